@@ -438,6 +438,106 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
                                                  const int64_t* o_strides, int64_t B, int64_t H, int HD,
                                                  void* stream);
 
+/* ---- State space layer: selective scan, short causal convolution, layer norm --------------------
+ * No reference counterpart.  Sizes: Dm channels, N states per channel (1..64), G groups of Dm / G
+ * channels that share B and C.  Operands in io_dtype: u, delta, z, y [Bn, T, Dm] and B, C
+ * [Bn, T, G, N] (innermost stride 1, other strides in elements, any alignment of an element, a
+ * stride of 0 for a broadcast input); fp32 and contiguous: A [Dm, N], D and delta_bias [Dm] (either
+ * may be NULL), states [*, Dm, N].
+ * A workspace is 16-byte aligned and belongs to one call at a time.
+ *
+ * Selective scan, per channel d and state n:
+ *     dt = delta + delta_bias, through softplus when `softplus`;  h <- exp(dt A) h + dt u B
+ *     y = (sum_n C h + D u) * silu(z)                     (no gate when z is NULL)
+ * strides[14] = (batch, token) of u, delta, z, y, then (batch, token, group) of B, C.  s0 (NULL:
+ * zeros) and s_final (NULL: not wanted): [Bn, Dm, N].  kept: NULL, or fp32 [Bn, ceil(T / 32), N, Dm]
+ * that receives the state of every 32nd token for triune_hip_ssm_bwd.  flags bits 8..15 force the
+ * length of a segment in units of 32 tokens (0: automatic). */
+size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags);
+int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const void* B, const void* C, const float* A,
+                        const float* D, const float* delta_bias, int io_dtype, const int64_t* strides, int softplus,
+                        const float* s0, void* y, float* s_final, float* kept, int64_t Bn, int64_t T, int64_t Dm,
+                        int64_t G, int N, int flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over packed sequences: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of u, delta, z, y
+ * [total_tokens, Dm] and B, C [total_tokens, G, N] are sequence i (int32 offsets on the device, ascending; rows
+ * outside them are neither read nor written).  strides[8] = token of u, delta, z, y, then (token,
+ * group) of B, C.  Sequence i starts from row slots[i] (i when slots is NULL) of s0 and leaves its
+ * last state in that row of s_final; s0 and s_final may be one pool.  Rows outside
+ * [0, n_state_rows) start from zero and keep nothing; other slots must be distinct. */
+size_t triune_hip_ssm_scan_varlen_workspace_size(int64_t n_seqs, int64_t total_tokens, int64_t Dm, int64_t G, int N,
+                                                 int flags);
+int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, const void* B, const void* C,
+                               const float* A, const float* D, const float* delta_bias, int io_dtype,
+                               const int64_t* strides, int softplus, const int32_t* cu_seqlens, int64_t n_seqs,
+                               int64_t total_tokens, const float* s0, float* s_final, const int32_t* slots,
+                               int64_t n_state_rows, void* y, int64_t Dm, int64_t G, int N, int flags,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of the dense scan from `kept` of the forward call.  strides[14] as there with dy in
+ * y's place.  ds_final: [Bn, Dm, N] or NULL.  Outputs, contiguous: du, ddelta, dz (with z) [Bn, T, Dm] and dB, dC
+ * [Bn, T, G, N] in io_dtype; fp32 dA [Dm, N], dD and ddelta_bias [Dm] (NULL: not wanted), ds0
+ * [Bn, Dm, N] (NULL: not wanted).  Sums are taken in a fixed order. */
+size_t triune_hip_ssm_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags);
+int triune_hip_ssm_bwd(const void* u, const void* delta, const void* z, const void* B, const void* C, const float* A,
+                       const float* D, const float* delta_bias, const void* dy, int io_dtype, const int64_t* strides,
+                       int softplus, const float* kept, const float* ds_final, void* du, void* ddelta, void* dz,
+                       void* dB, void* dC, float* dA, float* dD, float* ddelta_bias, float* ds0, int64_t Bn, int64_t T,
+                       int64_t Dm, int64_t G, int N, int flags, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* One token for each of Bn rows: u, delta, z, y [Bn, Dm], B, C [Bn, G, N]; strides[8] = row of u,
+ * delta, z, y, then (row, group) of B, C.  Row b reads and writes row slots[b] (b when slots is
+ * NULL) of state_in / state_out [n_state_rows, Dm, N], which may be one buffer; a slot outside
+ * [0, n_state_rows) reads and writes no state and gets zero outputs. */
+int triune_hip_ssm_decode_step(const void* u, const void* delta, const void* z, const void* B, const void* C,
+                               const float* A, const float* D, const float* delta_bias, int io_dtype,
+                               const int64_t* strides, int softplus, const float* state_in, float* state_out,
+                               const int32_t* slots, int64_t n_state_rows, void* y, int64_t Bn, int64_t Dm, int64_t G,
+                               int N, void* stream);
+
+/* Short causal depthwise convolution, W in 2..4 taps:
+ *     p_t = bias + sum_j w[d, j] x[t - W + 1 + j],  y = silu(p) when `silu`, else p
+ * x, y [Bn, T, Dm] in io_dtype (strides[4] = (batch, token) of x, y); w [Dm, W] and bias [Dm] (or
+ * NULL) contiguous in w_dtype (io_dtype or fp32).  s0: the W - 1 tokens before the first, [Bn, W - 1, Dm] contiguous in
+ * io_dtype (NULL: zeros); s_final (or NULL): the last W - 1 after the call, laid out the same. */
+int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io_dtype, int w_dtype,
+                          const int64_t* strides, int silu, const void* s0, void* s_final, void* y, int64_t Bn,
+                          int64_t T, int64_t Dm, int W, void* stream);
+/* Packed sequences over state rows, as triune_hip_ssm_scan_varlen; strides[2] = token of x, y. */
+int triune_hip_short_conv_varlen(const void* x, const void* w, const void* bias, int io_dtype, int w_dtype,
+                                 const int64_t* strides, int silu, const int32_t* cu_seqlens, int64_t n_seqs,
+                                 int64_t total_tokens, const void* s0, void* s_final, const int32_t* slots,
+                                 int64_t n_state_rows, void* y, int64_t Dm, int W, void* stream);
+/* One token for each of Bn rows over state rows, as triune_hip_ssm_decode_step; strides[2] = row of
+ * x, y. */
+int triune_hip_short_conv_decode_step(const void* x, const void* w, const void* bias, int io_dtype, int w_dtype,
+                                      const int64_t* strides, int silu, const void* state_in, void* state_out,
+                                      const int32_t* slots, int64_t n_state_rows, void* y, int64_t Bn, int64_t Dm,
+                                      int W, void* stream);
+/* Gradients of the dense convolution; strides[4] = (batch, token) of x, dy.  ds_final [Bn, W - 1, Dm]
+ * or NULL; dx [Bn, T, Dm] contiguous; dw, dbias in w_dtype, ds0 [Bn, W - 1, Dm] (each NULL: not wanted; the workspace
+ * is used for dw and dbias only).  Sums are taken in a fixed order. */
+size_t triune_hip_short_conv_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int W);
+int triune_hip_short_conv_bwd(const void* x, const void* w, const void* bias, const void* dy, int io_dtype,
+                              int w_dtype, const int64_t* strides, int silu, const void* s0, const void* ds_final,
+                              void* dx, void* dw, void* dbias, void* ds0, int64_t Bn, int64_t T, int64_t Dm, int W,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Layer norm of R rows of D elements (D <= 16384): y = (x - mean) rstd w + b, with
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  x: row stride x_stride, y contiguous, both io_dtype; w, b [D] (each may be
+ * NULL) in io_dtype or fp32; mean, rstd: fp32 [R] for the backward, or both NULL. */
+int triune_hip_layer_norm(const void* x, int64_t x_stride, const void* w, const void* b, int io_dtype, int w_dtype,
+                          int b_dtype, float eps, void* y, float* mean, float* rstd, int64_t R, int64_t D,
+                          void* stream);
+/* Its gradients: dx contiguous in io_dtype, dw in w_dtype and db in b_dtype (each NULL: not wanted;
+ * the workspace is used for these two only).  Sums are taken in a fixed order. */
+size_t triune_hip_layer_norm_bwd_workspace_size(int64_t R, int64_t D);
+int triune_hip_layer_norm_bwd(const void* x, int64_t x_stride, const void* w, const void* dy, int64_t dy_stride,
+                              int io_dtype, int w_dtype, int b_dtype, const float* mean, const float* rstd, void* dx,
+                              void* dw, void* db, int64_t R, int64_t D, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

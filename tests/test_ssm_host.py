@@ -1,0 +1,151 @@
+"""CPU: what the state space layer's entry points refuse before anything is launched."""
+
+import ctypes
+
+import pytest
+import torch
+
+import triune_amd
+import triune_amd._lib as L
+
+FAKE = ctypes.c_void_p(0x1000)  # aligned, never read: validation fails first or there is nothing to do
+ODD = ctypes.c_void_p(0x1001)
+NULL, SHAPE, DTYPE, LAYOUT, WORKSPACE = -1, -2, -3, -4, -5
+
+
+def st(n):
+    return (ctypes.c_int64 * n)(*([64] * n))
+
+
+def caller(name, order, **base):
+    fn = getattr(L.lib(), name)
+
+    def call(**kw):
+        a = {**base, **kw}
+        return fn(*[a[k] for k in order])
+
+    return call
+
+
+SCAN = "u dl z B C A D bias io st soft s0 y fin kept Bn T Dm G N flags ws wsb stream".split()
+VARLEN = "u dl z B C A D bias io st soft cu n total s0 fin slots rows y Dm G N flags ws wsb stream".split()
+BWD = ("u dl z B C A D bias dy io st soft kept dfin du dd dz dB dC dA dD db ds0 Bn T Dm G N flags ws wsb "
+       "stream").split()
+STEP = "u dl z B C A D bias io st soft s_in s_out slots rows y Bn Dm G N stream".split()
+
+
+def _scan_base(names):
+    base = {k: FAKE for k in names}
+    base.update(io=1, st=st(14), soft=1, z=None, D=None, bias=None, slots=None, ws=None, wsb=0, stream=None, flags=0,
+                Bn=2, T=64, Dm=64, G=1, N=16, n=2, total=64, rows=2, dz=None)
+    return base
+
+
+@pytest.mark.parametrize("name,order", [("triune_hip_ssm_scan", SCAN), ("triune_hip_ssm_scan_varlen", VARLEN),
+                                        ("triune_hip_ssm_bwd", BWD), ("triune_hip_ssm_decode_step", STEP)])
+def test_scan_entries_refuse(name, order):
+    call = caller(name, order, **_scan_base(order))
+    for k in ("u", "dl", "B", "C", "A", "st"):
+        assert call(**{k: None}) == NULL
+    assert call(io=7) == DTYPE
+    for kw in ({"N": 0}, {"N": 65}, {"G": 0}, {"G": 3}, {"Dm": 0}, {"Dm": 1 << 28}):
+        assert call(**kw) == SHAPE, kw
+    for k in ("u", "dl", "B", "C", "A", "D", "bias"):
+        assert call(**{k: ODD}) == LAYOUT, k
+    if "T" in order:
+        assert call(T=-1) == SHAPE and call(T=1 << 30) == SHAPE and call(Bn=-1) == SHAPE
+        assert call(Bn=1 << 40, T=1 << 29) == SHAPE  # more workgroups than a grid holds
+    if "rows" in order:
+        assert call(rows=1) == SHAPE  # fewer state rows than sequences and no slots
+        assert call(slots=ODD) == LAYOUT
+    if "cu" in order:
+        assert call(cu=None) == NULL and call(cu=ODD) == LAYOUT and call(total=-1) == SHAPE
+
+
+def test_scan_entries_need_their_workspace():
+    call = caller("triune_hip_ssm_bwd", BWD, **_scan_base(BWD))
+    need = L.lib().triune_hip_ssm_bwd_workspace_size(2, 64, 64, 1, 16, 0)
+    assert need > 0
+    assert call(ws=None, wsb=need) == WORKSPACE and call(ws=FAKE, wsb=need - 1) == WORKSPACE
+    assert call(ws=ctypes.c_void_p(0x1004), wsb=need) == LAYOUT
+    for k in ("kept", "du", "dd", "dB", "dC", "dA", "dy"):
+        assert call(**{k: None}) == NULL, k
+    assert call(z=FAKE) == NULL  # a gate without its gradient
+    assert call(Bn=0) == SHAPE and call(T=0) == SHAPE
+    scan = caller("triune_hip_ssm_scan", SCAN, **_scan_base(SCAN))
+    flags = 1 << 8  # segments of 32 tokens
+    need = L.lib().triune_hip_ssm_scan_workspace_size(2, 64, 64, 1, 16, flags)
+    assert need >= 2 * 2 * 17 * 64 * 4
+    assert scan(flags=flags, ws=FAKE, wsb=need - 1) == WORKSPACE
+
+
+def test_empty_calls_launch_nothing():
+    assert caller("triune_hip_ssm_scan", SCAN, **_scan_base(SCAN))(T=0) == 0
+    assert caller("triune_hip_ssm_scan", SCAN, **_scan_base(SCAN))(Bn=0) == 0
+    assert caller("triune_hip_ssm_scan_varlen", VARLEN, **_scan_base(VARLEN))(n=0) == 0
+    assert caller("triune_hip_ssm_decode_step", STEP, **_scan_base(STEP))(Bn=0) == 0
+    assert L.lib().triune_hip_ssm_scan_workspace_size(0, 64, 64, 1, 16, 0) == 0
+
+
+CONV = "x w bias io wdt st silu s0 fin y Bn T Dm W stream".split()
+CONV_V = "x w bias io wdt st silu cu n total s0 fin slots rows y Dm W stream".split()
+CONV_S = "x w bias io wdt st silu s0 fin slots rows y Bn Dm W stream".split()
+CONV_B = "x w bias dy io wdt st silu s0 dfin dx dw db ds0 Bn T Dm W ws wsb stream".split()
+
+
+def _conv_base(names):
+    base = {k: FAKE for k in names}
+    base.update(io=1, wdt=1, st=st(4), silu=1, bias=None, slots=None, ws=None, wsb=0, stream=None, Bn=2, T=64, Dm=64, W=4,
+                n=2, total=64, rows=2)
+    return base
+
+
+@pytest.mark.parametrize("name,order", [
+    ("triune_hip_short_conv", CONV), ("triune_hip_short_conv_varlen", CONV_V),
+    ("triune_hip_short_conv_decode_step", CONV_S), ("triune_hip_short_conv_bwd", CONV_B)])
+def test_conv_entries_refuse(name, order):
+    call = caller(name, order, **_conv_base(order))
+    for k in ("x", "w", "st"):
+        assert call(**{k: None}) == NULL
+    assert call(io=7) == DTYPE and call(wdt=2) == DTYPE and call(io=0, wdt=1) == DTYPE
+    for kw in ({"W": 1}, {"W": 5}, {"Dm": 0}, {"Dm": 1 << 28}):
+        assert call(**kw) == SHAPE, kw
+    for k in ("x", "w", "bias", "s0"):
+        assert call(**{k: ODD}) == LAYOUT, k
+    if "rows" in order:
+        assert call(rows=1) == SHAPE and call(slots=ODD) == LAYOUT
+    if "T" in order:
+        assert call(T=1 << 30) == SHAPE and call(Bn=1 << 24, T=1 << 20) == SHAPE
+    if "cu" in order:
+        assert call(cu=None) == NULL and call(cu=ODD) == LAYOUT
+    if "ws" in order:
+        need = L.lib().triune_hip_short_conv_bwd_workspace_size(2, 64, 64, 4)
+        assert need > 0 and call(ws=FAKE, wsb=need - 1) == WORKSPACE and call(dy=None) == NULL
+
+
+NORM = "x xs w b io wdt bdt eps y mean rstd R D stream".split()
+NORM_B = "x xs w dy ys io wdt bdt mean rstd dx dw db R D ws wsb stream".split()
+
+
+def test_norm_entries_refuse():
+    base = dict(x=FAKE, xs=64, w=FAKE, b=FAKE, io=1, wdt=1, bdt=0, eps=1e-5, y=FAKE, mean=None, rstd=None, R=4, D=64,
+                stream=None, dy=FAKE, ys=64, dx=FAKE, dw=FAKE, db=FAKE, ws=None, wsb=0)
+    fwd = caller("triune_hip_layer_norm", NORM, **base)
+    bwd = caller("triune_hip_layer_norm_bwd", NORM_B, **{**base, "mean": FAKE, "rstd": FAKE})
+    for call in (fwd, bwd):
+        assert call(x=None) == NULL and call(io=5) == DTYPE and call(wdt=2) == DTYPE and call(bdt=2) == DTYPE
+        assert call(D=0) == SHAPE and call(D=16385) == SHAPE and call(R=-1) == SHAPE
+        assert call(x=ODD) == LAYOUT and call(w=ODD) == LAYOUT
+    assert fwd(y=None) == NULL and fwd(mean=FAKE) == NULL and fwd(R=0) == 0
+    need = L.lib().triune_hip_layer_norm_bwd_workspace_size(4, 64)
+    assert need > 0 and bwd(ws=FAKE, wsb=need - 1) == WORKSPACE and bwd(R=0) == SHAPE and bwd(dx=None) == NULL
+
+
+def test_operators_refuse_cpu_tensors():
+    x, w = torch.zeros(1, 4, 8), torch.zeros(8, 4)
+    with pytest.raises(ValueError, match="CPU"):
+        triune_amd.short_conv(x, w)
+    with pytest.raises(ValueError, match="CPU"):
+        triune_amd.layer_norm(x)
+    with pytest.raises(ValueError, match="CPU"):
+        triune_amd.ssm_scan(x, x, w, torch.zeros(1, 4, 4), torch.zeros(1, 4, 4))

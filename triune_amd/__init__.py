@@ -16,6 +16,15 @@ from .fast_gla import (
 from .gla import gated_deltanet, gla
 from .gla_prep import (fused_qkv_g_prep_chunk_gla, fused_qkv_g_prep_inplace, fused_qkvg_decode_step,
                        fused_qkvg_decode_step_pool)
+from .norm import layer_norm
+from .ssm import (
+    short_conv,
+    short_conv_decode_step,
+    short_conv_varlen,
+    ssm_decode_step,
+    ssm_scan,
+    ssm_scan_varlen,
+)
 
 __all__ = [
     "FusedRecurrentScan",
@@ -31,4 +40,11 @@ __all__ = [
     "gated_deltanet",
     "gla",
     "gla_decode_step",
+    "layer_norm",
+    "short_conv",
+    "short_conv_decode_step",
+    "short_conv_varlen",
+    "ssm_decode_step",
+    "ssm_scan",
+    "ssm_scan_varlen",
 ]

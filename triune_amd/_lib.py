@@ -145,6 +145,55 @@ def _bind(lib):
              _vp],
             _i,
         ),
+        "triune_hip_ssm_scan_workspace_size": ([_i64, _i64, _i64, _i64, _i, _i], _sz),
+        "triune_hip_ssm_scan": (
+            [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64p, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _i,
+             _vp, _sz, _vp],
+            _i,
+        ),
+        "triune_hip_ssm_scan_varlen_workspace_size": ([_i64, _i64, _i64, _i64, _i, _i], _sz),
+        "triune_hip_ssm_scan_varlen": (
+            [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64p, _i, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64,
+             _i64, _i, _i, _vp, _sz, _vp],
+            _i,
+        ),
+        "triune_hip_ssm_bwd_workspace_size": ([_i64, _i64, _i64, _i64, _i, _i], _sz),
+        "triune_hip_ssm_bwd": (
+            [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64p, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+             _vp, _vp, _i64, _i64, _i64, _i64, _i, _i, _vp, _sz, _vp],
+            _i,
+        ),
+        "triune_hip_ssm_decode_step": (
+            [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i64p, _i, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i,
+             _vp],
+            _i,
+        ),
+        "triune_hip_short_conv": (
+            [_vp, _vp, _vp, _i, _i, _i64p, _i, _vp, _vp, _vp, _i64, _i64, _i64, _i, _vp],
+            _i,
+        ),
+        "triune_hip_short_conv_varlen": (
+            [_vp, _vp, _vp, _i, _i, _i64p, _i, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i, _vp],
+            _i,
+        ),
+        "triune_hip_short_conv_decode_step": (
+            [_vp, _vp, _vp, _i, _i, _i64p, _i, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i, _vp],
+            _i,
+        ),
+        "triune_hip_short_conv_bwd_workspace_size": ([_i64, _i64, _i64, _i], _sz),
+        "triune_hip_short_conv_bwd": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i64p, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _vp, _sz, _vp],
+            _i,
+        ),
+        "triune_hip_layer_norm": (
+            [_vp, _i64, _vp, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp],
+            _i,
+        ),
+        "triune_hip_layer_norm_bwd_workspace_size": ([_i64, _i64], _sz),
+        "triune_hip_layer_norm_bwd": (
+            [_vp, _i64, _vp, _vp, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp],
+            _i,
+        ),
     }
     for name, (argtypes, restype) in sig.items():
         fn = getattr(lib, name)
@@ -192,6 +241,21 @@ EXPORTS = (
     "triune_hip_gla_fused_decode_step",
     "triune_hip_gla_fused_decode_step_slots",
     "triune_hip_gla_fused_decode_step_slots_count",
+    "triune_hip_ssm_scan_workspace_size",
+    "triune_hip_ssm_scan",
+    "triune_hip_ssm_scan_varlen_workspace_size",
+    "triune_hip_ssm_scan_varlen",
+    "triune_hip_ssm_bwd_workspace_size",
+    "triune_hip_ssm_bwd",
+    "triune_hip_ssm_decode_step",
+    "triune_hip_short_conv",
+    "triune_hip_short_conv_varlen",
+    "triune_hip_short_conv_decode_step",
+    "triune_hip_short_conv_bwd_workspace_size",
+    "triune_hip_short_conv_bwd",
+    "triune_hip_layer_norm",
+    "triune_hip_layer_norm_bwd_workspace_size",
+    "triune_hip_layer_norm_bwd",
 )
 
 
@@ -251,6 +315,28 @@ def plan(t: torch.Tensor, name: str, *args) -> int:
     """The value of one of the library's size or support queries (a function of its arguments and of
     the device) for a call on t's device."""
     return _plan(t.get_device(), name, *args)
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """Run entry point `name` on t's device and its current stream (appended to args), whichever device
+    is current; raises TriuneHipError for any error it returns."""
+    L = lib()
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(L, name)(*args, stream_of(t))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(L, name)(*args, stream_of(t))
+    if rc != 0:
+        check(rc, name)
+
+
+def plan_on(t: torch.Tensor, name: str, *args) -> int:
+    """plan() with t's device current (the library asks the current device for its size)."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return plan(t, name, *args)
+    with torch.cuda.device(t.get_device()):
+        return plan(t, name, *args)
 
 
 _CTRL: dict = {}

@@ -1,0 +1,258 @@
+// layer_norm.hip -- layer norm over the last dim on gfx950, and its gradients.
+//
+//     xh = (x - mean) rstd;  y = xh w + b
+//     with g = dy w:  dx = rstd (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+// Bound by memory: a row is read once and stays in registers for its mean, its variance about that
+// mean (two passes over registers, so no cancellation) and its outputs.  A wave takes a row up to
+// 2048 wide, four waves one up to 8192, sixteen one up to 16384.  The backward's blocks walk rows
+// and hold their columns' dw and db in registers; a last kernel adds the blocks' parts in a fixed
+// order.
+#include "ssm.h"
+
+namespace triune {
+
+namespace {
+
+// The sum over the TPR threads of a row, in each of them.  `s` is used by rows of several waves.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float x, float* s) {
+    x = xor_sum<16>(xor_sum<32>(dpp_sum16(x)));
+    if constexpr (TPR > 64) {
+        const int w = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[w] = x;
+        __syncthreads();
+        x = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 64; ++i) x += s[i];
+    }
+    return x;
+}
+
+constexpr int block_threads(int tpr) { return tpr == 64 ? 256 : tpr; }
+
+// Columns of thread t: groups of eight, TPR * 8 apart.
+template <int TPR>
+__device__ __forceinline__ int column(int t, int k) {
+    return (k * TPR + t) * 8;
+}
+
+__device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, float none, float (&x)[8]) {
+    if (!p || n <= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = none;
+    } else if (dt == DT_F32) {
+        const Raw8<float> r = load_raw8((const float*)p + c, n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = r.v[j];
+    } else if (dt == DT_BF16) {
+        const Raw8<__bf16> r = load_raw8((const __bf16*)p + c, n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)r.v[j];
+    } else {
+        const Raw8<_Float16> r = load_raw8((const _Float16*)p + c, n);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)r.v[j];
+    }
+}
+
+}  // namespace
+
+template <typename T, int TPR, int K>
+__global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) {
+    constexpr int RPB = block_threads(TPR) / TPR;
+    __shared__ float s_red[16];
+    const int t = threadIdx.x % TPR;
+    const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (RPB > 1 && r >= a.R) return;  // whole waves
+    const T* px = (const T*)a.x + r * a.x_st;
+    T* py = (T*)a.y + r * a.D;
+    const float width = (float)a.D;  // divided by: a constant row's mean is its value where its sum is exact
+    Raw8<T> raw[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = column<TPR>(t, k);
+        raw[k] = load_raw8(px + c, a.D - c);
+    }
+    float x[K][8], s = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += x[k][j] = (float)raw[k].v[j];
+    const float mean = row_sum<TPR>(s, s_red) / width;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int left = a.D - column<TPR>(t, k);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[k][j] = j < left ? x[k][j] - mean : 0.f;
+            s = __builtin_fmaf(x[k][j], x[k][j], s);
+        }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(s, s_red) / width + a.eps);
+    if (a.mean && t == 0) {
+        a.mean[r] = mean;
+        a.rstd[r] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = column<TPR>(t, k), left = a.D - c;
+        if (left <= 0) continue;
+        float w[8], b[8], y[8];
+        load_par(a.w, a.w_dt, c, left, 1.f, w);
+        load_par(a.b, a.b_dt, c, left, 0.f, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[k][j] * rstd, w[j], b[j]);
+        store_raw8(py + c, left, y);
+    }
+}
+
+template <typename T, int TPR, int K>
+__global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdParams g) {
+    const NormParams& a = g.f;
+    constexpr int RPB = block_threads(TPR) / TPR;
+    __shared__ float s_red[16];
+    __shared__ float s_par[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * 8 : 1];
+    const int t = threadIdx.x % TPR, rl = threadIdx.x / TPR;
+    const float inv = 1.f / (float)a.D;
+    float w[K][8], dw[K][8], db[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = column<TPR>(t, k);
+        load_par(a.w, a.w_dt, c, a.D - c, 1.f, w[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dw[k][j] = db[k][j] = 0.f;
+    }
+    for (int64_t r = (int64_t)blockIdx.x * RPB + rl; r < a.R; r += (int64_t)gridDim.x * RPB) {
+        const T *px = (const T*)a.x + r * a.x_st, *py = (const T*)g.dy + r * g.dy_st;
+        T* pd = (T*)g.dx + r * a.D;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        Raw8<T> rx[K], ry[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = column<TPR>(t, k);
+            rx[k] = load_raw8(px + c, a.D - c);
+            ry[k] = load_raw8(py + c, a.D - c);
+        }
+        float s1 = 0.f, s2 = 0.f;
+        float xh[K][8];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                xh[k][j] = ((float)rx[k].v[j] - mean) * rstd;
+                const float dy = (float)ry[k].v[j], gg = dy * w[k][j];
+                s1 += gg;  // past the row's end dy is 0
+                s2 = __builtin_fmaf(gg, xh[k][j], s2);
+                dw[k][j] = __builtin_fmaf(dy, xh[k][j], dw[k][j]);
+                db[k][j] += dy;
+            }
+        }
+        const float m1 = row_sum<TPR>(s1, s_red) * inv, m2 = row_sum<TPR>(s2, s_red) * inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = column<TPR>(t, k), left = a.D - c;
+            if (left <= 0) continue;
+            float o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                o[j] = rstd * ((float)ry[k].v[j] * w[k][j] - __builtin_fmaf(xh[k][j], m2, m1));
+            store_raw8(pd + c, left, o);
+        }
+    }
+    if (!g.part) return;
+    float* pp = g.part + (int64_t)blockIdx.x * 2 * a.D;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = q ? db[k][j] : dw[k][j];
+            const int c = column<TPR>(t, k);
+            if constexpr (RPB > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s_par[rl][j * TPR + t] = v[j];
+                __syncthreads();
+                for (int e = threadIdx.x; e < TPR * 8; e += block_threads(TPR)) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int i = 0; i < RPB; ++i) s += s_par[i][(e & 7) * TPR + (e >> 3)];
+                    const int col = k * TPR * 8 + e;
+                    if (col < a.D) pp[(int64_t)q * a.D + col] = s;
+                }
+            } else if (c < a.D) {
+                store_raw8(pp + (int64_t)q * a.D + c, a.D - c, v);
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void norm_bwd_sum_kernel(NormBwdParams g) {
+    const int per = 2 * g.f.D, l = threadIdx.x & 63, id = blockIdx.x * 64 + l, w = threadIdx.x >> 6;
+    __shared__ float red[4][64];
+    float s = 0.f;
+    if (id < per)
+        for (int64_t p = w; p < g.parts; p += 4) s += g.part[p * per + id];
+    red[w][l] = s;
+    __syncthreads();
+    if (w || id >= per) return;
+    s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    if (id < g.f.D) {
+        if (g.dw) store_dt(g.dw, g.f.w_dt, id, s);
+    } else if (g.db) {
+        store_dt(g.db, g.f.b_dt, id - g.f.D, s);
+    }
+}
+
+int64_t norm_bwd_parts(int64_t R, int D, int cus) {
+    const int64_t rpb = D <= 2048 ? 4 : 1, blocks = (R + rpb - 1) / rpb, most = (int64_t)cus * 2;
+    return blocks < most ? blocks : most;
+}
+
+namespace {
+
+template <typename T, int TPR, int K>
+hipError_t norm_run(const NormParams& a, hipStream_t s) {
+    constexpr int RPB = block_threads(TPR) / TPR;
+    norm_kernel<T, TPR, K><<<dim3((unsigned)((a.R + RPB - 1) / RPB)), block_threads(TPR), 0, s>>>(a);
+    return hipGetLastError();
+}
+template <typename T, int TPR, int K>
+hipError_t norm_run(const NormBwdParams& g, hipStream_t s) {
+    norm_bwd_kernel<T, TPR, K><<<dim3((unsigned)g.parts), block_threads(TPR), 0, s>>>(g);
+    return hipGetLastError();
+}
+
+template <typename T, typename P>
+hipError_t norm_width(const P& p, int D, hipStream_t s) {
+    if (D <= 512) return norm_run<T, 64, 1>(p, s);
+    if (D <= 1024) return norm_run<T, 64, 2>(p, s);
+    if (D <= 1536) return norm_run<T, 64, 3>(p, s);
+    if (D <= 2048) return norm_run<T, 64, 4>(p, s);
+    if (D <= 4096) return norm_run<T, 256, 2>(p, s);
+    if (D <= 8192) return norm_run<T, 256, 4>(p, s);
+    return norm_run<T, 1024, 2>(p, s);
+}
+
+template <typename P>
+hipError_t norm_dtype(const P& p, int D, int dt, hipStream_t s) {
+    if (dt == DT_F32) return norm_width<float>(p, D, s);
+    if (dt == DT_BF16) return norm_width<__bf16>(p, D, s);
+    return norm_width<_Float16>(p, D, s);
+}
+
+}  // namespace
+
+hipError_t launch_norm(const NormParams& a, int dt, hipStream_t s) { return norm_dtype(a, a.D, dt, s); }
+
+hipError_t launch_norm_bwd(const NormBwdParams& g, int dt, hipStream_t s) {
+    const hipError_t e = norm_dtype(g, g.f.D, dt, s);
+    if (e != hipSuccess || !g.part) return e;
+    norm_bwd_sum_kernel<<<dim3((unsigned)((2 * g.f.D + 63) / 64)), 256, 0, s>>>(g);
+    return hipGetLastError();
+}
+
+}  // namespace triune

@@ -1,0 +1,402 @@
+// short_conv.hip -- the short causal depthwise convolution on gfx950: prompts, packed prompts, single
+// tokens and gradients.
+//
+//     p_t = bias + sum_j w_j x_{t-W+1+j}  (j < W; tokens before the first come from the state),
+//     y_t = silu(p_t) or p_t
+// Bound by memory: every value is read and written once.  A thread owns eight channels (16 bytes of a
+// 16-bit row, so a wave's access is whole cache lines) and walks a run of tokens with the last W - 1
+// of them in registers, so a token is read again only as the next run's first W - 1.
+#include "ssm.h"
+
+namespace triune {
+
+namespace {
+
+constexpr int RUN = 16;      // tokens of a forward run: a halo of 3 in 16, and runs enough for short prompts
+constexpr int BWD_RUN = 32;  // the gradient reads two tensors' halo
+constexpr int STEP = 4;      // tokens whose loads are in flight together
+
+// Lanes along the channels (a power of two, at most a wave): the rest of the block takes further runs.
+int channel_lanes(int D) {
+    int n = 1;
+    while (n < 64 && n * 8 < D) n *= 2;
+    return n;
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const Raw8<T>& r, float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)r.v[j];
+}
+
+template <int W>
+struct Taps {
+    float w[W][8], b[8];
+};
+template <int W>
+__device__ __forceinline__ void load_taps(const ConvParams& a, int c, int n, Taps<W>& k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool ok = i < n;
+#pragma unroll
+        for (int j = 0; j < W; ++j) k.w[j][i] = ok ? load_dt(a.w, a.w_dt, (int64_t)(c + i) * W + j) : 0.f;
+        k.b[i] = ok && a.bias ? load_dt(a.bias, a.w_dt, c + i) : 0.f;
+    }
+}
+
+// Row i (0 .. W - 2, oldest first) of a sequence's state, zeros without one.
+template <typename T, int W>
+__device__ __forceinline__ Raw8<T> state_row(const ConvParams& a, int64_t row, int i, int c, int n) {
+    i = i < 0 ? 0 : i;  // only where a packed call's offsets do not ascend
+    return load_raw8((const T*)a.s0 + (row * (W - 1) + i) * a.Dm + c, a.s0 && row >= 0 ? n : 0);
+}
+
+}  // namespace
+
+template <typename T, int W, bool PACKED>
+__global__ __launch_bounds__(256) void conv_kernel(ConvParams a, int cl, int cblocks) {
+    const int lc = threadIdx.x & (cl - 1), rl = threadIdx.x / cl, runs_pb = 256 / cl;
+    const int64_t rb = blockIdx.x / cblocks;
+    const int c = ((int)(blockIdx.x - rb * cblocks) * cl + lc) * 8;
+    const int n = min(a.Dm - c, 8);
+    if (n <= 0) return;
+    const int64_t run = rb * runs_pb + rl, per = (a.T + RUN - 1) / RUN;
+    int64_t seq, t0, t1, beg, end;  // tokens t0 .. t1 - 1; the sequence that holds t0 is beg .. end - 1
+    if constexpr (PACKED) {
+        t0 = run * RUN;
+        t1 = min(t0 + RUN, min((int64_t)a.cu[a.n_seqs], a.T));
+        t0 = max(t0, max((int64_t)a.cu[0], (int64_t)0));
+        if (t0 >= t1) return;
+        int64_t lo = 0, hi = a.n_seqs;  // cu[lo] <= t0 < cu[hi]
+        while (hi - lo > 1) {
+            const int64_t m = (lo + hi) >> 1;
+            if (a.cu[m] <= t0) lo = m; else hi = m;
+        }
+        seq = lo;
+        beg = max((int64_t)a.cu[seq], (int64_t)0);
+        end = a.cu[seq + 1];
+    } else {
+        seq = run / per;
+        if (seq >= a.n_seqs) return;
+        t0 = (run - seq * per) * RUN;
+        t1 = min(t0 + RUN, a.T);
+        beg = 0;
+        end = a.T;
+    }
+    const T* px = (const T*)a.x + (PACKED ? 0 : seq * a.x_sb) + c;
+    T* py = (T*)a.y + (PACKED ? 0 : seq * a.y_sb) + c;
+    Taps<W> k;
+    load_taps<W>(a, c, n, k);
+    float win[W - 1][8];  // tokens t - W + 1 .. t - 1
+    Raw8<T> last[W - 1];  // the same as they came, for the state
+    auto window = [&](int64_t t) {
+        const int64_t row = ssm_row(a.slots, a.n_slots, seq);
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) {
+            const int64_t s = t - (W - 1) + i;
+            last[i] = s >= beg ? load_raw8(px + s * a.x_st, n) : state_row<T, W>(a, row, (int)(s - beg) + W - 1, c, n);
+            widen(last[i], win[i]);
+        }
+    };
+    window(t0);
+    for (int64_t t = t0; t < t1; t += STEP) {
+        Raw8<T> r[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) r[i] = load_raw8(px + (t + i) * a.x_st, t + i < t1 ? n : 0);
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+            if (t + i >= t1) break;
+            if (PACKED && t + i >= end) {  // the next sequence that holds tokens
+                while (t + i >= end && seq + 1 < a.n_seqs) end = a.cu[++seq + 1];
+                beg = max((int64_t)a.cu[seq], (int64_t)0);
+                window(t + i);
+            }
+            float x[8], y[8];
+            widen(r[i], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float p = __builtin_fmaf(k.w[W - 1][e], x[e], k.b[e]);
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) p = __builtin_fmaf(k.w[j][e], win[j][e], p);
+                y[e] = a.silu ? silu_gate(p) : p;
+#pragma unroll
+                for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
+                win[W - 2][e] = x[e];
+            }
+            store_raw8(py + (t + i) * a.y_st, n, y);
+            if constexpr (!PACKED) {
+#pragma unroll
+                for (int j = 0; j < W - 2; ++j) last[j] = last[j + 1];
+                last[W - 2] = r[i];
+            }
+        }
+    }
+    if (!PACKED && a.fin && t1 == a.T) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) {
+            float v[8];
+            widen(last[j], v);
+            store_raw8((T*)a.fin + (seq * (W - 1) + j) * a.Dm + c, n, v);
+        }
+    }
+}
+
+// Packed calls: the states after the sequences, in a launch of its own because a pool's rows are
+// read by every run at a sequence's start.  One thread per (sequence, eight channels).
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_state_kernel(ConvParams a) {
+    const int64_t groups = (a.Dm + 7) / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t seq = id / groups;
+    if (seq >= a.n_seqs) return;
+    const int c = (int)(id - seq * groups) * 8, n = min(a.Dm - c, 8);
+    const int64_t row = ssm_row(a.slots, a.n_slots, seq);
+    if (row < 0) return;
+    const int64_t beg = min(max((int64_t)a.cu[seq], (int64_t)0), a.T);
+    const int64_t len = min(max((int64_t)a.cu[seq + 1], beg), a.T) - beg;
+    Raw8<T> r[W - 1];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        const int64_t s = len - (W - 1) + i;
+        r[i] = s >= 0 ? load_raw8((const T*)a.x + (beg + s) * a.x_st + c, n)
+                      : state_row<T, W>(a, row, (int)s + W - 1, c, n);
+    }
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        float v[8];
+        widen(r[i], v);
+        store_raw8((T*)a.fin + (row * (W - 1) + i) * a.Dm + c, n, v);
+    }
+}
+
+// One token for every row.  One thread per (row, VEC channels).
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_step_kernel(ConvParams a) {
+    const int64_t groups = (a.Dm + 7) / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t b = id / groups;
+    if (b >= a.n_seqs) return;
+    const int c = (int)(id - b * groups) * 8, n = min(a.Dm - c, 8);
+    const int64_t row = ssm_row(a.slots, a.n_slots, b);
+    Raw8<T> r[W];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) r[i] = state_row<T, W>(a, row, i, c, n);
+    r[W - 1] = load_raw8((const T*)a.x + b * a.x_sb + c, n);
+    Taps<W> k;
+    load_taps<W>(a, c, n, k);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float p = k.b[e];
+#pragma unroll
+        for (int j = 0; j < W; ++j) p = __builtin_fmaf(k.w[j][e], (float)r[j].v[e], p);
+        y[e] = row >= 0 ? (a.silu ? silu_gate(p) : p) : 0.f;
+    }
+    store_raw8((T*)a.y + b * a.y_sb + c, n, y);
+    if (row < 0) return;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        float v[8];
+        widen(r[i + 1], v);
+        store_raw8((T*)a.fin + (row * (W - 1) + i) * a.Dm + c, n, v);
+    }
+}
+
+// Gradients.  With dp_t = dy_t silu'(p_t): dx_s = sum_j w_j dp_{s+W-1-j} (s < 0: the state's rows),
+// dw_j = sum_t dp_t x_{t-W+1+j}, dbias = sum_t dp_t.  A run walks its tokens and W - 1 more, whose
+// dp it forms again; the gradient of token t - W + 1 is whole once dp_t is in.  Runs of a block add
+// their dw in LDS, blocks through memory in a fixed order.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, int cblocks) {
+    const ConvParams& a = g.f;
+    __shared__ float s_red[256][9];
+    const int lc = threadIdx.x & (cl - 1), rl = threadIdx.x / cl, runs_pb = 256 / cl;
+    const int64_t rb = blockIdx.x / cblocks;
+    const int c = ((int)(blockIdx.x - rb * cblocks) * cl + lc) * 8;
+    const int n = min(a.Dm - c, 8);
+    const int64_t run = rb * runs_pb + rl, per = (a.T + BWD_RUN - 1) / BWD_RUN;
+    const int64_t seq = run / per;
+    float dw[W + 1][8];  // dw, then dbias
+#pragma unroll
+    for (int j = 0; j <= W; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[j][e] = 0.f;
+    if (n > 0 && seq < a.n_seqs) {
+        const int64_t t0 = (run - seq * per) * BWD_RUN, t1 = min(t0 + BWD_RUN, a.T);
+        // the gradients of t0 .. t1 - 1, before them the state's rows (first run)
+        const int64_t from = t0 == 0 ? -(W - 1) : t0;
+        const T* px = (const T*)a.x + seq * a.x_sb + c;
+        const T* py = (const T*)g.dy + seq * g.dy_sb + c;
+        T* pd = (T*)g.dx + seq * a.T * a.Dm + c;
+        Taps<W> k;
+        load_taps<W>(a, c, n, k);
+        float win[W - 1][8], acc[W][8];  // acc[i]: the gradient of token t - W + 1 + i
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) {
+            const int64_t s = t0 - (W - 1) + i;
+            const Raw8<T> r = s >= 0 ? load_raw8(px + s * a.x_st, n) : state_row<T, W>(a, seq, (int)s + W - 1, c, n);
+            widen(r, win[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
+        const int64_t stop = t1 + W - 1;
+        for (int64_t t = t0; t < stop; t += STEP) {
+            Raw8<T> rx[STEP], ry[STEP];
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) {
+                const int m = t + i < stop && t + i < a.T ? n : 0;
+                rx[i] = load_raw8(px + (t + i) * a.x_st, m);
+                ry[i] = load_raw8(py + (t + i) * g.dy_st, m);
+            }
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) {
+                const int64_t tt = t + i;
+                if (tt >= stop) break;
+                float x[8], dy[8];
+                widen(rx[i], x);
+                widen(ry[i], dy);
+                const bool own = tt < t1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float dp = dy[e];
+                    if (a.silu) {
+                        float p = __builtin_fmaf(k.w[W - 1][e], x[e], k.b[e]);
+#pragma unroll
+                        for (int j = 0; j < W - 1; ++j) p = __builtin_fmaf(k.w[j][e], win[j][e], p);
+                        const float s = sigmoid(p);
+                        dp *= s * __builtin_fmaf(p, 1.f - s, 1.f);
+                    }
+                    if (tt >= a.T) dp = 0.f;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) acc[j][e] = __builtin_fmaf(k.w[j][e], dp, acc[j][e]);
+                    const float d = own ? dp : 0.f;
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) dw[j][e] = __builtin_fmaf(d, win[j][e], dw[j][e]);
+                    dw[W - 1][e] = __builtin_fmaf(d, x[e], dw[W - 1][e]);
+                    dw[W][e] += d;
+#pragma unroll
+                    for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
+                    win[W - 2][e] = x[e];
+                }
+                const int64_t s = tt - (W - 1);  // acc[0] is its whole gradient
+                if (s >= from) {
+                    float out[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) out[e] = acc[0][e];
+                    if (g.dfin && s >= a.T - (W - 1)) {
+                        float f[8];
+                        widen(load_raw8((const T*)g.dfin + (seq * (W - 1) + s - (a.T - (W - 1))) * a.Dm + c, n), f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) out[e] += f[e];
+                    }
+                    if (s >= 0) store_raw8(pd + s * a.Dm, n, out);
+                    else if (g.ds0) store_raw8((T*)g.ds0 + (seq * (W - 1) + s + W - 1) * a.Dm + c, n, out);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                    for (int j = 0; j < W - 1; ++j) acc[j][e] = acc[j + 1][e];
+                    acc[W - 1][e] = 0.f;
+                }
+            }
+        }
+    }
+    if (!g.part) return;
+#pragma unroll
+    for (int j = 0; j <= W; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_red[threadIdx.x][e] = dw[j][e];
+        __syncthreads();
+        for (int q = threadIdx.x; q < cl * 8; q += 256) {
+            const int ch = ((int)(blockIdx.x - rb * cblocks) * cl) * 8 + q;
+            float s = 0.f;
+            for (int r = 0; r < runs_pb; ++r) s += s_red[r * cl + (q >> 3)][q & 7];
+            if (ch < a.Dm) g.part[(rb * (W + 1) + j) * a.Dm + ch] = s;
+        }
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(256) void conv_bwd_sum_kernel(ConvBwdParams g) {
+    const ConvParams& a = g.f;
+    const int per = (a.W + 1) * a.Dm, id = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    __shared__ float red[4][64];
+    float s = 0.f;
+    if (id < per)
+        for (int64_t p = w; p < g.parts; p += 4) s += g.part[p * per + id];
+    red[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w || id >= per) return;
+    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    const int j = id / a.Dm, ch = id - j * a.Dm;
+    if (j < a.W) {
+        if (g.dw) store_dt(g.dw, a.w_dt, (int64_t)ch * a.W + j, s);
+    } else if (g.dbias) {
+        store_dt(g.dbias, a.w_dt, ch, s);
+    }
+}
+
+int64_t conv_bwd_parts(int64_t n_seqs, int64_t T, int D) {
+    const int64_t runs = n_seqs * ((T + BWD_RUN - 1) / BWD_RUN), pb = 256 / channel_lanes(D);
+    return (runs + pb - 1) / pb;
+}
+
+namespace {
+
+struct Grid {
+    int cl, cblocks;
+    int64_t blocks;
+};
+Grid run_grid(int64_t runs, int D) {
+    Grid g;
+    g.cl = channel_lanes(D);
+    g.cblocks = (D + g.cl * 8 - 1) / (g.cl * 8);
+    g.blocks = (runs + 256 / g.cl - 1) / (256 / g.cl) * g.cblocks;
+    return g;
+}
+dim3 thread_blocks(int64_t n) { return dim3((unsigned)((n + 255) / 256)); }
+
+template <typename T, int W>
+hipError_t conv_w(const ConvParams& a, hipStream_t s) {
+    const int64_t per = (a.T + RUN - 1) / RUN;
+    const Grid g = run_grid(a.cu ? per : a.n_seqs * per, a.Dm);
+    if (a.cu) conv_kernel<T, W, true><<<dim3((unsigned)g.blocks), 256, 0, s>>>(a, g.cl, g.cblocks);
+    else conv_kernel<T, W, false><<<dim3((unsigned)g.blocks), 256, 0, s>>>(a, g.cl, g.cblocks);
+    return hipGetLastError();
+}
+template <typename T, int W>
+hipError_t conv_state_w(const ConvParams& a, hipStream_t s) {
+    conv_state_kernel<T, W><<<thread_blocks(a.n_seqs * ((a.Dm + 7) / 8)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <typename T, int W>
+hipError_t conv_step_w(const ConvParams& a, hipStream_t s) {
+    conv_step_kernel<T, W><<<thread_blocks(a.n_seqs * ((a.Dm + 7) / 8)), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <typename T, int W>
+hipError_t conv_bwd_w(const ConvBwdParams& b, hipStream_t s) {
+    const ConvParams& a = b.f;
+    const Grid g = run_grid(a.n_seqs * ((a.T + BWD_RUN - 1) / BWD_RUN), a.Dm);
+    conv_bwd_kernel<T, W><<<dim3((unsigned)g.blocks), 256, 0, s>>>(b, g.cl, g.cblocks);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !b.part) return e;
+    conv_bwd_sum_kernel<<<dim3((unsigned)(((W + 1) * a.Dm + 63) / 64)), 256, 0, s>>>(b);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+#define CONV_DISPATCH(FN, W_, DT, ...)                                      \
+    switch (W_) {                                                           \
+        case 2: return DT == DT_F32 ? FN<float, 2>(__VA_ARGS__) : DT == DT_BF16 ? FN<__bf16, 2>(__VA_ARGS__) : FN<_Float16, 2>(__VA_ARGS__); \
+        case 3: return DT == DT_F32 ? FN<float, 3>(__VA_ARGS__) : DT == DT_BF16 ? FN<__bf16, 3>(__VA_ARGS__) : FN<_Float16, 3>(__VA_ARGS__); \
+        default: return DT == DT_F32 ? FN<float, 4>(__VA_ARGS__) : DT == DT_BF16 ? FN<__bf16, 4>(__VA_ARGS__) : FN<_Float16, 4>(__VA_ARGS__); \
+    }
+
+hipError_t launch_conv(const ConvParams& a, int dt, hipStream_t s) { CONV_DISPATCH(conv_w, a.W, dt, a, s) }
+hipError_t launch_conv_state(const ConvParams& a, int dt, hipStream_t s) { CONV_DISPATCH(conv_state_w, a.W, dt, a, s) }
+hipError_t launch_conv_step(const ConvParams& a, int dt, hipStream_t s) { CONV_DISPATCH(conv_step_w, a.W, dt, a, s) }
+hipError_t launch_conv_bwd(const ConvBwdParams& b, int dt, hipStream_t s) { CONV_DISPATCH(conv_bwd_w, b.f.W, dt, b, s) }
+
+}  // namespace triune

@@ -1,0 +1,252 @@
+// ssm.h -- parameter blocks and launchers of the state space layer's kernels: the selective scan
+// (ssm.hip, ssm_bwd.hip), the short causal convolution (short_conv.hip) and layer norm
+// (layer_norm.hip).  Internal to libtriune_hip.
+#pragma once
+
+#include "common.h"
+
+namespace triune {
+
+constexpr int SSM_BLOCK = 64;  // channels of a workgroup: one per lane
+constexpr int SSM_CKPT = 32;   // tokens between two states that the forward keeps for the backward
+constexpr int SSM_MAX_N = 64;  // states per channel
+
+// A [tokens, channels] operand of a batch of sequences: element strides, innermost stride 1.
+struct SsmTok {
+    const void* p;
+    int64_t sb, st;
+};
+
+struct SsmParams {
+    SsmTok u, dl, z, y;       // z.p null: no gate
+    const void *B, *C;        // [.., G, N] rows
+    int64_t b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+    const float *A, *D, *bias;  // [Dm, N], [Dm] or null, [Dm] or null
+    int softplus;
+    const float* s0;          // [rows, Dm, N] or null
+    float* fin;               // [rows, Dm, N] or null
+    const int32_t* slots;     // packed over a pool: the row of each sequence, else null
+    int64_t n_slots;
+    float* ckpt;              // [Bn, ceil(T / SSM_CKPT), N, Dm] or null
+    float* ws_state;          // [n_work, N, Dm]: a segment's own end state, then the state it starts from
+    float* ws_sum;            // [n_work, Dm]: summed step sizes
+    int64_t n_seqs, T;        // T: length of a dense sequence, or all tokens of a packed call
+    int Dm, G, N;
+    int blocks;               // channel blocks of a group
+    int seg, nseg;            // tokens of a segment, segments of a dense sequence
+    int64_t n_work;
+    const int32_t *cu, *seg_off;  // packed: [n_seqs + 1] token and segment offsets
+};
+
+struct SsmBwdParams {
+    SsmParams f;              // ws_state / ws_sum: the gradient's segment ends (nseg > 1)
+    SsmTok dy;
+    const float* dfin;        // [Bn, Dm, N] or null
+    void *du, *ddl, *dz;      // [Bn, T, Dm] contiguous, I/O dtype (dz null with z.p)
+    float* part_bc;           // [G * blocks, Bn * T, waves, 8]
+    float* part_par;          // [n_work, N + 2, Dm]: A's rows, D, bias
+    void *dB, *dC;            // [Bn, T, G, N] contiguous, I/O dtype
+    float *dA, *dD, *dbias;   // [Dm, N], [Dm], [Dm]; null where not wanted
+    float* ds0;               // [Bn, Dm, N] or null
+};
+
+struct SsmStepParams {
+    SsmTok u, dl, z, y;       // [Bn, Dm] rows: sb is the row stride
+    const void *B, *C;
+    int64_t b_sb, b_sg, c_sb, c_sg;
+    const float *A, *D, *bias;
+    int softplus;
+    const float* s_in;
+    float* s_out;
+    const int32_t* slots;
+    int64_t n_rows;           // rows of the state
+    int64_t Bn;
+    int Dm, G, N;
+};
+
+int ssm_waves(int N);                 // waves of a scan workgroup: four states each
+hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* seg_off, hipStream_t s);
+hipError_t launch_ssm_states(const SsmParams& a, int io_dt, hipStream_t s);
+hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s);
+hipError_t launch_ssm_scan(const SsmParams& a, int io_dt, hipStream_t s);
+hipError_t launch_ssm_step(const SsmStepParams& a, int io_dt, hipStream_t s);
+hipError_t launch_ssm_bwd_states(const SsmBwdParams& a, int io_dt, hipStream_t s);
+hipError_t launch_ssm_bwd_carry(const SsmBwdParams& a, hipStream_t s);
+hipError_t launch_ssm_bwd(const SsmBwdParams& a, int io_dt, hipStream_t s);
+hipError_t launch_ssm_bwd_sum(const SsmBwdParams& a, int io_dt, hipStream_t s);
+
+// ---- short causal convolution --------------------------------------------------------------
+struct ConvParams {
+    const void* x;            // [Bn, T, Dm] or packed rows, element strides
+    int64_t x_sb, x_st;
+    const void *w, *bias;     // [Dm, W] and [Dm] (or null) of w_dt
+    int w_dt, silu;
+    const void* s0;           // [rows, W - 1, Dm] of the I/O dtype, or null (zeros)
+    void* fin;                // the same after the call, or null
+    const int32_t* slots;     // the state row of each sequence, else null
+    int64_t n_slots;          // state rows
+    void* y;
+    int64_t y_sb, y_st;
+    int64_t n_seqs, T;        // T: length of a dense sequence, or all rows of a packed call
+    int Dm, W;
+    const int32_t* cu;        // packed: [n_seqs + 1]
+};
+
+struct ConvBwdParams {
+    ConvParams f;
+    const void* dy;           // [Bn, T, Dm]
+    int64_t dy_sb, dy_st;
+    const void* dfin;         // [Bn, W - 1, Dm] contiguous or null
+    void* dx;                 // [Bn, T, Dm] contiguous
+    void* ds0;                // [Bn, W - 1, Dm] contiguous or null
+    float* part;              // [parts, W + 1, Dm]
+    int64_t parts;
+    void *dw, *dbias;         // of w_dt, or null
+};
+
+int64_t conv_bwd_parts(int64_t n_seqs, int64_t T, int Dm);
+hipError_t launch_conv(const ConvParams& a, int io_dt, hipStream_t s);
+hipError_t launch_conv_state(const ConvParams& a, int io_dt, hipStream_t s);
+hipError_t launch_conv_step(const ConvParams& a, int io_dt, hipStream_t s);
+hipError_t launch_conv_bwd(const ConvBwdParams& a, int io_dt, hipStream_t s);
+
+// ---- layer norm ----------------------------------------------------------------------------
+constexpr int NORM_MAX_D = 16384;
+
+struct NormParams {
+    const void* x;            // [R, D], row stride x_st
+    int64_t x_st;
+    const void *w, *b;        // [D] of w_dt / b_dt, or null
+    int w_dt, b_dt;
+    float eps;
+    void* y;                  // [R, D] contiguous
+    float *mean, *rstd;       // [R] or null
+    int64_t R;
+    int D;
+};
+
+struct NormBwdParams {
+    NormParams f;             // x, w, mean, rstd, R, D
+    const void* dy;
+    int64_t dy_st;
+    void* dx;                 // [R, D] contiguous
+    float* part;              // [parts, 2, D], or null without parameter gradients
+    int64_t parts;
+    void *dw, *db;            // of w_dt / b_dt, or null
+};
+
+int64_t norm_bwd_parts(int64_t R, int D, int cus);
+hipError_t launch_norm(const NormParams& a, int io_dt, hipStream_t s);
+hipError_t launch_norm_bwd(const NormBwdParams& a, int io_dt, hipStream_t s);
+
+// ---- device helpers ---------------------------------------------------------------------------
+__device__ __forceinline__ float silu_gate(float z) { return z * sigmoid(z); }
+
+// log(1 + e^-|x|) + max(x, 0).  With s = e / (2 + e), log(1 + e) = 2 atanh(s), whose series in s^2
+// <= 1/9 is cut to a fitted polynomial (relative error 4e-9): the form keeps the relative precision
+// where e is small (step sizes of 1e-3 have e = 1e-3, of which log(1 + e) would lose ten bits).
+__device__ __forceinline__ float softplus(float x) {
+    const float e = fast_exp(-fabsf(x));
+    const float s = e * __builtin_amdgcn_rcpf(2.f + e), t = s * s;
+    float p = 0.28174665570259094f;
+    p = __builtin_fmaf(p, t, 0.27961426973342896f);
+    p = __builtin_fmaf(p, t, 0.40024852752685547f);
+    p = __builtin_fmaf(p, t, 0.6666631698608398f);
+    p = __builtin_fmaf(p, t, 2.0f);
+    return __builtin_fmaf(s, p, fmaxf(x, 0.f));
+}
+
+// Eight elements of any alignment in one access (the memory pipeline takes unaligned vectors), or the
+// n < 8 that a row's last group holds.
+template <typename T>
+struct __attribute__((packed, aligned(alignof(T)))) Raw8 {
+    T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int n) {
+    Raw8<T> r;
+    if (n >= 8) {
+        r = *reinterpret_cast<const Raw8<T>*>(p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_raw8(T* p, int n, const float (&x)[8]) {
+    Raw8<T> r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = (T)x[j];
+    if (n >= 8) {
+        *reinterpret_cast<Raw8<T>*>(p) = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) p[j] = r.v[j];
+    }
+}
+
+__device__ __forceinline__ float load_dt(const void* p, int dt, int64_t i) {
+    if (dt == DT_F32) return ((const float*)p)[i];
+    if (dt == DT_BF16) return (float)((const __bf16*)p)[i];
+    return (float)((const _Float16*)p)[i];
+}
+__device__ __forceinline__ void store_dt(void* p, int dt, int64_t i, float x) {
+    if (dt == DT_F32) ((float*)p)[i] = x;
+    else if (dt == DT_BF16) ((__bf16*)p)[i] = (__bf16)x;
+    else ((_Float16*)p)[i] = (_Float16)x;
+}
+
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
+
+// The tokens of work item w: sequence, first token (of the sequence), length, whether it is the
+// sequence's last segment.  False when there is no such item (packed calls bound their number).
+struct SsmSeg {
+    int64_t seq, row0, t0;  // row0: first token of the sequence in a packed tensor
+    int len, index;
+    bool last;
+};
+__device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSeg& s) {
+    if (!a.cu) {
+        s.seq = w / a.nseg;
+        s.index = (int)(w - s.seq * a.nseg);
+        s.row0 = 0;
+        s.t0 = (int64_t)s.index * a.seg;
+        s.len = (int)min((int64_t)a.seg, a.T - s.t0);
+        s.last = s.index == a.nseg - 1;
+        return true;
+    }
+    int64_t lo = w, first = w;  // without segment offsets every sequence is one segment
+    s.last = true;
+    if (a.seg_off) {
+        if (w >= a.seg_off[a.n_seqs]) return false;
+        lo = 0;
+        int64_t hi = a.n_seqs;  // seg_off[lo] <= w < seg_off[hi]
+        while (hi - lo > 1) {
+            const int64_t m = (lo + hi) >> 1;
+            if (a.seg_off[m] <= w) lo = m; else hi = m;
+        }
+        first = a.seg_off[lo];
+        s.last = w + 1 == a.seg_off[lo + 1];
+    }
+    // offsets outside the packed rows are cut to them
+    const int64_t beg = min(max((int64_t)a.cu[lo], (int64_t)0), a.T);
+    const int64_t n = min(max((int64_t)a.cu[lo + 1], beg), a.T) - beg;
+    s.seq = lo;
+    s.index = (int)(w - first);
+    s.row0 = beg;
+    s.t0 = (int64_t)s.index * a.seg;
+    s.len = (int)min((int64_t)a.seg, n - s.t0);
+    if (s.len < 0) s.len = 0;
+    return true;
+}
+
+// Row of the state tensors for a sequence, or -1 for a slot outside the pool.
+__device__ __forceinline__ int64_t ssm_row(const int32_t* slots, int64_t n_slots, int64_t seq) {
+    if (!slots) return seq;
+    const int64_t r = slots[seq];
+    return r >= 0 && r < n_slots ? r : -1;
+}
+
+}  // namespace triune
