@@ -442,7 +442,7 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
  * No reference counterpart.  Sizes: Dm channels, N states per channel (1..64), G groups of Dm / G
  * channels that share B and C.  Operands in io_dtype: u, delta, z, y [Bn, T, Dm] and B, C
  * [Bn, T, G, N] (innermost stride 1, other strides in elements, any alignment of an element, a
- * stride of 0 for a broadcast input); fp32 and contiguous: A [Dm, N], D and delta_bias [Dm] (either
+ * stride of 0 for a broadcast input; the scan takes token strides below 2^22, y's at least Dm); fp32 and contiguous: A [Dm, N], D and delta_bias [Dm] (either
  * may be NULL), states [*, Dm, N].
  * A workspace is 16-byte aligned and belongs to one call at a time.
  *
@@ -450,8 +450,8 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
  *     dt = delta + delta_bias, through softplus when `softplus`;  h <- exp(dt A) h + dt u B
  *     y = (sum_n C h + D u) * silu(z)                     (no gate when z is NULL)
  * strides[14] = (batch, token) of u, delta, z, y, then (batch, token, group) of B, C.  s0 (NULL:
- * zeros) and s_final (NULL: not wanted): [Bn, Dm, N].  kept: NULL, or fp32 [Bn, ceil(T / 32), N, Dm]
- * that receives the state of every 32nd token for triune_hip_ssm_bwd.  flags bits 8..15 force the
+ * zeros) and s_final (NULL: not wanted): [Bn, Dm, N].  kept: NULL, or fp32 [Bn, ceil(T / K), N, Dm],
+ * K = 32 (16 for N > 32), that receives the state of every K-th token for triune_hip_ssm_bwd.  flags bits 8..15 force the
  * length of a segment in units of 32 tokens (0: automatic). */
 size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags);
 int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const void* B, const void* C, const float* A,

@@ -32,29 +32,47 @@ int compute_units() {
     return n;
 }
 
+// The kernels address a tile's 32 rows by 32-bit byte offsets.
+constexpr int64_t kMaxTokenStride = 1 << 22;
+bool strides_ok(std::initializer_list<int64_t> st) {
+    for (const int64_t s : st)
+        if (s < 0 || s >= kMaxTokenStride) return false;
+    return true;
+}
+
 bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
-    return Dm > 0 && Dm < (1 << 28) && G > 0 && Dm % G == 0 && N > 0 && N <= SSM_MAX_N;
+    return Dm > 0 && Dm < kMaxTokenStride && G > 0 && Dm % G == 0 && N > 0 && N <= SSM_MAX_N;
 }
-int64_t group_blocks(int64_t Dm, int64_t G) { return (Dm / G + SSM_BLOCK - 1) / SSM_BLOCK; }
+// Workgroups that the channels of one group take, of all groups.
+int64_t group_blocks(int64_t Dm, int64_t G, int N) {
+    return (Dm / G + 63) / 64;
+}
+int64_t all_blocks(int64_t Dm, int64_t G, int N) { return G * group_blocks(Dm, G, N); }
 
-// Workgroups that give every SIMD of the chip two waves.
-int64_t ssm_slots(int N) {
+// Waves a compute unit (four SIMDs) that a call has without splitting the time axis for that to be left,
+// and that it gets where it is split.  Two waves on a SIMD keep it three quarters busy; splitting costs the
+// decays a second time.  8 x 2048 tokens of 4096 channels, N = 16: 306 us unsplit with eight waves a
+// unit, 445 split; 4 x 4096 of 1536: 183 us split for 24 waves, 201 for 16, 188 for 12.
+constexpr int kEnoughWaves = 8, kSplitWaves = 24;
+// Workgroups of `waves` waves a compute unit.
+int64_t ssm_slots(int N, int waves) {
     const int nw = ssm_waves(N);
-    return (int64_t)compute_units() * (nw >= 8 ? 1 : 8 / nw);
+    return (int64_t)compute_units() * (nw >= waves ? 1 : waves / nw);
 }
 
-int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * SSM_CKPT; }
+int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * SSM_UNIT; }
 
-// Tokens of a segment of a dense call (a multiple of SSM_CKPT; the whole sequence unless splitting
+// Tokens of a segment of a dense call (a multiple of SSM_UNIT; the whole sequence unless splitting
 // pays).  Splitting reads and decays every token twice, so `least` segments have to fit the chip.
 int64_t dense_segment(int64_t n_seqs, int64_t T, int64_t blocks, int N, int flags, int64_t least) {
-    const int64_t whole = (T + SSM_CKPT - 1) / SSM_CKPT * SSM_CKPT;
+    const int64_t whole = (T + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
     if (forced_segment(flags)) return forced_segment(flags) < whole ? forced_segment(flags) : whole;
-    int64_t n = ssm_slots(N) / (n_seqs * blocks);
+    if (n_seqs * blocks >= ssm_slots(N, kEnoughWaves)) return whole;
+    int64_t n = ssm_slots(N, kSplitWaves) / (n_seqs * blocks);
     const int64_t most = T / 64;
     if (n > most) n = most;
     if (n < least) return whole;
-    return ((T + n - 1) / n + SSM_CKPT - 1) / SSM_CKPT * SSM_CKPT;
+    return ((T + n - 1) / n + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
 }
 
 struct ScanPlan {
@@ -72,7 +90,7 @@ void plan_bytes(ScanPlan& p, int64_t Dm, int N, int64_t n_off) {
 
 ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int flags, int64_t least) {
     ScanPlan p{};
-    p.seg = dense_segment(n_seqs, T, G * group_blocks(Dm, G), N, flags, least);
+    p.seg = dense_segment(n_seqs, T, all_blocks(Dm, G, N), N, flags, least);
     p.nseg = (T + p.seg - 1) / p.seg;
     p.n_work = n_seqs * p.nseg;
     plan_bytes(p, Dm, N, 0);
@@ -83,13 +101,13 @@ ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int 
 // sequences enough for two rounds of the chip.  nseg > 1 says that there are segments.
 ScanPlan plan_packed(int64_t n_seqs, int64_t total, int64_t Dm, int64_t G, int N, int flags) {
     ScanPlan p{};
-    const int64_t whole = (total + SSM_CKPT - 1) / SSM_CKPT * SSM_CKPT, blocks = G * group_blocks(Dm, G);
-    const int64_t slots = ssm_slots(N);
+    const int64_t whole = (total + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT, blocks = all_blocks(Dm, G, N);
+    const int64_t slots = ssm_slots(N, kSplitWaves);
     p.seg = forced_segment(flags);
     if (!p.seg) {
-        p.seg = (total * blocks / slots + SSM_CKPT - 1) / SSM_CKPT * SSM_CKPT;
+        p.seg = (total * blocks / slots + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
         if (p.seg < 64) p.seg = 64;
-        if (n_seqs * blocks >= 2 * slots) p.seg = whole;
+        if (n_seqs * blocks >= 2 * ssm_slots(N, kEnoughWaves)) p.seg = whole;
     }
     p.nseg = p.seg < whole ? 2 : 1;
     p.n_work = p.nseg > 1 ? total / p.seg + n_seqs : n_seqs;
@@ -106,7 +124,7 @@ BwdPlan plan_bwd(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags)
     BwdPlan p{};
     p.s = plan_scan(Bn, T, Dm, G, N, flags, 2);
     p.off_bc = p.s.total;
-    p.off_par = p.off_bc + align_up((size_t)(G * group_blocks(Dm, G)) * Bn * T * ssm_waves(N) * 8 * 4);
+    p.off_par = p.off_bc + align_up((size_t)all_blocks(Dm, G, N) * Bn * T * ssm_waves(N) * 8 * 4);
     p.total = p.off_par + align_up((size_t)p.s.n_work * (N + 2) * Dm * 4);
     return p;
 }
@@ -117,7 +135,7 @@ void set_sizes(SsmParams& a, int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, i
     a.Dm = (int)Dm;
     a.G = (int)G;
     a.N = N;
-    a.blocks = (int)group_blocks(Dm, G);
+    a.blocks = (int)group_blocks(Dm, G, N);
     a.seg = (int)p.seg;
     a.nseg = (int)p.nseg;
     a.n_work = p.n_work;
@@ -158,9 +176,11 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
     if (!all_aligned(io_dtype, {u, delta, z, B, C, y}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, s0, s_final, kept}))
         return TRIUNE_ERR_LAYOUT;
+    if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]}) || strides[7] < Dm)
+        return TRIUNE_ERR_LAYOUT;
     if (Bn == 0 || T == 0) return TRIUNE_OK;
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags, 3);
-    if (p.n_work > kMaxGrid / (G * group_blocks(Dm, G)) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (p.n_work > kMaxGrid / all_blocks(Dm, G, N) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, strides[0], strides[1]};
@@ -200,10 +220,12 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
     if (!all_aligned(io_dtype, {u, delta, z, B, C, y}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, s0, s_final, cu_seqlens, slots}))
         return TRIUNE_ERR_LAYOUT;
+    if (!strides_ok({strides[0], strides[1], strides[2], strides[3], strides[4], strides[6]}) || strides[3] < Dm)
+        return TRIUNE_ERR_LAYOUT;
     if (n_seqs == 0) return TRIUNE_OK;
     // with no tokens every sequence's state still passes through: one empty segment each
     const ScanPlan p = plan_packed(n_seqs, total_tokens > 0 ? total_tokens : 1, Dm, G, N, flags);
-    if (p.n_work > kMaxGrid / (G * group_blocks(Dm, G)) || n_seqs > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (p.n_work > kMaxGrid / all_blocks(Dm, G, N) || n_seqs > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, 0, strides[0]};
@@ -244,8 +266,9 @@ int triune_hip_ssm_bwd(const void* u, const void* delta, const void* z, const vo
     if (!all_aligned(io_dtype, {u, delta, z, B, C, dy, du, ddelta, dz, dB, dC}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, kept, ds_final, dA, dD, ddelta_bias, ds0}))
         return TRIUNE_ERR_LAYOUT;
+    if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]})) return TRIUNE_ERR_LAYOUT;
     const BwdPlan p = plan_bwd(Bn, T, Dm, G, N, flags);
-    if (p.s.n_work > kMaxGrid / (G * group_blocks(Dm, G)) || Bn > kMaxGrid / (Dm * N) || Bn * T > kMaxGrid / (G * N))
+    if (p.s.n_work > kMaxGrid / all_blocks(Dm, G, N) || Bn > kMaxGrid / (Dm * N) || Bn * T > kMaxGrid / (G * N))
         return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     char* ws = (char*)workspace;

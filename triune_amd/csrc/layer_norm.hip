@@ -190,16 +190,17 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
     }
 }
 
-__global__ __launch_bounds__(256) void norm_bwd_sum_kernel(NormBwdParams g) {
+// Sixteen threads per value, each every sixteenth part, then these: a fixed order.
+__global__ __launch_bounds__(1024) void norm_bwd_sum_kernel(NormBwdParams g) {
     const int per = 2 * g.f.D, l = threadIdx.x & 63, id = blockIdx.x * 64 + l, w = threadIdx.x >> 6;
-    __shared__ float red[4][64];
+    __shared__ float red[16][64];
     float s = 0.f;
     if (id < per)
-        for (int64_t p = w; p < g.parts; p += 4) s += g.part[p * per + id];
+        for (int64_t p = w; p < g.parts; p += 16) s += g.part[p * per + id];
     red[w][l] = s;
     __syncthreads();
     if (w || id >= per) return;
-    s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    for (int i = 1; i < 16; ++i) s += red[i][l];
     if (id < g.f.D) {
         if (g.dw) store_dt(g.dw, g.f.w_dt, id, s);
     } else if (g.db) {
@@ -251,7 +252,7 @@ hipError_t launch_norm(const NormParams& a, int dt, hipStream_t s) { return norm
 hipError_t launch_norm_bwd(const NormBwdParams& g, int dt, hipStream_t s) {
     const hipError_t e = norm_dtype(g, g.f.D, dt, s);
     if (e != hipSuccess || !g.part) return e;
-    norm_bwd_sum_kernel<<<dim3((unsigned)((2 * g.f.D + 63) / 64)), 256, 0, s>>>(g);
+    norm_bwd_sum_kernel<<<dim3((unsigned)((2 * g.f.D + 63) / 64)), 1024, 0, s>>>(g);
     return hipGetLastError();
 }
 

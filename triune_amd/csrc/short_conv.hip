@@ -317,17 +317,18 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
     }
 }
 
-__global__ __launch_bounds__(256) void conv_bwd_sum_kernel(ConvBwdParams g) {
+// Sixteen threads per value, each every sixteenth part, then these: a fixed order.
+__global__ __launch_bounds__(1024) void conv_bwd_sum_kernel(ConvBwdParams g) {
     const ConvParams& a = g.f;
     const int per = (a.W + 1) * a.Dm, id = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    __shared__ float red[4][64];
+    __shared__ float red[16][64];
     float s = 0.f;
     if (id < per)
-        for (int64_t p = w; p < g.parts; p += 4) s += g.part[p * per + id];
+        for (int64_t p = w; p < g.parts; p += 16) s += g.part[p * per + id];
     red[w][threadIdx.x & 63] = s;
     __syncthreads();
     if (w || id >= per) return;
-    s = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
     const int j = id / a.Dm, ch = id - j * a.Dm;
     if (j < a.W) {
         if (g.dw) store_dt(g.dw, a.w_dt, (int64_t)ch * a.W + j, s);
@@ -381,7 +382,7 @@ hipError_t conv_bwd_w(const ConvBwdParams& b, hipStream_t s) {
     conv_bwd_kernel<T, W><<<dim3((unsigned)g.blocks), 256, 0, s>>>(b, g.cl, g.cblocks);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !b.part) return e;
-    conv_bwd_sum_kernel<<<dim3((unsigned)(((W + 1) * a.Dm + 63) / 64)), 256, 0, s>>>(b);
+    conv_bwd_sum_kernel<<<dim3((unsigned)(((W + 1) * a.Dm + 63) / 64)), 1024, 0, s>>>(b);
     return hipGetLastError();
 }
 

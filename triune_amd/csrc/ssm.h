@@ -5,10 +5,14 @@
 
 #include "common.h"
 
+#include <initializer_list>
+
 namespace triune {
 
-constexpr int SSM_BLOCK = 64;  // channels of a workgroup: one per lane
-constexpr int SSM_CKPT = 32;   // tokens between two states that the forward keeps for the backward
+constexpr int SSM_UNIT = 32;   // segments are multiples of this many tokens
+// Tokens between two states that the forward keeps for the backward, which holds its walks between them
+// in LDS.
+inline int ssm_kept_every(int N) { return N <= 32 ? 32 : 16; }
 constexpr int SSM_MAX_N = 64;  // states per channel
 
 // A [tokens, channels] operand of a batch of sequences: element strides, innermost stride 1.
@@ -27,7 +31,7 @@ struct SsmParams {
     float* fin;               // [rows, Dm, N] or null
     const int32_t* slots;     // packed over a pool: the row of each sequence, else null
     int64_t n_slots;
-    float* ckpt;              // [Bn, ceil(T / SSM_CKPT), N, Dm] or null
+    float* ckpt;              // [Bn, ceil(T / ssm_kept_every), N, Dm] or null
     float* ws_state;          // [n_work, N, Dm]: a segment's own end state, then the state it starts from
     float* ws_sum;            // [n_work, Dm]: summed step sizes
     int64_t n_seqs, T;        // T: length of a dense sequence, or all tokens of a packed call
@@ -64,7 +68,14 @@ struct SsmStepParams {
     int Dm, G, N;
 };
 
-int ssm_waves(int N);                 // waves of a scan workgroup: four states each
+int ssm_waves(int N);  // waves of a scan workgroup
+// Whether four channels of every row of these (and the groups) are aligned to their size together.
+inline bool ssm_by_four(int group_channels, int io_dt, std::initializer_list<SsmTok> ts) {
+    const uintptr_t m = io_dt == DT_F32 ? 15 : 7;
+    for (const SsmTok& t : ts)
+        if (t.p && ((reinterpret_cast<uintptr_t>(t.p) & m) || ((t.sb | t.st) & 3))) return false;
+    return group_channels % 4 == 0;
+}
 hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* seg_off, hipStream_t s);
 hipError_t launch_ssm_states(const SsmParams& a, int io_dt, hipStream_t s);
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s);
@@ -140,7 +151,9 @@ hipError_t launch_norm(const NormParams& a, int io_dt, hipStream_t s);
 hipError_t launch_norm_bwd(const NormBwdParams& a, int io_dt, hipStream_t s);
 
 // ---- device helpers ---------------------------------------------------------------------------
-__device__ __forceinline__ float silu_gate(float z) { return z * sigmoid(z); }
+// 1 / (1 + e^-x) with the hardware reciprocal (1 ulp); e^-x past the largest number gives 0.
+__device__ __forceinline__ float fast_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-x)); }
+__device__ __forceinline__ float silu_gate(float z) { return z * fast_sigmoid(z); }
 
 // log(1 + e^-|x|) + max(x, 0).  With s = e / (2 + e), log(1 + e) = 2 atanh(s), whose series in s^2
 // <= 1/9 is cut to a fitted polynomial (relative error 4e-9): the form keeps the relative precision
@@ -153,7 +166,7 @@ __device__ __forceinline__ float softplus(float x) {
     p = __builtin_fmaf(p, t, 0.40024852752685547f);
     p = __builtin_fmaf(p, t, 0.6666631698608398f);
     p = __builtin_fmaf(p, t, 2.0f);
-    return __builtin_fmaf(s, p, fmaxf(x, 0.f));
+    return __builtin_fmaf(s, p, 0.5f * (x + fabsf(x)));  // max(x, 0) without fmaxf's second max for NaN
 }
 
 // Eight elements of any alignment in one access (the memory pipeline takes unaligned vectors), or the
@@ -196,6 +209,155 @@ __device__ __forceinline__ void store_dt(void* p, int dt, int64_t i, float x) {
     if (dt == DT_F32) ((float*)p)[i] = x;
     else if (dt == DT_BF16) ((__bf16*)p)[i] = (__bf16)x;
     else ((_Float16*)p)[i] = (_Float16)x;
+}
+
+// A in units of the hardware's exp2.  Infinite values are cut to the largest number, so that a step of 0
+// (a token past a tile's end) is a decay of 1 for them too.
+__device__ __forceinline__ float log2_decay(float A) {
+    const float x = A * LOG2E, most = 3.4028234e38f;
+    return x < -most ? -most : x > most ? most : x;
+}
+
+// N consecutive states of a channel whose row holds `left` more (zeros past them).
+template <int N>
+__device__ __forceinline__ void load_states(const float* p, int left, float (&x)[N]) {
+    if (left >= N && !(reinterpret_cast<uintptr_t>(p) & 15)) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = j < left ? p[j] : 0.f;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_states(float* p, int left, const float (&x)[N]) {
+    if (left >= N && !(reinterpret_cast<uintptr_t>(p) & 15)) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) *reinterpret_cast<f32x4*>(p + j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < left) p[j] = x[j];
+    }
+}
+
+// The value that lane k of a channel's L lanes holds, in all of them (a DPP operand of its user).
+template <int CTRL>
+__device__ __forceinline__ float dpp_read(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+template <int L>
+__device__ __forceinline__ float lane_of(float x, int k) {
+    if constexpr (L == 1) {
+        return x;
+    } else if constexpr (L == 2) {
+        return k == 0 ? dpp_read<0xA0>(x) : dpp_read<0xF5>(x);  // quad_perm [0,0,2,2], [1,1,3,3]
+    } else if constexpr (L == 4) {
+        return k == 0 ? dpp_read<0x00>(x) : k == 1 ? dpp_read<0x55>(x) : k == 2 ? dpp_read<0xAA>(x) : dpp_read<0xFF>(x);
+    } else {
+        static_assert(L == 16, "no such broadcast");
+        switch (k) {  // row_newbcast
+            case 0: return dpp_read<0x150>(x);
+            case 1: return dpp_read<0x151>(x);
+            case 2: return dpp_read<0x152>(x);
+            case 3: return dpp_read<0x153>(x);
+            case 4: return dpp_read<0x154>(x);
+            case 5: return dpp_read<0x155>(x);
+            case 6: return dpp_read<0x156>(x);
+            case 7: return dpp_read<0x157>(x);
+            case 8: return dpp_read<0x158>(x);
+            case 9: return dpp_read<0x159>(x);
+            case 10: return dpp_read<0x15A>(x);
+            case 11: return dpp_read<0x15B>(x);
+            case 12: return dpp_read<0x15C>(x);
+            case 13: return dpp_read<0x15D>(x);
+            case 14: return dpp_read<0x15E>(x);
+            default: return dpp_read<0x15F>(x);
+        }
+    }
+}
+// The sum over a channel's L lanes, in all of them.
+template <int L>
+__device__ __forceinline__ float channel_sum(float x) {
+    if constexpr (L >= 2) x = dpp_add<0xB1>(x);    // lane ^ 1
+    if constexpr (L >= 4) x = dpp_add<0x4E>(x);    // lane ^ 2
+    if constexpr (L >= 8) x = dpp_add<0x141>(x);   // the other four of eight
+    if constexpr (L >= 16) x = dpp_add<0x140>(x);  // the other eight of sixteen
+    return x;
+}
+
+// Rows of a tile through a buffer resource: it starts at the tile's first row and ends with the last
+// valid one, so rows past the end (all of them, past the last tile or without a tensor) read 0 and are
+// not written.  Accesses step through the vector offset, which the range check covers; a
+// branch around them, or one for whole tiles, would make the compiler join registers behind it, which
+// waits for the loads it should leave in flight.
+constexpr int TILE_SKIP = 0x40000000;  // an offset past every resource: reads 0, writes nothing
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const T* p, int64_t st, int64_t rows, uint32_t width) {
+    const int64_t n = p && rows > 0 ? ((rows - 1) * st + width) * (int64_t)sizeof(T) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), (short)0, (int)min(n, (int64_t)TILE_SKIP), 0x00020000);
+}
+
+// V elements (1, or 4 aligned to their size together) in one access.
+template <typename T, int V>
+struct Vec {
+    T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> tile_load(__amdgpu_buffer_rsrc_t r, int voff) {
+    constexpr int B = sizeof(T) * V;
+    static_assert(B == 2 || B == 4 || B == 8 || B == 16, "no such access");
+    if constexpr (B == 2) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b16(r, voff, 0, 0));
+    else if constexpr (B == 4) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b32(r, voff, 0, 0));
+    else if constexpr (B == 8) return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b64(r, voff, 0, 0));
+    else return __builtin_bit_cast(Vec<T, V>, __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0));
+}
+template <typename T, int V>
+__device__ __forceinline__ void tile_store(const float (&y)[V], __amdgpu_buffer_rsrc_t r, int voff) {
+    constexpr int B = sizeof(T) * V;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    Vec<T, V> x;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.v[j] = (T)y[j];
+    if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), r, voff, 0, 0);
+    else if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, voff, 0, 0);
+    else if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, voff, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, voff, 0, 0);
+}
+// N accesses `st` bytes apart.  The offset is hidden from the optimizer, which would keep the N sums of it
+// in registers over the loop on tiles.
+template <typename T, int V, int N>
+__device__ __forceinline__ void tile_load_rows(__amdgpu_buffer_rsrc_t r, int voff, int st, Vec<T, V> (&x)[N]) {
+    if constexpr (N > 2) asm volatile("" : "+v"(voff));
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = tile_load<T, V>(r, voff + i * st);
+}
+template <typename T, int V, int N>
+__device__ __forceinline__ void tile_store_rows(__amdgpu_buffer_rsrc_t r, int voff, int st, const float (&y)[N][V]) {
+    if constexpr (N > 2) asm volatile("" : "+v"(voff));
+#pragma unroll
+    for (int i = 0; i < N; ++i) tile_store<T, V>(y[i], r, voff + i * st);
+}
+// V floats of an LDS row.
+template <int V>
+__device__ __forceinline__ void lds_store(float* p, const float (&x)[V]) {
+    if constexpr (V == 4) *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+    else p[0] = x[0];
+}
+template <int V>
+__device__ __forceinline__ void lds_add(const float* p, float (&x)[V]) {
+    if constexpr (V == 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += v[j];
+    } else {
+        x[0] += p[0];
+    }
 }
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }

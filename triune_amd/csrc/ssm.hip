@@ -3,163 +3,232 @@
 // For each channel d with states n:
 //     dt_t = softplus(delta_t + bias);  h_t = exp(dt_t A_n) h_{t-1} + dt_t u_t B_t,n
 //     y_t  = (sum_n C_t,n h_t,n + D u_t) silu(z_t)
-// A channel's decays differ by state, so nothing of it factors into matrix products: each (token,
-// channel, state) costs an exp2 (8.5 cycles per wave on a SIMD, measured) and four plain
-// operations, and that, not the memory, bounds the kernel.
-//
-// Work split: a lane is a channel, a wave holds four states of 64 channels in registers, a
-// workgroup all states of 64 channels.  Tiles of 32 tokens go through LDS: every (token, channel)
-// is loaded and its softplus taken once for all states (by one of the waves), B and C are read
-// as broadcasts, and the waves' parts of y meet there.  Calls with too few (sequence, channel block) pairs
-// for the chip split the time axis into segments: a pass for each segment's own end state (its
-// decay over the segment is exp(A sum dt), so only the sum of dt is kept), a scan over segments, and
-// the pass that writes the outputs.
 #include "ssm.h"
 
 namespace triune {
 
+// Waves of a workgroup, by the number of states: four states each.
 int ssm_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
-// STATES: only the segment's end state from zero, and its sum of dt.
-template <typename T, int NW, bool STATES>
+// NW: waves; V: channels that a lane loads and stores together (4 where alignment allows); STATES: only
+// the segment's end state from zero, and its sum of dt.
+template <typename T, int NW, int V, bool STATES>
 __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
-    constexpr int TT = NW == 16 ? 16 : 32;  // sixteen waves' parts of y for 32 tokens would fill the LDS
-    constexpr int TPW = TT / NW;            // tokens a wave loads and stores
-    constexpr int BW = STATES ? 4 : 8;
-    __shared__ float2 s_du[TT][64];     // dt, dt u
-    __shared__ float s_bc[TT][NW][BW];  // a wave's four B, then its four C
-    __shared__ float s_y[STATES ? 1 : NW][STATES ? 1 : TT][64];
+    constexpr int NS = 4, NT = 64 * NW;
+    constexpr int TT = NW == 1 || NW == 16 ? 16 : 32;  // tokens of a tile: sixteen waves' parts of y fill the LDS
+    constexpr int LPR = 64 / V;                        // lanes of a token's row
+    constexpr int TS = NT / LPR;                       // tokens of one access of the workgroup
+    constexpr int K = (TT + TS - 1) / TS;              // accesses of a tile
+    constexpr int KB = TT * 4 * NW / NT;               // elements of B (and C) that a thread loads
+    constexpr int BW = STATES ? NS : 2 * NS;
+    constexpr int U = 2;                               // tokens whose operands are read together
+    constexpr int ES = sizeof(T);
+    __shared__ __attribute__((aligned(16))) float s_d[2][TT][64];       // dt, dt u
+    __shared__ __attribute__((aligned(16))) float s_bc[TT][NW][BW];     // a wave's B, then its C
+    __shared__ __attribute__((aligned(16))) float s_y[STATES ? 1 : NW][STATES ? 1 : TT][64];
 
     const int nblk = a.G * a.blocks;
     const int64_t work = blockIdx.x / nblk;
     const int cb = (int)(blockIdx.x - work * nblk);
     SsmSeg sg;
     if (!ssm_segment(a, work, sg)) return;
-    const int Dg = a.Dm / a.G, grp = cb / a.blocks;
-    const int lane = threadIdx.x & 63, w = wave_index();
-    const int in_grp = (cb - grp * a.blocks) * SSM_BLOCK + lane;
-    const bool chv = in_grp < Dg;
-    const int ch = grp * Dg + in_grp;
-    const int n0 = 4 * w;
+    const int Dg = a.Dm / a.G, grp = cb / a.blocks, c0 = (cb - grp * a.blocks) * 64;
+    const int lane = threadIdx.x & 63, w = wave_index(), n0 = NS * w;
+    // the walk's channel; lanes past the group's channels repeat its first and store nothing
+    const bool chv = c0 + lane < Dg;
+    const int ch = grp * Dg + (chv ? c0 + lane : 0);
+    // the channels and the first token that this thread loads and stores, of a tile
+    const int cl = (threadIdx.x % LPR) * V, tl = threadIdx.x / LPR;
+    const bool lv = c0 + cl < Dg && (TS <= TT || tl < TT);
+    const int lch = grp * Dg + (lv ? c0 + cl : 0);
+    // the state and the first token that it loads B and C of
+    const int bn = threadIdx.x % (4 * NW), bt = threadIdx.x / (4 * NW);
 
     const int64_t tok = sg.row0 + sg.t0, bat = a.cu ? 0 : sg.seq;
-    const T* pu = (const T*)a.u.p + bat * a.u.sb + tok * a.u.st + (chv ? ch : 0);
-    const T* pd = (const T*)a.dl.p + bat * a.dl.sb + tok * a.dl.st + (chv ? ch : 0);
-    const T* pz = a.z.p ? (const T*)a.z.p + bat * a.z.sb + tok * a.z.st + (chv ? ch : 0) : nullptr;
-    T* py = (T*)const_cast<void*>(a.y.p) + bat * a.y.sb + tok * a.y.st + (chv ? ch : 0);
+    const T* pu = (const T*)a.u.p + bat * a.u.sb + tok * a.u.st;
+    const T* pd = (const T*)a.dl.p + bat * a.dl.sb + tok * a.dl.st;
+    const T* pz = a.z.p ? (const T*)a.z.p + bat * a.z.sb + tok * a.z.st : nullptr;
+    T* py = (T*)const_cast<void*>(a.y.p) + bat * a.y.sb + tok * a.y.st;
     const T* pB = (const T*)a.B + bat * a.b_sb + tok * a.b_st + grp * a.b_sg;
     const T* pC = (const T*)a.C + bat * a.c_sb + tok * a.c_st + grp * a.c_sg;
 
-    float Al[4], h[4];
+    float Al[NS], h[NS], bias[V], Dv[V];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        Al[j] = chv && n0 + j < a.N ? a.A[(int64_t)ch * a.N + n0 + j] * LOG2E : 0.f;
+    for (int j = 0; j < NS; ++j) {
+        Al[j] = n0 + j < a.N ? log2_decay(a.A[(int64_t)ch * a.N + n0 + j]) : 0.f;
         h[j] = 0.f;
     }
-    const float bias = a.bias && chv ? a.bias[ch] : 0.f, Dv = a.D && chv ? a.D[ch] : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = a.bias ? a.bias[lch + j] : 0.f;
+        Dv[j] = a.D ? a.D[lch + j] : 0.f;
+    }
     const int64_t row = STATES ? 0 : ssm_row(a.slots, a.n_slots, sg.seq);
-    if (!STATES && chv) {
+    if constexpr (!STATES) {
         if (a.ws_state) {  // segmented: the entering state comes from the scan over segments
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) h[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
         } else if (a.s0 && row >= 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) h[j] = a.s0[(row * a.Dm + ch) * a.N + n0 + j];
         }
+        if (n0 >= a.N)  // waves without states add nothing to y
+            for (int t = 0; t < TT; ++t) s_y[w][t][lane] = 0.f;
     }
 
-    T ru[TPW], rd[TPW], rz[STATES ? 1 : TPW];
+    // A tile's loads, issued a tile ahead.
+    Vec<T, V> ru[K], rd[K], rz[STATES ? 1 : K];
+    Vec<T, 1> rb[KB], rc[STATES ? 1 : KB];
+    const int vu = lv ? (tl * (int)a.u.st + lch) * ES : TILE_SKIP, vd = lv ? (tl * (int)a.dl.st + lch) * ES : TILE_SKIP;
+    const int vz = lv ? (tl * (int)a.z.st + lch) * ES : TILE_SKIP, vy = lv ? (tl * (int)a.y.st + lch) * ES : TILE_SKIP;
+    const int vb = bn < a.N ? (bt * (int)a.b_st + bn) * ES : TILE_SKIP;
+    const int vc = bn < a.N ? (bt * (int)a.c_st + bn) * ES : TILE_SKIP;
     auto fetch = [&](int t0) {
-#pragma unroll
-        for (int i = 0; i < TPW; ++i) {
-            const int t = t0 + i * NW + w;
-            const bool ok = t < sg.len && chv;
-            ru[i] = ok ? pu[t * a.u.st] : (T)0.f;
-            rd[i] = ok ? pd[t * a.dl.st] : (T)0.f;
-            if constexpr (!STATES) rz[i] = ok && pz ? pz[t * a.z.st] : (T)0.f;
+        const int left = sg.len - t0;
+        tile_load_rows(tile_rows(pu + t0 * a.u.st, a.u.st, left, a.Dm), vu, TS * ES * (int)a.u.st, ru);
+        tile_load_rows(tile_rows(pd + t0 * a.dl.st, a.dl.st, left, a.Dm), vd, TS * ES * (int)a.dl.st, rd);
+        tile_load_rows(tile_rows(pB + t0 * a.b_st, a.b_st, left, a.N), vb, 16 * ES * (int)a.b_st, rb);
+        if constexpr (!STATES) {
+            tile_load_rows(tile_rows(pz ? pz + t0 * a.z.st : pz, a.z.st, left, a.Dm), vz, TS * ES * (int)a.z.st, rz);
+            tile_load_rows(tile_rows(pC + t0 * a.c_st, a.c_st, left, a.N), vc, 16 * ES * (int)a.c_st, rc);
         }
     };
-    float sum = 0.f;
-    fetch(0);
-    for (int t0 = 0; t0 < sg.len; t0 += TT) {
-        float cu[STATES ? 1 : TPW], cz[STATES ? 1 : TPW];
+    struct Block {
+        float dt[U], du[U], b[U][BW];
+    };
+    auto read = [&](Block& x, int t) {
 #pragma unroll
-        for (int i = 0; i < TPW; ++i) {
-            const int t = i * NW + w;
-            const float x = (float)rd[i] + bias, uu = (float)ru[i];
-            const float dt = t0 + t < sg.len ? (a.softplus ? softplus(x) : x) : 0.f;
-            s_du[t][lane] = make_float2(dt, dt * uu);
+        for (int i = 0; i < U; ++i) {
+            x.dt[i] = s_d[0][t + i][lane];
+            x.du[i] = s_d[1][t + i][lane];
+#pragma unroll
+            for (int j = 0; j < BW; ++j) x.b[i][j] = s_bc[t + i][w][j];
+        }
+    };
+    auto walk = [&](const Block& x, int t) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            float y = 0.f;
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.dt[i] * Al[j]), h[j], x.du[i] * x.b[i][j]);
+                if constexpr (!STATES) y = j ? __builtin_fmaf(x.b[i][NS + j], h[j], y) : x.b[i][NS] * h[0];
+            }
+            if constexpr (!STATES) s_y[w][t + i][lane] = y;
+        }
+    };
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.f;
+    fetch(0);
+    if constexpr (!STATES) {
+        // Stores that write nothing, so that the loop is entered with as many accesses after its first
+        // loads as it has on its way round: else those loads would be waited for together with a
+        // tile's stores, which come after them.
+        const float none[K][V] = {};
+        tile_store_rows<T>(tile_rows(py, 0, 0, 0), TILE_SKIP, 0, none);
+    }
+    for (int t0 = 0; t0 < sg.len; t0 += TT) {
+        const bool whole = t0 + TT <= sg.len;
+        Vec<T, V> cu[STATES ? 1 : K], cz[STATES ? 1 : K];
+        float dt[K][V], du[K][V];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                dt[i][j] = (float)rd[i].v[j] + bias[j];
+                du[i][j] = (float)ru[i].v[j];
+            }
+            if constexpr (!STATES) cu[i] = ru[i], cz[i] = rz[i];
+        }
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) dt[i][j] = softplus(dt[i][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) du[i][j] *= dt[i][j];
+            if (!whole && t0 + i * TS + tl >= sg.len) {  // past the end: no step, which leaves the state as it is
+#pragma unroll
+                for (int j = 0; j < V; ++j) dt[i][j] = du[i][j] = 0.f;
+            }
+            if (TS <= TT || tl < TT) {
+                lds_store<V>(&s_d[0][i * TS + tl][cl], dt[i]);
+                lds_store<V>(&s_d[1][i * TS + tl][cl], du[i]);
+            }
             if constexpr (STATES) {
-                sum += dt;
-            } else {
-                cu[i] = uu;
-                cz[i] = (float)rz[i];
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] += TS <= TT || tl < TT ? dt[i][j] : 0.f;
             }
         }
-        for (int e = threadIdx.x; e < TT * 4 * NW; e += 64 * NW) {
-            const int t = e / (4 * NW), n = e % (4 * NW);
-            const bool ok = t0 + t < sg.len && n < a.N;
-            s_bc[t][n >> 2][n & 3] = ok ? (float)pB[(t0 + t) * a.b_st + n] : 0.f;
-            if constexpr (!STATES) s_bc[t][n >> 2][4 + (n & 3)] = ok ? (float)pC[(t0 + t) * a.c_st + n] : 0.f;
-        }
-        if (t0 + TT < sg.len) fetch(t0 + TT);
-        if (!STATES && a.ckpt && chv && (sg.t0 + t0) % SSM_CKPT == 0) {
-            const int64_t nck = (a.T + SSM_CKPT - 1) / SSM_CKPT, ck = sg.seq * nck + (sg.t0 + t0) / SSM_CKPT;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < KB; ++i) {
+            const bool in = whole || t0 + i * 16 + bt < sg.len;
+            s_bc[i * 16 + bt][bn >> 2][bn & 3] = in ? (float)rb[i].v[0] : 0.f;
+            if constexpr (!STATES) s_bc[i * 16 + bt][bn >> 2][NS + (bn & 3)] = (float)rc[i].v[0];
+        }
+        fetch(t0 + TT);
+        constexpr int EVERY = NW == 16 ? 16 : 32;  // ssm_kept_every
+        if (!STATES && a.ckpt && chv && (sg.t0 + t0) % EVERY == 0) {
+            const int64_t nck = (a.T + EVERY - 1) / EVERY, ck = sg.seq * nck + (sg.t0 + t0) / EVERY;
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) a.ckpt[(ck * a.N + n0 + j) * a.Dm + ch] = h[j];
         }
         __syncthreads();
-        const int nt = min(TT, sg.len - t0);
         if (n0 < a.N) {
-#pragma unroll 4
-            for (int t = 0; t < nt; ++t) {
-                const float2 d = s_du[t][lane];
-                const f32x4 b = *reinterpret_cast<const f32x4*>(&s_bc[t][w][0]);
-                float y = 0.f;
-                f32x4 c;
-                if constexpr (!STATES) c = *reinterpret_cast<const f32x4*>(&s_bc[t][w][4]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(d.x * Al[j]), h[j], d.y * b[j]);
-                    if constexpr (!STATES) y = __builtin_fmaf(c[j], h[j], y);
-                }
-                if constexpr (!STATES) s_y[w][t][lane] = y;
+            Block p, q;  // read one block ahead
+            read(p, 0);
+#pragma unroll 1
+            for (int t = 0; t < TT; t += 2 * U) {
+                read(q, t + U);
+                walk(p, t);
+                read(p, t + 2 * U < TT ? t + 2 * U : 0);
+                walk(q, t + U);
             }
         }
         __syncthreads();
         if constexpr (!STATES) {
-            const int live = (a.N + 3) >> 2;  // waves that hold states
+            float y[K][V];
 #pragma unroll
-            for (int i = 0; i < TPW; ++i) {
-                const int t = i * NW + w;
-                float y = Dv * cu[i];
-                for (int k = 0; k < live; ++k) y += s_y[k][t][lane];
-                if (pz) y *= silu_gate(cz[i]);
-                if (t0 + t < sg.len && chv) py[(t0 + t) * a.y.st] = (T)y;
+            for (int i = 0; i < K; ++i) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) y[i][j] = Dv[j] * (float)cu[i].v[j];
+                if (TS > TT && tl >= TT) continue;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) lds_add<V>(&s_y[k][i * TS + tl][cl], y[i]);
             }
+            if (pz) {
+#pragma unroll
+                for (int i = 0; i < K; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[i][j] *= silu_gate((float)cz[i].v[j]);
+            }
+            tile_store_rows<T>(tile_rows(py + t0 * a.y.st, a.y.st, sg.len - t0, a.Dm), vy, TS * ES * (int)a.y.st, y);
         }
     }
     if constexpr (STATES) {
         if (chv) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) a.ws_state[(work * a.N + n0 + j) * a.Dm + ch] = h[j];
         }
-        float* red = reinterpret_cast<float*>(&s_du[0][0]);  // every wave is past its reads of s_du
-        red[w * 64 + lane] = sum;
+        constexpr int ROWS = TS < TT ? TS : TT;
+        if (TS <= TT || tl < TT) lds_store<V>(&s_d[0][tl][cl], sum);  // every wave is past its reads of s_d
         __syncthreads();
         if (w == 0 && chv) {
             float s = 0.f;
-#pragma unroll
-            for (int k = 0; k < NW; ++k) s += red[k * 64 + lane];
+            for (int k = 0; k < ROWS; ++k) s += s_d[0][k][lane];
             a.ws_sum[work * a.Dm + ch] = s;
         }
     } else if (a.fin && sg.last && row >= 0 && chv) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NS; ++j)
             if (n0 + j < a.N) a.fin[(row * a.Dm + ch) * a.N + n0 + j] = h[j];
     }
 }
@@ -171,16 +240,29 @@ __global__ __launch_bounds__(256) void ssm_carry_kernel(SsmParams a) {
     if (id >= a.n_seqs * per) return;
     const int64_t seq = id / per;
     const int n = (int)((id - seq * per) / a.Dm), ch = (int)((id - seq * per) % a.Dm);
+    const int64_t at = (int64_t)ch * a.N + n;
     int64_t w0 = seq * a.nseg, w1 = w0 + a.nseg;
     if (a.cu) w0 = a.seg_off[seq], w1 = min((int64_t)a.seg_off[seq + 1], a.n_work);
-    const float Al = a.A[(int64_t)ch * a.N + n] * LOG2E;
+    const float Al = log2_decay(a.A[at]);
     const int64_t row = ssm_row(a.slots, a.n_slots, seq);
-    float S = a.s0 && row >= 0 ? a.s0[(row * a.Dm + ch) * a.N + n] : 0.f;
-    for (int64_t w = w0; w < w1; ++w) {
-        float* p = a.ws_state + w * per + (int64_t)n * a.Dm + ch;
-        const float local = *p;
-        *p = S;
-        S = __builtin_fmaf(__builtin_amdgcn_exp2f(a.ws_sum[w * a.Dm + ch] * Al), S, local);
+    float S = a.s0 && row >= 0 ? a.s0[row * per + at] : 0.f;
+    float* p = a.ws_state + (int64_t)n * a.Dm + ch;
+    const float* ps = a.ws_sum + ch;
+    constexpr int AHEAD = 8;  // segments whose loads are in flight together
+    for (int64_t w = w0; w < w1; w += AHEAD) {
+        float local[AHEAD], sum[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int64_t v = min(w + i, w1 - 1);
+            local[i] = p[v * per];
+            sum[i] = ps[v * a.Dm];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (w + i >= w1) break;
+            p[(w + i) * per] = S;
+            S = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[i] * Al), S, local[i]);
+        }
     }
 }
 
@@ -224,11 +306,11 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams a) {
         if constexpr (VEC) {
             const f32x4 s = *reinterpret_cast<const f32x4*>(ps), m = *reinterpret_cast<const f32x4*>(pA);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = s[j], Al[j] = m[j] * LOG2E;
+            for (int j = 0; j < 4; ++j) h[j] = s[j], Al[j] = log2_decay(m[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) h[j] = ps[j], Al[j] = pA[j] * LOG2E;
+                if (n0 + j < a.N) h[j] = ps[j], Al[j] = log2_decay(pA[j]);
         }
     }
     const int grp = c / (a.Dm / a.G);
@@ -265,24 +347,25 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams a) {
     }
 }
 
-template <typename T, bool STATES>
+template <typename T, int V, bool STATES>
 static hipError_t scan_waves(const SsmParams& a, hipStream_t s) {
     const dim3 grid((unsigned)(a.n_work * a.G * a.blocks));
     switch (ssm_waves(a.N)) {
-        case 1: ssm_scan_kernel<T, 1, STATES><<<grid, 64, 0, s>>>(a); break;
-        case 2: ssm_scan_kernel<T, 2, STATES><<<grid, 128, 0, s>>>(a); break;
-        case 4: ssm_scan_kernel<T, 4, STATES><<<grid, 256, 0, s>>>(a); break;
-        case 8: ssm_scan_kernel<T, 8, STATES><<<grid, 512, 0, s>>>(a); break;
-        default: ssm_scan_kernel<T, 16, STATES><<<grid, 1024, 0, s>>>(a); break;
+        case 1: ssm_scan_kernel<T, 1, V, STATES><<<grid, 64, 0, s>>>(a); break;
+        case 2: ssm_scan_kernel<T, 2, V, STATES><<<grid, 128, 0, s>>>(a); break;
+        case 4: ssm_scan_kernel<T, 4, V, STATES><<<grid, 256, 0, s>>>(a); break;
+        case 8: ssm_scan_kernel<T, 8, V, STATES><<<grid, 512, 0, s>>>(a); break;
+        default: ssm_scan_kernel<T, 16, V, STATES><<<grid, 1024, 0, s>>>(a); break;
     }
     return hipGetLastError();
 }
 
 template <bool STATES>
 static hipError_t scan_dtype(const SsmParams& a, int dt, hipStream_t s) {
-    if (dt == DT_F32) return scan_waves<float, STATES>(a, s);
-    if (dt == DT_BF16) return scan_waves<__bf16, STATES>(a, s);
-    return scan_waves<_Float16, STATES>(a, s);
+    const bool v4 = ssm_by_four(a.Dm / a.G, dt, {a.u, a.dl, a.z, a.y});
+    if (dt == DT_F32) return v4 ? scan_waves<float, 4, STATES>(a, s) : scan_waves<float, 1, STATES>(a, s);
+    if (dt == DT_BF16) return v4 ? scan_waves<__bf16, 4, STATES>(a, s) : scan_waves<__bf16, 1, STATES>(a, s);
+    return v4 ? scan_waves<_Float16, 4, STATES>(a, s) : scan_waves<_Float16, 1, STATES>(a, s);
 }
 
 hipError_t launch_ssm_states(const SsmParams& a, int dt, hipStream_t s) { return scan_dtype<true>(a, dt, s); }
@@ -301,7 +384,7 @@ hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* off, hipStream_t s) {
 
 template <typename T, bool VEC>
 static hipError_t step_lanes(const SsmStepParams& a, hipStream_t s) {
-    const int lpc = ssm_waves(a.N), cpb = 256 / lpc;
+    const int lpc = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16, cpb = 256 / lpc;
     const dim3 grid((unsigned)(a.Bn * ((a.Dm + cpb - 1) / cpb)));
     switch (lpc) {
         case 1: ssm_step_kernel<T, 1, VEC><<<grid, 256, 0, s>>>(a); break;

@@ -29,7 +29,11 @@ __all__ = [
 ]
 
 MAX_STATES = 64
-_KEPT_EVERY = 32  # tokens between the states the forward keeps for the backward
+
+
+def _kept_every(N):
+    """Tokens between the states that the forward keeps for the backward."""
+    return 32 if N <= 32 else 16
 
 
 def _one_device(first, *rest):
@@ -41,8 +45,27 @@ def _one_device(first, *rest):
             raise ValueError("all tensors must be on one HIP device")
 
 
-def _rows(x):
-    return x if x.stride(-1) == 1 else x.contiguous()
+_MAX_TOKEN_STRIDE = 1 << 22  # the scan's kernels address a tile's rows in 32 bits
+
+
+def _rows(x, tok=None):
+    """x with a unit innermost stride, and a stride of its token dim tok that the kernels take (a copy
+    where it has not)."""
+    if x.stride(-1) == 1 and (tok is None or x.stride(tok) < _MAX_TOKEN_STRIDE or x.shape[tok] == 1):
+        return x
+    return x.contiguous()
+
+
+def _lead(x, tok):
+    """The strides up to x's token dim; 0 for a single token's."""
+    st = x.stride()[:tok + 1]
+    return st if x.shape[tok] != 1 else (*st[:tok], 0)
+
+
+def _lead_out(y, tok):
+    """The same of an output, whose rows are never on top of each other."""
+    st = y.stride()[:tok + 1]
+    return st if y.shape[tok] != 1 else (*st[:tok], y.shape[-1])
 
 
 def _needs_grad(*ts) -> bool:
@@ -54,7 +77,7 @@ def _no_grad_path(what, *ts):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
-def _out(out, shape, dtype, like):
+def _out(out, shape, dtype, like, tok=None):
     if out is None:
         return torch.empty(shape, device=like.device, dtype=dtype)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
@@ -62,6 +85,8 @@ def _out(out, shape, dtype, like):
     if any(n > 1 and s < shape[-1] for n, s in zip(shape[:-1], out.stride()[:-1])) or (
             shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError("out needs a unit innermost stride and rows that do not overlap")
+    if tok is not None and out.shape[tok] > 1 and out.stride(tok) >= _MAX_TOKEN_STRIDE:
+        raise ValueError(f"out's token stride must be below {_MAX_TOKEN_STRIDE}")
     return out
 
 
@@ -126,10 +151,9 @@ def _c(x):
     return None if x is None else x.contiguous()
 
 
-def _group_strides(x, lead, G):
+def _group_strides(x, lead):
     """Strides of B or C in front of its states: (lead ..., group)."""
-    st = x.stride()
-    return st[:lead + 1] if x.dim() == lead + 2 else (*st[:lead], 0)
+    return (*_lead(x, lead - 1), x.stride(lead) if x.dim() == lead + 2 else 0)
 
 
 def _scan(u, delta, A, B, C, D, z, bias, softplus, s0, out, keep, flags=0):
@@ -137,20 +161,20 @@ def _scan(u, delta, A, B, C, D, z, bias, softplus, s0, out, keep, flags=0):
     Bn, T, Dm = u.shape
     N = A.shape[1]
     G = B.shape[2] if B.dim() == 4 else 1
-    u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
-    z = None if z is None else _rows(z)
+    u, delta, B, C = _rows(u, 1), _rows(delta, 1), _rows(B, 1), _rows(C, 1)
+    z = None if z is None else _rows(z, 1)
     A, D, bias = A.contiguous(), _c(D), _c(bias)
     if s0 is not None:
         s0 = s0.to(torch.float32).contiguous()
-    y = _out(out, u.shape, u.dtype, u)
+    y = _out(out, u.shape, u.dtype, u, 1)
     fin = torch.empty(Bn, Dm, N, device=u.device, dtype=torch.float32)
     kept = None
     if keep:
-        kept = torch.empty(Bn, -(-T // _KEPT_EVERY), N, Dm, device=u.device, dtype=torch.float32)
+        kept = torch.empty(Bn, -(-T // _kept_every(N)), N, Dm, device=u.device, dtype=torch.float32)
     wsb = plan_on(u, "triune_hip_ssm_scan_workspace_size", Bn, T, Dm, G, N, flags)
     ws = torch.empty(wsb, device=u.device, dtype=torch.uint8) if wsb else None
-    st = strides(u.stride()[:2], delta.stride()[:2], (0, 0) if z is None else z.stride()[:2], y.stride()[:2],
-                 _group_strides(B, 2, G), _group_strides(C, 2, G))
+    st = strides(_lead(u, 1), _lead(delta, 1), (0, 0) if z is None else _lead(z, 1), _lead_out(y, 1),
+                 _group_strides(B, 2), _group_strides(C, 2))
     call_on(u, "triune_hip_ssm_scan", ptr(u), ptr(delta), ptr(z), ptr(B), ptr(C), ptr(A), ptr(D), ptr(bias),
             dtype_code(u), st, int(softplus), ptr(s0), ptr(y), ptr(fin), ptr(kept), Bn, T, Dm, G, N, flags, ptr(ws),
             wsb)
@@ -162,10 +186,10 @@ def _scan_bwd(u, delta, A, B, C, D, z, bias, softplus, kept, dy, dfin, want_s0, 
     N = A.shape[1]
     G = B.shape[2] if B.dim() == 4 else 1
     dev, f32 = u.device, torch.float32
-    u, delta, Br, Cr = _rows(u), _rows(delta), _rows(B), _rows(C)
-    zr = None if z is None else _rows(z)
+    u, delta, Br, Cr = _rows(u, 1), _rows(delta, 1), _rows(B, 1), _rows(C, 1)
+    zr = None if z is None else _rows(z, 1)
     Ac, Dc, bc = A.contiguous(), _c(D), _c(bias)
-    dy = torch.zeros_like(u) if dy is None else _rows(dy.to(u.dtype))
+    dy = torch.zeros(Bn, T, Dm, device=dev, dtype=u.dtype) if dy is None else _rows(dy.to(u.dtype), 1)
     dfin = None if dfin is None else dfin.to(f32).contiguous()
     du, dd = (torch.empty(Bn, T, Dm, device=dev, dtype=u.dtype) for _ in range(2))
     dz = None if z is None else torch.empty_like(du)
@@ -176,8 +200,8 @@ def _scan_bwd(u, delta, A, B, C, D, z, bias, softplus, kept, dy, dfin, want_s0, 
     ds0 = torch.empty(Bn, Dm, N, device=dev, dtype=f32) if want_s0 else None
     wsb = plan_on(u, "triune_hip_ssm_bwd_workspace_size", Bn, T, Dm, G, N, flags)
     ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
-    st = strides(u.stride()[:2], delta.stride()[:2], (0, 0) if zr is None else zr.stride()[:2], dy.stride()[:2],
-                 _group_strides(Br, 2, G), _group_strides(Cr, 2, G))
+    st = strides(_lead(u, 1), _lead(delta, 1), (0, 0) if zr is None else _lead(zr, 1), _lead(dy, 1),
+                 _group_strides(Br, 2), _group_strides(Cr, 2))
     call_on(u, "triune_hip_ssm_bwd", ptr(u), ptr(delta), ptr(zr), ptr(Br), ptr(Cr), ptr(Ac), ptr(Dc), ptr(bc), ptr(dy),
             dtype_code(u), st, int(softplus), ptr(kept), ptr(dfin), ptr(du), ptr(dd), ptr(dz), ptr(dB), ptr(dC),
             ptr(dA), ptr(dD), ptr(db), ptr(ds0), Bn, T, Dm, G, N, flags, ptr(ws), wsb)
@@ -281,18 +305,18 @@ def ssm_scan_varlen(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=No
         s0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
         fin = torch.empty(n, Dm, N, device=u.device, dtype=torch.float32)
     sl = _slots(slots, n, u.device)
-    y = _out(out, u.shape, u.dtype, u)
+    y = _out(out, u.shape, u.dtype, u, 0)
     if total == 0:
         if state_pool is None:
             fin.zero_() if s0 is None else fin.copy_(s0)
     elif n > 0:
-        u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
-        z = None if z is None else _rows(z)
+        u, delta, B, C = _rows(u, 0), _rows(delta, 0), _rows(B, 0), _rows(C, 0)
+        z = None if z is None else _rows(z, 0)
         A, D, delta_bias = A.contiguous(), _c(D), _c(delta_bias)
         wsb = plan_on(u, "triune_hip_ssm_scan_varlen_workspace_size", n, total, Dm, G, N, 0)
         ws = torch.empty(wsb, device=u.device, dtype=torch.uint8) if wsb else None
-        st = strides(u.stride()[:1], delta.stride()[:1], (0,) if z is None else z.stride()[:1], y.stride()[:1],
-                     _group_strides(B, 1, G), _group_strides(C, 1, G))
+        st = strides(_lead(u, 0), _lead(delta, 0), (0,) if z is None else _lead(z, 0), _lead_out(y, 0),
+                     _group_strides(B, 1), _group_strides(C, 1))
         call_on(u, "triune_hip_ssm_scan_varlen", ptr(u), ptr(delta), ptr(z), ptr(B), ptr(C), ptr(A), ptr(D),
                 ptr(delta_bias), dtype_code(u), st, int(delta_softplus), ptr(cu), n, total, ptr(s0), ptr(fin), ptr(sl),
                 fin.shape[0], ptr(y), Dm, G, N, 0, ptr(ws), wsb)
@@ -342,7 +366,7 @@ def ssm_decode_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, d
         z = None if z is None else _rows(z)
         A, D, delta_bias = A.contiguous(), _c(D), _c(delta_bias)
         st = strides(u.stride()[:1], delta.stride()[:1], (0,) if z is None else z.stride()[:1], y.stride()[:1],
-                     _group_strides(B, 1, G), _group_strides(C, 1, G))
+                     _group_strides(B, 1), _group_strides(C, 1))
         call_on(u, "triune_hip_ssm_decode_step", ptr(u), ptr(delta), ptr(z), ptr(B), ptr(C), ptr(A), ptr(D),
                 ptr(delta_bias), dtype_code(u), st, int(delta_softplus), ptr(s_in), ptr(s_out), ptr(sl),
                 s_in.shape[0], ptr(y), n, Dm, G, N)
