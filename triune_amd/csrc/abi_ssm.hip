@@ -320,7 +320,7 @@ int triune_hip_ssm_decode_step(const void* u, const void* delta, const void* z, 
     a.C = C, a.c_sb = strides[6], a.c_sg = strides[7];
     a.A = A, a.D = D, a.bias = delta_bias, a.softplus = softplus;
     a.s_in = state_in, a.s_out = state_out, a.slots = slots, a.n_rows = n_state_rows;
-    a.Bn = Bn, a.Dm = (int)Dm, a.G = (int)G, a.N = N;
+    a.Bn = Bn, a.Dm = (int)Dm, a.G = (int)G, a.N = N, a.cus = compute_units();
     return status(launch_ssm_step(a, io_dtype, (hipStream_t)stream));
 }
 
@@ -332,8 +332,8 @@ static int conv_check(const void* x, const void* w, const void* bias, const void
     if (!dtype_ok(io_dtype) || (w_dtype != io_dtype && w_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
     if (n < 0 || T < 0 || T >= (1 << 30) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return TRIUNE_ERR_SHAPE;
     if (!all_aligned(io_dtype, {x, y, s0, fin}) || !all_aligned(w_dtype, {w, bias})) return TRIUNE_ERR_LAYOUT;
-    // runs of 16 tokens x eight channels, and (sequence, eight channels) pairs, are numbered in 31 bits
-    if (n > 0 && (Dm + 7) / 8 > kMaxGrid / (n * ((T + 15) / 16 + 1))) return TRIUNE_ERR_SHAPE;
+    // runs of 16 tokens x four channels, and (sequence, four channels) pairs, are numbered in 31 bits
+    if (n > 0 && (Dm + 3) / 4 > kMaxGrid / (n * ((T + 15) / 16 + 1))) return TRIUNE_ERR_SHAPE;
     return TRIUNE_OK;
 }
 
@@ -392,7 +392,8 @@ int triune_hip_short_conv_decode_step(const void* x, const void* w, const void* 
 
 size_t triune_hip_short_conv_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int W) {
     if (Bn <= 0 || T <= 0 || T >= (1 << 30) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return 0;
-    return align_up((size_t)conv_bwd_parts(Bn, T, (int)Dm) * (W + 1) * Dm * 4);
+    const int run = conv_bwd_run(Bn, T, (int)Dm, compute_units());
+    return align_up((size_t)conv_bwd_parts(Bn, T, (int)Dm, run) * (W + 1) * Dm * 4);
 }
 
 int triune_hip_short_conv_bwd(const void* x, const void* w, const void* bias, const void* dy, int io_dtype,
@@ -408,7 +409,8 @@ int triune_hip_short_conv_bwd(const void* x, const void* w, const void* bias, co
     g.f.x_sb = strides[0], g.f.x_st = strides[1];
     g.dy = dy, g.dy_sb = strides[2], g.dy_st = strides[3];
     g.dfin = ds_final, g.dx = dx, g.ds0 = ds0;
-    g.parts = conv_bwd_parts(Bn, T, (int)Dm);
+    g.run = conv_bwd_run(Bn, T, (int)Dm, compute_units());
+    g.parts = conv_bwd_parts(Bn, T, (int)Dm, g.run);
     if (dw || dbias) {
         if (const int e = check_ws(workspace, workspace_bytes, triune_hip_short_conv_bwd_workspace_size(Bn, T, Dm, W)))
             return e;
@@ -437,7 +439,7 @@ int triune_hip_layer_norm(const void* x, int64_t x_stride, const void* w, const 
     if (const int e = norm_check(x, w, b, io_dtype, w_dtype, b_dtype, R, D)) return e;
     if (!aligned(y, io_dtype) || !all_aligned(TRIUNE_DT_F32, {mean, rstd})) return TRIUNE_ERR_LAYOUT;
     if (R == 0) return TRIUNE_OK;
-    NormParams a{x, x_stride, w, b, w_dtype, b_dtype, eps, y, mean, rstd, R, (int)D};
+    NormParams a{x, x_stride, w, b, w_dtype, b_dtype, eps, y, mean, rstd, R, (int)D, compute_units()};
     return status(launch_norm(a, io_dtype, (hipStream_t)stream));
 }
 
@@ -457,7 +459,7 @@ int triune_hip_layer_norm_bwd(const void* x, int64_t x_stride, const void* w, co
     if (R == 0) return TRIUNE_ERR_SHAPE;
     NormBwdParams g{};
     g.f = NormParams{x, x_stride, w, nullptr, w_dtype, b_dtype, 0.f, nullptr, const_cast<float*>(mean),
-                     const_cast<float*>(rstd), R, (int)D};
+                     const_cast<float*>(rstd), R, (int)D, compute_units()};
     g.dy = dy, g.dy_st = dy_stride, g.dx = dx, g.dw = dw, g.db = db;
     g.parts = norm_bwd_parts(R, (int)D, compute_units());
     if (dw || db) {

@@ -29,6 +29,9 @@ __device__ __forceinline__ float row_sum(float x, float* s) {
     return x;
 }
 
+// Blocks of 256 threads a compute unit, each walking rows (16384 rows of 1536, bf16, forward and backward:
+// 81 us with 4 and 2, 95 with 8 and 4, whose parts of dw and db are twice as many).
+constexpr int FWD_BLOCKS = 4, BWD_BLOCKS = 2;
 constexpr int block_threads(int tpr) { return tpr == 64 ? 256 : tpr; }
 
 // Columns of thread t: groups of eight, TPR * 8 apart.
@@ -42,15 +45,15 @@ __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, fl
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = none;
     } else if (dt == DT_F32) {
-        const Raw8<float> r = load_raw8((const float*)p + c, n);
+        const Raw<float, 8> r = load_raw<8>((const float*)p + c, n);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = r.v[j];
     } else if (dt == DT_BF16) {
-        const Raw8<__bf16> r = load_raw8((const __bf16*)p + c, n);
+        const Raw<__bf16, 8> r = load_raw<8>((const __bf16*)p + c, n);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = (float)r.v[j];
     } else {
-        const Raw8<_Float16> r = load_raw8((const _Float16*)p + c, n);
+        const Raw<_Float16, 8> r = load_raw<8>((const _Float16*)p + c, n);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = (float)r.v[j];
     }
@@ -58,53 +61,66 @@ __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, fl
 
 }  // namespace
 
+// Blocks walk rows, the next row's loads in flight during this one's sums; w and b are loaded once.
 template <typename T, int TPR, int K>
 __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) {
     constexpr int RPB = block_threads(TPR) / TPR;
     __shared__ float s_red[16];
     const int t = threadIdx.x % TPR;
-    const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (RPB > 1 && r >= a.R) return;  // whole waves
-    const T* px = (const T*)a.x + r * a.x_st;
-    T* py = (T*)a.y + r * a.D;
     const float width = (float)a.D;  // divided by: a constant row's mean is its value where its sum is exact
-    Raw8<T> raw[K];
+    Raw<T, 8> raw[K];
+    auto fetch = [&](int64_t row) {
+        const T* px = (const T*)a.x + row * a.x_st;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = column<TPR>(t, k);
+            raw[k] = load_raw<8>(px + c, a.D - c);
+        }
+    };
+    fetch(r);
+    float w[K][8], b[K][8];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = column<TPR>(t, k);
-        raw[k] = load_raw8(px + c, a.D - c);
+        load_par(a.w, a.w_dt, c, a.D - c, 1.f, w[k]);
+        load_par(a.b, a.b_dt, c, a.D - c, 0.f, b[k]);
     }
-    float x[K][8], s = 0.f;
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    for (; r < a.R; r += step) {
+        float x[K][8], s = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += x[k][j] = (float)raw[k].v[j];
-    const float mean = row_sum<TPR>(s, s_red) / width;
-    s = 0.f;
+            for (int j = 0; j < 8; ++j) s += x[k][j] = (float)raw[k].v[j];
+        if (r + step < a.R) fetch(r + step);
+        const float mean = row_sum<TPR>(s, s_red) / width;
+        s = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int left = a.D - column<TPR>(t, k);
+        for (int k = 0; k < K; ++k) {
+            const int left = a.D - column<TPR>(t, k);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[k][j] = j < left ? x[k][j] - mean : 0.f;
-            s = __builtin_fmaf(x[k][j], x[k][j], s);
+            for (int j = 0; j < 8; ++j) {
+                x[k][j] = j < left ? x[k][j] - mean : 0.f;
+                s = __builtin_fmaf(x[k][j], x[k][j], s);
+            }
         }
-    }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(s, s_red) / width + a.eps);
-    if (a.mean && t == 0) {
-        a.mean[r] = mean;
-        a.rstd[r] = rstd;
-    }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, s_red) / width + a.eps);
+        if (a.mean && t == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        T* py = (T*)a.y + r * a.D;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = column<TPR>(t, k), left = a.D - c;
-        if (left <= 0) continue;
-        float w[8], b[8], y[8];
-        load_par(a.w, a.w_dt, c, left, 1.f, w);
-        load_par(a.b, a.b_dt, c, left, 0.f, b);
+        for (int k = 0; k < K; ++k) {
+            const int c = column<TPR>(t, k), left = a.D - c;
+            if (left <= 0) continue;
+            float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[k][j] * rstd, w[j], b[j]);
-        store_raw8(py + c, left, y);
+            for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[k][j] * rstd, w[k][j], b[k][j]);
+            store_raw<8>(py + c, left, y);
+        }
     }
 }
 
@@ -124,17 +140,32 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[k][j] = db[k][j] = 0.f;
     }
-    for (int64_t r = (int64_t)blockIdx.x * RPB + rl; r < a.R; r += (int64_t)gridDim.x * RPB) {
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Raw<T, 8> nx[K], ny[K];
+    float nmean, nrstd;
+    auto fetch = [&](int64_t r) {
         const T *px = (const T*)a.x + r * a.x_st, *py = (const T*)g.dy + r * g.dy_st;
-        T* pd = (T*)g.dx + r * a.D;
-        const float mean = a.mean[r], rstd = a.rstd[r];
-        Raw8<T> rx[K], ry[K];
+        nmean = a.mean[r];
+        nrstd = a.rstd[r];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = column<TPR>(t, k);
-            rx[k] = load_raw8(px + c, a.D - c);
-            ry[k] = load_raw8(py + c, a.D - c);
+            nx[k] = load_raw<8>(px + c, a.D - c);
+            ny[k] = load_raw<8>(py + c, a.D - c);
         }
+    };
+    // the next row's loads in flight where its registers are free
+    constexpr bool AHEAD = TPR <= 256 && K <= 3;
+    int64_t r = (int64_t)blockIdx.x * RPB + rl;
+    if (AHEAD && r < a.R) fetch(r);
+    for (; r < a.R; r += step) {
+        if constexpr (!AHEAD) fetch(r);
+        T* pd = (T*)g.dx + r * a.D;
+        const float mean = nmean, rstd = nrstd;
+        Raw<T, 8> rx[K], ry[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
+        if (AHEAD && r + step < a.R) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
         float xh[K][8];
 #pragma unroll
@@ -158,7 +189,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 o[j] = rstd * ((float)ry[k].v[j] * w[k][j] - __builtin_fmaf(xh[k][j], m2, m1));
-            store_raw8(pd + c, left, o);
+            store_raw<8>(pd + c, left, o);
         }
     }
     if (!g.part) return;
@@ -184,7 +215,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
                     if (col < a.D) pp[(int64_t)q * a.D + col] = s;
                 }
             } else if (c < a.D) {
-                store_raw8(pp + (int64_t)q * a.D + c, a.D - c, v);
+                store_raw<8>(pp + (int64_t)q * a.D + c, a.D - c, v);
             }
         }
     }
@@ -194,9 +225,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
 __global__ __launch_bounds__(1024) void norm_bwd_sum_kernel(NormBwdParams g) {
     const int per = 2 * g.f.D, l = threadIdx.x & 63, id = blockIdx.x * 64 + l, w = threadIdx.x >> 6;
     __shared__ float red[16][64];
-    float s = 0.f;
-    if (id < per)
-        for (int64_t p = w; p < g.parts; p += 16) s += g.part[p * per + id];
+    float s = id < per ? sum_parts(g.part + id, per, w, g.parts) : 0.f;
     red[w][l] = s;
     __syncthreads();
     if (w || id >= per) return;
@@ -209,7 +238,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_sum_kernel(NormBwdParams g) {
 }
 
 int64_t norm_bwd_parts(int64_t R, int D, int cus) {
-    const int64_t rpb = D <= 2048 ? 4 : 1, blocks = (R + rpb - 1) / rpb, most = (int64_t)cus * 2;
+    const int64_t rpb = D <= 2048 ? 4 : 1, blocks = (R + rpb - 1) / rpb, most = (int64_t)cus * BWD_BLOCKS;
     return blocks < most ? blocks : most;
 }
 
@@ -218,7 +247,8 @@ namespace {
 template <typename T, int TPR, int K>
 hipError_t norm_run(const NormParams& a, hipStream_t s) {
     constexpr int RPB = block_threads(TPR) / TPR;
-    norm_kernel<T, TPR, K><<<dim3((unsigned)((a.R + RPB - 1) / RPB)), block_threads(TPR), 0, s>>>(a);
+    const int64_t blocks = (a.R + RPB - 1) / RPB, most = (int64_t)a.cus * FWD_BLOCKS * 256 / block_threads(TPR);
+    norm_kernel<T, TPR, K><<<dim3((unsigned)(blocks < most ? blocks : most)), block_threads(TPR), 0, s>>>(a);
     return hipGetLastError();
 }
 template <typename T, int TPR, int K>

@@ -65,7 +65,7 @@ struct SsmStepParams {
     const int32_t* slots;
     int64_t n_rows;           // rows of the state
     int64_t Bn;
-    int Dm, G, N;
+    int Dm, G, N, cus;        // cus: compute units
 };
 
 int ssm_waves(int N);  // waves of a scan workgroup
@@ -112,10 +112,12 @@ struct ConvBwdParams {
     void* ds0;                // [Bn, W - 1, Dm] contiguous or null
     float* part;              // [parts, W + 1, Dm]
     int64_t parts;
+    int run;                  // tokens of a run
     void *dw, *dbias;         // of w_dt, or null
 };
 
-int64_t conv_bwd_parts(int64_t n_seqs, int64_t T, int Dm);
+int conv_bwd_run(int64_t n_seqs, int64_t T, int Dm, int cus);
+int64_t conv_bwd_parts(int64_t n_seqs, int64_t T, int Dm, int run);
 hipError_t launch_conv(const ConvParams& a, int io_dt, hipStream_t s);
 hipError_t launch_conv_state(const ConvParams& a, int io_dt, hipStream_t s);
 hipError_t launch_conv_step(const ConvParams& a, int io_dt, hipStream_t s);
@@ -133,7 +135,7 @@ struct NormParams {
     void* y;                  // [R, D] contiguous
     float *mean, *rstd;       // [R] or null
     int64_t R;
-    int D;
+    int D, cus;               // cus: compute units
 };
 
 struct NormBwdParams {
@@ -169,35 +171,51 @@ __device__ __forceinline__ float softplus(float x) {
     return __builtin_fmaf(s, p, 0.5f * (x + fabsf(x)));  // max(x, 0) without fmaxf's second max for NaN
 }
 
-// Eight elements of any alignment in one access (the memory pipeline takes unaligned vectors), or the
-// n < 8 that a row's last group holds.
-template <typename T>
-struct __attribute__((packed, aligned(alignof(T)))) Raw8 {
-    T v[8];
+// N elements of any alignment in one access (the memory pipeline takes unaligned vectors), or the
+// n < N that a row's last group holds.
+template <typename T, int N>
+struct __attribute__((packed, aligned(alignof(T)))) Raw {
+    T v[N];
 };
-template <typename T>
-__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int n) {
-    Raw8<T> r;
-    if (n >= 8) {
-        r = *reinterpret_cast<const Raw8<T>*>(p);
+template <int N, typename T>
+__device__ __forceinline__ Raw<T, N> load_raw(const T* p, int n) {
+    Raw<T, N> r;
+    if (n >= N) {
+        r = *reinterpret_cast<const Raw<T, N>*>(p);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
+        for (int j = 0; j < N; ++j) r.v[j] = j < n ? p[j] : (T)0.f;
     }
     return r;
 }
-template <typename T>
-__device__ __forceinline__ void store_raw8(T* p, int n, const float (&x)[8]) {
-    Raw8<T> r;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r.v[j] = (T)x[j];
-    if (n >= 8) {
-        *reinterpret_cast<Raw8<T>*>(p) = r;
+template <int N, typename T>
+__device__ __forceinline__ void store_raw(T* p, int n, const Raw<T, N>& r) {
+    if (n >= N) {
+        *reinterpret_cast<Raw<T, N>*>(p) = r;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < N; ++j)
             if (j < n) p[j] = r.v[j];
     }
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_raw(T* p, int n, const float (&x)[N]) {
+    Raw<T, N> r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.v[j] = (T)x[j];
+    store_raw<N>(p, n, r);
+}
+
+// The sum of n values `st` apart, every sixteenth from the first, four of them in flight.
+__device__ __forceinline__ float sum_parts(const float* p, int64_t st, int64_t first, int64_t n) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    int64_t k = first;
+    for (; k + 48 < n; k += 64) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += p[(k + 16 * i) * st];
+    }
+    for (int i = 0; k < n; k += 16, ++i) s[i] += p[k * st];
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 __device__ __forceinline__ float load_dt(const void* p, int dt, int64_t i) {
@@ -243,51 +261,6 @@ __device__ __forceinline__ void store_states(float* p, int left, const float (&x
         for (int j = 0; j < N; ++j)
             if (j < left) p[j] = x[j];
     }
-}
-
-// The value that lane k of a channel's L lanes holds, in all of them (a DPP operand of its user).
-template <int CTRL>
-__device__ __forceinline__ float dpp_read(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-template <int L>
-__device__ __forceinline__ float lane_of(float x, int k) {
-    if constexpr (L == 1) {
-        return x;
-    } else if constexpr (L == 2) {
-        return k == 0 ? dpp_read<0xA0>(x) : dpp_read<0xF5>(x);  // quad_perm [0,0,2,2], [1,1,3,3]
-    } else if constexpr (L == 4) {
-        return k == 0 ? dpp_read<0x00>(x) : k == 1 ? dpp_read<0x55>(x) : k == 2 ? dpp_read<0xAA>(x) : dpp_read<0xFF>(x);
-    } else {
-        static_assert(L == 16, "no such broadcast");
-        switch (k) {  // row_newbcast
-            case 0: return dpp_read<0x150>(x);
-            case 1: return dpp_read<0x151>(x);
-            case 2: return dpp_read<0x152>(x);
-            case 3: return dpp_read<0x153>(x);
-            case 4: return dpp_read<0x154>(x);
-            case 5: return dpp_read<0x155>(x);
-            case 6: return dpp_read<0x156>(x);
-            case 7: return dpp_read<0x157>(x);
-            case 8: return dpp_read<0x158>(x);
-            case 9: return dpp_read<0x159>(x);
-            case 10: return dpp_read<0x15A>(x);
-            case 11: return dpp_read<0x15B>(x);
-            case 12: return dpp_read<0x15C>(x);
-            case 13: return dpp_read<0x15D>(x);
-            case 14: return dpp_read<0x15E>(x);
-            default: return dpp_read<0x15F>(x);
-        }
-    }
-}
-// The sum over a channel's L lanes, in all of them.
-template <int L>
-__device__ __forceinline__ float channel_sum(float x) {
-    if constexpr (L >= 2) x = dpp_add<0xB1>(x);    // lane ^ 1
-    if constexpr (L >= 4) x = dpp_add<0x4E>(x);    // lane ^ 2
-    if constexpr (L >= 8) x = dpp_add<0x141>(x);   // the other four of eight
-    if constexpr (L >= 16) x = dpp_add<0x140>(x);  // the other eight of sixteen
-    return x;
 }
 
 // Rows of a tile through a buffer resource: it starts at the tile's first row and ends with the last

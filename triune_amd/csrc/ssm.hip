@@ -3,6 +3,22 @@
 // For each channel d with states n:
 //     dt_t = softplus(delta_t + bias);  h_t = exp(dt_t A_n) h_{t-1} + dt_t u_t B_t,n
 //     y_t  = (sum_n C_t,n h_t,n + D u_t) silu(z_t)
+// A channel's decays differ by state, so nothing of it factors into matrix products: each (token, channel,
+// state) costs an exp2 and four plain operations, 23.5 cycles of a SIMD per wave measured (8.4 for the
+// exp2; a plain operation 2.9 where two waves issue it, 5.5 alone, and 4.4 with a scalar or DPP
+// operand), each (token, channel) about 200 more for softplus, gate, conversions and its LDS traffic.
+// That, not the memory, bounds the kernel.
+//
+// Work split: a lane is a channel in the walk over the tokens, a wave holds four states of 64 channels
+// in registers, a workgroup all states of 64 channels.  Tiles of tokens go through LDS: every (token,
+// channel) is loaded and its softplus taken once for all states, by lanes of four channels, B and C are
+// read as broadcasts, and the waves' parts of y meet there.  A form without that traffic (four lanes
+// a channel, dt and dt u as DPP operands, y summed by DPP) issued as many operations, each slower:
+// 437 us for 8 x 2048 tokens of 4096 channels (N = 16, bf16) against 306.
+//
+// Calls with too few (sequence, channel block) pairs for the chip split the time axis into segments: a
+// pass for each segment's own end state (its decay over the segment is exp(A sum dt), so only the sum
+// of dt is kept), a scan over segments, and the pass that writes the outputs.
 #include "ssm.h"
 
 namespace triune {
@@ -289,61 +305,74 @@ __global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int32_t* o
     }
 }
 
-// One token for every row.  A lane holds up to four states of a channel, LPC lanes a channel.
-template <typename T, int LPC, bool VEC>
-__global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams a) {
+// Four elements of any alignment (the last of a row: those that it holds).
+template <typename T>
+__device__ __forceinline__ void load_four(const T* p, int left, float (&x)[4]) {
+    struct __attribute__((packed, aligned(alignof(T)))) Four {
+        T v[4];
+    };
+    if (left >= 4) {
+        const Four r = *reinterpret_cast<const Four*>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (float)r.v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = j < left ? (float)p[j] : 0.f;
+    }
+}
+
+// One token for every row.  A lane holds up to four states of a channel, LPC neighbouring lanes a
+// channel; a block keeps its channels' A, D and bias over the rows that it walks, the next row's
+// states and operands in flight.  Bound by the states, read and written once.
+template <typename T, int LPC>
+__global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams a, int blocks) {
     constexpr int CPB = 256 / LPC;  // channels of a block
-    const int64_t nblk = (a.Dm + CPB - 1) / CPB;
-    const int64_t b = blockIdx.x / nblk;
-    const int ch = (int)(blockIdx.x - b * nblk) * CPB + threadIdx.x / LPC, q = threadIdx.x % LPC, n0 = 4 * q;
+    const int ch = (int)(blockIdx.x % blocks) * CPB + threadIdx.x / LPC, q = threadIdx.x % LPC, n0 = 4 * q;
     const bool chv = ch < a.Dm;
-    const int c = chv ? ch : 0;
-    const int64_t row = ssm_row(a.slots, a.n_rows, b);
-    float h[4] = {0.f, 0.f, 0.f, 0.f}, Al[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool live = chv && row >= 0 && n0 < a.N;
-    if (live) {
-        const float *ps = a.s_in + (row * a.Dm + c) * a.N + n0, *pA = a.A + (int64_t)c * a.N + n0;
-        if constexpr (VEC) {
-            const f32x4 s = *reinterpret_cast<const f32x4*>(ps), m = *reinterpret_cast<const f32x4*>(pA);
+    const int c = chv ? ch : 0, left = chv ? a.N - n0 : 0, grp = c / (a.Dm / a.G);
+    float Al[4];
+    load_states<4>(a.A + (int64_t)c * a.N + n0, left, Al);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = s[j], Al[j] = log2_decay(m[j]);
-        } else {
+    for (int j = 0; j < 4; ++j) Al[j] = log2_decay(Al[j]);
+    const float bias = a.bias ? a.bias[c] : 0.f, Dv = a.D ? a.D[c] : 0.f;
+    struct Row {
+        int64_t row;
+        float h[4], B[4], C[4];
+        T u, dl, z;
+    } x;
+    auto fetch = [&](int64_t b) {
+        x.row = ssm_row(a.slots, a.n_rows, b);
+        load_states<4>(a.s_in + (x.row * a.Dm + c) * a.N + n0, x.row >= 0 ? left : 0, x.h);
+        load_four((const T*)a.B + b * a.b_sb + grp * a.b_sg + n0, left, x.B);
+        load_four((const T*)a.C + b * a.c_sb + grp * a.c_sg + n0, left, x.C);
+        x.u = ((const T*)a.u.p)[b * a.u.sb + c];
+        x.dl = ((const T*)a.dl.p)[b * a.dl.sb + c];
+        x.z = a.z.p ? ((const T*)a.z.p)[b * a.z.sb + c] : (T)0.f;
+    };
+    const int64_t step = gridDim.x / blocks;
+    int64_t b = blockIdx.x / blocks;
+    fetch(b);
+    for (; b < a.Bn; b += step) {
+        const Row r = x;
+        if (b + step < a.Bn) fetch(b + step);
+        const float uu = (float)r.u, xx = (float)r.dl + bias;
+        const float dt = a.softplus ? softplus(xx) : xx, dtu = dt * uu;
+        float h[4], y = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) h[j] = ps[j], Al[j] = log2_decay(pA[j]);
+        for (int j = 0; j < 4; ++j) {
+            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * Al[j]), r.h[j], dtu * r.B[j]);
+            y = __builtin_fmaf(r.C[j], h[j], y);
         }
-    }
-    const int grp = c / (a.Dm / a.G);
-    const T *pB = (const T*)a.B + b * a.b_sb + grp * a.b_sg + n0, *pC = (const T*)a.C + b * a.c_sb + grp * a.c_sg + n0;
-    const float x = (float)((const T*)a.dl.p)[b * a.dl.sb + c] + (a.bias ? a.bias[c] : 0.f);
-    const float uu = (float)((const T*)a.u.p)[b * a.u.sb + c];
-    const float dt = a.softplus ? softplus(x) : x, dtu = dt * uu;
-    float y = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool ok = n0 + j < a.N;
-        const float bb = ok ? (float)pB[j] : 0.f, cc = ok ? (float)pC[j] : 0.f;
-        h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * Al[j]), h[j], dtu * bb);
-        y = __builtin_fmaf(cc, h[j], y);
-    }
-    if (live) {
-        float* ps = a.s_out + (row * a.Dm + c) * a.N + n0;
-        if constexpr (VEC) {
-            *reinterpret_cast<f32x4*>(ps) = f32x4{h[0], h[1], h[2], h[3]};
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n0 + j < a.N) ps[j] = h[j];
+        if (r.row >= 0 && left > 0) store_states<4>(a.s_out + (r.row * a.Dm + c) * a.N + n0, left, h);
+        if constexpr (LPC >= 2) y = dpp_add<0xB1>(y);
+        if constexpr (LPC >= 4) y = dpp_add<0x4E>(y);
+        if constexpr (LPC >= 8) y = dpp_add<0x141>(y);
+        if constexpr (LPC >= 16) y = dpp_add<0x140>(y);
+        if (q == 0 && chv) {
+            y = __builtin_fmaf(Dv, uu, y);
+            if (a.z.p) y *= silu_gate((float)r.z);
+            ((T*)const_cast<void*>(a.y.p))[b * a.y.sb + c] = (T)(r.row >= 0 ? y : 0.f);
         }
-    }
-    if constexpr (LPC >= 2) y = dpp_add<0xB1>(y);
-    if constexpr (LPC >= 4) y = dpp_add<0x4E>(y);
-    if constexpr (LPC >= 8) y = dpp_add<0x141>(y);
-    if constexpr (LPC >= 16) y = dpp_add<0x140>(y);
-    if (q == 0 && chv) {
-        if (a.D) y = __builtin_fmaf(a.D[c], uu, y);
-        if (a.z.p) y *= silu_gate((float)((const T*)a.z.p)[b * a.z.sb + c]);
-        ((T*)const_cast<void*>(a.y.p))[b * a.y.sb + c] = (T)(row >= 0 ? y : 0.f);
     }
 }
 
@@ -382,26 +411,29 @@ hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* off, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T>
 static hipError_t step_lanes(const SsmStepParams& a, hipStream_t s) {
-    const int lpc = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16, cpb = 256 / lpc;
-    const dim3 grid((unsigned)(a.Bn * ((a.Dm + cpb - 1) / cpb)));
+    const int lpc = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
+    const int64_t blocks = (a.Dm * (int64_t)lpc + 255) / 256;
+    // rows that are walked side by side: eight blocks a compute unit (256 sessions of 1536 channels, N = 16:
+    // 15.0 us; 16.8 with four, 16.6 with sixteen, 19.1 with a block per row and 64 channels)
+    int64_t rows = a.cus * 8 / blocks;
+    rows = rows < 1 ? 1 : rows > a.Bn ? a.Bn : rows;
+    const dim3 grid((unsigned)(blocks * rows));
     switch (lpc) {
-        case 1: ssm_step_kernel<T, 1, VEC><<<grid, 256, 0, s>>>(a); break;
-        case 2: ssm_step_kernel<T, 2, VEC><<<grid, 256, 0, s>>>(a); break;
-        case 4: ssm_step_kernel<T, 4, VEC><<<grid, 256, 0, s>>>(a); break;
-        case 8: ssm_step_kernel<T, 8, VEC><<<grid, 256, 0, s>>>(a); break;
-        default: ssm_step_kernel<T, 16, VEC><<<grid, 256, 0, s>>>(a); break;
+        case 1: ssm_step_kernel<T, 1><<<grid, 256, 0, s>>>(a, (int)blocks); break;
+        case 2: ssm_step_kernel<T, 2><<<grid, 256, 0, s>>>(a, (int)blocks); break;
+        case 4: ssm_step_kernel<T, 4><<<grid, 256, 0, s>>>(a, (int)blocks); break;
+        case 8: ssm_step_kernel<T, 8><<<grid, 256, 0, s>>>(a, (int)blocks); break;
+        default: ssm_step_kernel<T, 16><<<grid, 256, 0, s>>>(a, (int)blocks); break;
     }
     return hipGetLastError();
 }
 
 hipError_t launch_ssm_step(const SsmStepParams& a, int dt, hipStream_t s) {
-    const bool vec = a.N % 4 == 0 && !((reinterpret_cast<uintptr_t>(a.s_in) | reinterpret_cast<uintptr_t>(a.s_out) |
-                                        reinterpret_cast<uintptr_t>(a.A)) & 15);
-    if (dt == DT_F32) return vec ? step_lanes<float, true>(a, s) : step_lanes<float, false>(a, s);
-    if (dt == DT_BF16) return vec ? step_lanes<__bf16, true>(a, s) : step_lanes<__bf16, false>(a, s);
-    return vec ? step_lanes<_Float16, true>(a, s) : step_lanes<_Float16, false>(a, s);
+    if (dt == DT_F32) return step_lanes<float>(a, s);
+    if (dt == DT_BF16) return step_lanes<__bf16>(a, s);
+    return step_lanes<_Float16>(a, s);
 }
 
 }  // namespace triune

@@ -5,14 +5,18 @@
 //     ddt = sum_n (p A + dh B u)   du = dt sum_n dh B + D gy     dA = sum_t p dt
 //     ddelta = ddt softplus'(x)    dz = dy silu'(z) (sum_n C h + D u)
 //
-// Lanes, waves and tiles are those of the forward (ssm.hip).  The forward kept the state of every
-// 32nd token; a workgroup walks its tiles from the last to the first.  In a tile it runs the states
-// forward once to have the one that each sub-tile starts from, then takes the sub-tiles backward:
-// a sub-tile's decays and states are formed again and stay in registers (sixteen tokens of four
-// states: 128 registers), so nothing of size tokens x channels x states goes to memory.  Sums over states
-// (for dt, u, z) meet in LDS; sums over channels (dB, dC) are taken across the lanes, eight values
-// of a token together by halving exchanges, and stored per workgroup; a last kernel adds the
-// workgroups' parts in a fixed order, so the gradients do not depend on timing.
+// Lanes, waves and tiles are those of the forward (ssm.hip).  The forward kept a state for each tile; a
+// workgroup walks its tiles from the last to the first.  In a tile it runs the states forward once to
+// have the one that each walk of eight tokens starts from, then takes the walks backward: a walk's decays
+// and states are formed again and stay in registers (64 of them), so nothing of size tokens x channels x
+// states goes to memory.  Sums over states (for dt, u, z) meet in LDS; sums over channels (dB, dC) are
+// taken across the lanes, eight values of a token together by halving exchanges (fp32 matrix products
+// with columns of the identity, which add four lanes, took 179 cycles per wave and state alone), and
+// stored per workgroup; a last kernel adds the workgroups' parts in a fixed order, so the gradients do
+// not depend on timing.
+//
+// Bound by vector issue at two waves a SIMD: 25 vector operations and 1.75 exp2 per wave and state (about
+// 105 cycles).  4 x 2048 tokens of 1536 channels, N = 16, bf16: 218 us where that is 134.
 #include "ssm.h"
 
 namespace triune {
@@ -449,34 +453,32 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void ssm_bwd_kernel(SsmB
     }
 }
 
-// dB, dC: the channel blocks' parts added in their order.  One thread per (token, group, state).
+// The parts added in a fixed order.  The first bc_blocks blocks: dB, dC over channel blocks, one thread per
+// (token, group, state).  The others: dA, dD, dbias over work items, sixteen threads per (row, channel),
+// each every sixteenth item, then these.
 template <typename T>
-__global__ __launch_bounds__(256) void ssm_bwd_bc_kernel(SsmBwdParams g, int nw) {
-    const SsmParams& a = g.f;
-    const int64_t toks = a.n_seqs * a.T, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= toks * a.G * a.N) return;
-    const int64_t tg = id / a.N, tok = tg / a.G;
-    const int n = (int)(id - tg * a.N), grp = (int)(tg - tok * a.G);
-    const float* p = g.part_bc + (((int64_t)grp * a.blocks * toks + tok) * nw + (n >> 2)) * 8 + (n & 3);
-    float sb = 0.f, sc = 0.f;
-    for (int k = 0; k < a.blocks; ++k) {
-        sb += p[k * toks * nw * 8];
-        sc += p[k * toks * nw * 8 + 4];
-    }
-    ((T*)g.dB)[id] = (T)sb;
-    ((T*)g.dC)[id] = (T)sc;
-}
-
-// dA, dD, dbias: the work items' parts added in a fixed order: sixteen threads per (row, channel), each
-// every sixteenth item, then these.
-__global__ __launch_bounds__(1024) void ssm_bwd_par_kernel(SsmBwdParams g) {
+__global__ __launch_bounds__(1024) void ssm_bwd_sum_kernel(SsmBwdParams g, int nw, int bc_blocks) {
     const SsmParams& a = g.f;
     __shared__ float red[16][64];
+    if (blockIdx.x < bc_blocks) {
+        const int64_t toks = a.n_seqs * a.T, id = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+        if (id >= toks * a.G * a.N) return;
+        const int64_t tg = id / a.N, tok = tg / a.G;
+        const int n = (int)(id - tg * a.N), grp = (int)(tg - tok * a.G);
+        const float* p = g.part_bc + (((int64_t)grp * a.blocks * toks + tok) * nw + (n >> 2)) * 8 + (n & 3);
+        float sb = 0.f, sc = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < a.blocks; ++k) {
+            sb += p[k * toks * nw * 8];
+            sc += p[k * toks * nw * 8 + 4];
+        }
+        ((T*)g.dB)[id] = (T)sb;
+        ((T*)g.dC)[id] = (T)sc;
+        return;
+    }
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t per = (int64_t)(a.N + 2) * a.Dm, id = (int64_t)blockIdx.x * 64 + l;
-    float s = 0.f;
-    if (id < per)
-        for (int64_t k = w; k < a.n_work; k += 16) s += g.part_par[k * per + id];
+    const int64_t per = (int64_t)(a.N + 2) * a.Dm, id = (int64_t)(blockIdx.x - bc_blocks) * 64 + l;
+    float s = id < per ? sum_parts(g.part_par + id, per, w, a.n_work) : 0.f;
     red[w][l] = s;
     __syncthreads();
     if (w || id >= per) return;
@@ -541,14 +543,11 @@ hipError_t launch_ssm_bwd_carry(const SsmBwdParams& g, hipStream_t s) {
 
 hipError_t launch_ssm_bwd_sum(const SsmBwdParams& g, int dt, hipStream_t s) {
     const int64_t n = g.f.n_seqs * g.f.T * g.f.G * g.f.N, m = (int64_t)(g.f.N + 2) * g.f.Dm;
-    const dim3 grid((unsigned)((n + 255) / 256));
-    const int nw = ssm_waves(g.f.N);
-    if (dt == DT_F32) ssm_bwd_bc_kernel<float><<<grid, 256, 0, s>>>(g, nw);
-    else if (dt == DT_BF16) ssm_bwd_bc_kernel<__bf16><<<grid, 256, 0, s>>>(g, nw);
-    else ssm_bwd_bc_kernel<_Float16><<<grid, 256, 0, s>>>(g, nw);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    ssm_bwd_par_kernel<<<dim3((unsigned)((m + 63) / 64)), 1024, 0, s>>>(g);
+    const int nw = ssm_waves(g.f.N), bc = (int)((n + 1023) / 1024);
+    const dim3 grid((unsigned)(bc + (m + 63) / 64));
+    if (dt == DT_F32) ssm_bwd_sum_kernel<float><<<grid, 1024, 0, s>>>(g, nw, bc);
+    else if (dt == DT_BF16) ssm_bwd_sum_kernel<__bf16><<<grid, 1024, 0, s>>>(g, nw, bc);
+    else ssm_bwd_sum_kernel<_Float16><<<grid, 1024, 0, s>>>(g, nw, bc);
     return hipGetLastError();
 }
 

@@ -69,7 +69,11 @@ def _lead_out(y, tok):
 
 
 def _needs_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_grad_path(what, *ts):
@@ -95,7 +99,9 @@ def _slots(slots, n, dev):
         return None
     if slots.numel() != n or slots.dim() != 1:
         raise ValueError(f"slots must hold one index for each of the {n} rows")
-    return slots.to(device=dev, dtype=torch.int32).contiguous()
+    if slots.dtype != torch.int32 or slots.device != dev:
+        slots = slots.to(device=dev, dtype=torch.int32)
+    return slots.contiguous()
 
 
 def _cu(cu_seqlens, dev):
@@ -123,26 +129,28 @@ def _check_scan(u, delta, A, B, C, D, z, delta_bias):
     """(Dm, G, N) of a call with token tensors [*lead, channels]."""
     _one_device(u, delta, A, B, C, D, z, delta_bias)
     dtype_code(u)
-    Dm = u.shape[-1]
-    if delta.shape != u.shape or (z is not None and z.shape != u.shape):
-        raise ValueError(f"delta and z must have u's shape {tuple(u.shape)}")
+    shape, dt = u.shape, u.dtype
+    Dm = shape[-1]
+    if delta.shape != shape or (z is not None and z.shape != shape):
+        raise ValueError(f"delta and z must have u's shape {tuple(shape)}")
     if A.dim() != 2 or A.shape[0] != Dm:
         raise ValueError(f"A must be [{Dm}, N]")
     N = A.shape[1]
     if not 1 <= N <= MAX_STATES or Dm < 1:
         raise ValueError(f"{N} states per channel are not supported (1 to {MAX_STATES})")
-    lead = u.dim() - 1
-    if B.shape != C.shape or B.shape[:lead] != u.shape[:lead] or B.shape[-1] != N or B.dim() not in (lead + 1, lead + 2):
-        raise ValueError(f"B and C must be {[*u.shape[:-1], N]} or [..., groups, {N}]")
-    G = B.shape[-2] if B.dim() == lead + 2 else 1
+    lead, bs = len(shape) - 1, B.shape
+    if bs != C.shape or bs[:lead] != shape[:lead] or bs[-1] != N or len(bs) not in (lead + 1, lead + 2):
+        raise ValueError(f"B and C must be {[*shape[:-1], N]} or [..., groups, {N}]")
+    G = bs[-2] if len(bs) == lead + 2 else 1
     if G < 1 or Dm % G:
         raise ValueError(f"{G} groups do not divide {Dm} channels")
-    if any(t is not None and t.dtype != u.dtype for t in (delta, z, B, C)):
+    if delta.dtype != dt or B.dtype != dt or C.dtype != dt or (z is not None and z.dtype != dt):
         raise TypeError("u, delta, z, B and C must share one dtype")
-    for name, t, shape in (("A", A, None), ("D", D, (Dm,)), ("delta_bias", delta_bias, (Dm,))):
-        if t is not None and t.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32")
-        if t is not None and shape is not None and tuple(t.shape) != shape:
+    f32 = torch.float32
+    if A.dtype != f32 or (D is not None and D.dtype != f32) or (delta_bias is not None and delta_bias.dtype != f32):
+        raise TypeError("A, D and delta_bias must be float32")
+    for name, t in (("D", D), ("delta_bias", delta_bias)):
+        if t is not None and (t.dim() != 1 or t.shape[0] != Dm):
             raise ValueError(f"{name} must be [{Dm}]")
     return Dm, G, N
 
