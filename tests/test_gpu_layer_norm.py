@@ -147,6 +147,9 @@ def test_graph_replays_and_determinism(dev):
 def test_empty_and_refusals(dev):
     x, w, b = inputs(dev, 4, 8)
     assert layer_norm(x[:0], w, b).shape == (0, 8)
+    leaves = [t.clone().requires_grad_() for t in (x[:0], w, b)]
+    for t, g in zip(leaves, torch.autograd.grad(layer_norm(*leaves).sum(), leaves)):
+        assert g.shape == t.shape and bool((g == 0).all())
     for a in ((x, w[:4]), (x, w, b[:4]), (x[:, :0],), (torch.zeros(2, 16385, device=dev),)):
         with pytest.raises(ValueError):
             layer_norm(*a)

@@ -173,6 +173,10 @@ def test_empty_and_refusals(dev):
     x, w, b, s = inputs(dev, 2, 5, 8, 4)
     y, fin = short_conv(x[:, :0], w, b, s)
     assert y.shape == (2, 0, 8) and torch.equal(fin, s)
+    leaves = [t.clone().requires_grad_() for t in (x[:, :0], w, b, s)]
+    y, fin = short_conv(*leaves)
+    for t, g in zip(leaves, torch.autograd.grad((y.sum(), fin.sum()), leaves)):
+        assert g.shape == t.shape and bool((g == (1 if t is leaves[3] else 0)).all())
     for a in ((x[0], w), (x, w[:4]), (x, w[:, :1]), (x, w, b[:4]), (x, w, b, s[:1]), (x, w, b, s, "gelu")):
         with pytest.raises(ValueError):
             short_conv(*a)

@@ -137,6 +137,16 @@ def test_empty(dev):
     assert y.shape == (0, 4, 8) and s.shape == (0, 8, 4)
 
 
+def test_empty_gradients(dev):
+    """No tokens: the initial state's gradient is the final state's, every other gradient is zero."""
+    args, kw = inputs(dev, 2, 0, 8, 4)
+    leaves = [t.requires_grad_() for t in (*args, *kw.values())]
+    y, s = ssm_scan(*args, **kw)
+    got = torch.autograd.grad((y.sum(), s.sum()), leaves)
+    for x, g in zip(leaves, got):
+        assert g.shape == x.shape and bool((g == (1 if x is kw["initial_state"] else 0)).all())
+
+
 # ---- packed ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("lens", [[1], [5, 0, 33, 1, 64, 100], [0, 0], [300, 2], [3] * 70])
 @pytest.mark.parametrize("G", [1, 2])

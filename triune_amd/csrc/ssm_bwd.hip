@@ -236,12 +236,12 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void ssm_bwd_kernel(SsmB
     float A[NS], Al[NS], e[NS], dA[NS], bias[V], Dv[V], dD[V], db[V];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-        const bool ok = n0 + j < a.N;
+        const bool ok = chv && n0 + j < a.N;  // lanes without a channel add zeros to dB and dC
         A[j] = ok ? a.A[(int64_t)ch * a.N + n0 + j] : 0.f;
         Al[j] = log2_decay(A[j]);
         dA[j] = e[j] = 0.f;
-        if (ok && chv && a.nseg > 1) e[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
-        else if (ok && chv && g.dfin) e[j] = g.dfin[(sg.seq * a.Dm + ch) * a.N + n0 + j];
+        if (ok && a.nseg > 1) e[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
+        else if (ok && g.dfin) e[j] = g.dfin[(sg.seq * a.Dm + ch) * a.N + n0 + j];
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {

@@ -40,7 +40,7 @@ def _forward(x, weight, bias, eps, stats):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
+        y, mean, rstd = _forward(x, weight, bias, eps, True) if x.numel() else (torch.empty_like(x), None, None)
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
@@ -49,6 +49,9 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
+        if mean is None:  # no rows
+            db = None if ctx.bias_dtype is None else torch.zeros(x.shape[-1], device=x.device, dtype=ctx.bias_dtype)
+            return torch.zeros_like(x), None if weight is None else torch.zeros_like(weight), db, None
         rows, up = _flat(x), _flat(dy.to(x.dtype))
         R, D = rows.shape
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
@@ -81,8 +84,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise ValueError("eps must not be negative")
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if x.numel() == 0:
-        return x.clone()
     if _needs_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
+    if x.numel() == 0:
+        return torch.empty_like(x)
     return _forward(x, weight, bias, float(eps), False)[0]

@@ -216,13 +216,23 @@ def _scan_bwd(u, delta, A, B, C, D, z, bias, softplus, kept, dy, dfin, want_s0, 
     return du, dd, dA, dB, dC, dD, dz, db, ds0
 
 
+def _no_tokens(u, N, s0):
+    """The final state of a call without tokens or sequences."""
+    if s0 is None:
+        return torch.zeros(u.shape[0], u.shape[-1], N, device=u.device, dtype=torch.float32)
+    return s0.to(torch.float32).clone()
+
+
 class _SsmScan(torch.autograd.Function):
     """ssm_scan with gradients.  The forward keeps the state of every 32nd token (N / 8 bytes per token
     and channel: 2 beside the 8 of u, delta, z and y in 16 bits at N = 16) as a saved tensor."""
 
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, bias, s0, softplus):
-        y, fin, kept = _scan(u, delta, A, B, C, D, z, bias, softplus, s0, None, True)
+        if u.shape[0] == 0 or u.shape[1] == 0:
+            y, fin, kept = torch.empty_like(u), _no_tokens(u, A.shape[1], s0), None
+        else:
+            y, fin, kept = _scan(u, delta, A, B, C, D, z, bias, softplus, s0, None, True)
         ctx.save_for_backward(u, delta, A, B, C, D, z, bias, kept)
         ctx.softplus, ctx.s0_dtype = softplus, None if s0 is None else s0.dtype
         ctx.set_materialize_grads(False)
@@ -235,6 +245,9 @@ class _SsmScan(torch.autograd.Function):
         if dy is None and dfin is None:
             return (None,) * 10
         want = ctx.s0_dtype is not None and ctx.needs_input_grad[8]
+        if kept is None:  # no tokens: the final state is the initial state
+            zero = [None if t is None else torch.zeros_like(t) for t in (u, delta, A, B, C, D, z, bias)]
+            return (*zero, dfin.to(ctx.s0_dtype) if want and dfin is not None else None, None)
         du, dd, dA, dB, dC, dD, dz, db, ds0 = _scan_bwd(u, delta, A, B, C, D, z, bias, ctx.softplus, kept, dy, dfin,
                                                         want)
         return du, dd, dA, dB, dC, dD, dz, db, ds0.to(ctx.s0_dtype) if want else None, None
@@ -265,12 +278,10 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=
         raise ValueError("out is for calls without gradients")
     if out is not None:
         _one_device(u, out)
-    if Bn == 0 or T == 0:  # nothing to scan: the final state is the initial state
-        s = (torch.zeros(Bn, Dm, N, device=u.device, dtype=torch.float32) if initial_state is None
-             else initial_state.to(torch.float32).clone())
-        return (u.clone() if grad else _out(out, u.shape, u.dtype, u)), s
     if grad:
         return _SsmScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus))
+    if Bn == 0 or T == 0:  # nothing to scan: the final state is the initial state
+        return _out(out, u.shape, u.dtype, u), _no_tokens(u, N, initial_state)
     return _scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state, out, False)[:2]
 
 
@@ -414,10 +425,20 @@ def _conv(x, weight, bias, silu, s0, out):
     return y, fin
 
 
+def _no_conv_tokens(x, W, s0):
+    """The final state of a call without tokens or sequences."""
+    if s0 is None:
+        return torch.zeros(x.shape[0], W - 1, x.shape[-1], device=x.device, dtype=x.dtype)
+    return s0.to(x.dtype).clone()
+
+
 class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, s0, silu):
-        y, fin = _conv(x, weight, bias, silu, s0, None)
+        if x.shape[0] == 0 or x.shape[1] == 0:
+            y, fin = torch.empty_like(x), _no_conv_tokens(x, weight.shape[1], s0)
+        else:
+            y, fin = _conv(x, weight, bias, silu, s0, None)
         ctx.save_for_backward(x, weight, bias, s0)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -431,6 +452,9 @@ class _ShortConv(torch.autograd.Function):
             return (None,) * 5
         Bn, T, Dm = x.shape
         W = weight.shape[1]
+        if Bn == 0 or T == 0:  # the final state is the initial state
+            zero = [None if t is None else torch.zeros_like(t) for t in (x, weight, bias)]
+            return (*zero, None if s0 is None or dfin is None else dfin.to(s0.dtype), None)
         dev = x.device
         xr, wc, bc = _rows(x), weight.contiguous(), _c(bias)
         dy = torch.zeros_like(xr) if dy is None else _rows(dy.to(x.dtype))
@@ -470,12 +494,10 @@ def short_conv(x, weight, bias=None, initial_state=None, activation="silu", out=
         raise ValueError("out is for calls without gradients")
     if out is not None:
         _one_device(x, out)
-    if Bn == 0 or T == 0:
-        s = (torch.zeros(Bn, W - 1, Dm, device=x.device, dtype=x.dtype) if initial_state is None
-             else initial_state.to(x.dtype).clone())
-        return (x.clone() if grad else _out(out, x.shape, x.dtype, x)), s
     if grad:
         return _ShortConv.apply(x, weight, bias, initial_state, silu)
+    if Bn == 0 or T == 0:
+        return _out(out, x.shape, x.dtype, x), _no_conv_tokens(x, W, initial_state)
     return _conv(x, weight, bias, silu, initial_state, out)
 
 
