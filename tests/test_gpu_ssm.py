@@ -117,6 +117,27 @@ def test_extremes(dev):
     check(ssm_scan(*args, **kw), want(args, kw), F32)
 
 
+def test_masked_tokens(dev):
+    """delta of -inf or of the type's lowest value is a step of 0 (the state stays, and gradients), one
+    near the largest forgets all."""
+    for dtype in (F32, BF):
+        args, kw = inputs(dev, 2, 70, 68, 16, dtype=dtype, seed=21)
+        args[1][:, 3] = args[1][:, 64] = float("-inf")
+        args[1][:, 4] = args[1][1, 40:] = torch.finfo(dtype).min
+        args[1][:, 20], args[0][:, 20] = 2e38, 0.0
+        check(ssm_scan(*args, **kw), want(args, kw), dtype)
+        x = [t[:, 3] if t.dim() == 3 else t for t in args]
+        k = {**kw, "z": kw["z"][:, 3]}
+        s0 = k.pop("initial_state")
+        assert torch.equal(ssm_decode_step(*x, s0, **k)[1], s0)
+    args[1][:, 20] = 1.0
+    leaves = [t.requires_grad_() for t in args]
+    y, s = ssm_scan(*leaves, **kw)
+    grads = torch.autograd.grad(y.float().sum() + s.sum(), leaves)
+    assert all(bool(t.isfinite().all()) for t in grads)
+    assert bool((grads[1][:, [3, 4, 64]] == 0).all()) and bool((grads[3][:, [3, 4, 64]] == 0).all())
+
+
 def test_nan_stays_in_its_row(dev):
     """A NaN of one batch row, channel or later token reaches no other row, channel or earlier token."""
     args, kw = inputs(dev, 3, 70, 70, 16, seed=4)

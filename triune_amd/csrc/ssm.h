@@ -168,7 +168,7 @@ __device__ __forceinline__ float softplus(float x) {
     p = __builtin_fmaf(p, t, 0.40024852752685547f);
     p = __builtin_fmaf(p, t, 0.6666631698608398f);
     p = __builtin_fmaf(p, t, 2.0f);
-    return __builtin_fmaf(s, p, 0.5f * (x + fabsf(x)));  // max(x, 0) without fmaxf's second max for NaN
+    return __builtin_fmaf(s, p, __builtin_amdgcn_fmed3f(x, 0.f, __builtin_inff()));  // max(x, 0); s carries a NaN
 }
 
 // N elements of any alignment in one access (the memory pipeline takes unaligned vectors), or the
