@@ -500,7 +500,7 @@ int triune_hip_ssm_decode_step(const void* u, const void* delta, const void* z, 
  *     p_t = bias + sum_j w[d, j] x[t - W + 1 + j],  y = silu(p) when `silu`, else p
  * x, y [Bn, T, Dm] in io_dtype (strides[4] = (batch, token) of x, y); w [Dm, W] and bias [Dm] (or
  * NULL) contiguous in w_dtype (io_dtype or fp32).  s0: the W - 1 tokens before the first, [Bn, W - 1, Dm] contiguous in
- * io_dtype (NULL: zeros); s_final (or NULL): the last W - 1 after the call, laid out the same. */
+ * io_dtype (NULL: zeros); s_final (or NULL): the last W - 1 after the call, laid out the same, not over s0. */
 int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io_dtype, int w_dtype,
                           const int64_t* strides, int silu, const void* s0, void* s_final, void* y, int64_t Bn,
                           int64_t T, int64_t Dm, int W, void* stream);

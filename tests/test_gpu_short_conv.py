@@ -197,3 +197,11 @@ def test_empty_and_refusals(dev):
         short_conv_varlen(x[:1], w, cu, state_pool=s)
     with pytest.raises(ValueError, match="gradient"):
         short_conv_varlen(x[:1], w.clone().requires_grad_(), cu)
+
+
+def test_pools_that_want_gradients_are_refused(dev):
+    x, w = torch.zeros(8, 6, device=dev), torch.zeros(6, 4, device=dev)
+    cu, slots = torch.tensor([0, 8], dtype=torch.int32, device=dev), torch.tensor([0], dtype=torch.int32, device=dev)
+    pool = torch.zeros(2, 3, 6, device=dev, requires_grad=True)
+    with pytest.raises(ValueError):
+        short_conv_varlen(x, w, cu, state_pool=pool, slots=slots)

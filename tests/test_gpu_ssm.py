@@ -507,3 +507,15 @@ def test_refusals(dev):
         ssm_decode_step(*step, pool[:2].half(), inplace=True)
     with pytest.raises(ValueError):
         ssm_decode_step(*step, pool.transpose(1, 2)[:2])
+
+
+def test_pools_that_want_gradients_are_refused(dev):
+    """A pool is written in place, without a gradient."""
+    args, kw = inputs(dev, 1, 8, 8, 4)
+    packed = [t[0] if t.dim() == 3 else t for t in args]
+    cu, slots = torch.tensor([0, 8], dtype=torch.int32, device=dev), torch.tensor([0], dtype=torch.int32, device=dev)
+    pool = torch.zeros(2, 8, 4, device=dev, requires_grad=True)
+    with pytest.raises(ValueError):
+        ssm_scan_varlen(*packed, cu, state_pool=pool, slots=slots)
+    with torch.no_grad():
+        assert ssm_scan_varlen(*packed, cu, state_pool=pool, slots=slots)[1] is pool

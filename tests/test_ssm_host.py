@@ -149,3 +149,20 @@ def test_operators_refuse_cpu_tensors():
         triune_amd.layer_norm(x)
     with pytest.raises(ValueError, match="CPU"):
         triune_amd.ssm_scan(x, x, w, torch.zeros(1, 4, 4), torch.zeros(1, 4, 4))
+
+
+def test_counts_past_the_plans_numbers():
+    """Counts whose products with channels or tokens pass 64 bits are refused, not multiplied."""
+    lib, many = L.lib(), 1 << 60
+    for call in (caller("triune_hip_ssm_scan", SCAN, **_scan_base(SCAN)),
+                 caller("triune_hip_ssm_bwd", BWD, **_scan_base(BWD)),
+                 caller("triune_hip_short_conv", CONV, **_conv_base(CONV)),
+                 caller("triune_hip_short_conv_bwd", CONV_B, **_conv_base(CONV_B))):
+        assert call(Bn=many) == SHAPE
+    for call in (caller("triune_hip_ssm_scan_varlen", VARLEN, **_scan_base(VARLEN)),
+                 caller("triune_hip_short_conv_varlen", CONV_V, **_conv_base(CONV_V))):
+        assert call(n=many, rows=many) == SHAPE
+    assert lib.triune_hip_ssm_scan_workspace_size(many, 64, 64, 1, 16, 0) == 0
+    assert lib.triune_hip_ssm_bwd_workspace_size(many, 64, 64, 1, 16, 0) == 0
+    assert lib.triune_hip_ssm_scan_varlen_workspace_size(many, 64, 64, 1, 16, 0) == 0
+    assert lib.triune_hip_short_conv_bwd_workspace_size(many, 64, 64, 4) == 0

@@ -40,14 +40,15 @@ bool strides_ok(std::initializer_list<int64_t> st) {
     return true;
 }
 
+// Sequences and tokens within the numbers that the plans multiply.
+bool tokens_ok(int64_t n, int64_t T) { return n >= 0 && n <= kMaxGrid && T >= 0 && T < (1 << 30); }
+
 bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
     return Dm > 0 && Dm < kMaxTokenStride && G > 0 && Dm % G == 0 && N > 0 && N <= SSM_MAX_N;
 }
 // Workgroups that the channels of one group take, of all groups.
-int64_t group_blocks(int64_t Dm, int64_t G, int N) {
-    return (Dm / G + 63) / 64;
-}
-int64_t all_blocks(int64_t Dm, int64_t G, int N) { return G * group_blocks(Dm, G, N); }
+int64_t group_blocks(int64_t Dm, int64_t G) { return (Dm / G + 63) / 64; }
+int64_t all_blocks(int64_t Dm, int64_t G) { return G * group_blocks(Dm, G); }
 
 // Waves a compute unit (four SIMDs) that a call has without splitting the time axis for that to be left,
 // and that it gets where it is split.  Two waves on a SIMD keep it three quarters busy; splitting costs the
@@ -90,7 +91,7 @@ void plan_bytes(ScanPlan& p, int64_t Dm, int N, int64_t n_off) {
 
 ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int flags, int64_t least) {
     ScanPlan p{};
-    p.seg = dense_segment(n_seqs, T, all_blocks(Dm, G, N), N, flags, least);
+    p.seg = dense_segment(n_seqs, T, all_blocks(Dm, G), N, flags, least);
     p.nseg = (T + p.seg - 1) / p.seg;
     p.n_work = n_seqs * p.nseg;
     plan_bytes(p, Dm, N, 0);
@@ -101,7 +102,7 @@ ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int 
 // sequences enough for two rounds of the chip.  nseg > 1 says that there are segments.
 ScanPlan plan_packed(int64_t n_seqs, int64_t total, int64_t Dm, int64_t G, int N, int flags) {
     ScanPlan p{};
-    const int64_t whole = (total + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT, blocks = all_blocks(Dm, G, N);
+    const int64_t whole = (total + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT, blocks = all_blocks(Dm, G);
     const int64_t slots = ssm_slots(N, kSplitWaves);
     p.seg = forced_segment(flags);
     if (!p.seg) {
@@ -124,7 +125,7 @@ BwdPlan plan_bwd(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags)
     BwdPlan p{};
     p.s = plan_scan(Bn, T, Dm, G, N, flags, 2);
     p.off_bc = p.s.total;
-    p.off_par = p.off_bc + align_up((size_t)all_blocks(Dm, G, N) * Bn * T * ssm_waves(N) * 8 * 4);
+    p.off_par = p.off_bc + align_up((size_t)all_blocks(Dm, G) * Bn * T * ssm_waves(N) * 8 * 4);
     p.total = p.off_par + align_up((size_t)p.s.n_work * (N + 2) * Dm * 4);
     return p;
 }
@@ -135,7 +136,7 @@ void set_sizes(SsmParams& a, int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, i
     a.Dm = (int)Dm;
     a.G = (int)G;
     a.N = N;
-    a.blocks = (int)group_blocks(Dm, G, N);
+    a.blocks = (int)group_blocks(Dm, G);
     a.seg = (int)p.seg;
     a.nseg = (int)p.nseg;
     a.n_work = p.n_work;
@@ -162,7 +163,7 @@ bool all_aligned(int dt, std::initializer_list<const void*> ps) {
 extern "C" {
 
 size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags) {
-    if (Bn <= 0 || T <= 0 || T >= (1 << 30) || !ssm_shape_ok(Dm, G, N)) return 0;
+    if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || !ssm_shape_ok(Dm, G, N)) return 0;
     return plan_scan(Bn, T, Dm, G, N, flags, 3).total;
 }
 
@@ -172,7 +173,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
                         int64_t G, int N, int flags, void* workspace, size_t workspace_bytes, void* stream) {
     if (!u || !delta || !B || !C || !A || !y || !strides) return TRIUNE_ERR_NULL;
     if (!dtype_ok(io_dtype)) return TRIUNE_ERR_DTYPE;
-    if (Bn < 0 || T < 0 || T >= (1 << 30) || !ssm_shape_ok(Dm, G, N)) return TRIUNE_ERR_SHAPE;
+    if (!tokens_ok(Bn, T) || !ssm_shape_ok(Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (!all_aligned(io_dtype, {u, delta, z, B, C, y}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, s0, s_final, kept}))
         return TRIUNE_ERR_LAYOUT;
@@ -180,7 +181,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
         return TRIUNE_ERR_LAYOUT;
     if (Bn == 0 || T == 0) return TRIUNE_OK;
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags, 3);
-    if (p.n_work > kMaxGrid / all_blocks(Dm, G, N) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (p.n_work > kMaxGrid / all_blocks(Dm, G) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, strides[0], strides[1]};
@@ -202,7 +203,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
 
 size_t triune_hip_ssm_scan_varlen_workspace_size(int64_t n_seqs, int64_t total_tokens, int64_t Dm, int64_t G, int N,
                                                  int flags) {
-    if (n_seqs <= 0 || total_tokens <= 0 || total_tokens >= (1 << 30) || !ssm_shape_ok(Dm, G, N)) return 0;
+    if (n_seqs <= 0 || total_tokens <= 0 || !tokens_ok(n_seqs, total_tokens) || !ssm_shape_ok(Dm, G, N)) return 0;
     return plan_packed(n_seqs, total_tokens, Dm, G, N, flags).total;
 }
 
@@ -214,8 +215,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
                                void* workspace, size_t workspace_bytes, void* stream) {
     if (!u || !delta || !B || !C || !A || !y || !strides || !cu_seqlens) return TRIUNE_ERR_NULL;
     if (!dtype_ok(io_dtype)) return TRIUNE_ERR_DTYPE;
-    if (n_seqs < 0 || total_tokens < 0 || total_tokens >= (1 << 30) || n_state_rows < 0 || !ssm_shape_ok(Dm, G, N))
-        return TRIUNE_ERR_SHAPE;
+    if (!tokens_ok(n_seqs, total_tokens) || n_state_rows < 0 || !ssm_shape_ok(Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (!slots && (s0 || s_final) && n_state_rows < n_seqs) return TRIUNE_ERR_SHAPE;
     if (!all_aligned(io_dtype, {u, delta, z, B, C, y}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, s0, s_final, cu_seqlens, slots}))
@@ -225,7 +225,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
     if (n_seqs == 0) return TRIUNE_OK;
     // with no tokens every sequence's state still passes through: one empty segment each
     const ScanPlan p = plan_packed(n_seqs, total_tokens > 0 ? total_tokens : 1, Dm, G, N, flags);
-    if (p.n_work > kMaxGrid / all_blocks(Dm, G, N) || n_seqs > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (p.n_work > kMaxGrid / all_blocks(Dm, G) || n_seqs > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, 0, strides[0]};
@@ -249,7 +249,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
 }
 
 size_t triune_hip_ssm_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags) {
-    if (Bn <= 0 || T <= 0 || T >= (1 << 30) || !ssm_shape_ok(Dm, G, N)) return 0;
+    if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || !ssm_shape_ok(Dm, G, N)) return 0;
     return plan_bwd(Bn, T, Dm, G, N, flags).total;
 }
 
@@ -262,13 +262,13 @@ int triune_hip_ssm_bwd(const void* u, const void* delta, const void* z, const vo
     if (!u || !delta || !B || !C || !A || !dy || !strides || !kept || !du || !ddelta || (z && !dz) || !dB || !dC || !dA)
         return TRIUNE_ERR_NULL;
     if (!dtype_ok(io_dtype)) return TRIUNE_ERR_DTYPE;
-    if (Bn <= 0 || T <= 0 || T >= (1 << 30) || !ssm_shape_ok(Dm, G, N)) return TRIUNE_ERR_SHAPE;
+    if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || !ssm_shape_ok(Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (!all_aligned(io_dtype, {u, delta, z, B, C, dy, du, ddelta, dz, dB, dC}) ||
         !all_aligned(TRIUNE_DT_F32, {A, D, delta_bias, kept, ds_final, dA, dD, ddelta_bias, ds0}))
         return TRIUNE_ERR_LAYOUT;
     if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]})) return TRIUNE_ERR_LAYOUT;
     const BwdPlan p = plan_bwd(Bn, T, Dm, G, N, flags);
-    if (p.s.n_work > kMaxGrid / all_blocks(Dm, G, N) || Bn > kMaxGrid / (Dm * N) || Bn * T > kMaxGrid / (G * N))
+    if (p.s.n_work > kMaxGrid / all_blocks(Dm, G) || Bn > kMaxGrid / (Dm * N) || Bn * T > kMaxGrid / (G * N))
         return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     char* ws = (char*)workspace;
@@ -330,7 +330,7 @@ static int conv_check(const void* x, const void* w, const void* bias, const void
                       int W) {
     if (!x || !w || !y || !strides) return TRIUNE_ERR_NULL;
     if (!dtype_ok(io_dtype) || (w_dtype != io_dtype && w_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
-    if (n < 0 || T < 0 || T >= (1 << 30) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return TRIUNE_ERR_SHAPE;
+    if (!tokens_ok(n, T) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return TRIUNE_ERR_SHAPE;
     if (!all_aligned(io_dtype, {x, y, s0, fin}) || !all_aligned(w_dtype, {w, bias})) return TRIUNE_ERR_LAYOUT;
     // runs of 16 tokens x four channels, and (sequence, four channels) pairs, are numbered in 31 bits
     if (n > 0 && (Dm + 3) / 4 > kMaxGrid / (n * ((T + 15) / 16 + 1))) return TRIUNE_ERR_SHAPE;
@@ -391,7 +391,7 @@ int triune_hip_short_conv_decode_step(const void* x, const void* w, const void* 
 }
 
 size_t triune_hip_short_conv_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int W) {
-    if (Bn <= 0 || T <= 0 || T >= (1 << 30) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return 0;
+    if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return 0;
     const int run = conv_bwd_run(Bn, T, (int)Dm, compute_units());
     return align_up((size_t)conv_bwd_parts(Bn, T, (int)Dm, run) * (W + 1) * Dm * 4);
 }

@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void conv_state_kernel(ConvParams a) {
     }
 }
 
-// One token for every row.  One thread per (row, VEC channels).
+// One token for every row.  One thread per (row, four channels).
 template <typename T, int W>
 __global__ __launch_bounds__(256) void conv_step_kernel(ConvParams a) {
     const int64_t groups = (a.Dm + E - 1) / E, id = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -218,11 +218,6 @@ __device__ __forceinline__ float sum_parts(const float* p, int64_t st, int64_t f
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-__device__ __forceinline__ float load_dt(const void* p, int dt, int64_t i) {
-    if (dt == DT_F32) return ((const float*)p)[i];
-    if (dt == DT_BF16) return (float)((const __bf16*)p)[i];
-    return (float)((const _Float16*)p)[i];
-}
 __device__ __forceinline__ void store_dt(void* p, int dt, int64_t i, float x) {
     if (dt == DT_F32) ((float*)p)[i] = x;
     else if (dt == DT_BF16) ((__bf16*)p)[i] = (__bf16)x;

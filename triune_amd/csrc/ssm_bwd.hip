@@ -142,39 +142,6 @@ __global__ __launch_bounds__(64 * NW) void ssm_bwd_states_kernel(SsmBwdParams g)
     }
 }
 
-// The scan over segments from the last: each one's own gradient at its start is replaced by the
-// gradient that enters at its end; what leaves the first segment is the initial state's gradient.
-__global__ __launch_bounds__(256) void ssm_bwd_carry_kernel(SsmBwdParams g) {
-    const SsmParams& a = g.f;
-    const int64_t per = (int64_t)a.N * a.Dm, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.n_seqs * per) return;
-    const int64_t seq = id / per;
-    const int n = (int)((id - seq * per) / a.Dm), ch = (int)((id - seq * per) % a.Dm);
-    const float Al = log2_decay(a.A[(int64_t)ch * a.N + n]);
-    const int64_t at = (seq * a.Dm + ch) * a.N + n;
-    float E = g.dfin ? g.dfin[at] : 0.f;
-    const int64_t w0 = seq * a.nseg;
-    float* p = a.ws_state + (int64_t)n * a.Dm + ch;
-    const float* ps = a.ws_sum + ch;
-    constexpr int AHEAD = 8;  // segments whose loads are in flight together
-    for (int64_t w = w0 + a.nseg - 1; w >= w0; w -= AHEAD) {
-        float local[AHEAD], sum[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int64_t v = max(w - i, w0);
-            local[i] = p[v * per];
-            sum[i] = ps[v * a.Dm];
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (w - i < w0) break;
-            p[(w - i) * per] = E;
-            E = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[i] * Al), E, local[i]);
-        }
-    }
-    if (g.ds0) g.ds0[at] = E;
-}
-
 // The sums over a wave's lanes of v[0..8), by halving exchanges: a level leaves half of the values to each
 // half of the lanes.  Lane l holds the one of value l / 8.
 __device__ __forceinline__ float lanes_sum8(const float (&v)[8]) {
@@ -201,7 +168,7 @@ __device__ __forceinline__ float lanes_sum8(const float (&v)[8]) {
 __device__ __forceinline__ void reread() { asm volatile("" ::: "memory"); }
 
 template <typename T, int NW, int V>
-__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : 2) void ssm_bwd_kernel(SsmBwdParams g) {
+__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : NW == 1 ? 1 : 2) void ssm_bwd_kernel(SsmBwdParams g) {
     const SsmParams& a = g.f;
     constexpr int NS = 4, NT = 64 * NW, TT = NW == 16 ? 16 : 32, LPR = 64 / V, TS = NT / LPR;  // TT: ssm_kept_every
     constexpr int K = (TT + TS - 1) / TS, KB = TT * 4 * NW / NT, ES = sizeof(T);
@@ -533,12 +500,6 @@ hipError_t launch_ssm_bwd(const SsmBwdParams& g, int dt, hipStream_t s) {
     if (dt == DT_F32) return v4 ? bwd_waves<float, 4>(g, s) : bwd_waves<float, 1>(g, s);
     if (dt == DT_BF16) return v4 ? bwd_waves<__bf16, 4>(g, s) : bwd_waves<__bf16, 1>(g, s);
     return v4 ? bwd_waves<_Float16, 4>(g, s) : bwd_waves<_Float16, 1>(g, s);
-}
-
-hipError_t launch_ssm_bwd_carry(const SsmBwdParams& g, hipStream_t s) {
-    const int64_t n = g.f.n_seqs * g.f.N * g.f.Dm;
-    ssm_bwd_carry_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(g);
-    return hipGetLastError();
 }
 
 hipError_t launch_ssm_bwd_sum(const SsmBwdParams& g, int dt, hipStream_t s) {

@@ -296,7 +296,7 @@ def ssm_scan_varlen(u, delta, A, B, C, cu_seqlens, D=None, z=None, delta_bias=No
     sequence i starts from state_pool[slots[i]] and leaves its final state there, and the second
     item returned is state_pool; a slot outside the pool (-1 for a padded row) starts from zero and
     keeps nothing."""
-    _no_grad_path("ssm_scan_varlen", u, delta, A, B, C, D, z, delta_bias, initial_state)
+    _no_grad_path("ssm_scan_varlen", u, delta, A, B, C, D, z, delta_bias, initial_state, state_pool)
     lead1 = u.dim() == 3
     if lead1:
         if u.shape[0] != 1:
@@ -506,7 +506,7 @@ def short_conv_varlen(x, weight, cu_seqlens, bias=None, initial_state=None, acti
     """short_conv over packed ragged prompts x [N, channels] or [1, N, channels], without gradients;
     cu_seqlens, initial_state [n, W - 1, channels], state_pool [rows, W - 1, channels] in x's
     dtype, slots and the returned pair as in ssm_scan_varlen."""
-    _no_grad_path("short_conv_varlen", x, weight, bias, initial_state)
+    _no_grad_path("short_conv_varlen", x, weight, bias, initial_state, state_pool)
     lead1 = x.dim() == 3
     if lead1:
         if x.shape[0] != 1 or (out is not None and (out.dim() != 3 or out.shape[0] != 1)):
