@@ -352,6 +352,7 @@ int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io
     if (Bn == 0 || T == 0) return TRIUNE_OK;
     ConvParams a = conv_params(x, w, bias, w_dtype, silu, s0, s_final, y, Bn, T, Dm, W);
     a.x_sb = strides[0], a.x_st = strides[1], a.y_sb = strides[2], a.y_st = strides[3];
+    a.run = conv_run(Bn, T, (int)Dm, compute_units());
     return status(launch_conv(a, io_dtype, (hipStream_t)stream));
 }
 
@@ -367,6 +368,7 @@ int triune_hip_short_conv_varlen(const void* x, const void* w, const void* bias,
     if (n_seqs == 0) return TRIUNE_OK;
     ConvParams a = conv_params(x, w, bias, w_dtype, silu, s0, s_final, y, n_seqs, total_tokens, Dm, W);
     a.x_st = strides[0], a.y_st = strides[1];
+    a.run = conv_run(1, total_tokens, (int)Dm, compute_units());
     a.cu = cu_seqlens, a.slots = slots, a.n_slots = n_state_rows;
     const hipStream_t s = (hipStream_t)stream;
     if (total_tokens > 0)
@@ -392,7 +394,7 @@ int triune_hip_short_conv_decode_step(const void* x, const void* w, const void* 
 
 size_t triune_hip_short_conv_bwd_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int W) {
     if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || Dm <= 0 || Dm >= (1 << 28) || W < 2 || W > 4) return 0;
-    const int run = conv_bwd_run(Bn, T, (int)Dm, compute_units());
+    const int run = conv_run(Bn, T, (int)Dm, compute_units());
     return align_up((size_t)conv_bwd_parts(Bn, T, (int)Dm, run) * (W + 1) * Dm * 4);
 }
 
@@ -409,8 +411,8 @@ int triune_hip_short_conv_bwd(const void* x, const void* w, const void* bias, co
     g.f.x_sb = strides[0], g.f.x_st = strides[1];
     g.dy = dy, g.dy_sb = strides[2], g.dy_st = strides[3];
     g.dfin = ds_final, g.dx = dx, g.ds0 = ds0;
-    g.run = conv_bwd_run(Bn, T, (int)Dm, compute_units());
-    g.parts = conv_bwd_parts(Bn, T, (int)Dm, g.run);
+    g.f.run = conv_run(Bn, T, (int)Dm, compute_units());
+    g.parts = conv_bwd_parts(Bn, T, (int)Dm, g.f.run);
     if (dw || dbias) {
         if (const int e = check_ws(workspace, workspace_bytes, triune_hip_short_conv_bwd_workspace_size(Bn, T, Dm, W)))
             return e;

@@ -5,9 +5,10 @@
 //     y_t = silu(p_t) or p_t
 // Bound by memory: every value is read and written once.  A thread owns four channels (a wave's access
 // is whole cache lines) and walks a run of tokens with the last W - 1 of them in registers, so a
-// token is read again only as the next run's first W - 1.  Four channels and two tokens of loads in flight:
-// 4 x 16384 tokens of 768 channels (W = 4, bf16) in 61 us (3.3 TB/s), against 73 with eight channels
-// and four tokens, whose registers leave three waves on a SIMD.
+// token is read again only as the next run's first W - 1.  Whole runs inside a sequence load the next two tokens
+// before they work on two and have no condition around an access; the others go token by token.
+// 4 x 16384 tokens of 768 channels (W = 4, bf16): 47 us (4.3 TB/s), 61 with the conditions in the loop; forward and
+// gradients of 8 x 2048 tokens of 1536 channels 86 us, 102 with them (93 with one token ahead, 98 with four).
 #include "ssm.h"
 
 namespace triune {
@@ -15,7 +16,6 @@ namespace triune {
 namespace {
 
 constexpr int E = 4;     // channels of a thread
-constexpr int RUN = 16;  // tokens of a forward run: a halo of 3 in 16, and runs enough for short prompts
 constexpr int STEP = 2;  // tokens whose loads are in flight together
 
 // Lanes along the channels (a power of two, at most a wave): the rest of the block takes further runs.
@@ -65,18 +65,32 @@ __device__ __forceinline__ Raw<T, E> state_row(const ConvParams& a, int64_t row,
 
 }  // namespace
 
+// A token's outputs p from its inputs x and the window of the W - 1 before it, which moves on.
+template <int W>
+__device__ __forceinline__ void taps(const Taps<W>& k, float (&win)[W - 1][E], const float (&x)[E], float (&p)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        p[e] = __builtin_fmaf(k.w[W - 1][e], x[e], k.b[e]);
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) p[e] = __builtin_fmaf(k.w[j][e], win[j][e], p[e]);
+#pragma unroll
+        for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
+        win[W - 2][e] = x[e];
+    }
+}
+
 template <typename T, int W, bool PACKED>
 __global__ __launch_bounds__(256) void conv_kernel(ConvParams a, int cl, int cblocks) {
     const int lc = threadIdx.x & (cl - 1), rl = threadIdx.x / cl, runs_pb = 256 / cl;
-    const int64_t rb = blockIdx.x / cblocks;
+    const uint32_t rb = blockIdx.x / (uint32_t)cblocks;
     const int c = ((int)(blockIdx.x - rb * cblocks) * cl + lc) * E;
     const int n = min(a.Dm - c, E);
     if (n <= 0) return;
-    const int64_t run = rb * runs_pb + rl, per = (a.T + RUN - 1) / RUN;
+    const uint32_t run = rb * runs_pb + rl, per = (uint32_t)((a.T + a.run - 1) / a.run);
     int64_t seq, t0, t1, beg, end;  // tokens t0 .. t1 - 1; the sequence that holds t0 is beg .. end - 1
     if constexpr (PACKED) {
-        t0 = run * RUN;
-        t1 = min(t0 + RUN, min((int64_t)a.cu[a.n_seqs], a.T));
+        t0 = (int64_t)run * a.run;
+        t1 = min(t0 + a.run, min((int64_t)a.cu[a.n_seqs], a.T));
         t0 = max(t0, max((int64_t)a.cu[0], (int64_t)0));
         if (t0 >= t1) return;
         int64_t lo = 0, hi = a.n_seqs;  // cu[lo] <= t0 < cu[hi]
@@ -90,8 +104,8 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams a, int cl, int cbl
     } else {
         seq = run / per;
         if (seq >= a.n_seqs) return;
-        t0 = (run - seq * per) * RUN;
-        t1 = min(t0 + RUN, a.T);
+        t0 = (int64_t)(run - (uint32_t)seq * per) * a.run;
+        t1 = min(t0 + a.run, a.T);
         beg = 0;
         end = a.T;
     }
@@ -109,31 +123,54 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams a, int cl, int cbl
         }
     };
     window(t0);
-    for (int64_t t = t0; t < t1; t += STEP) {
+    if (n == E && t1 - t0 == a.run && t1 <= end) {
+        // A whole run of one sequence: no access depends on a condition, which would make the compiler wait for
+        // loads where it joins their registers.
+        const T* p = px + t0 * a.x_st;
+        T* q = py + t0 * a.y_st;
         Raw<T, E> r[STEP];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) r[i] = load_raw<E>(px + (t + i) * a.x_st, t + i < t1 ? n : 0);
+        for (int i = 0; i < STEP; ++i) r[i] = load_raw<E>(p + i * a.x_st, E);
+#pragma unroll 1
+        for (int t = 0; t < a.run; t += STEP) {
+            float o[STEP][E];
+            const int64_t ahead = t + STEP < a.run ? STEP * a.x_st : 0;  // the last step's loads are its own again
+            p += ahead;
+            Raw<T, E> next[STEP];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) {
-            if (t + i >= t1) break;
-            if (PACKED && t + i >= end) {  // the next sequence that holds tokens
-                while (t + i >= end && seq + 1 < a.n_seqs) end = a.cu[++seq + 1];
+            for (int i = 0; i < STEP; ++i) next[i] = load_raw<E>(p + i * a.x_st, E);
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) {
+                float x[E];
+                widen(r[i], x);
+                taps<W>(k, win, x, o[i]);
+                r[i] = next[i];
+            }
+            if (a.silu) {
+#pragma unroll
+                for (int i = 0; i < STEP; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[i][e] = silu_gate(o[i][e]);
+            }
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) store_raw<E>(q + i * a.y_st, E, o[i]);
+            q += STEP * a.y_st;
+        }
+    } else {
+        for (int64_t t = t0; t < t1; ++t) {
+            if (PACKED && t >= end) {  // the next sequence that holds tokens
+                while (t >= end && seq + 1 < a.n_seqs) end = a.cu[++seq + 1];
                 beg = max((int64_t)a.cu[seq], (int64_t)0);
-                window(t + i);
+                window(t);
             }
-            float x[E], y[E];
-            widen(r[i], x);
+            float x[E], o[E];
+            widen(load_raw<E>(px + t * a.x_st, n), x);
+            taps<W>(k, win, x, o);
+            if (a.silu) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float p = __builtin_fmaf(k.w[W - 1][e], x[e], k.b[e]);
-#pragma unroll
-                for (int j = 0; j < W - 1; ++j) p = __builtin_fmaf(k.w[j][e], win[j][e], p);
-                y[e] = a.silu ? silu_gate(p) : p;
-#pragma unroll
-                for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
-                win[W - 2][e] = x[e];
+                for (int e = 0; e < E; ++e) o[e] = silu_gate(o[e]);
             }
-            store_raw<E>(py + (t + i) * a.y_st, n, y);
+            store_raw<E>(py + t * a.y_st, n, o);
         }
     }
     if (!PACKED && a.fin && t1 == a.T) {
@@ -210,10 +247,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
     const ConvParams& a = g.f;
     __shared__ float s_red[256][E + 1];
     const int lc = threadIdx.x & (cl - 1), rl = threadIdx.x / cl, runs_pb = 256 / cl;
-    const int64_t rb = blockIdx.x / cblocks;
+    const uint32_t rb = blockIdx.x / (uint32_t)cblocks;
     const int c = ((int)(blockIdx.x - rb * cblocks) * cl + lc) * E;
     const int n = min(a.Dm - c, E);
-    const int64_t run = rb * runs_pb + rl, per = (a.T + g.run - 1) / g.run;
+    const uint32_t run = rb * runs_pb + rl, per = (uint32_t)((a.T + a.run - 1) / a.run);
     const int64_t seq = run / per;
     float dw[W + 1][E];  // dw, then dbias
 #pragma unroll
@@ -221,9 +258,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
 #pragma unroll
         for (int e = 0; e < E; ++e) dw[j][e] = 0.f;
     if (n > 0 && seq < a.n_seqs) {
-        const int64_t t0 = (run - seq * per) * g.run, t1 = min(t0 + g.run, a.T);
-        // the gradients of t0 .. t1 - 1, before them the state's rows (first run)
-        const int64_t from = t0 == 0 ? -(W - 1) : t0;
+        const int64_t t0 = (int64_t)(run - (uint32_t)seq * per) * a.run, t1 = min(t0 + a.run, a.T), stop = t1 + W - 1;
         const T* px = (const T*)a.x + seq * a.x_sb + c;
         const T* py = (const T*)g.dy + seq * g.dy_sb + c;
         T* pd = (T*)g.dx + seq * a.T * a.Dm + c;
@@ -240,65 +275,92 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
         for (int i = 0; i < W; ++i)
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
-        const int64_t stop = t1 + W - 1;
-        for (int64_t t = t0; t < stop; t += STEP) {
-            Raw<T, E> rx[STEP], ry[STEP];
+        // Takes a token in (own: of this run, whose dw it adds to; in: of the sequence) and its dp to acc, of which acc[0] is whole then.
+        auto token = [&](const Raw<T, E>& rx, const Raw<T, E>& ry, bool own, bool in, float (&out)[E]) {
+            float x[E], dp[E], p[E], old[W - 1][E];
+            widen(rx, x);
+            widen(ry, dp);
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-                const int m = t + i < stop && t + i < a.T ? n : 0;
-                rx[i] = load_raw<E>(px + (t + i) * a.x_st, m);
-                ry[i] = load_raw<E>(py + (t + i) * g.dy_st, m);
+            for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+                for (int e = 0; e < E; ++e) old[j][e] = win[j][e];
+            taps<W>(k, win, x, p);
+            if (a.silu) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float s = fast_sigmoid(p[e]);
+                    dp[e] *= s * __builtin_fmaf(p[e], 1.f - s, 1.f);
+                }
             }
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-                const int64_t tt = t + i;
-                if (tt >= stop) break;
-                float x[E], dy[E];
-                widen(rx[i], x);
-                widen(ry[i], dy);
-                const bool own = tt < t1;
+            for (int e = 0; e < E; ++e) {
+                if (!in) dp[e] = 0.f;
+                if (own) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    float dp = dy[e];
-                    if (a.silu) {
-                        float p = __builtin_fmaf(k.w[W - 1][e], x[e], k.b[e]);
-#pragma unroll
-                        for (int j = 0; j < W - 1; ++j) p = __builtin_fmaf(k.w[j][e], win[j][e], p);
-                        const float s = sigmoid(p);
-                        dp *= s * __builtin_fmaf(p, 1.f - s, 1.f);
-                    }
-                    if (tt >= a.T) dp = 0.f;
-#pragma unroll
-                    for (int j = 0; j < W; ++j) acc[j][e] = __builtin_fmaf(k.w[j][e], dp, acc[j][e]);
-                    const float d = own ? dp : 0.f;
-#pragma unroll
-                    for (int j = 0; j < W - 1; ++j) dw[j][e] = __builtin_fmaf(d, win[j][e], dw[j][e]);
-                    dw[W - 1][e] = __builtin_fmaf(d, x[e], dw[W - 1][e]);
-                    dw[W][e] += d;
-#pragma unroll
-                    for (int j = 0; j < W - 2; ++j) win[j][e] = win[j + 1][e];
-                    win[W - 2][e] = x[e];
+                    for (int j = 0; j < W - 1; ++j) dw[j][e] = __builtin_fmaf(dp[e], old[j][e], dw[j][e]);
+                    dw[W - 1][e] = __builtin_fmaf(dp[e], x[e], dw[W - 1][e]);
+                    dw[W][e] += dp[e];
                 }
-                const int64_t s = tt - (W - 1);  // acc[0] is its whole gradient
-                if (s >= from) {
+                out[e] = __builtin_fmaf(k.w[0][e], dp[e], acc[0][e]);
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) acc[j][e] = __builtin_fmaf(k.w[j + 1][e], dp[e], acc[j + 1][e]);
+                acc[W - 1][e] = 0.f;
+            }
+        };
+        if (n == E && t0 > 0 && t1 - t0 == a.run && stop <= a.T) {
+            // a whole run within the sequence, as in the forward: no access depends on a condition but the first
+            // W - 1 stores, whose tokens are the run's before
+            px += t0 * a.x_st;
+            py += t0 * g.dy_st;
+            pd += (t0 - (W - 1)) * a.Dm;
+            Raw<T, E> rx[STEP], ry[STEP];
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) rx[i] = load_raw<E>(px + i * a.x_st, E), ry[i] = load_raw<E>(py + i * g.dy_st, E);
+#pragma unroll 1
+            for (int t = 0; t < a.run; t += STEP) {
+                px += STEP * a.x_st;
+                py += STEP * g.dy_st;
+                Raw<T, E> nx[STEP], ny[STEP];
+#pragma unroll
+                for (int i = 0; i < STEP; ++i) {  // behind the run: its W - 1 tokens
+                    const int j = t + STEP < a.run || i < W - 1 ? i : 0;
+                    nx[i] = load_raw<E>(px + j * a.x_st, E);
+                    ny[i] = load_raw<E>(py + j * g.dy_st, E);
+                }
+#pragma unroll
+                for (int i = 0; i < STEP; ++i) {
                     float out[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) out[e] = acc[0][e];
-                    if (g.dfin && s >= a.T - (W - 1)) {
-                        float f[E];
-                        widen(load_raw<E>((const T*)g.dfin + (seq * (W - 1) + s - (a.T - (W - 1))) * a.Dm + c, n), f);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) out[e] += f[e];
-                    }
-                    if (s >= 0) store_raw<E>(pd + s * a.Dm, n, out);
-                    else if (g.ds0) store_raw<E>((T*)g.ds0 + (seq * (W - 1) + s + W - 1) * a.Dm + c, n, out);
+                    token(rx[i], ry[i], true, true, out);
+                    if (t + i >= W - 1) store_raw<E>(pd, E, out);
+                    pd += a.Dm;
+                    rx[i] = nx[i];
+                    ry[i] = ny[i];
                 }
+            }
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
+            for (int i = 0; i < W - 1; ++i) {
+                if (i >= STEP) rx[i % STEP] = load_raw<E>(px + i * a.x_st, E), ry[i % STEP] = load_raw<E>(py + i * g.dy_st, E);
+                float out[E];
+                token(rx[i % STEP], ry[i % STEP], false, true, out);
+                store_raw<E>(pd, E, out);
+                pd += a.Dm;
+            }
+        } else {
+            const int64_t from = t0 == 0 ? -(W - 1) : t0;  // before the first run's tokens the state's rows
+            for (int64_t t = t0; t < stop; ++t) {
+                const int m = t < a.T ? n : 0;
+                float out[E];
+                token(load_raw<E>(px + t * a.x_st, m), load_raw<E>(py + t * g.dy_st, m), t < t1, t < a.T, out);
+                const int64_t s = t - (W - 1);
+                if (s < from) continue;
+                if (g.dfin && s >= a.T - (W - 1)) {
+                    float f[E];
+                    widen(load_raw<E>((const T*)g.dfin + (seq * (W - 1) + s - (a.T - (W - 1))) * a.Dm + c, n), f);
 #pragma unroll
-                    for (int j = 0; j < W - 1; ++j) acc[j][e] = acc[j + 1][e];
-                    acc[W - 1][e] = 0.f;
+                    for (int e = 0; e < E; ++e) out[e] += f[e];
                 }
+                if (s >= 0) store_raw<E>(pd + s * a.Dm, n, out);
+                else if (g.ds0) store_raw<E>((T*)g.ds0 + (seq * (W - 1) + s + W - 1) * a.Dm + c, n, out);
             }
         }
     }
@@ -336,10 +398,9 @@ __global__ __launch_bounds__(1024) void conv_bwd_sum_kernel(ConvBwdParams g) {
     }
 }
 
-// Tokens of a gradient's run: its halo (of two tensors) and its part of dw are less in longer ones, but
-// sixteen where 32 leave the chip under eight waves a compute unit (8 x 2048 tokens of 1536 channels:
-// 102 us forward and backward with 32, 116 with 16; 3 x 3001 of 1001: 77 with 32, 61 with 16).
-int conv_bwd_run(int64_t n_seqs, int64_t T, int D, int cus) {
+// Tokens of a run: its halo (W - 1 tokens, of two tensors in the gradients) and its part of dw are less in longer
+// ones, but sixteen where 32 leave the chip under eight waves a compute unit.
+int conv_run(int64_t n_seqs, int64_t T, int D, int cus) {
     const int64_t threads = n_seqs * ((T + 31) / 32) * ((D + E - 1) / E);
     return threads >= (int64_t)cus * 8 * 64 ? 32 : 16;
 }
@@ -365,7 +426,7 @@ dim3 thread_blocks(int64_t n) { return dim3((unsigned)((n + 255) / 256)); }
 
 template <typename T, int W>
 hipError_t conv_w(const ConvParams& a, hipStream_t s) {
-    const int64_t per = (a.T + RUN - 1) / RUN;
+    const int64_t per = (a.T + a.run - 1) / a.run;
     const Grid g = run_grid(a.cu ? per : a.n_seqs * per, a.Dm);
     if (a.cu) conv_kernel<T, W, true><<<dim3((unsigned)g.blocks), 256, 0, s>>>(a, g.cl, g.cblocks);
     else conv_kernel<T, W, false><<<dim3((unsigned)g.blocks), 256, 0, s>>>(a, g.cl, g.cblocks);
@@ -384,7 +445,7 @@ hipError_t conv_step_w(const ConvParams& a, hipStream_t s) {
 template <typename T, int W>
 hipError_t conv_bwd_w(const ConvBwdParams& b, hipStream_t s) {
     const ConvParams& a = b.f;
-    const Grid g = run_grid(a.n_seqs * ((a.T + b.run - 1) / b.run), a.Dm);
+    const Grid g = run_grid(a.n_seqs * ((a.T + a.run - 1) / a.run), a.Dm);
     conv_bwd_kernel<T, W><<<dim3((unsigned)g.blocks), 256, 0, s>>>(b, g.cl, g.cblocks);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !b.part) return e;

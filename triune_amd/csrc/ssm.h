@@ -100,6 +100,7 @@ struct ConvParams {
     int64_t y_sb, y_st;
     int64_t n_seqs, T;        // T: length of a dense sequence, or all rows of a packed call
     int Dm, W;
+    int run;                  // tokens of a thread's run
     const int32_t* cu;        // packed: [n_seqs + 1]
 };
 
@@ -112,11 +113,10 @@ struct ConvBwdParams {
     void* ds0;                // [Bn, W - 1, Dm] contiguous or null
     float* part;              // [parts, W + 1, Dm]
     int64_t parts;
-    int run;                  // tokens of a run
     void *dw, *dbias;         // of w_dt, or null
 };
 
-int conv_bwd_run(int64_t n_seqs, int64_t T, int Dm, int cus);
+int conv_run(int64_t n_seqs, int64_t T, int Dm, int cus);
 int64_t conv_bwd_parts(int64_t n_seqs, int64_t T, int Dm, int run);
 hipError_t launch_conv(const ConvParams& a, int io_dt, hipStream_t s);
 hipError_t launch_conv_state(const ConvParams& a, int io_dt, hipStream_t s);
