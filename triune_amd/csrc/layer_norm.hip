@@ -40,6 +40,19 @@ __device__ __forceinline__ int column(int t, int k) {
     return (k * TPR + t) * 8;
 }
 
+// Eight elements of a row from column c, zeros past its end.  EIGHTS: the width is a multiple of eight, so a
+// group is in the row or past it, and the load depends on no condition (which would make the compiler wait
+// where it joins the registers, so that no row is in flight).  256 rows of 384 (bf16): 3.7 us, 4.5 with the
+// conditions; 16384 rows of 1536 forward and backward 80.3 and 81.2.
+template <bool EIGHTS, typename T>
+__device__ __forceinline__ Raw<T, 8> load_group(const T* p, int c, int D) {
+    if constexpr (!EIGHTS) return load_raw<8>(p + c, D - c);
+    Raw<T, 8> r = load_raw<8>(p + (c < D ? c : 0), 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = c < D ? r.v[j] : (T)0.f;
+    return r;
+}
+
 __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, float none, float (&x)[8]) {
     if (!p || n <= 0) {
 #pragma unroll
@@ -62,7 +75,7 @@ __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, fl
 }  // namespace
 
 // Blocks walk rows, the next row's loads in flight during this one's sums; w and b are loaded once.
-template <typename T, int TPR, int K>
+template <typename T, int TPR, int K, bool EIGHTS>
 __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) {
     constexpr int RPB = block_threads(TPR) / TPR;
     __shared__ float s_red[16];
@@ -76,7 +89,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = column<TPR>(t, k);
-            raw[k] = load_raw<8>(px + c, a.D - c);
+            raw[k] = load_group<EIGHTS>(px, c, a.D);
         }
     };
     fetch(r);
@@ -94,7 +107,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += x[k][j] = (float)raw[k].v[j];
-        if (r + step < a.R) fetch(r + step);
+        if (EIGHTS || r + step < a.R) fetch(r + step < a.R ? r + step : r);
         const float mean = row_sum<TPR>(s, s_red) / width;
         s = 0.f;
 #pragma unroll
@@ -124,7 +137,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
     }
 }
 
-template <typename T, int TPR, int K>
+template <typename T, int TPR, int K, bool EIGHTS>
 __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdParams g) {
     const NormParams& a = g.f;
     constexpr int RPB = block_threads(TPR) / TPR;
@@ -150,8 +163,8 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = column<TPR>(t, k);
-            nx[k] = load_raw<8>(px + c, a.D - c);
-            ny[k] = load_raw<8>(py + c, a.D - c);
+            nx[k] = load_group<EIGHTS>(px, c, a.D);
+            ny[k] = load_group<EIGHTS>(py, c, a.D);
         }
     };
     // the next row's loads in flight where its registers are free
@@ -165,7 +178,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
         Raw<T, 8> rx[K], ry[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
-        if (AHEAD && r + step < a.R) fetch(r + step);
+        if (AHEAD && (EIGHTS || r + step < a.R)) fetch(r + step < a.R ? r + step : r);
         float s1 = 0.f, s2 = 0.f;
         float xh[K][8];
 #pragma unroll
@@ -244,35 +257,35 @@ int64_t norm_bwd_parts(int64_t R, int D, int cus) {
 
 namespace {
 
-template <typename T, int TPR, int K>
+template <typename T, int TPR, int K, bool EIGHTS>
 hipError_t norm_run(const NormParams& a, hipStream_t s) {
     constexpr int RPB = block_threads(TPR) / TPR;
     const int64_t blocks = (a.R + RPB - 1) / RPB, most = (int64_t)a.cus * FWD_BLOCKS * 256 / block_threads(TPR);
-    norm_kernel<T, TPR, K><<<dim3((unsigned)(blocks < most ? blocks : most)), block_threads(TPR), 0, s>>>(a);
+    norm_kernel<T, TPR, K, EIGHTS><<<dim3((unsigned)(blocks < most ? blocks : most)), block_threads(TPR), 0, s>>>(a);
     return hipGetLastError();
 }
-template <typename T, int TPR, int K>
+template <typename T, int TPR, int K, bool EIGHTS>
 hipError_t norm_run(const NormBwdParams& g, hipStream_t s) {
-    norm_bwd_kernel<T, TPR, K><<<dim3((unsigned)g.parts), block_threads(TPR), 0, s>>>(g);
+    norm_bwd_kernel<T, TPR, K, EIGHTS><<<dim3((unsigned)g.parts), block_threads(TPR), 0, s>>>(g);
     return hipGetLastError();
 }
 
-template <typename T, typename P>
+template <typename T, bool EIGHTS, typename P>
 hipError_t norm_width(const P& p, int D, hipStream_t s) {
-    if (D <= 512) return norm_run<T, 64, 1>(p, s);
-    if (D <= 1024) return norm_run<T, 64, 2>(p, s);
-    if (D <= 1536) return norm_run<T, 64, 3>(p, s);
-    if (D <= 2048) return norm_run<T, 64, 4>(p, s);
-    if (D <= 4096) return norm_run<T, 256, 2>(p, s);
-    if (D <= 8192) return norm_run<T, 256, 4>(p, s);
-    return norm_run<T, 1024, 2>(p, s);
+    if (D <= 512) return norm_run<T, 64, 1, EIGHTS>(p, s);
+    if (D <= 1024) return norm_run<T, 64, 2, EIGHTS>(p, s);
+    if (D <= 1536) return norm_run<T, 64, 3, EIGHTS>(p, s);
+    if (D <= 2048) return norm_run<T, 64, 4, EIGHTS>(p, s);
+    if (D <= 4096) return norm_run<T, 256, 2, EIGHTS>(p, s);
+    if (D <= 8192) return norm_run<T, 256, 4, EIGHTS>(p, s);
+    return norm_run<T, 1024, 2, EIGHTS>(p, s);
 }
 
 template <typename P>
 hipError_t norm_dtype(const P& p, int D, int dt, hipStream_t s) {
-    if (dt == DT_F32) return norm_width<float>(p, D, s);
-    if (dt == DT_BF16) return norm_width<__bf16>(p, D, s);
-    return norm_width<_Float16>(p, D, s);
+    if (dt == DT_F32) return D % 8 ? norm_width<float, false>(p, D, s) : norm_width<float, true>(p, D, s);
+    if (dt == DT_BF16) return D % 8 ? norm_width<__bf16, false>(p, D, s) : norm_width<__bf16, true>(p, D, s);
+    return D % 8 ? norm_width<_Float16, false>(p, D, s) : norm_width<_Float16, true>(p, D, s);
 }
 
 }  // namespace
