@@ -29,8 +29,8 @@ __device__ __forceinline__ float row_sum(float x, float* s) {
     return x;
 }
 
-// Blocks of 256 threads a compute unit, each walking rows (16384 rows of 1536, bf16, forward and backward:
-// 81 us with 4 and 2, 95 with 8 and 4, whose parts of dw and db are twice as many).
+// Blocks of 256 threads a compute unit, each walking rows.  The backward's parts of dw and db grow with them (16384
+// rows of 1536, bf16, forward and gradients: 69.5 us with two, 85.7 with one, 82.4 with four).
 constexpr int FWD_BLOCKS = 4, BWD_BLOCKS = 2;
 constexpr int block_threads(int tpr) { return tpr == 64 ? 256 : tpr; }
 
@@ -42,8 +42,8 @@ __device__ __forceinline__ int column(int t, int k) {
 
 // Eight elements of a row from column c, zeros past its end.  EIGHTS: the width is a multiple of eight, so a
 // group is in the row or past it, and the load depends on no condition (which would make the compiler wait
-// where it joins the registers, so that no row is in flight).  256 rows of 384 (bf16): 3.7 us, 4.5 with the
-// conditions; 16384 rows of 1536 forward and backward 80.3 and 81.2.
+// where it joins the registers, so that no row is in flight).  16384 rows of 1536 (bf16), forward and gradients: 73.4
+// us, 80.2 with the conditions.
 template <bool EIGHTS, typename T>
 __device__ __forceinline__ Raw<T, 8> load_group(const T* p, int c, int D) {
     if constexpr (!EIGHTS) return load_raw<8>(p + c, D - c);
@@ -74,14 +74,16 @@ __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, fl
 
 }  // namespace
 
-// Blocks walk rows, the next row's loads in flight during this one's sums; w and b are loaded once.
+// Blocks walk rows, the next row's loads in flight during this one's sums; w and b are loaded once, to LDS: in
+// registers they leave fewer waves a SIMD (16384 rows of 1536, bf16: 23.3 us (4.3 TB/s) and 27.6; 4096 of 8192: 35.3
+// and 45.7).
 template <typename T, int TPR, int K, bool EIGHTS>
 __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) {
     constexpr int RPB = block_threads(TPR) / TPR;
     __shared__ float s_red[16];
+    __shared__ __attribute__((aligned(16))) float s_par[2][K][2][TPR][4];  // w, b
     const int t = threadIdx.x % TPR;
     int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (RPB > 1 && r >= a.R) return;  // whole waves
     const float width = (float)a.D;  // divided by: a constant row's mean is its value where its sum is exact
     Raw<T, 8> raw[K];
     auto fetch = [&](int64_t row) {
@@ -92,14 +94,21 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
             raw[k] = load_group<EIGHTS>(px, c, a.D);
         }
     };
-    fetch(r);
-    float w[K][8], b[K][8];
+    if (RPB == 1 || r < a.R) fetch(r);
+    if (threadIdx.x < TPR) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = column<TPR>(t, k);
-        load_par(a.w, a.w_dt, c, a.D - c, 1.f, w[k]);
-        load_par(a.b, a.b_dt, c, a.D - c, 0.f, b[k]);
+        for (int k = 0; k < K; ++k) {
+            const int c = column<TPR>(t, k);
+            float w[8], b[8];
+            load_par(a.w, a.w_dt, c, a.D - c, 1.f, w);
+            load_par(a.b, a.b_dt, c, a.D - c, 0.f, b);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s_par[0][k][h][t][j] = w[4 * h + j], s_par[1][k][h][t][j] = b[4 * h + j];
+        }
     }
+    __syncthreads();
     const int64_t step = (int64_t)gridDim.x * RPB;
     for (; r < a.R; r += step) {
         float x[K][8], s = 0.f;
@@ -107,7 +116,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += x[k][j] = (float)raw[k].v[j];
-        if (EIGHTS || r + step < a.R) fetch(r + step < a.R ? r + step : r);
+        if (r + step < a.R) fetch(r + step);
         const float mean = row_sum<TPR>(s, s_red) / width;
         s = 0.f;
 #pragma unroll
@@ -131,7 +140,8 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) 
             if (left <= 0) continue;
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = __builtin_fmaf(x[k][j] * rstd, w[k][j], b[k][j]);
+            for (int j = 0; j < 8; ++j)
+                y[j] = __builtin_fmaf(x[k][j] * rstd, s_par[0][k][j >> 2][t][j & 3], s_par[1][k][j >> 2][t][j & 3]);
             store_raw<8>(py + c, left, y);
         }
     }
@@ -178,7 +188,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void norm_bwd_kernel(NormBwdPar
         Raw<T, 8> rx[K], ry[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) rx[k] = nx[k], ry[k] = ny[k];
-        if (AHEAD && (EIGHTS || r + step < a.R)) fetch(r + step < a.R ? r + step : r);
+        if (AHEAD && r + step < a.R) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
         float xh[K][8];
 #pragma unroll
