@@ -205,3 +205,29 @@ def test_pools_that_want_gradients_are_refused(dev):
     pool = torch.zeros(2, 3, 6, device=dev, requires_grad=True)
     with pytest.raises(ValueError):
         short_conv_varlen(x, w, cu, state_pool=pool, slots=slots)
+
+
+def test_runs_of_large_calls(dev):
+    """Calls that fill the chip take longer runs: the same bits as short pieces, dense and packed; dw and dbias
+    against 64 bits (32 tokens of a run, four runs of a block, 65 blocks' parts: within the 96 of test_gradients)."""
+    T, D, W = 8209, 2060, 4
+    x, w, b, s = inputs(dev, 1, T, D, W, BF)
+    cu = torch.tensor([0, 5, 5, 1003, 8209], dtype=torch.int32, device=dev)
+    y, fin = short_conv(x, w, b, s)
+    at, parts, state = 0, [], s
+    while at < T:
+        p, state = short_conv(x[:, at:at + 1021], w, b, state)
+        parts.append(p)
+        at += 1021
+    assert torch.equal(torch.cat(parts, 1), y) and torch.equal(state, fin)
+    yp, fp = short_conv_varlen(x[0], w, cu, b)
+    for i, (lo, hi) in enumerate(zip(cu.tolist(), cu.tolist()[1:])):
+        e = short_conv(x[:, lo:hi], w, b)
+        assert torch.equal(yp[lo:hi], e[0][0]) and torch.equal(fp[i], e[1][0])
+    dy = torch.randn(1, T, D, generator=torch.Generator().manual_seed(2)).to(BF).to(dev)
+    ds = torch.zeros_like(s)
+    leaves = [t.requires_grad_() for t in (x, w, b, s)]
+    got = torch.autograd.grad(short_conv(*leaves, activation=None), leaves, (dy, ds))
+    form = (x, w, b, s, False, dy, ds)
+    for t, g, r, e in zip(leaves, got, R.conv_grads(*form), R.conv_grads(*form, absolute=True)):
+        R.near(g, r, (2 * W + 30 + (96 if t is w or t is b else 0)) * R.U * e, BF)

@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
             const int ch = ((int)(blockIdx.x - rb * cblocks) * cl) * E + q;
             float s = 0.f;
             for (int r = 0; r < runs_pb; ++r) s += s_red[r * cl + q / E][q % E];
-            if (ch < a.Dm) g.part[(rb * (W + 1) + j) * a.Dm + ch] = s;
+            if (ch < a.Dm) g.part[((int64_t)rb * (W + 1) + j) * a.Dm + ch] = s;
         }
         __syncthreads();
     }
