@@ -519,3 +519,21 @@ def test_pools_that_want_gradients_are_refused(dev):
         ssm_scan_varlen(*packed, cu, state_pool=pool, slots=slots)
     with torch.no_grad():
         assert ssm_scan_varlen(*packed, cu, state_pool=pool, slots=slots)[1] is pool
+
+
+def test_more_segments_than_a_block_joins_at_once(dev):
+    """139 segments of 32 tokens with long memories, forward and gradients, and a packed call whose one long prompt
+    has more segments than the average that the join is laid out for."""
+    args, kw = inputs(dev, 1, 4430, 10, 5, slow=True, seed=31)
+    y, s, _ = S._scan(*args, kw["D"], kw["z"], kw["delta_bias"], True, kw["initial_state"], None, False, 1 << 8)
+    check((y, s), want(args, kw), F32)
+    grad_check(dev, args, kw, F32, flags=1 << 8)
+    lens = [3, 4400, *[1] * 26, 1]
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+    s0 = kw["initial_state"].expand(len(lens), -1, -1)
+    kw["initial_state"] = None
+    yp, fin = ssm_scan_varlen(*args, cu, **{**kw, "initial_state": s0})
+    for i in (0, 1, len(lens) - 1):
+        c = slice(int(cu[i]), int(cu[i + 1]))
+        part = [args[0][:, c], args[1][:, c], args[2], args[3][:, c], args[4][:, c]]
+        check((yp[:, c], fin[i:i + 1]), R.scan(*part, kw["D"], kw["z"][:, c], kw["delta_bias"], True, s0[:1]), F32)
