@@ -442,8 +442,8 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
  * No reference counterpart.  Sizes: Dm channels, N states per channel (1..64), G groups of Dm / G
  * channels that share B and C.  Operands in io_dtype: u, delta, z, y [Bn, T, Dm] and B, C
  * [Bn, T, G, N] (innermost stride 1, other strides in elements, any alignment of an element, a
- * stride of 0 for a broadcast input; the scan takes token strides below 2^22, y's at least Dm); fp32 and contiguous: A [Dm, N], D and delta_bias [Dm] (either
- * may be NULL), states [*, Dm, N].
+ * stride of 0 for a broadcast input; the scan takes token strides below 2^22, y's at least Dm); fp32
+ * and contiguous: A [Dm, N], D and delta_bias [Dm] (either may be NULL), states [*, Dm, N].
  * A workspace is 16-byte aligned and belongs to one call at a time.
  *
  * Selective scan, per channel d and state n:

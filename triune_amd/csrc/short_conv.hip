@@ -119,7 +119,8 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvParams a, int cl, int cbl
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) {
             const int64_t s = t - (W - 1) + i;
-            widen(s >= beg ? load_raw<E>(px + s * a.x_st, n) : state_row<T, W>(a, row, (int)(s - beg) + W - 1, c, n), win[i]);
+            widen(s >= beg ? load_raw<E>(px + s * a.x_st, n) : state_row<T, W>(a, row, (int)(s - beg) + W - 1, c, n),
+                  win[i]);
         }
     };
     window(t0);
@@ -268,14 +269,14 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) {
             const int64_t s = t0 - (W - 1) + i;
-            const Raw<T, E> r = s >= 0 ? load_raw<E>(px + s * a.x_st, n) : state_row<T, W>(a, seq, (int)s + W - 1, c, n);
-            widen(r, win[i]);
+            widen(s >= 0 ? load_raw<E>(px + s * a.x_st, n) : state_row<T, W>(a, seq, (int)s + W - 1, c, n), win[i]);
         }
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
-        // Takes a token in (own: of this run, whose dw it adds to; in: of the sequence) and its dp to acc, of which acc[0] is whole then.
+        // Takes a token in (own: of this run, whose dw it adds to; in: of the sequence) and its dp to acc, of which
+        // acc[0] is whole then.
         auto token = [&](const Raw<T, E>& rx, const Raw<T, E>& ry, bool own, bool in, float (&out)[E]) {
             float x[E], dp[E], p[E], old[W - 1][E];
             widen(rx, x);
@@ -315,7 +316,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
             pd += (t0 - (W - 1)) * a.Dm;
             Raw<T, E> rx[STEP], ry[STEP];
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) rx[i] = load_raw<E>(px + i * a.x_st, E), ry[i] = load_raw<E>(py + i * g.dy_st, E);
+            for (int i = 0; i < STEP; ++i) {
+                rx[i] = load_raw<E>(px + i * a.x_st, E);
+                ry[i] = load_raw<E>(py + i * g.dy_st, E);
+            }
 #pragma unroll 1
             for (int t = 0; t < a.run; t += STEP) {
                 px += STEP * a.x_st;
@@ -339,7 +343,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvBwdParams g, int cl, 
             }
 #pragma unroll
             for (int i = 0; i < W - 1; ++i) {
-                if (i >= STEP) rx[i % STEP] = load_raw<E>(px + i * a.x_st, E), ry[i % STEP] = load_raw<E>(py + i * g.dy_st, E);
+                if (i >= STEP) {
+                    rx[i % STEP] = load_raw<E>(px + i * a.x_st, E);
+                    ry[i % STEP] = load_raw<E>(py + i * g.dy_st, E);
+                }
                 float out[E];
                 token(rx[i % STEP], ry[i % STEP], false, true, out);
                 store_raw<E>(pd, E, out);
