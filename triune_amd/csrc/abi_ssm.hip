@@ -53,9 +53,9 @@ int64_t all_blocks(int64_t Dm, int64_t G) { return G * group_blocks(Dm, G); }
 // Waves a compute unit (four SIMDs) that a call has without splitting the time axis for that to be left,
 // and that it gets where it is split.  Two waves on a SIMD keep it three quarters busy; splitting costs the
 // decays a second time.  8 x 2048 tokens of 4096 channels, N = 16: 306 us unsplit with eight waves a unit, 445
-// split.  Split calls take shares that several rounds of workgroups even out: 1 x 16384 of 768 channels 104 us
-// split for 32 waves, 108 for 24, 122 for 16, 106 for 48; 16 ragged prompts of 5034 tokens, 1536 channels: 86, 91,
-// 97 and 87.
+// split.  Split calls take shares that several rounds of workgroups even out: 1 x 16384 of 768 channels 106 us for
+// 24 to 48 waves (segments of 128 and 64 tokens), 122 for 16; 16 ragged prompts of 5034 tokens, 1536 channels: 86 for
+// 32, 91 for 24, 97 for 14, 87 for 64.
 constexpr int kEnoughWaves = 8, kSplitWaves = 32;
 // Workgroups of `waves` waves a compute unit.
 int64_t ssm_slots(int N, int waves) {
