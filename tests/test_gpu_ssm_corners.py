@@ -1,0 +1,84 @@
+"""GPU: corners of the state space layer's operators that their other tests leave."""
+
+import pytest
+import torch
+import ssm_ref as R
+
+from triune_amd import ssm as S
+from triune_amd import ssm_scan, ssm_scan_varlen
+
+pytestmark = pytest.mark.gpu
+
+F32 = torch.float32
+
+
+# ---- modes that grow --------------------------------------------------------------------------------
+# dt A = 2 a token: 92 binary exponents in 32 tokens, 185 in 64, past the largest number's 128.
+def growing(dev, B, T, D=40, N=16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    u, Bm, C = rn(B, T, D), rn(B, T, N), rn(B, T, N)
+    A = torch.full((D, N), 2.0) - 0.1 * torch.rand(D, N, generator=g)
+    A[:, 1] = -1.0  # beside them one that decays
+    return [t.to(dev) for t in (u, torch.ones(B, T, D), A, Bm, C)]
+
+
+def growing_check(got, args, s0=None):
+    y, fin, ey, ef, _ = R.scan(*args, soft=False, s0=s0)
+    R.near(got[0], y, ey, F32, "y")
+    R.near(got[1], fin, ef, F32, "state")
+
+
+@pytest.mark.parametrize("units", [0, 1, 2, 3])
+def test_zero_states_grow_to_zero(dev, units):
+    """Left padding (u = 0, no initial state) in front of 12 tokens: the state stays 0 whatever its decay product is,
+    so the split call gives what the unsplit one does."""
+    args = growing(dev, 2, 212)
+    args[0][:, :200] = 0
+    y, s, _ = S._scan(*args, None, None, None, False, None, None, False, units << 8)
+    growing_check((y, s), args)
+
+
+def test_zero_states_grow_to_zero_by_the_rule(dev):
+    """The same through the public calls, where the rule splits the time axis: dense and packed."""
+    args = growing(dev, 1, 4096)
+    args[0][:, :4084] = 0
+    assert S.plan_on(args[0], "triune_hip_ssm_scan_workspace_size", 1, 4096, 40, 1, 16, 0) > 0
+    growing_check(ssm_scan(*args, delta_softplus=False), args)
+    lens = [300, 3784, 12]
+    args[0][:, 288:300] = args[0][:, 4080:4084] = 1
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+    assert S.plan_on(args[0], "triune_hip_ssm_scan_varlen_workspace_size", 3, 4096, 40, 1, 16, 0) > 0
+    y, s = ssm_scan_varlen(*args, cu, delta_softplus=False)
+    for i, ln in enumerate(lens):
+        c = slice(int(cu[i]), int(cu[i]) + ln)
+        growing_check((y[:, c], s[i:i + 1]), [t if t.dim() == 2 else t[:, c] for t in args])
+
+
+@pytest.mark.parametrize("units", [0, 1, 2])
+def test_small_states_grow_within_range(dev, units):
+    """A state of 1e-30 grows by 2^207 to about 2^107, though the decay product of its first 64 tokens is past the
+    largest number; a large one decays by 2^-200 to a small one."""
+    args = growing(dev, 1, 72, seed=1)
+    args[0].zero_()
+    s0 = torch.full((1, 40, 16), 1e-30, device=dev)
+    args[2][:, 1], s0[:, :, 1] = -2.0, 1e30
+    y, s, _ = S._scan(*args, None, None, None, False, s0, None, False, units << 8)
+    growing_check((y, s), args, s0)
+
+
+@pytest.mark.parametrize("units", [0, 1, 2])
+def test_gradients_of_growing_modes(dev, units):
+    """Upstream of the first 12 tokens only: the gradient of every later state is 0 whatever it is decayed by."""
+    args = growing(dev, 2, 212, seed=2)
+    args[0][:, :200] = 0
+    s0 = torch.zeros(2, 40, 16, device=dev)
+    dy = torch.randn(2, 212, 40, generator=torch.Generator().manual_seed(3)).to(dev)
+    dy[:, 12:] = 0
+    _, _, kept = S._scan(*args, None, None, None, False, s0, None, True, units << 8)
+    got = S._scan_bwd(*args, None, None, None, False, kept, dy, None, True, units << 8)
+    form = (*args, None, None, None, False, s0, dy, None)
+    for x, r, e in zip(got, R.scan_grads(*form), R.scan_grads(*form, absolute=True)):
+        assert (x is None) == (r is None)
+        if r is not None:
+            R.near(x, r, 24 * (212 + 16) * R.U * e, F32)

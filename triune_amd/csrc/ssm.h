@@ -231,6 +231,21 @@ __device__ __forceinline__ float log2_decay(float A) {
     return x < -most ? -most : x > most ? most : x;
 }
 
+// 2^x as m 2^e with m in (1/2, 1], for a decay product over a segment: modes that grow (A > 0, or steps below
+// 0) take it past the largest number where the state that it scales, 0 or small, stays within.  scale(v) = v 2^x
+// then leaves the range only if the product does.  Past 300 no float's product is within; NaN stays.
+struct Pow2 {
+    float m;
+    int e;
+    __device__ __forceinline__ explicit Pow2(float x) {
+        x = x < -300.f ? -300.f : x > 300.f ? 300.f : x;
+        const float c = __builtin_ceilf(x);
+        m = __builtin_amdgcn_exp2f(x - c);
+        e = (int)__builtin_amdgcn_fmed3f(c, -300.f, 300.f);
+    }
+    __device__ __forceinline__ float scale(float v) const { return __builtin_ldexpf(m * v, e); }
+};
+
 // N consecutive states of a channel whose row holds `left` more (zeros past them).
 template <int N>
 __device__ __forceinline__ void load_states(const float* p, int left, float (&x)[N]) {

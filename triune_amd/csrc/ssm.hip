@@ -287,7 +287,7 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
         float all = 0.f, end = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            end = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[i] * Al), end, local[i]);
+            end = Pow2(sum[i] * Al).scale(end) + local[i];
             all += sum[i];
         }
         if (waves > 1) {
@@ -299,12 +299,12 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
         for (int q = 0; q < waves; ++q) {
             if (q == w) S = next;
             const float d = waves > 1 ? s_sum[q][lane] : all, e = waves > 1 ? s_end[q][lane] : end;
-            next = __builtin_fmaf(__builtin_amdgcn_exp2f(d * Al), next, e);
+            next = Pow2(d * Al).scale(next) + e;
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (i < m && chv) p[(BACK ? v0 - i : v0 + i) * per] = S;
-            S = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[i] * Al), S, local[i]);
+            S = Pow2(sum[i] * Al).scale(S) + local[i];
         }
         S = next;
         if (waves > 1) __syncthreads();
