@@ -82,3 +82,30 @@ def test_gradients_of_growing_modes(dev, units):
         assert (x is None) == (r is None)
         if r is not None:
             R.near(x, r, 24 * (212 + 16) * R.U * e, F32)
+
+
+# ---- infinite decays ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("soft", [True, False])
+@pytest.mark.parametrize("N", [3, 16, 40])
+def test_gradients_with_infinite_decay(dev, N, soft):
+    """A of -inf forgets at every step above 0, as a finite A far below does: the gradients are that one's, also at
+    tokens whose step is 0."""
+    B, T, D = 2, 70, 36
+    g = torch.Generator().manual_seed(N)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    u, delta, Bm, C, z, dy = rn(B, T, D), rn(B, T, D), rn(B, T, N), rn(B, T, N), rn(B, T, D), rn(B, T, D)
+    A, s0, ds = -torch.exp(rn(D, N)), rn(B, D, N), rn(B, D, N)
+    if soft:
+        delta[:, 5] = delta[:, 64] = float("-inf")
+    else:
+        delta = delta.abs() + 0.01
+    far = A.clone()
+    A[3, 1], A[7], A[35, 0] = (float("-inf"),) * 3
+    far[3, 1], far[7], far[35, 0] = (-1e30,) * 3
+    leaves = [t.requires_grad_() for t in (u, delta, A, Bm, C, z, s0)]
+    y, fin = ssm_scan(*leaves[:5], z=z, delta_softplus=soft, initial_state=s0)
+    got = torch.autograd.grad((y, fin), leaves, (dy, ds))
+    form = (u, delta, far, Bm, C, None, z, None, soft, s0, dy, ds)
+    ref, env = (R.scan_grads(*form, absolute=a) for a in (False, True))
+    for x, i, name in zip(got, (0, 1, 2, 3, 4, 6, 8), ("u", "delta", "A", "B", "C", "z", "initial_state")):
+        R.near(x, ref[i], 24 * (T + 16) * R.U * env[i], F32, name)

@@ -224,12 +224,15 @@ __device__ __forceinline__ void store_dt(void* p, int dt, int64_t i, float x) {
     else ((_Float16*)p)[i] = (_Float16)x;
 }
 
-// A in units of the hardware's exp2.  Infinite values are cut to the largest number, so that a step of 0
-// (a token past a tile's end) is a decay of 1 for them too.
-__device__ __forceinline__ float log2_decay(float A) {
-    const float x = A * LOG2E, most = 3.4028234e38f;
+// x with infinities cut to the largest numbers of their signs.
+__device__ __forceinline__ float finite(float x) {
+    const float most = 3.4028234e38f;
     return x < -most ? -most : x > most ? most : x;
 }
+
+// A in units of the hardware's exp2.  Infinite values are cut, so that a step of 0 (a token past a tile's
+// end) is a decay of 1 for them too.
+__device__ __forceinline__ float log2_decay(float A) { return finite(A * LOG2E); }
 
 // 2^x as m 2^e with m in (1/2, 1], for a decay product over a segment: modes that grow (A > 0, or steps below
 // 0) take it past the largest number where the state that it scales, 0 or small, stays within.  scale(v) = v 2^x
