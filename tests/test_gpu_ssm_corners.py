@@ -4,8 +4,9 @@ import pytest
 import torch
 import ssm_ref as R
 
+from triune_amd import (layer_norm, short_conv, short_conv_decode_step, short_conv_varlen, ssm_decode_step, ssm_scan,
+                        ssm_scan_varlen)
 from triune_amd import ssm as S
-from triune_amd import ssm_scan, ssm_scan_varlen
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +110,27 @@ def test_gradients_with_infinite_decay(dev, N, soft):
     ref, env = (R.scan_grads(*form, absolute=a) for a in (False, True))
     for x, i, name in zip(got, (0, 1, 2, 3, 4, 6, 8), ("u", "delta", "A", "B", "C", "z", "initial_state")):
         R.near(x, ref[i], 24 * (T + 16) * R.U * env[i], F32, name)
+
+
+# ---- forward-mode derivatives ---------------------------------------------------------------------------
+def test_forward_mode_is_refused(dev):
+    """A dual tensor does not require a gradient and has storage to read; its tangent would be dropped."""
+    fw = torch.autograd.forward_ad
+    rn = lambda *s: torch.randn(*s, device=dev)  # noqa: E731
+    u, A, Bm, w, state, pool = rn(1, 8, 8), -rn(8, 4).exp(), rn(1, 8, 4), rn(8, 4), rn(1, 3, 8), rn(1, 8, 4)
+    cu, slots = torch.tensor([0, 8], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    calls = [
+        lambda d: ssm_scan(d(u), u, A, Bm, Bm), lambda d: ssm_scan(u, u, d(A), Bm, Bm),
+        lambda d: ssm_scan(u, u, A, Bm, Bm, initial_state=d(pool)), lambda d: ssm_scan(u, u, A, Bm, Bm, z=d(u)),
+        lambda d: ssm_scan_varlen(u, d(u), A, Bm, Bm, cu), lambda d: ssm_decode_step(u[:, 0], u[:, 0], A, Bm[:, 0],
+                                                                                    Bm[:, 0], d(pool)),
+        lambda d: short_conv(d(u), w), lambda d: short_conv(u, d(w)), lambda d: short_conv(u, w, initial_state=d(state)),
+        lambda d: short_conv_varlen(u, d(w), cu), lambda d: short_conv_decode_step(d(u[:, 0]), w, state),
+        lambda d: layer_norm(d(u)), lambda d: layer_norm(u, d(w[:, 0].contiguous())),
+    ]
+    with fw.dual_level():
+        for call in calls:
+            call(lambda t: t)  # tensors without a tangent are taken there too
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    call(lambda t: fw.make_dual(t, torch.ones_like(t)))

@@ -166,3 +166,18 @@ def test_counts_past_the_plans_numbers():
     assert lib.triune_hip_ssm_bwd_workspace_size(many, 64, 64, 1, 16, 0) == 0
     assert lib.triune_hip_ssm_scan_varlen_workspace_size(many, 64, 64, 1, 16, 0) == 0
     assert lib.triune_hip_short_conv_bwd_workspace_size(many, 64, 64, 4) == 0
+
+
+def test_forward_mode_duals_are_refused():
+    """What every entry asks of its tensors: no tangent, recorded or not."""
+    fw, x = torch.autograd.forward_ad, torch.zeros(3)
+    from triune_amd.ssm import _needs_grad
+
+    assert not _needs_grad(x, None)
+    with fw.dual_level():
+        assert not _needs_grad(x, None) and _needs_grad(None, torch.zeros(3, requires_grad=True))
+        d = fw.make_dual(x, torch.ones(3))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                _needs_grad(None, x, d)
+    assert not _needs_grad(x)

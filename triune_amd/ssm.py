@@ -16,6 +16,7 @@ carry is float32; outputs are rounded once.  Tensors are on one HIP device; ther
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import call_on, dtype_code, plan_on, ptr, strides
 
@@ -69,6 +70,12 @@ def _lead_out(y, tok):
 
 
 def _needs_grad(*ts) -> bool:
+    """Whether a call on these is recorded.  Refuses forward-mode duals: they do not require a gradient, and
+    their tangents would be dropped."""
+    if forward_ad._current_level >= 0:  # inside dual_level()
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("there is no forward-mode derivative: an input carries a tangent")
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
