@@ -450,7 +450,7 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
  *     dt = delta + delta_bias, through softplus when `softplus`;  h <- exp(dt A) h + dt u B
  *     y = (sum_n C h + D u) * silu(z)                     (no gate when z is NULL)
  * strides[14] = (batch, token) of u, delta, z, y, then (batch, token, group) of B, C.  s0 (NULL:
- * zeros) and s_final (NULL: not wanted): [Bn, Dm, N].  kept: NULL, or fp32 [Bn, ceil(T / K), N, Dm],
+ * zeros) and s_final (NULL: not wanted): [Bn, Dm, N]; without tokens (T = 0) s0 goes to s_final.  kept: NULL, or fp32 [Bn, ceil(T / K), N, Dm],
  * K = 32 (16 for N > 32), that receives the state of every K-th token for triune_hip_ssm_bwd.  flags bits 8..15 force the
  * length of a segment in units of 32 tokens (0: automatic). */
 size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags);
@@ -500,7 +500,8 @@ int triune_hip_ssm_decode_step(const void* u, const void* delta, const void* z, 
  *     p_t = bias + sum_j w[d, j] x[t - W + 1 + j],  y = silu(p) when `silu`, else p
  * x, y [Bn, T, Dm] in io_dtype (strides[4] = (batch, token) of x, y); w [Dm, W] and bias [Dm] (or
  * NULL) contiguous in w_dtype (io_dtype or fp32).  s0: the W - 1 tokens before the first, [Bn, W - 1, Dm] contiguous in
- * io_dtype (NULL: zeros); s_final (or NULL): the last W - 1 after the call, laid out the same, not over s0. */
+ * io_dtype (NULL: zeros); s_final (or NULL): the last W - 1 after the call, laid out the same, not over s0 (T = 0:
+ * a copy of s0). */
 int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io_dtype, int w_dtype,
                           const int64_t* strides, int silu, const void* s0, void* s_final, void* y, int64_t Bn,
                           int64_t T, int64_t Dm, int W, void* stream);

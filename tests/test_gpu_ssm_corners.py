@@ -1,16 +1,19 @@
 """GPU: corners of the state space layer's operators that their other tests leave."""
 
+import ctypes
+
 import pytest
 import torch
 import ssm_ref as R
 
+import triune_amd._lib as L
 from triune_amd import (layer_norm, short_conv, short_conv_decode_step, short_conv_varlen, ssm_decode_step, ssm_scan,
                         ssm_scan_varlen)
 from triune_amd import ssm as S
 
 pytestmark = pytest.mark.gpu
 
-F32 = torch.float32
+BF, F32 = torch.bfloat16, torch.float32
 
 
 # ---- modes that grow --------------------------------------------------------------------------------
@@ -134,3 +137,32 @@ def test_forward_mode_is_refused(dev):
             for grad in (True, False):
                 with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
                     call(lambda t: fw.make_dual(t, torch.ones_like(t)))
+
+
+# ---- calls without tokens at the C entries ------------------------------------------------------------------
+def test_no_tokens_leave_the_initial_state(dev):
+    """T = 0 with sequences: the final state is the initial one, zeros without one, as in the packed calls; given as
+    one buffer it stays."""
+    lib, stream = L.lib(), torch.cuda.current_stream(dev).cuda_stream
+    p = lambda t: ctypes.c_void_p(None if t is None else t.data_ptr())  # noqa: E731
+    x = torch.zeros(64, device=dev)
+    st = (ctypes.c_int64 * 14)(*([64] * 14))
+    s0 = torch.randn(3, 10, 5, device=dev)
+
+    def scan(a, b):
+        return lib.triune_hip_ssm_scan(p(x), p(x), None, p(x), p(x), p(x), None, None, 0, st, 1, p(a), p(x), p(b), None, 3,
+                                       0, 10, 1, 5, 0, None, 0, stream)
+
+    for a in (s0, None):
+        b = torch.full_like(s0, 7.0)
+        assert scan(a, b) == 0
+        assert torch.equal(b, torch.zeros_like(s0) if a is None else s0)
+    keep = s0.clone()
+    assert scan(s0, s0) == 0 and scan(s0, None) == 0 and torch.equal(s0, keep)
+    for code, dtype in ((0, F32), (1, BF), (2, torch.float16)):
+        c0 = torch.randn(3, 3, 11, device=dev).to(dtype)
+        w = torch.zeros(44, device=dev)
+        for a in (c0, None):
+            b = torch.full_like(c0, 7.0)
+            assert lib.triune_hip_short_conv(p(x), p(w), None, code, 0, st, 1, p(a), p(b), p(x), 3, 0, 11, 4, stream) == 0
+            assert torch.equal(b, torch.zeros_like(c0) if a is None else c0)

@@ -181,7 +181,8 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
         return TRIUNE_ERR_LAYOUT;
     if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]}) || strides[7] < Dm)
         return TRIUNE_ERR_LAYOUT;
-    if (Bn == 0 || T == 0) return TRIUNE_OK;
+    if (Bn == 0) return TRIUNE_OK;
+    if (T == 0) return s_final ? status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream)) : TRIUNE_OK;
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags, 3);
     if (p.n_work > kMaxGrid / all_blocks(Dm, G) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
@@ -351,7 +352,11 @@ int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io
                           const int64_t* strides, int silu, const void* s0, void* s_final, void* y, int64_t Bn,
                           int64_t T, int64_t Dm, int W, void* stream) {
     if (const int e = conv_check(x, w, bias, y, strides, s0, s_final, io_dtype, w_dtype, Bn, T, Dm, W)) return e;
-    if (Bn == 0 || T == 0) return TRIUNE_OK;
+    if (Bn == 0) return TRIUNE_OK;
+    if (T == 0) {
+        const int bytes = io_dtype == TRIUNE_DT_F32 ? 4 : 2;
+        return s_final ? status(launch_state_copy(s0, s_final, Bn * (W - 1) * Dm, bytes, (hipStream_t)stream)) : TRIUNE_OK;
+    }
     ConvParams a = conv_params(x, w, bias, w_dtype, silu, s0, s_final, y, Bn, T, Dm, W);
     a.x_sb = strides[0], a.x_st = strides[1], a.y_sb = strides[2], a.y_st = strides[3];
     a.run = conv_run(Bn, T, (int)Dm, compute_units());

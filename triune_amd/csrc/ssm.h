@@ -76,6 +76,8 @@ inline bool ssm_by_four(int group_channels, int io_dt, std::initializer_list<Ssm
         if (t.p && ((reinterpret_cast<uintptr_t>(t.p) & m) || ((t.sb | t.st) & 3))) return false;
     return group_channels % 4 == 0;
 }
+// n elements of `bytes` (2 or 4) from one state tensor to another, zeros without a source: calls without tokens.
+hipError_t launch_state_copy(const void* from, void* to, int64_t n, int bytes, hipStream_t s);
 hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* seg_off, hipStream_t s);
 hipError_t launch_ssm_states(const SsmParams& a, int io_dt, hipStream_t s);
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s);

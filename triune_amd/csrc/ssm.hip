@@ -335,6 +335,11 @@ __global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int32_t* o
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(256) void state_copy_kernel(const T* from, T* to, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from ? from[i] : (T)0;
+}
+
 // One token for every row.  A lane holds up to four states of a channel, LPC neighbouring lanes a
 // channel; a block keeps its channels' A, D and bias over the rows that it walks, the next row's
 // states and operands in flight.  Bound by the states, read and written once.
@@ -430,6 +435,15 @@ hipError_t launch_ssm_bwd_carry(const SsmBwdParams& g, hipStream_t s) { return c
 
 hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* off, hipStream_t s) {
     ssm_offsets_kernel<<<1, 64, 0, s>>>(a, off);
+    return hipGetLastError();
+}
+
+hipError_t launch_state_copy(const void* from, void* to, int64_t n, int bytes, hipStream_t s) {
+    if (from == to || n == 0) return hipSuccess;
+    const int64_t blocks = (n + 255) / 256;
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    if (bytes == 4) state_copy_kernel<uint32_t><<<grid, 256, 0, s>>>((const uint32_t*)from, (uint32_t*)to, n);
+    else state_copy_kernel<uint16_t><<<grid, 256, 0, s>>>((const uint16_t*)from, (uint16_t*)to, n);
     return hipGetLastError();
 }
 
