@@ -166,3 +166,21 @@ def test_no_tokens_leave_the_initial_state(dev):
             b = torch.full_like(c0, 7.0)
             assert lib.triune_hip_short_conv(p(x), p(w), None, code, 0, st, 1, p(a), p(b), p(x), 3, 0, 11, 4, stream) == 0
             assert torch.equal(b, torch.zeros_like(c0) if a is None else c0)
+
+
+# ---- output buffers and slots -------------------------------------------------------------------------------
+def test_out_rows_of_two_dims_that_overlap_are_refused(dev):
+    """Strides that each span a row but put rows of several sequences on one another; interleaved rows are taken."""
+    u = torch.randn(2, 8, 8, device=dev)
+    A, Bm, w = -torch.ones(8, 4, device=dev), torch.randn(2, 8, 4, device=dev), torch.randn(8, 4, device=dev)
+    flat = torch.zeros(256, device=dev)
+    for st in ((8, 8, 1), (16, 8, 1), (56, 8, 1), (8, 12, 1)):
+        out = flat.as_strided((2, 8, 8), st)
+        with pytest.raises(ValueError, match="overlap"):
+            ssm_scan(u, u, A, Bm, Bm, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            short_conv(u, w, out=out)
+    for st in ((64, 8, 1), (8, 16, 1), (9, 18, 1), (100, 10, 1)):
+        out = flat.as_strided((2, 8, 8), st)
+        assert torch.equal(ssm_scan(u, u, A, Bm, Bm, out=out)[0], ssm_scan(u, u, A, Bm, Bm)[0])
+        assert torch.equal(short_conv(u, w, out=out)[0], short_conv(u, w)[0])

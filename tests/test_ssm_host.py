@@ -181,3 +181,17 @@ def test_forward_mode_duals_are_refused():
             with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
                 _needs_grad(None, x, d)
     assert not _needs_grad(x)
+
+
+def test_out_rows_that_overlap():
+    """Rows of two dims on one another, though each stride spans a row; interleaved rows are apart."""
+    from triune_amd.ssm import _out
+
+    flat, like = torch.zeros(256), torch.zeros(1)
+    for st in ((8, 8, 1), (16, 8, 1), (56, 8, 1), (8, 12, 1), (64, 4, 1), (64, 8, 2), (0, 8, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            _out(flat.as_strided((2, 8, 8), st), (2, 8, 8), torch.float32, like, 1)
+    for st in ((64, 8, 1), (8, 16, 1), (9, 18, 1), (100, 10, 1)):
+        _out(flat.as_strided((2, 8, 8), st), (2, 8, 8), torch.float32, like, 1)
+    for shape, st in (((1, 8, 8), (0, 8, 1)), ((2, 1, 8), (8, 0, 1)), ((2, 8, 1), (8, 1, 5)), ((0, 8, 8), (0, 0, 1))):
+        _out(flat.as_strided(shape, st), shape, torch.float32, like, 1)

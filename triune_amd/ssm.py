@@ -93,8 +93,11 @@ def _out(out, shape, dtype, like, tok=None):
         return torch.empty(shape, device=like.device, dtype=dtype)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"out must be {tuple(shape)} of {dtype}")
-    if any(n > 1 and s < shape[-1] for n, s in zip(shape[:-1], out.stride()[:-1])) or (
-            shape[-1] > 1 and out.stride(-1) != 1):
+    span, apart = shape[-1], shape[-1] < 2 or out.stride(-1) == 1
+    for s, n in sorted((s, n) for s, n in zip(out.stride()[:-1], shape[:-1]) if n > 1):
+        apart = apart and s >= span  # past all that the dims of smaller strides reach
+        span += (n - 1) * s
+    if not apart and out.numel():
         raise ValueError("out needs a unit innermost stride and rows that do not overlap")
     if tok is not None and out.shape[tok] > 1 and out.stride(tok) >= _MAX_TOKEN_STRIDE:
         raise ValueError(f"out's token stride must be below {_MAX_TOKEN_STRIDE}")
