@@ -184,3 +184,25 @@ def test_out_rows_of_two_dims_that_overlap_are_refused(dev):
         out = flat.as_strided((2, 8, 8), st)
         assert torch.equal(ssm_scan(u, u, A, Bm, Bm, out=out)[0], ssm_scan(u, u, A, Bm, Bm)[0])
         assert torch.equal(short_conv(u, w, out=out)[0], short_conv(u, w)[0])
+
+
+def test_wide_slots_are_outside_the_pool(dev):
+    """int64 slots past 32 bits are outside the pool, not the row that their low half names; slots are integers."""
+    D, N = 8, 4
+    u, Bm, w = torch.randn(3, D, device=dev), torch.randn(3, N, device=dev), torch.randn(D, 4, device=dev)
+    A = -torch.ones(D, N, device=dev)
+    pool, cpool = torch.randn(4, D, N, device=dev), torch.randn(4, 3, D, device=dev)
+    slots = torch.tensor([2, (1 << 32) + 1, -(1 << 32)], device=dev)
+    cu = torch.tensor([0, 1, 2, 3], device=dev, dtype=torch.int32)
+    near = torch.tensor([2, 4, -1], device=dev, dtype=torch.int32)  # the same rows, the others just outside
+    for call, s in (
+            (lambda s, k: ssm_decode_step(u, u, A, Bm, Bm, s, inplace=True, slots=k), pool),
+            (lambda s, k: ssm_scan_varlen(u, u, A, Bm, Bm, cu, state_pool=s, slots=k), pool),
+            (lambda s, k: short_conv_decode_step(u, w, s, inplace=True, slots=k), cpool),
+            (lambda s, k: short_conv_varlen(u, w, cu, state_pool=s, slots=k), cpool)):
+        a, b = s.clone(), s.clone()
+        ya, yb = call(a, slots)[0], call(b, near)[0]
+        assert torch.equal(a, b) and torch.equal(ya, yb) and torch.equal(a[[0, 1, 3]], s[[0, 1, 3]])
+        for bad in (near.float(), near >= 0):
+            with pytest.raises(TypeError, match="slots"):
+                call(s.clone(), bad)

@@ -195,3 +195,18 @@ def test_out_rows_that_overlap():
         _out(flat.as_strided((2, 8, 8), st), (2, 8, 8), torch.float32, like, 1)
     for shape, st in (((1, 8, 8), (0, 8, 1)), ((2, 1, 8), (8, 0, 1)), ((2, 8, 1), (8, 1, 5)), ((0, 8, 8), (0, 0, 1))):
         _out(flat.as_strided(shape, st), shape, torch.float32, like, 1)
+
+
+def test_slots_past_32_bits():
+    from triune_amd.ssm import _slots
+
+    dev, wide = torch.device("cpu"), [3, 0, -1, -7, (1 << 32) + 1, -(1 << 32), 1 << 31, -(1 << 31) - 1]
+    got = _slots(torch.tensor(wide), len(wide), dev)
+    assert got.dtype == torch.int32
+    for s, g in zip(wide, got.tolist()):
+        assert g == s if 0 <= s < 1 << 31 else g < 0 or g == (1 << 31) - 1  # stays outside every pool
+    for dt in (torch.int8, torch.int16, torch.uint8, torch.int32):
+        assert _slots(torch.tensor([3, 0], dtype=dt), 2, dev).tolist() == [3, 0]
+    for dt in (torch.float32, torch.float16, torch.bool, torch.complex64):
+        with pytest.raises(TypeError, match="slots"):
+            _slots(torch.zeros(2, dtype=dt), 2, dev)

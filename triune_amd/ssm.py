@@ -110,6 +110,10 @@ def _slots(slots, n, dev):
     if slots.numel() != n or slots.dim() != 1:
         raise ValueError(f"slots must hold one index for each of the {n} rows")
     if slots.dtype != torch.int32 or slots.device != dev:
+        if slots.dtype.is_floating_point or slots.dtype.is_complex or slots.dtype == torch.bool:
+            raise TypeError(f"slots must be integers, not {slots.dtype}")
+        if slots.dtype == torch.int64:  # past 32 bits is outside every pool, not the row of the low half
+            slots = slots.clamp(-1, 2**31 - 1)
         slots = slots.to(device=dev, dtype=torch.int32)
     return slots.contiguous()
 
