@@ -210,3 +210,15 @@ def test_slots_past_32_bits():
     for dt in (torch.float32, torch.float16, torch.bool, torch.complex64):
         with pytest.raises(TypeError, match="slots"):
             _slots(torch.zeros(2, dtype=dt), 2, dev)
+
+
+def test_tokens_wider_than_the_kernels_address():
+    """2^22 group states a token and more: refused by name, and not copied first; one token has no stride."""
+    from triune_amd.ssm import _rows
+
+    B = torch.zeros(1).expand(1, 2, 1 << 16, 64)
+    with pytest.raises(ValueError, match="too wide"):
+        _rows(B, 1)
+    with pytest.raises(ValueError, match="too wide"):
+        _rows(B[0], 0)
+    assert _rows(B[:, :1, :4], 1).shape == (1, 1, 4, 64) and _rows(B[:, :, : (1 << 16) - 1, :8], 1).is_contiguous()

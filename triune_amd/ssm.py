@@ -15,6 +15,8 @@ carry is float32; outputs are rounded once.  Tensors are on one HIP device; ther
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd import forward_ad
 
@@ -54,6 +56,8 @@ def _rows(x, tok=None):
     where it has not)."""
     if x.stride(-1) == 1 and (tok is None or x.stride(tok) < _MAX_TOKEN_STRIDE or x.shape[tok] == 1):
         return x
+    if tok is not None and x.shape[tok] != 1 and math.prod(x.shape[tok + 1:]) >= _MAX_TOKEN_STRIDE:
+        raise ValueError(f"tokens of {tuple(x.shape[tok + 1:])} are too wide: below {_MAX_TOKEN_STRIDE} values are supported")
     return x.contiguous()
 
 
@@ -271,8 +275,8 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=
     """Selective state space scan over [B, T, channels] prompts.
 
     u, delta, z: [B, T, Dm] (z: the gate, or None); A: float32 [Dm, N]; B, C: [B, T, N], or
-    [B, T, G, N] where G groups of Dm / G consecutive channels share theirs; D, delta_bias: float32
-    [Dm] or None; N at most 64.  dt is softplus(delta + delta_bias), or delta + delta_bias without
+    [B, T, G, N] where G groups of Dm / G consecutive channels share theirs (G N below 2^22 where T > 1);
+    D, delta_bias: float32 [Dm] or None; N at most 64.  dt is softplus(delta + delta_bias), or delta + delta_bias without
     delta_softplus.  initial_state: [B, Dm, N] or None (zeros).  out: optional [B, T, Dm] buffer
     in u's dtype that overlaps no input, for calls without gradients.  Returns (y [B, T, Dm] in u's
     dtype, final state float32 [B, Dm, N]).
