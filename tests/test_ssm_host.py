@@ -222,3 +222,13 @@ def test_tokens_wider_than_the_kernels_address():
     with pytest.raises(ValueError, match="too wide"):
         _rows(B[0], 0)
     assert _rows(B[:, :1, :4], 1).shape == (1, 1, 4, 64) and _rows(B[:, :, : (1 << 16) - 1, :8], 1).is_contiguous()
+
+
+def test_grids_past_32_bits_of_threads():
+    """Channel groups of one channel make a workgroup each, sixteen waves above 32 states: 2^32 threads are refused,
+    not launched."""
+    wide = dict(st=(ctypes.c_int64 * 14)(*([4096] * 14)), T=1, total=1024, n=1024, Bn=1024, rows=1024, Dm=4096, G=4096, N=64)
+    big, ws = L.lib().triune_hip_ssm_bwd_workspace_size(1024, 1, 4096, 4096, 64, 0), FAKE
+    assert caller("triune_hip_ssm_scan", SCAN, **{**_scan_base(SCAN), **wide})() == SHAPE
+    assert caller("triune_hip_ssm_scan_varlen", VARLEN, **{**_scan_base(VARLEN), **wide})() == SHAPE
+    assert caller("triune_hip_ssm_bwd", BWD, **{**_scan_base(BWD), **wide})(ws=ws, wsb=big) == SHAPE

@@ -50,6 +50,17 @@ bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
 int64_t group_blocks(int64_t Dm, int64_t G) { return (Dm / G + 63) / 64; }
 int64_t all_blocks(int64_t Dm, int64_t G) { return G * group_blocks(Dm, G); }
 
+// Whether n workgroups per channel block are a grid: 31 bits of workgroups and 32 of threads.
+bool grid_ok(int64_t n, int64_t blocks, int threads) {
+    const int64_t by_threads = (int64_t)0xffffffff / threads, most = by_threads < kMaxGrid ? by_threads : kMaxGrid;
+    return n <= most / blocks;
+}
+// The grids of a scan: its work items, and the join's blocks of up to sixteen waves.
+bool scan_grids_ok(int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int64_t G, int N) {
+    return grid_ok(n_work, all_blocks(Dm, G), 64 * ssm_waves(N)) && n_seqs <= kMaxGrid / (Dm * N) &&
+           (nseg <= 1 || grid_ok(n_seqs * N, (Dm + 63) / 64, 1024));
+}
+
 // Waves a compute unit (four SIMDs) that a call has without splitting the time axis for that to be left,
 // and that it gets where it is split.  Two waves on a SIMD keep it three quarters busy; splitting costs the
 // decays a second time.  8 x 2048 tokens of 4096 channels, N = 16: 306 us unsplit with eight waves a unit, 445
@@ -184,7 +195,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
     if (Bn == 0) return TRIUNE_OK;
     if (T == 0) return s_final ? status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream)) : TRIUNE_OK;
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags, 3);
-    if (p.n_work > kMaxGrid / all_blocks(Dm, G) || Bn > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(p.n_work, p.nseg, Bn, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, strides[0], strides[1]};
@@ -228,7 +239,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
     if (n_seqs == 0) return TRIUNE_OK;
     // with no tokens every sequence's state still passes through: one empty segment each
     const ScanPlan p = plan_packed(n_seqs, total_tokens > 0 ? total_tokens : 1, Dm, G, N, flags);
-    if (p.n_work > kMaxGrid / all_blocks(Dm, G) || n_seqs > kMaxGrid / (Dm * N)) return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(p.n_work, p.nseg, n_seqs, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, 0, strides[0]};
@@ -271,8 +282,7 @@ int triune_hip_ssm_bwd(const void* u, const void* delta, const void* z, const vo
         return TRIUNE_ERR_LAYOUT;
     if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]})) return TRIUNE_ERR_LAYOUT;
     const BwdPlan p = plan_bwd(Bn, T, Dm, G, N, flags);
-    if (p.s.n_work > kMaxGrid / all_blocks(Dm, G) || Bn > kMaxGrid / (Dm * N) || Bn * T > kMaxGrid / (G * N))
-        return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(p.s.n_work, p.s.nseg, Bn, Dm, G, N) || Bn * T > kMaxGrid / (G * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     char* ws = (char*)workspace;
     SsmBwdParams g{};
