@@ -232,3 +232,25 @@ def test_grids_past_32_bits_of_threads():
     assert caller("triune_hip_ssm_scan", SCAN, **{**_scan_base(SCAN), **wide})() == SHAPE
     assert caller("triune_hip_ssm_scan_varlen", VARLEN, **{**_scan_base(VARLEN), **wide})() == SHAPE
     assert caller("triune_hip_ssm_bwd", BWD, **{**_scan_base(BWD), **wide})(ws=ws, wsb=big) == SHAPE
+
+
+@pytest.mark.parametrize("N,split,whole", [
+    (16, [256, 304], [320, 352, 448, 504, 512]), (8, [512], [640, 768]), (32, [128], [160, 192]), (64, [64, 128], [160, 192])])
+def test_scans_are_split_where_that_is_faster(N, split, whole):
+    """Workgroups (8 prompts of 2048 tokens) on both sides of the measured crossover."""
+    size = L.lib().triune_hip_ssm_scan_workspace_size
+    for wgs in split:
+        assert size(8, 2048, wgs * 8, 1, N, 0) > 0, wgs
+    for wgs in whole:
+        assert size(8, 2048, wgs * 8, 1, N, 0) == 0, wgs
+
+
+@pytest.mark.parametrize("N,split,whole", [
+    (16, [256, 320, 400], [448, 504, 512]), (8, [512, 640], [832, 1024]), (32, [128, 160, 192], [208, 240]),
+    (64, [64, 128, 160], [192, 240])])
+def test_gradients_are_split_where_that_is_faster(N, split, whole):
+    size, unsplit = L.lib().triune_hip_ssm_bwd_workspace_size, 255 << 8
+    for wgs in split:
+        assert size(8, 2048, wgs * 8, 1, N, 0) > size(8, 2048, wgs * 8, 1, N, unsplit), wgs
+    for wgs in whole:
+        assert size(8, 2048, wgs * 8, 1, N, 0) == size(8, 2048, wgs * 8, 1, N, unsplit), wgs

@@ -61,13 +61,19 @@ bool scan_grids_ok(int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int
            (nseg <= 1 || grid_ok(n_seqs * N, (Dm + 63) / 64, 1024));
 }
 
-// Waves a compute unit (four SIMDs) that a call has without splitting the time axis for that to be left,
-// and that it gets where it is split.  Two waves on a SIMD keep it three quarters busy; splitting costs the
-// decays a second time.  8 x 2048 tokens of 4096 channels, N = 16: 306 us unsplit with eight waves a unit, 445
-// split.  Split calls take shares that several rounds of workgroups even out: 1 x 16384 of 768 channels 106 us for
+// A chip's worth of workgroups is eight waves a compute unit (four SIMDs); two waves on a SIMD keep it three quarters
+// busy.  Calls below the shares here split the time axis, which costs the decays a second time: unsplit they
+// take as long for one workgroup as for the whole chip, split their time follows the work.  bf16, 8 x 2048 tokens, us
+// unsplit and split, by workgroups:
+//   outputs    N = 16: 256 230 234, 320 305 302, 352 304 320, 448 307 395, 504 308 446;  N = 8: 512 346 335, 640 348 427;
+//              N = 32: 128 295 260, 160 296 333;  N = 64: 128 591 541, 160 591 725
+//   gradients  N = 16: 320 1052 844, 400 1058 1006, 448 1058 1099, 504 1067 1240;  N = 8: 640 1522 1487, 768 1544 1761;
+//              N = 32: 192 1231 1188, 240 1236 1457;  N = 64: 160 3549 2975, 240 3738 4337
+// Split calls take shares that several rounds of workgroups even out: 1 x 16384 of 768 channels 106 us for
 // 24 to 48 waves (segments of 128 and 64 tokens), 122 for 16; 16 ragged prompts of 5034 tokens, 1536 channels: 86 for
 // 32, 91 for 24, 97 for 14, 87 for 64.
 constexpr int kEnoughWaves = 8, kSplitWaves = 32;
+constexpr int kForwardShare = 10, kGradientShare = 13;  // sixteenths of the chip's workgroups
 // Workgroups of `waves` waves a compute unit.
 int64_t ssm_slots(int N, int waves) {
     const int nw = ssm_waves(N);
@@ -77,12 +83,14 @@ int64_t ssm_slots(int N, int waves) {
 int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * SSM_UNIT; }
 
 // Tokens of a segment of a dense call (a multiple of SSM_UNIT; the whole sequence unless splitting
-// pays).  Splitting reads and decays every token twice, so `least` segments have to fit the chip.
-int64_t dense_segment(int64_t n_seqs, int64_t T, int64_t blocks, int N, int flags, int64_t least) {
+// pays).  Two segments pay only where the sequence is short: `least` is the number that its length has to give, of
+// which the chip has to hold three (gradients of 192 workgroups at N = 64: 4229 us in two segments, 3650 unsplit).
+int64_t dense_segment(int64_t n_seqs, int64_t T, int64_t blocks, int N, int flags, int share, int64_t least) {
     const int64_t whole = (T + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
     if (forced_segment(flags)) return forced_segment(flags) < whole ? forced_segment(flags) : whole;
-    if (n_seqs * blocks >= ssm_slots(N, kEnoughWaves)) return whole;
+    if (16 * n_seqs * blocks >= share * ssm_slots(N, kEnoughWaves)) return whole;
     int64_t n = ssm_slots(N, kSplitWaves) / (n_seqs * blocks);
+    if (n < 3) return whole;
     const int64_t most = T / 64;
     if (n > most) n = most;
     if (n < least) return whole;
@@ -102,9 +110,10 @@ void plan_bytes(ScanPlan& p, int64_t Dm, int N, int64_t n_off) {
     p.total = p.off_seg + align_up((size_t)n_off * 4);
 }
 
-ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int flags, int64_t least) {
+ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int flags, bool gradients = false) {
     ScanPlan p{};
-    p.seg = dense_segment(n_seqs, T, all_blocks(Dm, G), N, flags, least);
+    p.seg = dense_segment(n_seqs, T, all_blocks(Dm, G), N, flags, gradients ? kGradientShare : kForwardShare,
+                          gradients ? 2 : 3);
     p.nseg = (T + p.seg - 1) / p.seg;
     p.n_work = n_seqs * p.nseg;
     plan_bytes(p, Dm, N, 0);
@@ -136,7 +145,7 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags) {
     BwdPlan p{};
-    p.s = plan_scan(Bn, T, Dm, G, N, flags, 2);
+    p.s = plan_scan(Bn, T, Dm, G, N, flags, true);
     p.off_bc = p.s.total;
     p.off_par = p.off_bc + align_up((size_t)all_blocks(Dm, G) * Bn * T * ssm_waves(N) * 8 * 4);
     p.total = p.off_par + align_up((size_t)p.s.n_work * (N + 2) * Dm * 4);
@@ -177,7 +186,7 @@ extern "C" {
 
 size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags) {
     if (Bn <= 0 || T <= 0 || !tokens_ok(Bn, T) || !ssm_shape_ok(Dm, G, N)) return 0;
-    return plan_scan(Bn, T, Dm, G, N, flags, 3).total;
+    return plan_scan(Bn, T, Dm, G, N, flags).total;
 }
 
 int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const void* B, const void* C, const float* A,
@@ -194,7 +203,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
         return TRIUNE_ERR_LAYOUT;
     if (Bn == 0) return TRIUNE_OK;
     if (T == 0) return s_final ? status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream)) : TRIUNE_OK;
-    const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags, 3);
+    const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags);
     if (!scan_grids_ok(p.n_work, p.nseg, Bn, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
