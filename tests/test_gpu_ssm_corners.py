@@ -206,3 +206,38 @@ def test_wide_slots_are_outside_the_pool(dev):
         for bad in (near.float(), near >= 0):
             with pytest.raises(TypeError, match="slots"):
                 call(s.clone(), bad)
+
+
+# ---- packed prompts, one far longer than the rest -----------------------------------------------------------
+@pytest.mark.parametrize("place", [0, 30, 65])
+@torch.no_grad()
+def test_one_long_prompt_among_many_short_ones(dev, place):
+    """Sequences enough to fill the chip, of which two are cut: states in a pool, one row padded, lengths on both
+    sides of the longest that stays whole (512) and of a segment (128), empty ones."""
+    lens = [ln for ln in (0, 1, 40, 128, 129, 512, 513, 33) for _ in range(2)] + [7, 19, 0, 64, 31] * 10
+    lens[place:place] = [5001]
+    n, D, N, total = len(lens), 1000, 16, sum(lens)
+    assert S.plan_on(torch.zeros(1, device=dev), "triune_hip_ssm_scan_varlen_workspace_size", n, total, D, 1, N, 0) > 0
+    g = torch.Generator().manual_seed(place)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    u, delta, Bm, C, z = rn(total, D), rn(total, D) - 4, rn(total, N), rn(total, N), rn(total, D)
+    A, Dp, pool = -torch.exp(rn(D, N)), rn(D), rn(n + 2, D, N)
+    before, slots = pool.clone(), torch.randperm(n + 2, generator=g)[:n].to(torch.int32)
+    pad = lens.index(129)
+    slots[pad] = -1
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    y, _ = ssm_scan_varlen(u, delta, A, Bm, C, cu.to(dev), Dp, z, state_pool=pool, slots=slots.to(dev))
+    near = [i for i, ln in enumerate(lens) if ln > 100] + [i for i, ln in enumerate(lens) if ln <= 40][::7]
+    for i in near:
+        c, sl = slice(int(cu[i]), int(cu[i + 1])), int(slots[i])
+        s0 = None if sl < 0 else before[sl:sl + 1]
+        part = [t[None, c] for t in (u, delta)] + [A] + [t[None, c] for t in (Bm, C)]
+        ry, rs, ey, es, _ = R.scan(*part, Dp, z[None, c], s0=s0)
+        R.near(y[None, c], ry, ey, F32, f"sequence {i} of {lens[i]}")
+        if sl >= 0:
+            R.near(pool[sl:sl + 1], rs, es, F32, f"state {i} of {lens[i]}")
+    rest = [r for r in range(n + 2) if r not in slots.tolist()]
+    assert torch.equal(pool[rest], before[rest])
+    again = before.clone()
+    y2, _ = ssm_scan_varlen(u, delta, A, Bm, C, cu.to(dev), Dp, z, state_pool=again, slots=slots.to(dev))
+    assert torch.equal(y, y2) and torch.equal(pool, again)

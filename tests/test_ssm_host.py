@@ -254,3 +254,12 @@ def test_gradients_are_split_where_that_is_faster(N, split, whole):
         assert size(8, 2048, wgs * 8, 1, N, 0) > size(8, 2048, wgs * 8, 1, N, unsplit), wgs
     for wgs in whole:
         assert size(8, 2048, wgs * 8, 1, N, 0) == size(8, 2048, wgs * 8, 1, N, unsplit), wgs
+
+
+def test_packed_scans_with_one_long_prompt_are_cut():
+    """Sequences enough for two rounds of the chip: 42 of 64 tokens and one of 16384 (1536 channels) have room for
+    segments, calls of few tokens have none and need none."""
+    size = L.lib().triune_hip_ssm_scan_varlen_workspace_size
+    assert size(43, 42 * 64 + 16384, 1536, 1, 16, 0) > 43 * 17 * 1536 * 4
+    assert size(201, 28000, 1536, 1, 16, 0) > 201 * 17 * 1536 * 4
+    assert size(100, 3000, 1536, 1, 16, 0) == 0 and size(43, 43, 1536, 1, 16, 0) == 0

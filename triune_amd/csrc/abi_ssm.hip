@@ -98,7 +98,7 @@ int64_t dense_segment(int64_t n_seqs, int64_t T, int64_t blocks, int N, int flag
 }
 
 struct ScanPlan {
-    int64_t seg, nseg, n_work;
+    int64_t seg, nseg, n_work, cut;
     size_t off_sum, off_seg, total;
 };
 
@@ -120,19 +120,30 @@ ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int 
     return p;
 }
 
-// Packed: lengths are on the device, so a segment is an equal share of all tokens, unless there are
-// sequences enough for two rounds of the chip.  nseg > 1 says that there are segments.
+// Packed: lengths are on the device, so a segment is an equal share of all tokens.  Where there are sequences enough
+// for two rounds of the chip they fill it by themselves, but for one far longer than the rest, which its
+// workgroups would walk alone: sequences up to twice a workgroup's share of one round stay whole, and longer ones are cut
+// into halves of it.  1536 channels, N = 16, bf16, us with every sequence whole and by this rule: 42 prompts of 64
+// tokens and one of 16384 1730 and 259, and one of 2048 251 and 78; 200 of 100 and one of 8000 1047 and 341; 48
+// log-uniform up to 8192 1139 and 965, 64 up to 2048 341 and 364.  Even lengths pay the launches that find
+// nothing to do: 43 of 512 166 and 174, 200 of 256 308 and 312, 256 of 64 111 and 127, 64 of 100 57 and 66, so calls
+// of few tokens stay whole (100 of 30: 37 and 45).  nseg > 1 says that there are segments.
 ScanPlan plan_packed(int64_t n_seqs, int64_t total, int64_t Dm, int64_t G, int N, int flags) {
     ScanPlan p{};
-    const int64_t whole = (total + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT, blocks = all_blocks(Dm, G);
-    const int64_t slots = ssm_slots(N, kSplitWaves);
+    const int64_t blocks = all_blocks(Dm, G), slots = ssm_slots(N, kSplitWaves);
     p.seg = forced_segment(flags);
     if (!p.seg) {
         p.seg = (total * blocks / slots + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
         if (p.seg < 64) p.seg = 64;
-        if (n_seqs * blocks >= 2 * ssm_slots(N, kEnoughWaves)) p.seg = whole;
+        const int64_t round = ssm_slots(N, kEnoughWaves);
+        if (n_seqs * blocks >= 2 * round) {
+            const int64_t share = total * blocks / round < 256 ? 256 : total * blocks / round;
+            p.seg = (share / 2 + SSM_UNIT - 1) / SSM_UNIT * SSM_UNIT;
+            p.cut = total <= 4096 ? total : 2 * share;
+        }
     }
-    p.nseg = p.seg < whole ? 2 : 1;
+    if (p.cut < p.seg) p.cut = p.seg;
+    p.nseg = p.cut < total ? 2 : 1;
     p.n_work = p.nseg > 1 ? total / p.seg + n_seqs : n_seqs;
     plan_bytes(p, Dm, N, n_seqs + 1);
     return p;
@@ -160,6 +171,7 @@ void set_sizes(SsmParams& a, int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, i
     a.N = N;
     a.blocks = (int)group_blocks(Dm, G);
     a.seg = (int)p.seg;
+    a.cut = p.cut;
     a.nseg = (int)p.nseg;
     a.n_work = p.n_work;
     if (p.nseg > 1) {

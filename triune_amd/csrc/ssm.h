@@ -38,8 +38,10 @@ struct SsmParams {
     int Dm, G, N;
     int blocks;               // channel blocks of a group
     int seg, nseg;            // tokens of a segment, segments of a dense sequence
+    int64_t cut;              // packed: sequences of more tokens than this are cut into segments
     int64_t n_work;
     const int32_t *cu, *seg_off;  // packed: [n_seqs + 1] token and segment offsets
+    bool by_followed;         // the join's blocks are laid out by the segments that another one follows
 };
 
 struct SsmBwdParams {
@@ -357,6 +359,17 @@ struct SsmSeg {
     int len, index;
     bool last;
 };
+// The packed sequence of the j-th segment that another one follows, of all sequences: seg_off[i] - i of them are in
+// front of sequence i.  -1 when there are not so many.
+__device__ __forceinline__ int64_t ssm_followed(const SsmParams& a, int64_t j) {
+    if (j >= a.seg_off[a.n_seqs] - a.n_seqs) return -1;
+    int64_t lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+        const int64_t m = (lo + hi) >> 1;
+        if (a.seg_off[m] - m <= j) lo = m; else hi = m;
+    }
+    return lo;
+}
 __device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSeg& s) {
     if (!a.cu) {
         s.seq = w / a.nseg;
@@ -387,8 +400,7 @@ __device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSe
     s.index = (int)(w - first);
     s.row0 = beg;
     s.t0 = (int64_t)s.index * a.seg;
-    s.len = (int)min((int64_t)a.seg, n - s.t0);
-    if (s.len < 0) s.len = 0;
+    s.len = (int)(s.last ? max(n - s.t0, (int64_t)0) : a.seg);
     return true;
 }
 

@@ -44,10 +44,16 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
     __shared__ __attribute__((aligned(16))) float s_y[STATES ? 1 : NW][STATES ? 1 : TT][64];
 
     const int nblk = a.G * a.blocks;
-    const int64_t work = blockIdx.x / nblk;
+    int64_t work = blockIdx.x / nblk;
     const int cb = (int)(blockIdx.x - work * nblk);
+    if (STATES && a.cu) {
+        const int64_t seq = ssm_followed(a, work);
+        if (seq < 0) return;
+        work += seq;
+    }
     SsmSeg sg;
     if (!ssm_segment(a, work, sg)) return;
+    if (STATES && sg.last) return;  // nothing follows that would start from its end
     const int Dg = a.Dm / a.G, grp = cb / a.blocks, c0 = (cb - grp * a.blocks) * 64;
     const int lane = threadIdx.x & 63, w = wave_index(), n0 = NS * w;
     // the walk's channel; lanes past the group's channels repeat its first and store nothing
@@ -81,7 +87,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
     }
     const int64_t row = STATES ? 0 : ssm_row(a.slots, a.n_slots, sg.seq);
     if constexpr (!STATES) {
-        if (a.ws_state) {  // segmented: the entering state comes from the scan over segments
+        if (a.ws_state && !(sg.last && sg.index == 0)) {  // segmented: the entering state comes from the scan over segments
 #pragma unroll
             for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) h[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
@@ -261,13 +267,21 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
     __shared__ float s_sum[16][64], s_end[16][64];
     const int lane = threadIdx.x & 63, w = wave_index(), waves = blockDim.x >> 6;
     const int cb = (a.Dm + 63) / 64;
-    const int64_t sn = blockIdx.x / cb, seq = sn / a.N;
+    const int64_t sn = blockIdx.x / cb;
+    int64_t seq = sn / a.N;
     const int n = (int)(sn - seq * a.N), c = (int)(blockIdx.x - sn * cb) * 64 + lane;
+    if (a.by_followed) {  // the block of a sequence's first segment takes the sequence
+        const int64_t j = seq;
+        seq = ssm_followed(a, j);
+        if (seq < 0 || a.seg_off[seq] - seq != j) return;
+    }
     const bool chv = c < a.Dm;
     const int ch = chv ? c : 0;
     const int64_t per = (int64_t)a.N * a.Dm, at = (int64_t)ch * a.N + n;
     int64_t first = seq * a.nseg, count = a.nseg;
     if (a.cu) first = a.seg_off[seq], count = min((int64_t)a.seg_off[seq + 1], a.n_work) - first;
+    if (a.cu && count == 1) return;
+    const int64_t from = BACK ? count : count - 1;  // segments whose own result is there
     const float Al = log2_decay(a.A[at]);
     const int64_t row = ssm_row(a.slots, a.n_slots, seq);
     float S = init && row >= 0 ? init[row * per + at] : 0.f;
@@ -281,8 +295,8 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int64_t v = BACK ? v0 - i : v0 + i;
-            local[i] = i < m ? p[v * per] : 0.f;
-            sum[i] = i < m ? ps[v * a.Dm] : 0.f;
+            local[i] = k + i < from ? p[v * per] : 0.f;
+            sum[i] = k + i < from ? ps[v * a.Dm] : 0.f;
         }
         float all = 0.f, end = 0.f;
 #pragma unroll
@@ -323,7 +337,7 @@ __global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int32_t* o
         if (i < a.n_seqs) {
             const int64_t beg = min(max((int64_t)a.cu[i], (int64_t)0), a.T);
             const int64_t len = min(max((int64_t)a.cu[i + 1], beg), a.T) - beg;
-            n = max((len + a.seg - 1) / a.seg, (int64_t)1);
+            n = len > a.cut ? (len + a.seg - 1) / a.seg : 1;
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
@@ -398,7 +412,8 @@ __global__ __launch_bounds__(256) void ssm_step_kernel(SsmStepParams a, int bloc
 
 template <typename T, int V, bool STATES>
 static hipError_t scan_waves(const SsmParams& a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.n_work * a.G * a.blocks));
+    const int64_t work = STATES && a.cu ? a.n_work - a.n_seqs : a.n_work;  // packed: those that another segment follows
+    const dim3 grid((unsigned)(work * a.G * a.blocks));
     switch (ssm_waves(a.N)) {
         case 1: ssm_scan_kernel<T, 1, V, STATES><<<grid, 64, 0, s>>>(a); break;
         case 2: ssm_scan_kernel<T, 2, V, STATES><<<grid, 128, 0, s>>>(a); break;
@@ -426,8 +441,12 @@ static hipError_t carry(const SsmParams& a, const float* init, float* out, hipSt
     // 8.9 us so, 14.5 with waves for four times as many)
     const int64_t segs = a.cu ? (a.n_work + a.n_seqs - 1) / a.n_seqs : a.nseg;
     const int waves = segs <= 8 ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
-    const int64_t blocks = a.n_seqs * a.N * ((a.Dm + 63) / 64);
-    ssm_carry_kernel<BACK><<<dim3((unsigned)blocks), 64 * waves, 0, s>>>(a, init, out);
+    // Packed: sequences of one segment need no join, so where fewer segments are followed by another than there are
+    // sequences, blocks are laid out by those (256 prompts of 64 tokens: 127 us a call, 155 by sequences).
+    SsmParams b = a;
+    b.by_followed = a.cu && a.n_work - a.n_seqs < a.n_seqs;
+    const int64_t blocks = (b.by_followed ? a.n_work - a.n_seqs : a.n_seqs) * a.N * ((a.Dm + 63) / 64);
+    ssm_carry_kernel<BACK><<<dim3((unsigned)blocks), 64 * waves, 0, s>>>(b, init, out);
     return hipGetLastError();
 }
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s) { return carry<false>(a, a.s0, nullptr, s); }
