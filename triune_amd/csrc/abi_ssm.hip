@@ -171,7 +171,6 @@ void set_sizes(SsmParams& a, int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, i
     a.N = N;
     a.blocks = (int)group_blocks(Dm, G);
     a.seg = (int)p.seg;
-    a.cut = p.cut;
     a.nseg = (int)p.nseg;
     a.n_work = p.n_work;
     if (p.nseg > 1) {
@@ -275,7 +274,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
     const hipStream_t s = (hipStream_t)stream;
     if (p.nseg > 1) {
         int32_t* off = (int32_t*)((char*)workspace + p.off_seg);
-        if (const int e = status(launch_ssm_offsets(a, off, s))) return e;
+        if (const int e = status(launch_ssm_offsets(a, p.cut, off, s))) return e;
         a.seg_off = off;
         if (const int e = status(launch_ssm_states(a, io_dtype, s))) return e;
         if (const int e = status(launch_ssm_carry(a, s))) return e;

@@ -38,10 +38,8 @@ struct SsmParams {
     int Dm, G, N;
     int blocks;               // channel blocks of a group
     int seg, nseg;            // tokens of a segment, segments of a dense sequence
-    int64_t cut;              // packed: sequences of more tokens than this are cut into segments
     int64_t n_work;
     const int32_t *cu, *seg_off;  // packed: [n_seqs + 1] token and segment offsets
-    bool by_followed;         // the join's blocks are laid out by the segments that another one follows
 };
 
 struct SsmBwdParams {
@@ -80,7 +78,8 @@ inline bool ssm_by_four(int group_channels, int io_dt, std::initializer_list<Ssm
 }
 // n elements of `bytes` (2 or 4) from one state tensor to another, zeros without a source: calls without tokens.
 hipError_t launch_state_copy(const void* from, void* to, int64_t n, int bytes, hipStream_t s);
-hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* seg_off, hipStream_t s);
+// Sequences of more than `cut` tokens are cut into segments.
+hipError_t launch_ssm_offsets(const SsmParams& a, int64_t cut, int32_t* seg_off, hipStream_t s);
 hipError_t launch_ssm_states(const SsmParams& a, int io_dt, hipStream_t s);
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s);
 hipError_t launch_ssm_scan(const SsmParams& a, int io_dt, hipStream_t s);
@@ -228,15 +227,17 @@ __device__ __forceinline__ void store_dt(void* p, int dt, int64_t i, float x) {
     else ((_Float16*)p)[i] = (_Float16)x;
 }
 
-// x with infinities cut to the largest numbers of their signs.
-__device__ __forceinline__ float finite(float x) {
-    const float most = 3.4028234e38f;
+// A in units of the hardware's exp2.  Infinite values are cut to the largest number, so that a step of 0
+// (a token past a tile's end) is a decay of 1 for them too.
+__device__ __forceinline__ float log2_decay(float A) {
+    const float x = A * LOG2E, most = 3.4028234e38f;
     return x < -most ? -most : x > most ? most : x;
 }
 
-// A in units of the hardware's exp2.  Infinite values are cut, so that a step of 0 (a token past a tile's
-// end) is a decay of 1 for them too.
-__device__ __forceinline__ float log2_decay(float A) { return finite(A * LOG2E); }
+// A as a factor of p = dh a h_{t-1} in the gradient.  Past 1e30 every step above 1e-28 has a decay, and a p, of
+// 0, whose product with an infinite A has to be 0; at a step of 0 the product stays finite, and softplus' slope of 0
+// takes it.
+__device__ __forceinline__ float slope_decay(float A) { return A < -1e30f ? -1e30f : A > 1e30f ? 1e30f : A; }
 
 // 2^x as m 2^e with m in (1/2, 1], for a decay product over a segment: modes that grow (A > 0, or steps below
 // 0) take it past the largest number where the state that it scales, 0 or small, stays within.  scale(v) = v 2^x
@@ -244,6 +245,7 @@ __device__ __forceinline__ float log2_decay(float A) { return finite(A * LOG2E);
 struct Pow2 {
     float m;
     int e;
+    __device__ __forceinline__ Pow2(float m, int e) : m(m), e(e) {}
     __device__ __forceinline__ explicit Pow2(float x) {
         x = x < -300.f ? -300.f : x > 300.f ? 300.f : x;
         const float c = __builtin_ceilf(x);

@@ -262,15 +262,16 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
 // waves before it leave.  128 segments of 768 channels, N = 16: 7.0 us; a thread per channel with eight
 // segments in flight 15.7.
 template <bool BACK>
-__global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const float* init, float* out) {
+__global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const float* init, float* out, bool by_followed) {
     constexpr int PER = 8;  // segments of a wave
-    __shared__ float s_sum[16][64], s_end[16][64];
+    __shared__ float s_m[16][64], s_end[16][64];  // a wave's decay (mantissa, exponent) and its end from zero
+    __shared__ int s_e[16][64];
     const int lane = threadIdx.x & 63, w = wave_index(), waves = blockDim.x >> 6;
     const int cb = (a.Dm + 63) / 64;
     const int64_t sn = blockIdx.x / cb;
     int64_t seq = sn / a.N;
     const int n = (int)(sn - seq * a.N), c = (int)(blockIdx.x - sn * cb) * 64 + lane;
-    if (a.by_followed) {  // the block of a sequence's first segment takes the sequence
+    if (by_followed) {  // the block of a sequence's first segment takes the sequence
         const int64_t j = seq;
         seq = ssm_followed(a, j);
         if (seq < 0 || a.seg_off[seq] - seq != j) return;
@@ -304,16 +305,17 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
             end = Pow2(sum[i] * Al).scale(end) + local[i];
             all += sum[i];
         }
+        const Pow2 own(all * Al);
         if (waves > 1) {
-            s_sum[w][lane] = all;
+            s_m[w][lane] = own.m;
+            s_e[w][lane] = own.e;
             s_end[w][lane] = end;
             __syncthreads();
         }
         float next = S;
         for (int q = 0; q < waves; ++q) {
             if (q == w) S = next;
-            const float d = waves > 1 ? s_sum[q][lane] : all, e = waves > 1 ? s_end[q][lane] : end;
-            next = Pow2(d * Al).scale(next) + e;
+            next = waves > 1 ? Pow2(s_m[q][lane], s_e[q][lane]).scale(next) + s_end[q][lane] : own.scale(next) + end;
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const floa
 }
 
 // Packed calls: seg_off[i] = segments of the sequences before i (one at least for each).  One wave.
-__global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int32_t* off) {
+__global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int64_t cut, int32_t* off) {
     const int lane = threadIdx.x;
     int64_t base = 0;
     if (lane == 0) off[0] = 0;
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int32_t* o
         if (i < a.n_seqs) {
             const int64_t beg = min(max((int64_t)a.cu[i], (int64_t)0), a.T);
             const int64_t len = min(max((int64_t)a.cu[i + 1], beg), a.T) - beg;
-            n = len > a.cut ? (len + a.seg - 1) / a.seg : 1;
+            n = len > cut ? (len + a.seg - 1) / a.seg : 1;
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
@@ -437,23 +439,23 @@ hipError_t launch_ssm_scan(const SsmParams& a, int dt, hipStream_t s) { return s
 
 template <bool BACK>
 static hipError_t carry(const SsmParams& a, const float* init, float* out, hipStream_t s) {
-    // waves for the segments of a sequence, the average one of a packed call (16 ragged prompts, 68 segments:
-    // 8.9 us so, 14.5 with waves for four times as many)
+    // Waves for the segments of a sequence.  Packed calls know the average alone and take two waves from five segments
+    // on: 16 ragged prompts of 5034 tokens (6 segments, the longest 23) 84 us a call with one wave, 81 with two, 82 with
+    // four, 90 with eight; 20 of 300 tokens (6) 54, 56, 59, 68; three, one of them of 5000 (28), 62, 54, 52, 51.
     const int64_t segs = a.cu ? (a.n_work + a.n_seqs - 1) / a.n_seqs : a.nseg;
-    const int waves = segs <= 8 ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
+    const int waves = segs <= (a.cu ? 4 : 8) ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
     // Packed: sequences of one segment need no join, so where fewer segments are followed by another than there are
     // sequences, blocks are laid out by those (256 prompts of 64 tokens: 127 us a call, 155 by sequences).
-    SsmParams b = a;
-    b.by_followed = a.cu && a.n_work - a.n_seqs < a.n_seqs;
-    const int64_t blocks = (b.by_followed ? a.n_work - a.n_seqs : a.n_seqs) * a.N * ((a.Dm + 63) / 64);
-    ssm_carry_kernel<BACK><<<dim3((unsigned)blocks), 64 * waves, 0, s>>>(b, init, out);
+    const bool by_followed = a.cu && a.n_work - a.n_seqs < a.n_seqs;
+    const int64_t blocks = (by_followed ? a.n_work - a.n_seqs : a.n_seqs) * a.N * ((a.Dm + 63) / 64);
+    ssm_carry_kernel<BACK><<<dim3((unsigned)blocks), 64 * waves, 0, s>>>(a, init, out, by_followed);
     return hipGetLastError();
 }
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s) { return carry<false>(a, a.s0, nullptr, s); }
 hipError_t launch_ssm_bwd_carry(const SsmBwdParams& g, hipStream_t s) { return carry<true>(g.f, g.dfin, g.ds0, s); }
 
-hipError_t launch_ssm_offsets(const SsmParams& a, int32_t* off, hipStream_t s) {
-    ssm_offsets_kernel<<<1, 64, 0, s>>>(a, off);
+hipError_t launch_ssm_offsets(const SsmParams& a, int64_t cut, int32_t* off, hipStream_t s) {
+    ssm_offsets_kernel<<<1, 64, 0, s>>>(a, cut, off);
     return hipGetLastError();
 }
 

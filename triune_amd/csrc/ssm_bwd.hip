@@ -204,9 +204,9 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : NW == 1 ? 1 : 2) void ssm_b
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
         const bool ok = chv && n0 + j < a.N;  // lanes without a channel add zeros to dB and dC
-        // cut as Al is: where the decay is 0, so is p, and p A has to be
-        A[j] = ok ? finite(a.A[(int64_t)ch * a.N + n0 + j]) : 0.f;
-        Al[j] = log2_decay(A[j]);
+        const float Aj = ok ? a.A[(int64_t)ch * a.N + n0 + j] : 0.f;
+        A[j] = slope_decay(Aj);
+        Al[j] = log2_decay(Aj);
         dA[j] = e[j] = 0.f;
         if (ok && a.nseg > 1) e[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
         else if (ok && g.dfin) e[j] = g.dfin[(sg.seq * a.Dm + ch) * a.N + n0 + j];
@@ -380,10 +380,7 @@ __global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : NW == 1 ? 1 : 2) void ssm_b
                 for (int j = 0; j < V; ++j) {
                     const float uu = (float)cu[i].v[j];
                     o[j] = __builtin_fmaf(s1[j], uu, s2[j]);
-                    if (a.softplus) {  // a step of 0 has no slope, though p A of an infinite A may pass the range
-                        const float slope = fast_sigmoid((float)cd[i].v[j] + bias[j]);
-                        o[j] = slope == 0.f ? 0.f : o[j] * slope;
-                    }
+                    if (a.softplus) o[j] *= fast_sigmoid((float)cd[i].v[j] + bias[j]);
                     dD[j] = __builtin_fmaf(gy[j], uu, dD[j]);
                     db[j] += t0 + t < sg.len ? o[j] : 0.f;
                 }
