@@ -241,3 +241,62 @@ def test_one_long_prompt_among_many_short_ones(dev, place):
     again = before.clone()
     y2, _ = ssm_scan_varlen(u, delta, A, Bm, C, cu.to(dev), Dp, z, state_pool=again, slots=slots.to(dev))
     assert torch.equal(y, y2) and torch.equal(pool, again)
+
+
+# ---- one token's terms at a time ----------------------------------------------------------------------------
+@pytest.mark.parametrize("units", [0, 1])
+def test_gradients_of_single_tokens_of_a_long_prompt(dev, units):
+    """Upstream at one token and input at one: dC, dB, dA and the rest hold that pair's terms alone, with the roundings
+    of the tokens between, so a term that a tile or segment drops or takes twice shows, which a bound on the sum over
+    thousands of tokens would let pass."""
+    T, D, N = 4430, 12, 5
+    g = torch.Generator().manual_seed(1)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    for src, dst in ((0, 0), (0, 31), (31, 32), (2047, 2049), (2015, 2080), (4416, 4429), (4429, 4429)):
+        u, dy = torch.zeros(1, T, D, device=dev), torch.zeros(1, T, D, device=dev)
+        u[:, src], dy[:, dst] = rn(1, D), rn(1, D)
+        delta, A, Bm, C, Dp = rn(1, T, D) - 5, -torch.exp(rn(D, N)), rn(1, T, N), rn(1, T, N), rn(D)
+        _, _, kept = S._scan(u, delta, A, Bm, C, Dp, None, None, True, None, None, True, units << 8)
+        got = S._scan_bwd(u, delta, A, Bm, C, Dp, None, None, True, kept, dy, None, False, units << 8)
+        form = (u, delta, A, Bm, C, Dp, None, None, True, None, dy, None)
+        for name, x, r, e in zip("u delta A B C D".split(), got, R.scan_grads(*form), R.scan_grads(*form, absolute=True)):
+            R.near(x, r, 24 * (dst - src + 33 + 16) * R.U * e, F32, f"{name} {src} {dst}")
+
+
+# ---- the public training path in a graph --------------------------------------------------------------------
+def test_training_steps_replay_from_a_graph(dev):
+    """Forward and backward of each operator through its public call, captured together and replayed with new inputs
+    and eager steps (on leaves of their own) between."""
+    rn = lambda *s: torch.randn(*s, device=dev)  # noqa: E731
+    B, T, D, N = 2, 200, 70, 16
+    ops = [
+        (lambda x, w, b: (layer_norm(x, w, b),), [rn(B * T, D).to(BF), rn(D).to(BF), rn(D).to(BF)]),
+        (lambda x, w, b, s: short_conv(x, w, b, s), [rn(B, T, D).to(BF), rn(D, 4), rn(D), rn(B, 3, D).to(BF)]),
+        (lambda u, d, A, Bm, C, Dp, z, bias, s: ssm_scan(u, d, A, Bm, C, Dp, z, bias, initial_state=s),
+         [rn(B, T, D), rn(B, T, D), -rn(D, N).exp(), rn(B, T, N), rn(B, T, N), rn(D), rn(B, T, D), rn(D), rn(B, D, N)]),
+    ]
+    for op, data in ops:
+        with torch.no_grad():
+            ups = [torch.randn_like(t) for t in op(*data)]
+
+        def step(inputs, ups=ups, op=op):
+            leaves = [t.detach().requires_grad_() for t in inputs]
+            return torch.autograd.grad(op(*leaves), leaves, ups)
+
+        side = torch.cuda.Stream(device=dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            step(data)
+        torch.cuda.current_stream(dev).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(data)
+        for n in range(3):
+            data[0].copy_(torch.randn(data[0].shape, generator=torch.Generator().manual_seed(n)))
+            for t in out:
+                t.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, step(data)):
+                assert torch.equal(a, b)
+        del graph
