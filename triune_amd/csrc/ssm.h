@@ -354,7 +354,7 @@ __device__ __forceinline__ void lds_add(const float* p, float (&x)[V]) {
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
-// The tokens of work item w: sequence, first token (of the sequence), length, whether it is the
+// The tokens of work item w (of packed sequence seq, searched for where that is negative): sequence, first token (of the sequence), length, whether it is the
 // sequence's last segment.  False when there is no such item (packed calls bound their number).
 struct SsmSeg {
     int64_t seq, row0, t0;  // row0: first token of the sequence in a packed tensor
@@ -372,7 +372,7 @@ __device__ __forceinline__ int64_t ssm_followed(const SsmParams& a, int64_t j) {
     }
     return lo;
 }
-__device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSeg& s) {
+__device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSeg& s, int64_t seq = -1) {
     if (!a.cu) {
         s.seq = w / a.nseg;
         s.index = (int)(w - s.seq * a.nseg);
@@ -386,8 +386,8 @@ __device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSe
     s.last = true;
     if (a.seg_off) {
         if (w >= a.seg_off[a.n_seqs]) return false;
-        lo = 0;
-        int64_t hi = a.n_seqs;  // seg_off[lo] <= w < seg_off[hi]
+        lo = seq < 0 ? 0 : seq;
+        int64_t hi = seq < 0 ? a.n_seqs : seq + 1;  // seg_off[lo] <= w < seg_off[hi]
         while (hi - lo > 1) {
             const int64_t m = (lo + hi) >> 1;
             if (a.seg_off[m] <= w) lo = m; else hi = m;

@@ -46,13 +46,14 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
     const int nblk = a.G * a.blocks;
     int64_t work = blockIdx.x / nblk;
     const int cb = (int)(blockIdx.x - work * nblk);
+    int64_t seq = -1;
     if (STATES && a.cu) {
-        const int64_t seq = ssm_followed(a, work);
+        seq = ssm_followed(a, work);
         if (seq < 0) return;
         work += seq;
     }
     SsmSeg sg;
-    if (!ssm_segment(a, work, sg)) return;
+    if (!ssm_segment(a, work, sg, seq)) return;
     if (STATES && sg.last) return;  // nothing follows that would start from its end
     const int Dg = a.Dm / a.G, grp = cb / a.blocks, c0 = (cb - grp * a.blocks) * 64;
     const int lane = threadIdx.x & 63, w = wave_index(), n0 = NS * w;
