@@ -127,7 +127,8 @@ def test_forward_mode_is_refused(dev):
         lambda d: ssm_scan(u, u, A, Bm, Bm, initial_state=d(pool)), lambda d: ssm_scan(u, u, A, Bm, Bm, z=d(u)),
         lambda d: ssm_scan_varlen(u, d(u), A, Bm, Bm, cu), lambda d: ssm_decode_step(u[:, 0], u[:, 0], A, Bm[:, 0],
                                                                                     Bm[:, 0], d(pool)),
-        lambda d: short_conv(d(u), w), lambda d: short_conv(u, d(w)), lambda d: short_conv(u, w, initial_state=d(state)),
+        lambda d: short_conv(d(u), w), lambda d: short_conv(u, d(w)),
+        lambda d: short_conv(u, w, initial_state=d(state)),
         lambda d: short_conv_varlen(u, d(w), cu), lambda d: short_conv_decode_step(d(u[:, 0]), w, state),
         lambda d: layer_norm(d(u)), lambda d: layer_norm(u, d(w[:, 0].contiguous())),
     ]
@@ -150,8 +151,8 @@ def test_no_tokens_leave_the_initial_state(dev):
     s0 = torch.randn(3, 10, 5, device=dev)
 
     def scan(a, b):
-        return lib.triune_hip_ssm_scan(p(x), p(x), None, p(x), p(x), p(x), None, None, 0, st, 1, p(a), p(x), p(b), None, 3,
-                                       0, 10, 1, 5, 0, None, 0, stream)
+        return lib.triune_hip_ssm_scan(p(x), p(x), None, p(x), p(x), p(x), None, None, 0, st, 1, p(a), p(x), p(b), None,
+                                       3, 0, 10, 1, 5, 0, None, 0, stream)
 
     for a in (s0, None):
         b = torch.full_like(s0, 7.0)
@@ -164,7 +165,8 @@ def test_no_tokens_leave_the_initial_state(dev):
         w = torch.zeros(44, device=dev)
         for a in (c0, None):
             b = torch.full_like(c0, 7.0)
-            assert lib.triune_hip_short_conv(p(x), p(w), None, code, 0, st, 1, p(a), p(b), p(x), 3, 0, 11, 4, stream) == 0
+            assert lib.triune_hip_short_conv(p(x), p(w), None, code, 0, st, 1, p(a), p(b), p(x), 3, 0, 11, 4,
+                                             stream) == 0
             assert torch.equal(b, torch.zeros_like(c0) if a is None else c0)
 
 
@@ -259,7 +261,8 @@ def test_gradients_of_single_tokens_of_a_long_prompt(dev, units):
         _, _, kept = S._scan(u, delta, A, Bm, C, Dp, None, None, True, None, None, True, units << 8)
         got = S._scan_bwd(u, delta, A, Bm, C, Dp, None, None, True, kept, dy, None, False, units << 8)
         form = (u, delta, A, Bm, C, Dp, None, None, True, None, dy, None)
-        for name, x, r, e in zip("u delta A B C D".split(), got, R.scan_grads(*form), R.scan_grads(*form, absolute=True)):
+        ref, env = (R.scan_grads(*form, absolute=a) for a in (False, True))
+        for name, x, r, e in zip("u delta A B C D".split(), got, ref, env):
             R.near(x, r, 24 * (dst - src + 33 + 16) * R.U * e, F32, f"{name} {src} {dst}")
 
 

@@ -227,7 +227,8 @@ def test_tokens_wider_than_the_kernels_address():
 def test_grids_past_32_bits_of_threads():
     """Channel groups of one channel make a workgroup each, sixteen waves above 32 states: 2^32 threads are refused,
     not launched."""
-    wide = dict(st=(ctypes.c_int64 * 14)(*([4096] * 14)), T=1, total=1024, n=1024, Bn=1024, rows=1024, Dm=4096, G=4096, N=64)
+    wide = dict(st=(ctypes.c_int64 * 14)(*([4096] * 14)), T=1, total=1024, n=1024, Bn=1024, rows=1024, Dm=4096, G=4096,
+                N=64)
     big, ws = L.lib().triune_hip_ssm_bwd_workspace_size(1024, 1, 4096, 4096, 64, 0), FAKE
     assert caller("triune_hip_ssm_scan", SCAN, **{**_scan_base(SCAN), **wide})() == SHAPE
     assert caller("triune_hip_ssm_scan_varlen", VARLEN, **{**_scan_base(VARLEN), **wide})() == SHAPE
@@ -235,7 +236,8 @@ def test_grids_past_32_bits_of_threads():
 
 
 @pytest.mark.parametrize("N,split,whole", [
-    (16, [256, 304], [320, 352, 448, 504, 512]), (8, [512], [640, 768]), (32, [128], [160, 192]), (64, [64, 128], [160, 192])])
+    (16, [256, 304], [320, 352, 448, 504, 512]), (8, [512], [640, 768]), (32, [128], [160, 192]),
+    (64, [64, 128], [160, 192])])
 def test_scans_are_split_where_that_is_faster(N, split, whole):
     """Workgroups (8 prompts of 2048 tokens) on both sides of the measured crossover."""
     size = L.lib().triune_hip_ssm_scan_workspace_size

@@ -65,8 +65,8 @@ bool scan_grids_ok(int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int
 // busy.  Calls below the shares here split the time axis, which costs the decays a second time: unsplit they
 // take as long for one workgroup as for the whole chip, split their time follows the work.  bf16, 8 x 2048 tokens, us
 // unsplit and split, by workgroups:
-//   outputs    N = 16: 256 230 234, 320 305 302, 352 304 320, 448 307 395, 504 308 446;  N = 8: 512 346 335, 640 348 427;
-//              N = 32: 128 295 260, 160 296 333;  N = 64: 128 591 541, 160 591 725
+//   outputs    N = 16: 256 230 234, 320 305 302, 352 304 320, 448 307 395, 504 308 446;  N = 8: 512 346 335,
+//              640 348 427;  N = 32: 128 295 260, 160 296 333;  N = 64: 128 591 541, 160 591 725
 //   gradients  N = 16: 320 1052 844, 400 1058 1006, 448 1058 1099, 504 1067 1240;  N = 8: 640 1522 1487, 768 1544 1761;
 //              N = 32: 192 1231 1188, 240 1236 1457;  N = 64: 160 3549 2975, 240 3738 4337
 // Split calls take shares that several rounds of workgroups even out: 1 x 16384 of 768 channels 106 us for
@@ -122,8 +122,8 @@ ScanPlan plan_scan(int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, int N, int 
 
 // Packed: lengths are on the device, so a segment is an equal share of all tokens.  Where there are sequences enough
 // for two rounds of the chip they fill it by themselves, but for one far longer than the rest, which its
-// workgroups would walk alone: sequences up to twice a workgroup's share of one round stay whole, and longer ones are cut
-// into halves of it.  1536 channels, N = 16, bf16, us with every sequence whole and by this rule: 42 prompts of 64
+// workgroups would walk alone: sequences up to twice a workgroup's share of one round stay whole, and longer ones are
+// cut into halves of it.  1536 channels, N = 16, bf16, us with every sequence whole and by this rule: 42 prompts of 64
 // tokens and one of 16384 1730 and 259, and one of 2048 251 and 78; 200 of 100 and one of 8000 1047 and 341; 48
 // log-uniform up to 8192 1139 and 965, 64 up to 2048 341 and 364.  Even lengths pay the launches that find
 // nothing to do: 43 of 512 166 and 174, 200 of 256 308 and 312, 256 of 64 111 and 127, 64 of 100 57 and 66, so calls
@@ -213,7 +213,10 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
     if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]}) || strides[7] < Dm)
         return TRIUNE_ERR_LAYOUT;
     if (Bn == 0) return TRIUNE_OK;
-    if (T == 0) return s_final ? status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream)) : TRIUNE_OK;
+    if (T == 0) {
+        if (!s_final) return TRIUNE_OK;
+        return status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream));
+    }
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags);
     if (!scan_grids_ok(p.n_work, p.nseg, Bn, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
@@ -384,8 +387,9 @@ int triune_hip_short_conv(const void* x, const void* w, const void* bias, int io
     if (const int e = conv_check(x, w, bias, y, strides, s0, s_final, io_dtype, w_dtype, Bn, T, Dm, W)) return e;
     if (Bn == 0) return TRIUNE_OK;
     if (T == 0) {
+        if (!s_final) return TRIUNE_OK;
         const int bytes = io_dtype == TRIUNE_DT_F32 ? 4 : 2;
-        return s_final ? status(launch_state_copy(s0, s_final, Bn * (W - 1) * Dm, bytes, (hipStream_t)stream)) : TRIUNE_OK;
+        return status(launch_state_copy(s0, s_final, Bn * (W - 1) * Dm, bytes, (hipStream_t)stream));
     }
     ConvParams a = conv_params(x, w, bias, w_dtype, silu, s0, s_final, y, Bn, T, Dm, W);
     a.x_sb = strides[0], a.x_st = strides[1], a.y_sb = strides[2], a.y_st = strides[3];

@@ -42,8 +42,8 @@ __device__ __forceinline__ int column(int t, int k) {
 
 // Eight elements of a row from column c, zeros past its end.  EIGHTS: the width is a multiple of eight, so a
 // group is in the row or past it, and the load depends on no condition (which would make the compiler wait
-// where it joins the registers, so that no row is in flight).  16384 rows of 1536 (bf16), forward and gradients: 73.4
-// us, 80.2 with the conditions.
+// where it joins the registers, so that no row is in flight).  16384 rows of 1536 (bf16), forward and gradients: 66.3
+// us, 80.9 with the conditions; 4096 of 8192: 102 and 128.
 template <bool EIGHTS, typename T>
 __device__ __forceinline__ Raw<T, 8> load_group(const T* p, int c, int D) {
     if constexpr (!EIGHTS) return load_raw<8>(p + c, D - c);
@@ -75,8 +75,8 @@ __device__ __forceinline__ void load_par(const void* p, int dt, int c, int n, fl
 }  // namespace
 
 // Blocks walk rows, the next row's loads in flight during this one's sums; w and b are loaded once, to LDS: in
-// registers they leave fewer waves a SIMD (16384 rows of 1536, bf16: 23.3 us (4.3 TB/s) and 27.6; 4096 of 8192: 35.3
-// and 45.7).
+// registers they leave fewer waves a SIMD (16384 rows of 1536, bf16, two inputs in turn, partly in the last-level
+// cache: 23.3 us and 27.6; 4096 of 8192: 35.3 and 45.7.  Three inputs, with mean and rstd stored: 26.6 us, 3.8 TB/s).
 template <typename T, int TPR, int K, bool EIGHTS>
 __global__ __launch_bounds__(block_threads(TPR)) void norm_kernel(NormParams a) {
     constexpr int RPB = block_threads(TPR) / TPR;

@@ -161,7 +161,7 @@ __device__ __forceinline__ float fast_sigmoid(float x) { return __builtin_amdgcn
 __device__ __forceinline__ float silu_gate(float z) { return z * fast_sigmoid(z); }
 
 // log(1 + e^-|x|) + max(x, 0).  With s = e / (2 + e), log(1 + e) = 2 atanh(s), whose series in s^2
-// <= 1/9 is cut to a fitted polynomial (relative error 4e-9): the form keeps the relative precision
+// <= 1/9 is cut to a fitted polynomial (relative error 8e-9): the form keeps the relative precision
 // where e is small (step sizes of 1e-3 have e = 1e-3, of which log(1 + e) would lose ten bits).
 __device__ __forceinline__ float softplus(float x) {
     const float e = fast_exp(-fabsf(x));
@@ -354,8 +354,9 @@ __device__ __forceinline__ void lds_add(const float* p, float (&x)[V]) {
 
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
-// The tokens of work item w (of packed sequence seq, searched for where that is negative): sequence, first token (of the sequence), length, whether it is the
-// sequence's last segment.  False when there is no such item (packed calls bound their number).
+// The tokens of work item w (of packed sequence seq, searched for where that is negative): sequence, first
+// token (of the sequence), length, whether it is the sequence's last segment.  False when there is no such item
+// (packed calls bound their number).
 struct SsmSeg {
     int64_t seq, row0, t0;  // row0: first token of the sequence in a packed tensor
     int len, index;

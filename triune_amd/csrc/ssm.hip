@@ -17,8 +17,8 @@
 // 437 us for 8 x 2048 tokens of 4096 channels (N = 16, bf16) against 306.
 //
 // Calls with too few (sequence, channel block) pairs for the chip split the time axis into segments: a
-// pass for each segment's own end state (its decay over the segment is exp(A sum dt), so only the sum
-// of dt is kept), a scan over segments, and the pass that writes the outputs.
+// pass for each segment's own end state but the last one's (its decay over the segment is exp(A sum dt), so only
+// the sum of dt is kept), a scan over segments, and the pass that writes the outputs.
 #include "ssm.h"
 
 namespace triune {
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
     }
     const int64_t row = STATES ? 0 : ssm_row(a.slots, a.n_slots, sg.seq);
     if constexpr (!STATES) {
-        if (a.ws_state && !(sg.last && sg.index == 0)) {  // segmented: the entering state comes from the scan over segments
+        if (a.ws_state && !(sg.last && sg.index == 0)) {  // of several: its entering state comes from the join
 #pragma unroll
             for (int j = 0; j < NS; ++j)
                 if (n0 + j < a.N) h[j] = a.ws_state[(work * a.N + n0 + j) * a.Dm + ch];
@@ -260,8 +260,8 @@ __global__ __launch_bounds__(64 * NW) void ssm_scan_kernel(SsmParams a) {
 // from (BACK: from the last to the first, each one's own gradient at its start by the one that enters at
 // its end).  A block takes 64 channels of a (sequence, state), its waves eight segments each at a time:
 // a wave folds its segments to one, the folds meet in LDS, and each wave finishes from the state that the
-// waves before it leave.  128 segments of 768 channels, N = 16: 7.0 us; a thread per channel with eight
-// segments in flight 15.7.
+// waves before it leave.  128 segments of 768 channels, N = 16: 7.6 us, 6.9 with decays that may overflow (Pow2);
+// a thread per channel with eight segments in flight 15.7.
 template <bool BACK>
 __global__ __launch_bounds__(1024) void ssm_carry_kernel(SsmParams a, const float* init, float* out, bool by_followed) {
     constexpr int PER = 8;  // segments of a wave
@@ -354,7 +354,8 @@ __global__ __launch_bounds__(64) void ssm_offsets_kernel(SsmParams a, int64_t cu
 
 template <typename T>
 __global__ __launch_bounds__(256) void state_copy_kernel(const T* from, T* to, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from ? from[i] : (T)0;
+    const int64_t step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) to[i] = from ? from[i] : (T)0;
 }
 
 // One token for every row.  A lane holds up to four states of a channel, LPC neighbouring lanes a
@@ -441,8 +442,9 @@ hipError_t launch_ssm_scan(const SsmParams& a, int dt, hipStream_t s) { return s
 template <bool BACK>
 static hipError_t carry(const SsmParams& a, const float* init, float* out, hipStream_t s) {
     // Waves for the segments of a sequence.  Packed calls know the average alone and take two waves from five segments
-    // on: 16 ragged prompts of 5034 tokens (6 segments, the longest 23) 84 us a call with one wave, 81 with two, 82 with
-    // four, 90 with eight; 20 of 300 tokens (6) 54, 56, 59, 68; three, one of them of 5000 (28), 62, 54, 52, 51.
+    // on: 16 ragged prompts of 5034 tokens (6 segments, the longest 23) 84 us a call with one wave, 81 with two,
+    // 82 with four, 90 with eight; 20 of 300 tokens (6) 54, 56, 59, 68; three, one of them of 5000 (28), 62, 54,
+    // 52, 51.
     const int64_t segs = a.cu ? (a.n_work + a.n_seqs - 1) / a.n_seqs : a.nseg;
     const int waves = segs <= (a.cu ? 4 : 8) ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
     // Packed: sequences of one segment need no join, so where fewer segments are followed by another than there are
@@ -474,7 +476,8 @@ static hipError_t step_lanes(const SsmStepParams& a, hipStream_t s) {
     const int lpc = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
     const int64_t blocks = (a.Dm * (int64_t)lpc + 255) / 256;
     // rows that are walked side by side: eight blocks a compute unit (256 sessions of 1536 channels, N = 16:
-    // 15.0 us; 16.8 with four, 16.6 with sixteen, 19.1 with a block per row and 64 channels)
+    // 14.9 us; 16.8 with four, 16.6 with sixteen, 19.1 with a block per row and 64 channels).  None of these divides
+    // the rows evenly: 85 side by side leave the last of four rounds one row.  Even divisions have not been tried.
     int64_t rows = a.cus * 8 / blocks;
     rows = rows < 1 ? 1 : rows > a.Bn ? a.Bn : rows;
     const dim3 grid((unsigned)(blocks * rows));

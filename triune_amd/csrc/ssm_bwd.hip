@@ -16,7 +16,7 @@
 // not depend on timing.
 //
 // Bound by vector issue at two waves a SIMD: 25 vector operations and 1.75 exp2 per wave and state (about
-// 105 cycles).  4 x 2048 tokens of 1536 channels, N = 16, bf16: 218 us where that is 134.
+// 105 cycles).  4 x 2048 tokens of 1536 channels, N = 16, bf16: 206 us where that is 134.
 #include "ssm.h"
 
 namespace triune {

@@ -3,7 +3,8 @@ training batch or of a decode step's tokens.  No reference counterpart.
 
     y = (x - mean) rstd weight + bias,   rstd = 1 / sqrt(mean((x - mean)^2) + eps)
 
-Statistics and sums are float32, outputs are rounded once.  There is no CPU path.
+Statistics and sums are float32, outputs are rounded once.  There is no CPU path and no forward-mode
+derivative.
 """
 
 from __future__ import annotations

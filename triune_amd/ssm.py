@@ -10,7 +10,9 @@ Layouts: token tensors [B, T, channels] (packed: [N, channels] or [1, N, channel
 (the innermost is made 1 by a copy where it is not), one dtype of float32, bfloat16 and float16;
 parameters A, D and delta_bias in float32; scan states float32 [B, channels, N], convolution states
 [B, W - 1, channels] in x's dtype (the last W - 1 inputs, oldest first).  Everything that the kernels sum or
-carry is float32; outputs are rounded once.  Tensors are on one HIP device; there is no CPU path.
+carry is float32; outputs are rounded once.  A may be positive and dt below 0 (modes that grow), but one token's
+exp(dt A) has to be a float32 number; A of -inf forgets at every step above 0.  Tensors are on one HIP device;
+there is no CPU path and no forward-mode derivative.
 """
 
 from __future__ import annotations
@@ -57,7 +59,7 @@ def _rows(x, tok=None):
     if x.stride(-1) == 1 and (tok is None or x.stride(tok) < _MAX_TOKEN_STRIDE or x.shape[tok] == 1):
         return x
     if tok is not None and x.shape[tok] != 1 and math.prod(x.shape[tok + 1:]) >= _MAX_TOKEN_STRIDE:
-        raise ValueError(f"tokens of {tuple(x.shape[tok + 1:])} are too wide: below {_MAX_TOKEN_STRIDE} values are supported")
+        raise ValueError(f"tokens of {tuple(x.shape[tok + 1:])} are too wide: they need below {_MAX_TOKEN_STRIDE} values")
     return x.contiguous()
 
 
@@ -276,8 +278,8 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=
 
     u, delta, z: [B, T, Dm] (z: the gate, or None); A: float32 [Dm, N]; B, C: [B, T, N], or
     [B, T, G, N] where G groups of Dm / G consecutive channels share theirs (G N below 2^22 where T > 1);
-    D, delta_bias: float32 [Dm] or None; N at most 64.  dt is softplus(delta + delta_bias), or delta + delta_bias without
-    delta_softplus.  initial_state: [B, Dm, N] or None (zeros).  out: optional [B, T, Dm] buffer
+    D, delta_bias: float32 [Dm] or None; N at most 64.  dt is softplus(delta + delta_bias), or delta + delta_bias
+    without delta_softplus.  initial_state: [B, Dm, N] or None (zeros).  out: optional [B, T, Dm] buffer
     in u's dtype that overlaps no input, for calls without gradients.  Returns (y [B, T, Dm] in u's
     dtype, final state float32 [B, Dm, N]).
 
