@@ -450,8 +450,8 @@ int triune_hip_gla_fused_decode_step_slots_count(const void* qkvg, int io_dtype,
  *     dt = delta + delta_bias, through softplus when `softplus`;  h <- exp(dt A) h + dt u B
  *     y = (sum_n C h + D u) * silu(z)                     (no gate when z is NULL)
  * strides[14] = (batch, token) of u, delta, z, y, then (batch, token, group) of B, C.  s0 (NULL:
- * zeros) and s_final (NULL: not wanted): [Bn, Dm, N]; without tokens (T = 0) s0 goes to s_final.  kept: NULL, or fp32 [Bn, ceil(T / K), N, Dm],
- * K = 32 (16 for N > 32), that receives the state of every K-th token for triune_hip_ssm_bwd.  flags bits 8..15 force the
+ * zeros) and s_final (NULL: not wanted): [Bn, Dm, N]; without tokens (T = 0) s0 goes to s_final.  kept: NULL, or
+ * fp32 [Bn, ceil(T / K), N, Dm], K = 32 (16 for N > 32), that receives the state of every K-th token for triune_hip_ssm_bwd.  flags bits 8..15 force the
  * length of a segment in units of 32 tokens (0: automatic). */
 size_t triune_hip_ssm_scan_workspace_size(int64_t Bn, int64_t T, int64_t Dm, int64_t G, int N, int flags);
 int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const void* B, const void* C, const float* A,

@@ -303,3 +303,17 @@ def test_training_steps_replay_from_a_graph(dev):
             for a, b in zip(out, step(data)):
                 assert torch.equal(a, b)
         del graph
+
+
+@torch.no_grad()
+def test_thousands_of_packed_sequences(dev):
+    """4200 sequences of two tokens, 64 states: the bits of the dense call."""
+    n, D, N = 4200, 1088, 64
+    g = torch.Generator().manual_seed(0)
+    rn = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    u, Bm, C, A, Dp = rn(n, 2, D), rn(n, 2, N), rn(n, 2, N), -rn(D, N).exp(), rn(D)
+    cu = torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device=dev)
+    assert S.plan_on(u, "triune_hip_ssm_scan_varlen_workspace_size", n, 2 * n, D, 1, N, 0) > 0
+    y, s = ssm_scan_varlen(u.flatten(0, 1), u.flatten(0, 1), A, Bm.flatten(0, 1), C.flatten(0, 1), cu, Dp)
+    yd, sd = ssm_scan(u, u, A, Bm, C, Dp)
+    assert torch.equal(y.view_as(yd), yd) and torch.equal(s, sd)

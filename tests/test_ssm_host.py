@@ -265,3 +265,12 @@ def test_packed_scans_with_one_long_prompt_are_cut():
     assert size(43, 42 * 64 + 16384, 1536, 1, 16, 0) > 43 * 17 * 1536 * 4
     assert size(201, 28000, 1536, 1, 16, 0) > 201 * 17 * 1536 * 4
     assert size(100, 3000, 1536, 1, 16, 0) == 0 and size(43, 43, 1536, 1, 16, 0) == 0
+
+
+def test_packed_scans_of_thousands_of_sequences_are_taken():
+    """The join's grid counts what it launches: blocks for the segments that are followed, of the waves they get."""
+    call = caller("triune_hip_ssm_scan_varlen", VARLEN, **_scan_base(VARLEN))
+    for n, total, Dm, N in ((4200, 8400, 1088, 64), (4096, 200000, 4096, 16), (20000, 40000, 768, 64)):
+        need = L.lib().triune_hip_ssm_scan_varlen_workspace_size(n, total, Dm, 1, N, 0)
+        kw = dict(n=n, rows=n, total=total, Dm=Dm, N=N, st=(ctypes.c_int64 * 8)(*([Dm] * 8)))
+        assert need > 0 and call(ws=FAKE, wsb=need - 1, **kw) == WORKSPACE, (n, total, Dm, N)

@@ -50,15 +50,17 @@ bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
 int64_t group_blocks(int64_t Dm, int64_t G) { return (Dm / G + 63) / 64; }
 int64_t all_blocks(int64_t Dm, int64_t G) { return G * group_blocks(Dm, G); }
 
-// Whether n workgroups per channel block are a grid: 31 bits of workgroups and 32 of threads.
+// Whether n times `blocks` workgroups are a grid: 31 bits of workgroups and 32 of threads.
 bool grid_ok(int64_t n, int64_t blocks, int threads) {
     const int64_t by_threads = (int64_t)0xffffffff / threads, most = by_threads < kMaxGrid ? by_threads : kMaxGrid;
     return n <= most / blocks;
 }
-// The grids of a scan: its work items, and the join's blocks of up to sixteen waves.
-bool scan_grids_ok(int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int64_t G, int N) {
-    return grid_ok(n_work, all_blocks(Dm, G), 64 * ssm_waves(N)) && n_seqs <= kMaxGrid / (Dm * N) &&
-           (nseg <= 1 || grid_ok(n_seqs * N, (Dm + 63) / 64, 1024));
+// The grids of a scan: its work items, and the join's.
+bool scan_grids_ok(bool packed, int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int64_t G, int N) {
+    if (!grid_ok(n_work, all_blocks(Dm, G), 64 * ssm_waves(N)) || n_seqs > kMaxGrid / (Dm * N)) return false;
+    if (nseg <= 1) return true;
+    const CarryGrid g = ssm_carry_grid(packed, n_seqs, n_work, nseg, Dm, N);
+    return grid_ok(g.blocks, 1, 64 * g.waves);
 }
 
 // A chip's worth of workgroups is eight waves a compute unit (four SIMDs); two waves on a SIMD keep it three quarters
@@ -218,7 +220,7 @@ int triune_hip_ssm_scan(const void* u, const void* delta, const void* z, const v
         return status(launch_state_copy(s0, s_final, Bn * Dm * N, 4, (hipStream_t)stream));
     }
     const ScanPlan p = plan_scan(Bn, T, Dm, G, N, flags);
-    if (!scan_grids_ok(p.n_work, p.nseg, Bn, Dm, G, N)) return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(false, p.n_work, p.nseg, Bn, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, strides[0], strides[1]};
@@ -262,7 +264,7 @@ int triune_hip_ssm_scan_varlen(const void* u, const void* delta, const void* z, 
     if (n_seqs == 0) return TRIUNE_OK;
     // with no tokens every sequence's state still passes through: one empty segment each
     const ScanPlan p = plan_packed(n_seqs, total_tokens > 0 ? total_tokens : 1, Dm, G, N, flags);
-    if (!scan_grids_ok(p.n_work, p.nseg, n_seqs, Dm, G, N)) return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(true, p.n_work, p.nseg, n_seqs, Dm, G, N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     SsmParams a{};
     a.u = {u, 0, strides[0]};
@@ -305,7 +307,7 @@ int triune_hip_ssm_bwd(const void* u, const void* delta, const void* z, const vo
         return TRIUNE_ERR_LAYOUT;
     if (!strides_ok({strides[1], strides[3], strides[5], strides[7], strides[9], strides[12]})) return TRIUNE_ERR_LAYOUT;
     const BwdPlan p = plan_bwd(Bn, T, Dm, G, N, flags);
-    if (!scan_grids_ok(p.s.n_work, p.s.nseg, Bn, Dm, G, N) || Bn * T > kMaxGrid / (G * N)) return TRIUNE_ERR_SHAPE;
+    if (!scan_grids_ok(false, p.s.n_work, p.s.nseg, Bn, Dm, G, N) || Bn * T > kMaxGrid / (G * N)) return TRIUNE_ERR_SHAPE;
     if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
     char* ws = (char*)workspace;
     SsmBwdParams g{};

@@ -69,6 +69,13 @@ struct SsmStepParams {
 };
 
 int ssm_waves(int N);  // waves of a scan workgroup
+// The join's launch.  by_followed: its blocks are laid out by the segments that another one follows.
+struct CarryGrid {
+    int64_t blocks;
+    int waves;
+    bool by_followed;
+};
+CarryGrid ssm_carry_grid(bool packed, int64_t n_seqs, int64_t n_work, int64_t nseg, int64_t Dm, int N);
 // Whether four channels of every row of these (and the groups) are aligned to their size together.
 inline bool ssm_by_four(int group_channels, int io_dt, std::initializer_list<SsmTok> ts) {
     const uintptr_t m = io_dt == DT_F32 ? 15 : 7;

@@ -439,19 +439,25 @@ static hipError_t scan_dtype(const SsmParams& a, int dt, hipStream_t s) {
 hipError_t launch_ssm_states(const SsmParams& a, int dt, hipStream_t s) { return scan_dtype<true>(a, dt, s); }
 hipError_t launch_ssm_scan(const SsmParams& a, int dt, hipStream_t s) { return scan_dtype<false>(a, dt, s); }
 
-template <bool BACK>
-static hipError_t carry(const SsmParams& a, const float* init, float* out, hipStream_t s) {
+CarryGrid ssm_carry_grid(bool packed, int64_t n_seqs, int64_t n_work, int64_t nseg, int64_t Dm, int N) {
     // Waves for the segments of a sequence.  Packed calls know the average alone and take two waves from five segments
     // on: 16 ragged prompts of 5034 tokens (6 segments, the longest 23) 84 us a call with one wave, 81 with two,
     // 82 with four, 90 with eight; 20 of 300 tokens (6) 54, 56, 59, 68; three, one of them of 5000 (28), 62, 54,
     // 52, 51.
-    const int64_t segs = a.cu ? (a.n_work + a.n_seqs - 1) / a.n_seqs : a.nseg;
-    const int waves = segs <= (a.cu ? 4 : 8) ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
+    const int64_t segs = packed ? (n_work + n_seqs - 1) / n_seqs : nseg;
+    CarryGrid g;
+    g.waves = segs <= (packed ? 4 : 8) ? 1 : segs <= 16 ? 2 : segs <= 32 ? 4 : segs <= 64 ? 8 : 16;
     // Packed: sequences of one segment need no join, so where fewer segments are followed by another than there are
     // sequences, blocks are laid out by those (256 prompts of 64 tokens: 127 us a call, 155 by sequences).
-    const bool by_followed = a.cu && a.n_work - a.n_seqs < a.n_seqs;
-    const int64_t blocks = (by_followed ? a.n_work - a.n_seqs : a.n_seqs) * a.N * ((a.Dm + 63) / 64);
-    ssm_carry_kernel<BACK><<<dim3((unsigned)blocks), 64 * waves, 0, s>>>(a, init, out, by_followed);
+    g.by_followed = packed && n_work - n_seqs < n_seqs;
+    g.blocks = (g.by_followed ? n_work - n_seqs : n_seqs) * N * ((Dm + 63) / 64);
+    return g;
+}
+
+template <bool BACK>
+static hipError_t carry(const SsmParams& a, const float* init, float* out, hipStream_t s) {
+    const CarryGrid g = ssm_carry_grid(a.cu, a.n_seqs, a.n_work, a.nseg, a.Dm, a.N);
+    ssm_carry_kernel<BACK><<<dim3((unsigned)g.blocks), 64 * g.waves, 0, s>>>(a, init, out, g.by_followed);
     return hipGetLastError();
 }
 hipError_t launch_ssm_carry(const SsmParams& a, hipStream_t s) { return carry<false>(a, a.s0, nullptr, s); }
