@@ -207,7 +207,7 @@ def test_slots_past_32_bits():
         assert g == s if 0 <= s < 1 << 31 else g < 0 or g == (1 << 31) - 1  # stays outside every pool
     for dt in (torch.int8, torch.int16, torch.uint8, torch.int32):
         assert _slots(torch.tensor([3, 0], dtype=dt), 2, dev).tolist() == [3, 0]
-    for dt in (torch.float32, torch.float16, torch.bool, torch.complex64):
+    for dt in (torch.float32, torch.float16, torch.bool, torch.complex64, torch.uint64, torch.uint32):
         with pytest.raises(TypeError, match="slots"):
             _slots(torch.zeros(2, dtype=dt), 2, dev)
 
@@ -274,3 +274,13 @@ def test_packed_scans_of_thousands_of_sequences_are_taken():
         need = L.lib().triune_hip_ssm_scan_varlen_workspace_size(n, total, Dm, 1, N, 0)
         kw = dict(n=n, rows=n, total=total, Dm=Dm, N=N, st=(ctypes.c_int64 * 8)(*([Dm] * 8)))
         assert need > 0 and call(ws=FAKE, wsb=need - 1, **kw) == WORKSPACE, (n, total, Dm, N)
+
+
+def test_offsets_past_32_bits():
+    """int64 offsets stay on their side of the packed rows, to which the kernels cut them."""
+    from triune_amd.ssm import _cu
+
+    dev = torch.device("cpu")
+    got = _cu(torch.tensor([-(1 << 32) + 3, 0, 7, (1 << 32) + 5]), dev)
+    assert got.dtype == torch.int32 and got.tolist() == [0, 0, 7, (1 << 31) - 1]
+    assert _cu(torch.tensor([0, 7], dtype=torch.int32), dev).tolist() == [0, 7]

@@ -110,14 +110,17 @@ def _out(out, shape, dtype, like, tok=None):
     return out
 
 
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
 def _slots(slots, n, dev):
     if slots is None:
         return None
     if slots.numel() != n or slots.dim() != 1:
         raise ValueError(f"slots must hold one index for each of the {n} rows")
     if slots.dtype != torch.int32 or slots.device != dev:
-        if slots.dtype.is_floating_point or slots.dtype.is_complex or slots.dtype == torch.bool:
-            raise TypeError(f"slots must be integers, not {slots.dtype}")
+        if slots.dtype not in _INTEGERS:
+            raise TypeError(f"slots must be int32 or another of {_INTEGERS}, not {slots.dtype}")
         if slots.dtype == torch.int64:  # past 32 bits is outside every pool, not the row of the low half
             slots = slots.clamp(-1, 2**31 - 1)
         slots = slots.to(device=dev, dtype=torch.int32)
@@ -127,6 +130,8 @@ def _slots(slots, n, dev):
 def _cu(cu_seqlens, dev):
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise ValueError("cu_seqlens must be int32 offsets [n + 1]")
+    if cu_seqlens.dtype == torch.int64:  # past 32 bits is behind every row, as for offsets that fit
+        cu_seqlens = cu_seqlens.clamp(0, 2**31 - 1)
     return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous()
 
 
