@@ -539,6 +539,37 @@ int triune_hip_layer_norm_bwd(const void* x, int64_t x_stride, const void* w, co
                               void* dw, void* db, int64_t R, int64_t D, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/* Decay attention: linear attention with one decay per head and token,
+ *     S_t = e^{g_t} S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t         (g above 0 counts as 0)
+ * q, k [B, T, Hk, Dk], v, o [B, T, H, Dv] in io_dtype, innermost stride 1, any other strides (in elements) and any
+ * alignment of an element; H / Hk consecutive heads of v share one of q and k; g [B, T, H] in io_dtype or fp32 (strides of
+ * 0 for constants).  Dk <= 128, Dv <= 16384, H < 65536.  strides[15] = (batch, token, head) of q, k, v, g, o.
+ * States: fp32 contiguous [B, H, Dk, Dv], s0 NULL: zeros, s_final NULL: not wanted; without tokens (T = 0) s0 goes to
+ * s_final.  o overlaps no input.  A workspace is 16-byte aligned and belongs to one call at a time.  flags bits 8..15
+ * force the length of a segment in units of 32 tokens (0: automatic). */
+size_t triune_hip_decay_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                            int flags);
+int triune_hip_decay_attn(const void* q, const void* k, const void* v, const void* g, int io_dtype, int g_dtype,
+                          const int64_t* strides, float scale, const float* s0, void* o, float* s_final, int64_t B,
+                          int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int flags, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* The same over packed sequences, offsets, slots and states as triune_hip_ssm_scan_varlen; strides[10] = (token, head)
+ * of q, k, v, g, o. */
+size_t triune_hip_decay_attn_varlen_workspace_size(int64_t n_seqs, int64_t total_tokens, int64_t H, int64_t Hk,
+                                                   int64_t Dk, int64_t Dv, int flags);
+int triune_hip_decay_attn_varlen(const void* q, const void* k, const void* v, const void* g, int io_dtype, int g_dtype,
+                                 const int64_t* strides, float scale, const int32_t* cu_seqlens, int64_t n_seqs,
+                                 int64_t total_tokens, const float* s0, float* s_final, const int32_t* slots,
+                                 int64_t n_state_rows, void* o, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                 int flags, void* workspace, size_t workspace_bytes, void* stream);
+/* One token for each of B rows; strides[10] = (batch, head) of q, k, v, g, o.  Row b uses state row slots[b] (b when
+ * slots is NULL) of state_in and state_out, which may be one tensor; a row outside [0, n_state_rows) has no state and
+ * zero outputs; other slots must be distinct. */
+int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* v, const void* g, int io_dtype,
+                                      int g_dtype, const int64_t* strides, float scale, const float* state_in,
+                                      float* state_out, const int32_t* slots, int64_t n_state_rows, void* o, int64_t B,
+                                      int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

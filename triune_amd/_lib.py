@@ -30,6 +30,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
+_f = ctypes.c_float
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
 _LIB = None
@@ -185,6 +186,22 @@ def _bind(lib):
             [_vp, _vp, _vp, _vp, _i, _i, _i64p, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i, _vp, _sz, _vp],
             _i,
         ),
+        "triune_hip_decay_attn_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i], _sz),
+        "triune_hip_decay_attn": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i, _vp, _sz,
+             _vp],
+            _i,
+        ),
+        "triune_hip_decay_attn_varlen_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i], _sz),
+        "triune_hip_decay_attn_varlen": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+             _i, _vp, _sz, _vp],
+            _i,
+        ),
+        "triune_hip_decay_attn_decode_step": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp],
+            _i,
+        ),
         "triune_hip_layer_norm": (
             [_vp, _i64, _vp, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp],
             _i,
@@ -253,6 +270,11 @@ EXPORTS = (
     "triune_hip_short_conv_decode_step",
     "triune_hip_short_conv_bwd_workspace_size",
     "triune_hip_short_conv_bwd",
+    "triune_hip_decay_attn_workspace_size",
+    "triune_hip_decay_attn",
+    "triune_hip_decay_attn_varlen_workspace_size",
+    "triune_hip_decay_attn_varlen",
+    "triune_hip_decay_attn_decode_step",
     "triune_hip_layer_norm",
     "triune_hip_layer_norm_bwd_workspace_size",
     "triune_hip_layer_norm_bwd",

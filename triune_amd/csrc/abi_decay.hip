@@ -1,0 +1,216 @@
+// abi_decay.hip -- extern "C" entry points of the decay attention layer's operators (declared in
+// include/triune_hip.h): argument checks, workspace layout and launches.
+#include "abi_common.h"
+#include "decay.h"
+
+using namespace triune;
+
+namespace {
+
+bool decay_shape_ok(int64_t H, int64_t Hk, int64_t Dk, int64_t Dv) {
+    return H > 0 && H < (1 << 16) && Hk > 0 && H % Hk == 0 && Dk > 0 && Dk <= DECAY_MAX_DK && Dv > 0 &&
+           Dv <= DECAY_MAX_DV;
+}
+int64_t slices_of(int64_t Dv) { return (Dv + decay_slice((int)Dv) - 1) / decay_slice((int)Dv); }
+
+// Sequences whose workgroups are a grid: what the plans below multiply then stays within 64 bits.
+bool seqs_ok(int64_t n_seqs, int64_t H, int64_t Dv) { return grid_ok(n_seqs, H * slices_of(Dv), 256); }
+
+int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * DECAY_CHUNK; }
+int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+// Workgroups that fill the chip.
+constexpr int kSlots = 4;
+
+struct DecayPlan {
+    int64_t seg, nseg, n_work, cut;
+    size_t off_sum, off_seg, total;
+};
+
+void plan_bytes(DecayPlan& p, int64_t H, int64_t Dk, int64_t Dv, int64_t n_off) {
+    p.off_sum = p.off_seg = p.total = 0;
+    if (p.nseg <= 1) return;
+    p.off_sum = align_up((size_t)(p.n_work * H) * decay_state_values((int)Dk, (int)Dv) * 4);
+    p.off_seg = p.off_sum + align_up((size_t)(p.n_work * H) * 8);
+    p.total = p.off_seg + align_up((size_t)n_off * 4);
+}
+
+DecayPlan plan_dense(int64_t n_seqs, int64_t T, int64_t H, int64_t Dk, int64_t Dv, int flags) {
+    DecayPlan p{};
+    const int64_t whole = round_up(T, DECAY_CHUNK), blocks = n_seqs * H * slices_of(Dv);
+    p.seg = forced_segment(flags);
+    if (!p.seg) {
+        int64_t n = (int64_t)compute_units() * kSlots / blocks;
+        if (n > T / 64) n = T / 64;
+        p.seg = n < 2 ? whole : round_up((T + n - 1) / n, DECAY_CHUNK);
+    }
+    if (p.seg > whole) p.seg = whole;
+    p.nseg = (T + p.seg - 1) / p.seg;
+    p.n_work = n_seqs * p.nseg;
+    plan_bytes(p, H, Dk, Dv, 0);
+    return p;
+}
+
+// Packed: lengths are on the device, so a segment is an equal share of all tokens.  nseg > 1 says that there may be
+// segments.
+DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int64_t Dv, int flags) {
+    DecayPlan p{};
+    p.seg = forced_segment(flags);
+    if (!p.seg) {
+        p.seg = round_up(total * H * slices_of(Dv) / ((int64_t)compute_units() * kSlots), DECAY_CHUNK);
+        if (p.seg < 64) p.seg = 64;
+    }
+    p.cut = p.seg;
+    p.nseg = p.cut < total ? 2 : 1;
+    p.n_work = p.nseg > 1 ? total / p.seg + n_seqs : n_seqs;
+    plan_bytes(p, H, Dk, Dv, n_seqs + 1);
+    return p;
+}
+
+bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t Dv) {
+    const int64_t values = decay_state_values((int)Dk, (int)Dv);
+    return grid_ok(p.n_work, H * slices_of(Dv), 256) && grid_ok(n_seqs, H * ((values + 255) / 256), 256) &&
+           n_seqs <= kMaxGrid / (H * Dk * Dv);
+}
+
+void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+               const DecayPlan& p, char* ws) {
+    a.n_seqs = n_seqs;
+    a.T = T;
+    a.H = (int)H;
+    a.per = (int)(H / Hk);
+    a.Dk = (int)Dk;
+    a.Dv = (int)Dv;
+    a.slices = (int)slices_of(Dv);
+    a.seg = (int)p.seg;
+    a.nseg = (int)p.nseg;
+    a.n_work = p.n_work;
+    if (p.nseg > 1) {
+        a.ws_state = (float*)ws;
+        a.ws_sum = (float*)(ws + p.off_sum);
+    }
+}
+
+int run_attn(const DecayParams& a, int nseg, int io_dtype, hipStream_t s) {
+    if (nseg > 1) {
+        if (const int e = status(launch_decay_states(a, io_dtype, s))) return e;
+        if (const int e = status(launch_decay_carry(a, s))) return e;
+    }
+    return status(launch_decay_attn(a, io_dtype, s));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t triune_hip_decay_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                            int flags) {
+    if (B <= 0 || T <= 0 || !tokens_ok(B, T) || !decay_shape_ok(H, Hk, Dk, Dv) || !seqs_ok(B, H, Dv)) return 0;
+    const DecayPlan p = plan_dense(B, T, H, Dk, Dv, flags);
+    return grids_ok(p, B, H, Dk, Dv) ? p.total : 0;
+}
+
+int triune_hip_decay_attn(const void* q, const void* k, const void* v, const void* g, int io_dtype, int g_dtype,
+                          const int64_t* strides, float scale, const float* s0, void* o, float* s_final, int64_t B,
+                          int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int flags, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    if (!q || !k || !v || !g || !o || !strides) return TRIUNE_ERR_NULL;
+    if (!dtype_ok(io_dtype) || (g_dtype != io_dtype && g_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
+    if (!tokens_ok(B, T) || !decay_shape_ok(H, Hk, Dk, Dv) || !seqs_ok(B, H, Dv)) return TRIUNE_ERR_SHAPE;
+    if (!all_aligned(io_dtype, {q, k, v, o}) || !aligned(g, g_dtype) ||
+        !all_aligned(TRIUNE_DT_F32, {s0, s_final}))
+        return TRIUNE_ERR_LAYOUT;
+    if (B == 0) return TRIUNE_OK;
+    if (T == 0) {
+        if (!s_final) return TRIUNE_OK;
+        return status(launch_state_copy(s0, s_final, B * H * Dk * Dv, 4, (hipStream_t)stream));
+    }
+    const DecayPlan p = plan_dense(B, T, H, Dk, Dv, flags);
+    if (!grids_ok(p, B, H, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
+    DecayParams a{};
+    a.q = {q, strides[0], strides[1], strides[2]};
+    a.k = {k, strides[3], strides[4], strides[5]};
+    a.v = {v, strides[6], strides[7], strides[8]};
+    a.g = {g, strides[9], strides[10], strides[11]};
+    a.o = {o, strides[12], strides[13], strides[14]};
+    a.g_dt = g_dtype, a.scale = scale, a.s0 = s0, a.fin = s_final;
+    set_sizes(a, B, T, H, Hk, Dk, Dv, p, (char*)workspace);
+    return run_attn(a, a.nseg, io_dtype, (hipStream_t)stream);
+}
+
+size_t triune_hip_decay_attn_varlen_workspace_size(int64_t n_seqs, int64_t total_tokens, int64_t H, int64_t Hk,
+                                                   int64_t Dk, int64_t Dv, int flags) {
+    if (n_seqs <= 0 || total_tokens <= 0 || !tokens_ok(n_seqs, total_tokens) || !decay_shape_ok(H, Hk, Dk, Dv) ||
+        !seqs_ok(n_seqs, H, Dv))
+        return 0;
+    const DecayPlan p = plan_packed(n_seqs, total_tokens, H, Dk, Dv, flags);
+    return grids_ok(p, n_seqs, H, Dk, Dv) ? p.total : 0;
+}
+
+int triune_hip_decay_attn_varlen(const void* q, const void* k, const void* v, const void* g, int io_dtype, int g_dtype,
+                                 const int64_t* strides, float scale, const int32_t* cu_seqlens, int64_t n_seqs,
+                                 int64_t total_tokens, const float* s0, float* s_final, const int32_t* slots,
+                                 int64_t n_state_rows, void* o, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                 int flags, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k || !v || !g || !o || !strides || !cu_seqlens) return TRIUNE_ERR_NULL;
+    if (!dtype_ok(io_dtype) || (g_dtype != io_dtype && g_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
+    if (!tokens_ok(n_seqs, total_tokens) || n_state_rows < 0 || !decay_shape_ok(H, Hk, Dk, Dv) ||
+        !seqs_ok(n_seqs, H, Dv))
+        return TRIUNE_ERR_SHAPE;
+    if (!slots && (s0 || s_final) && n_state_rows < n_seqs) return TRIUNE_ERR_SHAPE;
+    if (!all_aligned(io_dtype, {q, k, v, o}) || !aligned(g, g_dtype) ||
+        !all_aligned(TRIUNE_DT_F32, {s0, s_final, cu_seqlens, slots}))
+        return TRIUNE_ERR_LAYOUT;
+    if (n_seqs == 0) return TRIUNE_OK;
+    // with no tokens every sequence's state still passes through: one empty segment each
+    const DecayPlan p = plan_packed(n_seqs, total_tokens > 0 ? total_tokens : 1, H, Dk, Dv, flags);
+    if (!grids_ok(p, n_seqs, H, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (const int e = check_ws(workspace, workspace_bytes, p.total)) return e;
+    DecayParams a{};
+    a.q = {q, 0, strides[0], strides[1]};
+    a.k = {k, 0, strides[2], strides[3]};
+    a.v = {v, 0, strides[4], strides[5]};
+    a.g = {g, 0, strides[6], strides[7]};
+    a.o = {o, 0, strides[8], strides[9]};
+    a.g_dt = g_dtype, a.scale = scale, a.s0 = s0, a.fin = s_final;
+    a.slots = slots, a.n_slots = n_state_rows, a.cu = cu_seqlens;
+    set_sizes(a, n_seqs, total_tokens, H, Hk, Dk, Dv, p, (char*)workspace);
+    const hipStream_t s = (hipStream_t)stream;
+    if (p.nseg > 1) {
+        int32_t* off = (int32_t*)((char*)workspace + p.off_seg);
+        SsmParams lengths{};  // what the offsets' kernel reads of them
+        lengths.cu = cu_seqlens, lengths.n_seqs = n_seqs, lengths.T = total_tokens;
+        lengths.seg = (int)p.seg, lengths.n_work = p.n_work;
+        if (const int e = status(launch_ssm_offsets(lengths, p.cut, off, s))) return e;
+        a.seg_off = off;
+    }
+    return run_attn(a, a.nseg, io_dtype, s);
+}
+
+int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* v, const void* g, int io_dtype,
+                                      int g_dtype, const int64_t* strides, float scale, const float* state_in,
+                                      float* state_out, const int32_t* slots, int64_t n_state_rows, void* o, int64_t B,
+                                      int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, void* stream) {
+    if (!q || !k || !v || !g || !o || !strides || !state_in || !state_out) return TRIUNE_ERR_NULL;
+    if (!dtype_ok(io_dtype) || (g_dtype != io_dtype && g_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
+    if (B < 0 || n_state_rows < 0 || !decay_shape_ok(H, Hk, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (!slots && n_state_rows < B) return TRIUNE_ERR_SHAPE;
+    if (!all_aligned(io_dtype, {q, k, v, o}) || !aligned(g, g_dtype) ||
+        !all_aligned(TRIUNE_DT_F32, {state_in, state_out, slots}))
+        return TRIUNE_ERR_LAYOUT;
+    if (!grid_ok(B, H, 256)) return TRIUNE_ERR_SHAPE;
+    if (B == 0) return TRIUNE_OK;
+    DecayStepParams a{};
+    a.q = {q, strides[0], 0, strides[1]};
+    a.k = {k, strides[2], 0, strides[3]};
+    a.v = {v, strides[4], 0, strides[5]};
+    a.g = {g, strides[6], 0, strides[7]};
+    a.o = {o, strides[8], 0, strides[9]};
+    a.g_dt = g_dtype, a.scale = scale, a.s_in = state_in, a.s_out = state_out;
+    a.slots = slots, a.n_rows = n_state_rows, a.Bn = B;
+    a.H = (int)H, a.per = (int)(H / Hk), a.Dk = (int)Dk, a.Dv = (int)Dv;
+    return status(launch_decay_step(a, io_dtype, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -1,36 +1,12 @@
 // abi_ssm.hip -- extern "C" entry points of the state space layer's operators (declared in
 // include/triune_hip.h): argument checks, workspace layout and launches.
 #include "../../include/triune_hip.h"
+#include "abi_common.h"
 #include "ssm.h"
-
-#include <atomic>
 
 using namespace triune;
 
 namespace {
-
-constexpr int kMaxDevices = 64;
-constexpr int64_t kMaxGrid = 0x7fffffff;
-
-size_t align_up(size_t x) { return (x + 255) / 256 * 256; }
-int status(hipError_t e) { return e == hipSuccess ? TRIUNE_OK : TRIUNE_ERR_LAUNCH; }
-bool dtype_ok(int dt) { return dt == TRIUNE_DT_F32 || dt == TRIUNE_DT_BF16 || dt == TRIUNE_DT_F16; }
-bool aligned(const void* p, int dt) { return reinterpret_cast<uintptr_t>(p) % (dt == TRIUNE_DT_F32 ? 4 : 2) == 0; }
-
-// Compute units of the current device, asked once per device (MI355X: 256).
-int compute_units() {
-    static std::atomic<int> cache[kMaxDevices];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDevices) {
-        (void)hipGetLastError();
-        return 256;
-    }
-    int n = cache[dev].load(std::memory_order_relaxed);
-    if (n > 0) return n;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
 
 // The kernels address a tile's 32 rows by 32-bit byte offsets.
 constexpr int64_t kMaxTokenStride = 1 << 22;
@@ -40,9 +16,6 @@ bool strides_ok(std::initializer_list<int64_t> st) {
     return true;
 }
 
-// Sequences and tokens within the numbers that the plans multiply.
-bool tokens_ok(int64_t n, int64_t T) { return n >= 0 && n <= kMaxGrid && T >= 0 && T < (1 << 30); }
-
 bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
     return Dm > 0 && Dm < kMaxTokenStride && G > 0 && Dm % G == 0 && N > 0 && N <= SSM_MAX_N;
 }
@@ -50,11 +23,6 @@ bool ssm_shape_ok(int64_t Dm, int64_t G, int N) {
 int64_t group_blocks(int64_t Dm, int64_t G) { return (Dm / G + 63) / 64; }
 int64_t all_blocks(int64_t Dm, int64_t G) { return G * group_blocks(Dm, G); }
 
-// Whether n times `blocks` workgroups are a grid: 31 bits of workgroups and 32 of threads.
-bool grid_ok(int64_t n, int64_t blocks, int threads) {
-    const int64_t by_threads = (int64_t)0xffffffff / threads, most = by_threads < kMaxGrid ? by_threads : kMaxGrid;
-    return n <= most / blocks;
-}
 // The grids of a scan: its work items, and the join's.
 bool scan_grids_ok(bool packed, int64_t n_work, int64_t nseg, int64_t n_seqs, int64_t Dm, int64_t G, int N) {
     if (!grid_ok(n_work, all_blocks(Dm, G), 64 * ssm_waves(N)) || n_seqs > kMaxGrid / (Dm * N)) return false;
@@ -179,18 +147,6 @@ void set_sizes(SsmParams& a, int64_t n_seqs, int64_t T, int64_t Dm, int64_t G, i
         a.ws_state = (float*)ws;
         a.ws_sum = (float*)(ws + p.off_sum);
     }
-}
-
-int check_ws(const void* ws, size_t have, size_t need) {
-    if (need == 0) return TRIUNE_OK;
-    if (!ws || have < need) return TRIUNE_ERR_WORKSPACE;
-    return reinterpret_cast<uintptr_t>(ws) % 16 ? TRIUNE_ERR_LAYOUT : TRIUNE_OK;
-}
-
-bool all_aligned(int dt, std::initializer_list<const void*> ps) {
-    for (const void* p : ps)
-        if (!aligned(p, dt)) return false;
-    return true;
 }
 
 }  // namespace

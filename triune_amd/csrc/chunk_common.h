@@ -125,15 +125,6 @@ __device__ __forceinline__ Split8<NP> lds_frag(const char* base, int plane_bytes
     return f;
 }
 
-// ds_read_b64_tr_b16: within each 16-lane group, lane m supplies the address of four
-// consecutive 16-bit elements M[m][0..3]; lane i receives M[4j + (i >> 2)][i & 3], j = 0..3.
-__device__ __forceinline__ bf16x4 lds_read_tr(const __bf16* p) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    return __builtin_bit_cast(bf16x4, r);
-}
-
 // Fragment whose lane index is a plane column (K index down the rows): lane (g4, r16) gets
 // column col0 + r16 of rows row0 + 4*g4 + [0,4) (K slots 0..3) and row0 + 16 + 4*g4 + [0,4)
 // (slots 4..7).  Lane (g4, m) addresses row row0 + 4*g4 + (m >> 2), columns col0 + 4*(m & 3).

@@ -380,7 +380,9 @@ __device__ __forceinline__ int64_t ssm_followed(const SsmParams& a, int64_t j) {
     }
     return lo;
 }
-__device__ __forceinline__ bool ssm_segment(const SsmParams& a, int64_t w, SsmSeg& s, int64_t seq = -1) {
+// P: SsmParams, or another block with its n_seqs, T, seg, nseg, cu and seg_off.
+template <typename P>
+__device__ __forceinline__ bool ssm_segment(const P& a, int64_t w, SsmSeg& s, int64_t seq = -1) {
     if (!a.cu) {
         s.seq = w / a.nseg;
         s.index = (int)(w - s.seq * a.nseg);
