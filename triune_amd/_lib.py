@@ -198,6 +198,12 @@ def _bind(lib):
              _i, _vp, _sz, _vp],
             _i,
         ),
+        "triune_hip_decay_attn_bwd_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i], _sz),
+        "triune_hip_decay_attn_bwd": (
+            [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i64, _i64, _i64,
+             _i64, _i64, _i, _vp, _sz, _vp],
+            _i,
+        ),
         "triune_hip_decay_attn_decode_step": (
             [_vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp],
             _i,
@@ -274,6 +280,8 @@ EXPORTS = (
     "triune_hip_decay_attn",
     "triune_hip_decay_attn_varlen_workspace_size",
     "triune_hip_decay_attn_varlen",
+    "triune_hip_decay_attn_bwd_workspace_size",
+    "triune_hip_decay_attn_bwd",
     "triune_hip_decay_attn_decode_step",
     "triune_hip_layer_norm",
     "triune_hip_layer_norm_bwd_workspace_size",

@@ -67,10 +67,44 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
     return p;
 }
 
+// Gradients: segments of whole chunks, the states of every chunk, and sums of shared heads and of constant gates.
+struct GradPlan {
+    DecayPlan p;
+    int64_t chunk, nc;
+    size_t off_S, off_R, off_q, off_k, off_g, total;
+};
+
+GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int io_dtype, int g_head,
+                   int flags) {
+    GradPlan r{};
+    r.chunk = decay_grad_chunk(io_dtype == TRIUNE_DT_BF16);
+    r.nc = (T + r.chunk - 1) / r.chunk;
+    r.p = plan_dense(B, T, H, Dk, Dv, flags);
+    if (r.p.nseg > 1) {
+        r.p.seg = round_up(r.p.seg, r.chunk);
+        r.p.nseg = (T + r.p.seg - 1) / r.p.seg;
+        r.p.n_work = B * r.p.nseg;
+        plan_bytes(r.p, H, Dk, Dv, 0);
+    }
+    const size_t states = align_up((size_t)(B * H * r.nc) * decay_state_values((int)Dk, (int)Dv) * 4);
+    const size_t shared = H > Hk ? align_up((size_t)(B * T * H) * Dk * 4) : 0;
+    r.off_S = r.p.total;
+    r.off_R = r.off_S + states;
+    r.off_q = r.off_R + states;
+    r.off_k = r.off_q + shared;
+    r.off_g = r.off_k + shared;
+    r.total = r.off_g + (g_head ? align_up((size_t)(B * r.nc * H) * 4) : 0);
+    return r;
+}
+
 bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t Dv) {
     const int64_t values = decay_state_values((int)Dk, (int)Dv);
     return grid_ok(p.n_work, H * slices_of(Dv), 256) && grid_ok(n_seqs, H * ((values + 255) / 256), 256) &&
            n_seqs <= kMaxGrid / (H * Dk * Dv);
+}
+
+bool grad_grids_ok(const GradPlan& r, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv) {
+    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 512) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
 }
 
 void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -93,8 +127,8 @@ void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk,
 
 int run_attn(const DecayParams& a, int nseg, int io_dtype, hipStream_t s) {
     if (nseg > 1) {
-        if (const int e = status(launch_decay_states(a, io_dtype, s))) return e;
-        if (const int e = status(launch_decay_carry(a, s))) return e;
+        if (const int e = status(launch_decay_walk(DecayWalkParams{a, nullptr, 0}, false, io_dtype, s))) return e;
+        if (const int e = status(launch_decay_carry(a, false, s))) return e;
     }
     return status(launch_decay_attn(a, io_dtype, s));
 }
@@ -186,6 +220,60 @@ int triune_hip_decay_attn_varlen(const void* q, const void* k, const void* v, co
         a.seg_off = off;
     }
     return run_attn(a, a.nseg, io_dtype, s);
+}
+
+size_t triune_hip_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                                int io_dtype, int g_head, int flags) {
+    if (B <= 0 || T <= 0 || !tokens_ok(B, T) || !dtype_ok(io_dtype) || !decay_shape_ok(H, Hk, Dk, Dv) ||
+        !seqs_ok(B, H, Dv))
+        return 0;
+    const GradPlan r = plan_grad(B, T, H, Hk, Dk, Dv, io_dtype, g_head, flags);
+    return grad_grids_ok(r, B, T, H, Hk, Dk, Dv) ? r.total : 0;
+}
+
+int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const void* dout,
+                              int io_dtype, int g_dtype, const int64_t* strides, float scale, const float* s0,
+                              const float* ds_final, void* dq, void* dk, void* dv, void* dg, int g_head, float* ds0,
+                              int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int flags,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k || !v || !g || !dout || !strides || !dq || !dk || !dv || !dg) return TRIUNE_ERR_NULL;
+    if (!dtype_ok(io_dtype) || (g_dtype != io_dtype && g_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
+    if (B <= 0 || T <= 0 || !tokens_ok(B, T) || !decay_shape_ok(H, Hk, Dk, Dv) || !seqs_ok(B, H, Dv))
+        return TRIUNE_ERR_SHAPE;
+    if (!all_aligned(io_dtype, {q, k, v, dout, dq, dk, dv}) || !aligned(g, g_dtype) || !aligned(dg, g_dtype) ||
+        !all_aligned(TRIUNE_DT_F32, {s0, ds_final, ds0}))
+        return TRIUNE_ERR_LAYOUT;
+    const GradPlan r = plan_grad(B, T, H, Hk, Dk, Dv, io_dtype, g_head, flags);
+    if (!grad_grids_ok(r, B, T, H, Hk, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (const int e = check_ws(workspace, workspace_bytes, r.total)) return e;
+    char* ws = (char*)workspace;
+    const hipStream_t s = (hipStream_t)stream;
+    DecayGradParams p{};
+    DecayParams& a = p.f;
+    a.q = {q, strides[0], strides[1], strides[2]};
+    a.k = {k, strides[3], strides[4], strides[5]};
+    a.v = {v, strides[6], strides[7], strides[8]};
+    a.g = {g, strides[9], strides[10], strides[11]};
+    a.o = {dout, strides[12], strides[13], strides[14]};
+    a.g_dt = g_dtype, a.scale = scale;
+    set_sizes(a, B, T, H, Hk, Dk, Dv, r.p, ws);
+    p.S = (float*)(ws + r.off_S), p.R = (float*)(ws + r.off_R), p.nc = r.nc;
+    p.dq = dq, p.dk = dk, p.dv = dv, p.dg = dg;
+    if (H > Hk) p.part_q = (float*)(ws + r.off_q), p.part_k = (float*)(ws + r.off_k);
+    if (g_head) p.part_g = (float*)(ws + r.off_g);
+    for (const bool rev : {false, true}) {
+        DecayWalkParams x{a, nullptr, (int)r.chunk};
+        x.f.s0 = rev ? ds_final : s0;
+        x.f.fin = rev ? ds0 : nullptr;
+        if (rev) x.f.k = a.q, x.f.v = a.o;
+        if (r.p.nseg > 1) {
+            if (const int e = status(launch_decay_walk(x, rev, io_dtype, s))) return e;
+            if (const int e = status(launch_decay_carry(x.f, rev, s))) return e;
+        }
+        x.states = const_cast<float*>(rev ? p.R : p.S);
+        if (const int e = status(launch_decay_walk(x, rev, io_dtype, s))) return e;
+    }
+    return status(launch_decay_grad(p, io_dtype, s));
 }
 
 int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* v, const void* g, int io_dtype,

@@ -35,10 +35,31 @@ struct DecayParams {
 
 // Columns of a slice, and the values that a segment's state takes in the workspace.
 int decay_slice(int Dv);
+int decay_padded_dk(int Dk);
 int64_t decay_state_values(int Dk, int Dv);
-hipError_t launch_decay_states(const DecayParams& a, int io_dt, hipStream_t s);
-hipError_t launch_decay_carry(const DecayParams& a, hipStream_t s);
+// The walks that form states.  rev: gradients of states, from the end.
+struct DecayWalkParams {
+    DecayParams f;            // rows in k, columns in v
+    float* states;            // [n_seqs, H, ceil(T / every), values] or null: the segments' end states instead
+    int every;                // of 32 tokens' multiples; segments are multiples of it
+};
+hipError_t launch_decay_walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
+hipError_t launch_decay_carry(const DecayParams& a, bool rev, hipStream_t s);
 hipError_t launch_decay_attn(const DecayParams& a, int io_dt, hipStream_t s);
+
+// Tokens of a chunk of the gradients: 64, or 32 for operands in fp32, whose tiles take twice the LDS.
+constexpr int decay_grad_chunk(bool bf16) { return bf16 ? 64 : 32; }
+
+struct DecayGradParams {
+    DecayParams f;            // o: the gradient of the outputs
+    const float *S, *R;       // [n_seqs, H, nc, values]: states in front of the chunks, gradients of those behind them
+    int64_t nc;               // chunks of a sequence
+    void *dq, *dk, *dv;       // contiguous, I/O dtype
+    float *part_q, *part_k;   // [n_seqs T, H, Dk] where heads share q and k, else null
+    void* dg;                 // [n_seqs, T, H], or [H] with part_g
+    float* part_g;            // [n_seqs nc, H] or null
+};
+hipError_t launch_decay_grad(const DecayGradParams& p, int io_dt, hipStream_t s);
 
 struct DecayStepParams {
     DecayTok q, k, v, g, o;   // sb and sh: strides of the batch and the heads

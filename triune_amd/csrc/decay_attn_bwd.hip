@@ -1,0 +1,413 @@
+// decay_attn_bwd.hip -- gradients of decay attention (decay_attn.hip) on gfx950.
+//
+// Per chunk, with S_0 the state in front of it, R the gradient of the state behind it, and for j <= i
+//     A_ij = scale e^{G_i - G_j} (q_i . k_j),   B_ij = scale e^{G_i - G_j} (do_i . v_j):
+//     dq_i = sum_j B_ij k_j + scale e^{G_i} S_0 do_i
+//     dk_j = sum_i B_ij q_i + e^{G_C - G_j} R v_j
+//     dv_j = sum_i A_ij do_i + e^{G_C - G_j} R^T k_j
+//     dg_t = what passes from writes before t to reads at t or behind it:
+//            sum_{i >= t} q_i . dq'_i + sum_{j < t} k_j . dk'_j + e^{G_C} <S_0, R> + sum_{j < t <= i} (q_i . k_j) B_ij
+// with dq', dk' the terms with S_0 and R.  Only pairs that span t are added, so steep gates, whose own pairs are large
+// and spanning ones small, lose nothing to cancellation.
+//
+// The states in front of the chunks and the gradients behind them come from two walks (decay_walk_kernel), so a
+// workgroup takes one (chunk, head) by itself.  A and B are formed once, in tiles over the waves, and shared through
+// LDS; a wave owns 16-wide tiles of key dims (dq, dk) and of value dims (dv), so a state is read once for each use.
+#include "decay_mfma.h"
+
+namespace triune {
+
+namespace {
+
+// Causal tile idx: token rows I (read) and J <= I (written).
+__device__ __forceinline__ void tile_of(int idx, int& I, int& J) {
+    I = idx >= 6 ? 3 : idx >= 3 ? 2 : idx >= 1 ? 1 : 0;
+    J = idx - I * (I + 1) / 2;
+}
+__device__ __forceinline__ int tile_index(int I, int J) { return I * (I + 1) / 2 + J; }
+
+// Four values as NP planes of parts.
+template <typename TC, int NP>
+__device__ __forceinline__ void put4(TC* plane, int plane_size, int off, const f32x4& x) {
+    if constexpr (Mat<TC>::E == 8) {
+        float r[4] = {x[0], x[1], x[2], x[3]};
+        uint32_t w[NP][2];
+        split_pairs<NP, 2>(r, w);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<uint2*>(plane + p * plane_size + off) = uint2{w[p][0], w[p][1]};
+    } else {
+        *reinterpret_cast<f32x4*>(plane + off) = x;
+    }
+}
+
+// Sums over the lanes at and behind this one of its row of 16.
+__device__ __forceinline__ float row_suffix_scan(float x) {
+    x += row_shl<1>(x);
+    x += row_shl<2>(x);
+    x += row_shl<4>(x);
+    x += row_shl<8>(x);
+    return x;
+}
+
+template <int E>
+__device__ __forceinline__ void load_floats(const float* p, float (&x)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+    }
+}
+
+}  // namespace
+
+template <typename TIO, typename TC, int DK, int DVW, int NW>
+__global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) {
+    const DecayParams& a = p.f;
+    constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, CH = decay_grad_chunk(E == 8), CT = CH / 16, TJ = CH / KS;
+    constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(DVW), RC = tile_stride<TC>(CH), NTH = NW * 64;
+    constexpr int TILES = CT * (CT + 1) / 2, MT = (TILES + NW - 1) / NW, NP = E == 8 ? 2 : 1, PL = CH * RC;
+    constexpr int NDK = DK / 16 < NW ? 1 : DK / 16 / NW, NDV = DVW / 16 < NW ? 1 : DVW / 16 / NW;
+    using Frag = typename Mat<TC>::Frag;
+    __shared__ __attribute__((aligned(16))) TC s_q[CH * RK], s_k[CH * RK], s_v[CH * RV], s_d[CH * RV];
+    __shared__ __attribute__((aligned(16))) TC s_A[NP * PL], s_B[NP * PL];
+    __shared__ float s_g[2][CH], s_x[NW][CH], s_y[NW][CH], s_z[NW];
+    __shared__ float s_r[TILES][16], s_c[TILES][16], s_tot[TILES], s_diag[CT][16];
+    const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15;
+    const int h = (int)(blockIdx.x % a.H);
+    const int64_t sc = blockIdx.x / a.H, seq = sc / p.nc, c = sc - seq * p.nc, t0 = c * CH;
+    const int rows = (int)min((int64_t)CH, a.T - t0), hk = h / a.per;
+    const int64_t wide = (int64_t)DVW * a.slices, values = DK * wide;
+    const float* pS = p.S + ((seq * a.H + h) * p.nc + c) * values;
+    const float* pR = p.R + ((seq * a.H + h) * p.nc + c) * values;
+    auto at = [&](const DecayTok& t, int head) { return seq * t.sb + t0 * t.st + head * t.sh; };
+
+    load_tile<TIO, TC, CH, DK, NTH>(s_q, (const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
+    load_tile<TIO, TC, CH, DK, NTH>(s_k, (const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
+    if (w == 0) {
+        const Sum2 gs = chunk_sums<CH>(a.g, a.g_dt, at(a.g, h), rows, lane);
+        if (lane < CH) s_g[0][lane] = gs.hi, s_g[1][lane] = gs.lo;
+    }
+    if constexpr (E == 8) {  // a K step of 32 tokens takes the tile above the diagonal along: zeros
+        for (int u = threadIdx.x; u < CT / 2 * NP * 2 * 16 * 4; u += NTH) {
+            const int q = u & 3, row = (u >> 2) & 15, pl = (u >> 6) & 1, b = u >> 7 & (NP - 1), I = 2 * (u >> 8);
+            TC* to = (pl ? s_B : s_A) + b * PL + (16 * I + row) * RC + 16 * (I + 1) + 4 * q;
+            *reinterpret_cast<uint2*>(to) = uint2{0, 0};
+        }
+    }
+    __syncthreads();
+    auto sum_at = [&](int t) { return Sum2{s_g[0][t], s_g[1][t]}; };
+    const Sum2 end = sum_at(CH - 1);
+
+    f32x4 am[MT], bm[MT], dec[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        am[m] = bm[m] = dec[m] = zero4();
+        const int idx = w + NW * m;
+        if (idx >= TILES) continue;
+        int I, J;
+        tile_of(idx, I, J);
+#pragma unroll
+        for (int s = 0; s < DK / KS; ++s)
+            am[m] = Mat<TC>::mma(row_frag(s_k, RK, 16 * J + n, s, g), row_frag(s_q, RK, 16 * I + n, s, g), am[m]);
+        const Sum2 Gi = sum_at(16 * I + n);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            dec[m][r] = J < I || 4 * g + r <= n ? a.scale * decay_between(Gi, sum_at(16 * J + 4 * g + r)) : 0.f;
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = J < I || 4 * g + r <= n ? am[m][r] * dec[m][r] : 0.f;
+        put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
+    }
+
+    f32x4 dq[NDK][CT], dk[NDK][CT];
+#pragma unroll
+    for (int d = 0; d < NDK; ++d)
+#pragma unroll
+        for (int I = 0; I < CT; ++I) dq[d][I] = dk[d][I] = zero4();
+    float z = 0.f;
+    for (int sl = 0; sl < a.slices; ++sl) {
+        const int col0 = sl * DVW;
+        if (sl) __syncthreads();
+        load_tile<TIO, TC, CH, DVW, NTH>(s_v, (const TIO*)a.v.p + at(a.v, h) + col0, a.v.st, rows, a.Dv - col0);
+        load_tile<TIO, TC, CH, DVW, NTH>(s_d, (const TIO*)a.o.p + at(a.o, h) + col0, a.o.st, rows, a.Dv - col0);
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int idx = w + NW * m;
+            if (idx >= TILES) continue;
+            int I, J;
+            tile_of(idx, I, J);
+#pragma unroll
+            for (int s = 0; s < DVW / KS; ++s)
+                bm[m] = Mat<TC>::mma(row_frag(s_v, RV, 16 * J + n, s, g), row_frag(s_d, RV, 16 * I + n, s, g), bm[m]);
+        }
+#pragma unroll
+        for (int d = 0; d < NDK; ++d) {
+            const int t = w * NDK + d;
+            if (t >= DK / 16) continue;
+            const int64_t off = (16 * t + n) * wide + col0 + E * g;
+#pragma unroll
+            for (int s = 0; s < DVW / KS; ++s) {
+                float xs[E], xr[E];
+                load_floats<E>(pS + off + s * KS, xs);
+                load_floats<E>(pR + off + s * KS, xr);
+#pragma unroll
+                for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[e], xr[e], z);
+                const auto ps = parts<TC, 3>(xs);
+                const auto pr = parts<TC, 3>(xr);
+#pragma unroll
+                for (int I = 0; I < CT; ++I) {
+                    dq[d][I] = mma<TC>(ps, row_frag(s_d, RV, 16 * I + n, s, g), dq[d][I]);
+                    dk[d][I] = mma<TC>(pr, row_frag(s_v, RV, 16 * I + n, s, g), dk[d][I]);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < NDV; ++d) {
+            const int t = w * NDV + d;
+            if (t >= DVW / 16) continue;
+            f32x4 dv[CT];
+#pragma unroll
+            for (int J = 0; J < CT; ++J) dv[J] = zero4();
+#pragma unroll
+            for (int s = 0; s < DK / KS; ++s) {
+                float xr[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) xr[e] = pR[(s * KS + E * g + e) * wide + col0 + 16 * t + n];
+                const auto pr = parts<TC, 3>(xr);
+#pragma unroll
+                for (int J = 0; J < CT; ++J) dv[J] = mma<TC>(pr, row_frag(s_k, RK, 16 * J + n, s, g), dv[J]);
+            }
+#pragma unroll
+            for (int J = 0; J < CT; ++J) {
+                const int j = 16 * J + n;
+                dv[J] *= decay_between(end, sum_at(j));
+#pragma unroll
+                for (int s = 16 * J / KS; s < TJ; ++s) {
+                    const Frag x = col_frag<TC, false>(s_d, RV, t, s, g, n);
+#pragma unroll
+                    for (int b = NP - 1; b >= 0; --b)
+                        dv[J] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, J, s, g, n), dv[J]);
+                }
+                const int dim = col0 + 16 * t + 4 * g;
+                const float o[4] = {dv[J][0], dv[J][1], dv[J][2], dv[J][3]};
+                if (j < rows) store_raw<4>((TIO*)p.dv + ((seq * a.T + t0 + j) * a.H + h) * a.Dv + dim, a.Dv - dim, o);
+            }
+        }
+    }
+
+    // B, and the sums of (q . k) B over its tiles that the gates' gradients take
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int idx = w + NW * m;
+        if (idx >= TILES) continue;
+        int I, J;
+        tile_of(idx, I, J);
+        f32x4 x, M;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            x[r] = J < I || 4 * g + r <= n ? bm[m][r] * dec[m][r] : 0.f;
+            M[r] = J < I || 4 * g + r < n ? am[m][r] * x[r] : 0.f;
+        }
+        put4<TC, NP>(s_B, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
+        if (J < I) {
+            float col = (M[0] + M[1]) + (M[2] + M[3]);
+            col = xor_sum<32>(xor_sum<16>(col));
+            if (g == 0) s_c[idx][n] = col;
+            col = dpp_sum16(col);
+            if (lane == 0) s_tot[idx] = col;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float row = dpp_sum16(M[r]);
+                if (n == 0) s_r[idx][4 * g + r] = row;
+            }
+        } else {
+            // for every t = 4 g + r: written before t (rows of lower r and g), read at t or behind (n >= t)
+            const float all = (M[0] + M[1]) + (M[2] + M[3]);
+            const RowPair by1 = swap16(all);
+            const float by2 = swap32(by1.lo + by1.hi).lo;
+            float before = ((g & 1) ? by1.lo : 0.f) + ((g & 2) ? by2 : 0.f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float sum = dpp_sum16(n >= 4 * g + r ? before : 0.f);
+                if (n == 0) s_diag[I][4 * g + r] = sum;
+                before += M[r];
+            }
+        }
+    }
+    __syncthreads();
+
+    float xs[CT], ys[CT];
+#pragma unroll
+    for (int I = 0; I < CT; ++I) xs[I] = ys[I] = 0.f;
+#pragma unroll
+    for (int d = 0; d < NDK; ++d) {
+        const int t = w * NDK + d;
+        if (t >= DK / 16) continue;
+        const int dim = 16 * t + 4 * g;
+#pragma unroll
+        for (int I = 0; I < CT; ++I) {
+            const int i = 16 * I + n;
+            const Sum2 Gi = sum_at(i);
+            const float fq = a.scale * __builtin_amdgcn_exp2f(Gi.hi + Gi.lo), fk = decay_between(end, Gi);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                dq[d][I][r] *= fq;
+                dk[d][I][r] *= fk;
+                xs[I] = __builtin_fmaf((float)s_q[i * RK + dim + r], dq[d][I][r], xs[I]);
+                ys[I] = __builtin_fmaf((float)s_k[i * RK + dim + r], dk[d][I][r], ys[I]);
+            }
+#pragma unroll
+            for (int s = 0; s <= (16 * I + 15) / KS; ++s) {
+                const Frag x = col_frag<TC, false>(s_k, RK, t, s, g, n);
+#pragma unroll
+                for (int b = NP - 1; b >= 0; --b)
+                    dq[d][I] = Mat<TC>::mma(x, row_frag_tok(s_B + b * PL, RC, i, s, g), dq[d][I]);
+            }
+#pragma unroll
+            for (int s = 16 * I / KS; s < TJ; ++s) {
+                const Frag x = col_frag<TC, false>(s_q, RK, t, s, g, n);
+#pragma unroll
+                for (int b = NP - 1; b >= 0; --b)
+                    dk[d][I] = Mat<TC>::mma(x, col_frag<TC, false>(s_B + b * PL, RC, I, s, g, n), dk[d][I]);
+            }
+            if (i >= rows) continue;
+            const float oq[4] = {dq[d][I][0], dq[d][I][1], dq[d][I][2], dq[d][I][3]};
+            const float ok[4] = {dk[d][I][0], dk[d][I][1], dk[d][I][2], dk[d][I][3]};
+            const int64_t tok = seq * a.T + t0 + i;
+            if (p.part_q) {  // of one head of several that share q and k
+                const int64_t off = (tok * a.H + h) * a.Dk + dim;
+                store_raw<4>(p.part_q + off, a.Dk - dim, oq);
+                store_raw<4>(p.part_k + off, a.Dk - dim, ok);
+            } else {
+                const int64_t off = (tok * (a.H / a.per) + hk) * a.Dk + dim;
+                store_raw<4>((TIO*)p.dq + off, a.Dk - dim, oq);
+                store_raw<4>((TIO*)p.dk + off, a.Dk - dim, ok);
+            }
+        }
+    }
+#pragma unroll
+    for (int I = 0; I < CT; ++I) {
+        const float x = xor_sum<32>(xor_sum<16>(xs[I])), y = xor_sum<32>(xor_sum<16>(ys[I]));
+        if (g == 0) s_x[w][16 * I + n] = x, s_y[w][16 * I + n] = y;
+    }
+    z = xor_sum<16>(xor_sum<32>(dpp_sum16(z)));
+    if (lane == 0) s_z[w] = z;
+    __syncthreads();
+    if (w) return;
+
+    const int t = lane & (CH - 1), blk = t >> 4;
+    float x = 0.f, y = 0.f, across = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) x += s_x[k][t], y += s_y[k][t], across += s_z[k];
+    across *= __builtin_amdgcn_exp2f(end.hi + end.lo);
+    float rs = 0.f, cs = 0.f;
+    for (int I = blk + 1; I < CT; ++I) rs += s_r[tile_index(I, blk)][n];
+    for (int J = 0; J < blk; ++J) {
+        cs += s_c[tile_index(blk, J)][n];
+        for (int I = blk + 1; I < CT; ++I) across += s_tot[tile_index(I, J)];
+    }
+    // lanes 0 .. CH - 1: sums at and behind t of x, in front of t of y
+    x = row_suffix_scan(x);
+    y = row_inclusive_scan(y);
+    float later = 0.f, earlier = 0.f;
+#pragma unroll
+    for (int b = 0; b < CT; ++b) {
+        const float xb = lane_value(x, 16 * b), yb = lane_value(y, 16 * b + 15);
+        if (b > blk) later += xb;
+        if (b < blk) earlier += yb;
+    }
+    float dg = (x + later) + (row_shr<1>(y) + earlier) + across + row_shr<1>(row_inclusive_scan(rs)) +
+               row_suffix_scan(cs) + s_diag[blk][n];
+    const bool in = lane < CH && t < rows;
+    const float gate = in ? load_dt(a.g.p, a.g_dt, at(a.g, h) + t * a.g.st) : 0.f;
+    if (!in || gate > 0.f) dg = 0.f;
+    if (p.part_g) {
+        dg = xor_sum<16>(xor_sum<32>(dpp_sum16(dg)));
+        if (lane == 0) p.part_g[(seq * p.nc + c) * a.H + h] = dg;
+    } else if (in) {
+        store_dt(p.dg, a.g_dt, (seq * a.T + t0 + t) * a.H + h, dg);
+    }
+}
+
+// dq and dk of shared heads: the sum over the heads that share them, in their order.
+template <typename TIO>
+__global__ __launch_bounds__(256) void decay_share_kernel(DecayGradParams p, int64_t n) {
+    const DecayParams& a = p.f;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int64_t head = i / a.Dk, d = i - head * a.Dk;
+    float q = 0.f, k = 0.f;
+    for (int s = 0; s < a.per; ++s) {
+        const int64_t off = (head * a.per + s) * a.Dk + d;
+        q += p.part_q[off];
+        k += p.part_k[off];
+    }
+    ((TIO*)p.dq)[i] = (TIO)q;
+    ((TIO*)p.dk)[i] = (TIO)k;
+}
+
+// dg of constants per head: the chunks' sums, sixteen threads a head, then these, in a fixed order.
+__global__ __launch_bounds__(1024) void decay_gate_kernel(DecayGradParams p, int64_t parts) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, h = blockIdx.x * 64 + l, H = p.f.H;
+    __shared__ float red[16][64];
+    float s = h < H ? sum_parts(p.part_g + h, H, w, parts) : 0.f;
+    red[w][l] = s;
+    __syncthreads();
+    if (w || h >= H) return;
+    for (int i = 1; i < 16; ++i) s += red[i][l];
+    store_dt(p.dg, p.f.g_dt, h, s);
+}
+
+namespace {
+
+template <typename TIO, typename TC, int DK, int DVW>
+hipError_t grad_one(const DecayGradParams& p, hipStream_t s) {
+    constexpr int NW = DK == 128 || DVW == 128 ? 8 : 4;
+    decay_grad_kernel<TIO, TC, DK, DVW, NW>
+        <<<dim3((unsigned)(p.f.n_seqs * p.nc * p.f.H)), NW * 64, 0, s>>>(p);
+    return hipGetLastError();
+}
+template <typename TIO, typename TC, int DK>
+hipError_t grad_width(const DecayGradParams& p, hipStream_t s) {
+    switch (decay_slice(p.f.Dv)) {
+        case 32: return grad_one<TIO, TC, DK, 32>(p, s);
+        case 64: return grad_one<TIO, TC, DK, 64>(p, s);
+        default: return grad_one<TIO, TC, DK, 128>(p, s);
+    }
+}
+template <typename TIO, typename TC>
+hipError_t grad_dk(const DecayGradParams& p, hipStream_t s) {
+    switch (decay_padded_dk(p.f.Dk)) {
+        case 32: return grad_width<TIO, TC, 32>(p, s);
+        case 64: return grad_width<TIO, TC, 64>(p, s);
+        default: return grad_width<TIO, TC, 128>(p, s);
+    }
+}
+template <typename TIO>
+hipError_t share(const DecayGradParams& p, hipStream_t s) {
+    const int64_t n = p.f.n_seqs * p.f.T * (p.f.H / p.f.per) * p.f.Dk;
+    decay_share_kernel<TIO><<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(p, n);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_decay_grad(const DecayGradParams& p, int io_dt, hipStream_t s) {
+    hipError_t e = io_dt == DT_F32    ? grad_dk<float, float>(p, s)
+                   : io_dt == DT_BF16 ? grad_dk<__bf16, __bf16>(p, s)
+                                      : grad_dk<_Float16, float>(p, s);
+    if (e != hipSuccess) return e;
+    if (p.part_q) {
+        e = io_dt == DT_F32 ? share<float>(p, s) : io_dt == DT_BF16 ? share<__bf16>(p, s) : share<_Float16>(p, s);
+        if (e != hipSuccess) return e;
+    }
+    if (p.part_g) {
+        decay_gate_kernel<<<dim3((unsigned)((p.f.H + 63) / 64)), 1024, 0, s>>>(p, p.f.n_seqs * p.nc);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+}  // namespace triune

@@ -88,19 +88,124 @@ __device__ __forceinline__ typename Mat<TC>::Frag row_frag(const TC* tile, int R
     return *reinterpret_cast<const typename Mat<TC>::Frag*>(tile + row * RS + s * Mat<TC>::KS + Mat<TC>::E * g);
 }
 
-// Columns of a [32 tokens][D] tile as an operand whose K index is the token: fragment j of 32 / KS.  `PERM`: column m
+// Columns of a [tokens][D] tile as an operand whose K index is the token: K step j.  `PERM`: column m
 // of the operand is tile_dim(t, m), else 16 t + m.
 template <typename TC, bool PERM>
 __device__ __forceinline__ typename Mat<TC>::Frag col_frag(const TC* tile, int RS, int t, int j, int g, int n) {
     if constexpr (Mat<TC>::E == 8) {
         const int col = PERM ? 32 * (t >> 1) + 8 * (n & 3) + 4 * (t & 1) : 16 * t + 4 * (n & 3);
-        const __bf16* p = tile + (4 * g + (n >> 2)) * RS + col;
+        const __bf16* p = tile + (32 * j + 4 * g + (n >> 2)) * RS + col;
         const bf16x4 a = lds_read_tr(p), b = lds_read_tr(p + 16 * RS);
         return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     } else {
         const float* p = tile + (16 * j + 4 * g) * RS + 16 * t + n;
         return f32x4{p[0], p[RS], p[2 * RS], p[3 * RS]};
     }
+}
+
+// K step j of row `row`, its K indexes in the order of col_frag's.
+template <typename TC>
+__device__ __forceinline__ typename Mat<TC>::Frag row_frag_tok(const TC* tile, int RS, int row, int j, int g) {
+    if constexpr (Mat<TC>::E == 8) {
+        const __bf16* p = tile + row * RS + 32 * j + 4 * g;
+        const bf16x4 a = *reinterpret_cast<const bf16x4*>(p), b = *reinterpret_cast<const bf16x4*>(p + 16);
+        return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+        return row_frag(tile, RS, row, j, g);
+    }
+}
+
+// ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`.
+template <typename TIO, typename TC, int ROWS, int D, int NTH>
+__device__ __forceinline__ void load_tile(TC* tile, const TIO* p, int64_t st, int rows, int cols) {
+    constexpr int E = Mat<TC>::E, UNITS = D / E, RS = tile_stride<TC>(D);
+#pragma unroll
+    for (int u = threadIdx.x; u < ROWS * UNITS; u += NTH) {
+        const int row = u / UNITS, c = u % UNITS * E;
+        Raw<TIO, E> r = load_raw<E>(p + (row < rows ? row * st + c : 0), row < rows ? cols - c : 0);
+        typename Mat<TC>::Frag f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = (TC)r.v[e];
+        *reinterpret_cast<typename Mat<TC>::Frag*>(tile + row * RS + c) = f;
+    }
+}
+
+__device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a constant
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
+// The running sums of a chunk's gates: lane l holds token l's (of 32: l & 31's).  Tokens past the end count as 0.
+template <int CH>
+__device__ __forceinline__ Sum2 chunk_sums(const DecayTok& g, int dt, int64_t at, int rows, int lane) {
+    const int t = lane & (CH - 1);
+    Sum2 s = split_gate(t < rows ? log2_gate(load_dt(g.p, dt, at + t * g.st)) : 0.f);
+    s.hi = row_inclusive_scan(s.hi);
+    s.lo = row_inclusive_scan(s.lo);
+    const float h0 = lane_value(s.hi, 15), l0 = lane_value(s.lo, 15);
+    const float h2 = lane_value(s.hi, 47), l2 = lane_value(s.lo, 47);
+    if (lane & 16) s.hi += lane & 32 ? h2 : h0, s.lo += lane & 32 ? l2 : l0;
+    if constexpr (CH == 64) {
+        const float h1 = lane_value(s.hi, 31), l1 = lane_value(s.lo, 31);
+        if (lane & 32) s.hi += h1, s.lo += l1;
+    }
+    return s;
+}
+
+// Work items of a walk: (segment, head, slice), slices fastest.
+struct DecayWhere {
+    SsmSeg seg;
+    int64_t w, last;  // the work item, that of the sequence's last segment
+    int h, slice;
+};
+__device__ __forceinline__ bool decay_where(const DecayParams& a, DecayWhere& x) {
+    int64_t b = blockIdx.x;
+    x.slice = (int)(b % a.slices);
+    b /= a.slices;
+    x.h = (int)(b % a.H);
+    x.w = b / a.H;
+    if (!ssm_segment(a, x.w, x.seg)) return false;
+    x.last = !a.cu ? x.w - x.seg.index + a.nseg - 1 : a.seg_off ? a.seg_off[x.seg.seq + 1] - 1 : x.w;
+    return true;
+}
+// The first element of a work item's tokens.
+__device__ __forceinline__ int64_t decay_base(const DecayParams& a, const DecayWhere& x, const DecayTok& t, int head) {
+    return (a.cu ? 0 : x.seg.seq * t.sb) + (x.seg.row0 + x.seg.t0) * t.st + head * t.sh;
+}
+
+// A wave's slice of a state lies in accumulators, NT tiles of 16 columns by DT of 16 rows: row tile_dim(t, 4 g + r) and
+// column 16 (w NT + c) + n of the slice.  f(value, its place in a matrix with this row stride, whether that is in
+// [Dk, Dv]).
+template <typename TC, int NT, int DT, typename F>
+__device__ __forceinline__ void each_state(f32x4 (&S)[NT][DT], int col0, int Dk, int Dv, int64_t row_stride, F f) {
+    const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const int dv = col0 + 16 * (w * NT + c) + n;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int dk = tile_dim<TC>(t, 4 * g + r);
+                float x = S[c][t][r];
+                f(x, dk * row_stride + dv, dk < Dk && dv < Dv);
+                S[c][t][r] = x;
+            }
+    }
+}
+// The same in the workspace, in the order of the lanes.
+template <int NT, int DT>
+__device__ __forceinline__ void put_state(const f32x4 (&S)[NT][DT], float* to) {
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(to + (c * DT + t) * 256) = S[c][t];
+}
+template <int NT, int DT>
+__device__ __forceinline__ void get_state(f32x4 (&S)[NT][DT], const float* from) {
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) S[c][t] = *reinterpret_cast<const f32x4*>(from + (c * DT + t) * 256);
 }
 
 }  // namespace triune

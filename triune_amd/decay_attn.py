@@ -108,19 +108,76 @@ def _no_tokens(q, H, Dv, s0):
     return s0.to(torch.float32).clone()
 
 
+def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0):
+    B, T, H, Dv = v.shape
+    Hk, Dk = q.shape[2:]
+    dev, f32 = q.device, torch.float32
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    do = torch.zeros(B, T, H, Dv, device=dev, dtype=q.dtype) if do is None else _rows(do.to(q.dtype))
+    dfin = None if dfin is None else dfin.to(f32).contiguous()
+    dq, dk = (torch.empty(B, T, Hk, Dk, device=dev, dtype=q.dtype) for _ in range(2))
+    dv = torch.empty(B, T, H, Dv, device=dev, dtype=q.dtype)
+    dg = torch.empty(g.shape, device=dev, dtype=g.dtype)
+    ds0 = torch.empty(B, H, Dk, Dv, device=dev, dtype=f32) if want_s0 else None
+    head = int(g.dim() == 1)
+    wsb = plan_on(q, "triune_hip_decay_attn_bwd_workspace_size", B, T, H, Hk, Dk, Dv, dtype_code(q), head, flags)
+    ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
+    st = strides(*(_head_strides(x) for x in (q, k, v)), _head_strides(g, 3), _head_strides(do))
+    call_on(q, "triune_hip_decay_attn_bwd", ptr(q), ptr(k), ptr(v), ptr(g), ptr(do), dtype_code(q), dtype_code(g), st, scale,
+            ptr(s0), ptr(dfin), ptr(dq), ptr(dk), ptr(dv), ptr(dg), head, ptr(ds0), B, T, H, Hk, Dk, Dv, flags, ptr(ws), wsb)
+    return dq, dk, dv, dg, ds0
+
+
+class _DecayAttn(torch.autograd.Function):
+    """decay_attn with gradients.  The backward forms the states of every 64th token again, so nothing is kept
+    but the inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, s0, scale):
+        s0f = None if s0 is None else s0.to(torch.float32).contiguous()
+        if q.shape[0] == 0 or q.shape[1] == 0:
+            o, fin = torch.empty(v.shape, device=v.device, dtype=v.dtype), _no_tokens(q, *v.shape[2:], s0f)
+        else:
+            o, fin = _attn(q, k, v, g, scale, s0f, None)
+        ctx.save_for_backward(q, k, v, g, s0)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, fin
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dfin):
+        q, k, v, g, s0 = ctx.saved_tensors
+        if do is None and dfin is None:
+            return (None,) * 6
+        want = s0 is not None and ctx.needs_input_grad[4]
+        if q.shape[0] == 0 or q.shape[1] == 0:  # no tokens: the final state is the initial state
+            zero = [torch.zeros_like(t) for t in (q, k, v, g)]
+            return (*zero, dfin.to(s0.dtype) if want and dfin is not None else None, None)
+        s0f = None if s0 is None else s0.to(torch.float32).contiguous()
+        dq, dk, dv, dg, ds0 = _attn_bwd(q, k, v, g, ctx.scale, s0f, do, dfin, want)
+        return dq, dk, dv, dg, ds0.to(s0.dtype) if want else None, None
+
+
 def decay_attn(q, k, v, g, initial_state=None, scale=1.0, out=None):
     """Decay attention over [B, T, heads, dim] prompts.
 
     q, k: [B, T, Hk, Dk]; v: [B, T, H, Dv]; g: [B, T, H] or [H]; initial_state: [B, H, Dk, Dv] or None (zeros); out:
     optional [B, T, H, Dv] buffer in q's dtype that overlaps no input, for calls without gradients.  Returns (o
-    [B, T, H, Dv] in q's dtype, final state float32 [B, H, Dk, Dv])."""
+    [B, T, H, Dv] in q's dtype, final state float32 [B, H, Dk, Dv]).
+
+    Differentiable in every tensor argument (once): the gradients come from triune_hip_decay_attn_bwd and do not depend
+    on timing."""
     if q.dim() != 4:
         raise ValueError("q must be [B, T, heads, dim]")
     H, Hk, Dk, Dv = _check(q, k, v, g)
     B, T = q.shape[:2]
-    s0 = _initial(initial_state, q, (B, H, Dk, Dv))
     if _needs_grad(q, k, v, g, initial_state):
-        raise ValueError("gradients are not available")
+        if out is not None:
+            raise ValueError("out is for calls without gradients")
+        _initial(initial_state, q, (B, H, Dk, Dv))
+        return _DecayAttn.apply(q, k, v, g, initial_state, float(scale))
+    s0 = _initial(initial_state, q, (B, H, Dk, Dv))
     if B == 0 or T == 0:  # nothing to read: the final state is the initial state
         return _out(out, v), _no_tokens(q, H, Dv, s0)
     return _attn(q, k, v, g, float(scale), s0, out)
