@@ -581,6 +581,34 @@ int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* 
                                       float* state_out, const int32_t* slots, int64_t n_state_rows, void* o, int64_t B,
                                       int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, void* stream);
 
+/* RMS norm of R rows of D elements (D <= 16384), with the residual sum in front of it:
+ *     h = r + scale x (rounded to r_dtype),   y = h rstd w,   rstd = 1 / sqrt(mean h^2 + eps)
+ * scale: s [D], or alpha where s is NULL.  r and h NULL: y is the norm of x.  x, y in io_dtype; r, h in r_dtype (io_dtype
+ * or fp32); w, s [D] (each may be NULL) in io_dtype or fp32.  Row i of x starts (i / G) strides[0] + (i % G) strides[1]
+ * elements in, of r likewise with strides[2..3]; y, h contiguous.  rstd: fp32 [R] for the backward, or NULL. */
+int triune_hip_rms_norm(const void* x, const void* r, const void* w, const void* s, int io_dtype, int r_dtype,
+                        int w_dtype, int s_dtype, const int64_t* strides, float alpha, float eps, void* y, void* h,
+                        float* rstd, int64_t R, int64_t G, int64_t D, void* stream);
+/* Its gradients.  h: what was normalised (x without a residual), in h_dtype; dy and dh (in h_dtype; NULL: none) those of y
+ * and h; x is read for ds only.  dx in io_dtype, dr in h_dtype, both contiguous; dw in w_dtype, ds in s_dtype (each NULL:
+ * not wanted; the workspace is used for dw and ds only).  strides[8] = h, dy, dh, x.  R > 0.  Sums are taken in a fixed
+ * order. */
+size_t triune_hip_rms_norm_bwd_workspace_size(int64_t R, int64_t D);
+int triune_hip_rms_norm_bwd(const void* h, const void* dy, const void* dh, const void* x, const void* w,
+                            const void* s, int io_dtype, int h_dtype, int w_dtype, int s_dtype, const int64_t* strides,
+                            float alpha, const float* rstd, void* dx, void* dr, void* dw, void* ds, int64_t R,
+                            int64_t G, int64_t D, void* workspace, size_t workspace_bytes, void* stream);
+/* y = x rstd(x) w silu(z), rows and types as above; strides[4] = x, z. */
+int triune_hip_gated_rms_norm(const void* x, const void* z, const void* w, int io_dtype, int w_dtype,
+                              const int64_t* strides, float eps, void* y, float* rstd, int64_t R, int64_t G, int64_t D,
+                              void* stream);
+/* Its gradients (dx, dz contiguous, dw in w_dtype, each NULL: not wanted); strides[6] = x, z, dy; the workspace is that of
+ * triune_hip_rms_norm_bwd. */
+int triune_hip_gated_rms_norm_bwd(const void* x, const void* z, const void* dy, const void* w, int io_dtype,
+                                  int w_dtype, const int64_t* strides, const float* rstd, void* dx, void* dz, void* dw,
+                                  int64_t R, int64_t G, int64_t D, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,7 +17,7 @@ from .fast_gla import (
 from .gla import gated_deltanet, gla
 from .gla_prep import (fused_qkv_g_prep_chunk_gla, fused_qkv_g_prep_inplace, fused_qkvg_decode_step,
                        fused_qkvg_decode_step_pool)
-from .norm import layer_norm
+from .norm import add_rms_norm, gated_rms_norm, layer_norm, rms_norm
 from .ssm import (
     short_conv,
     short_conv_decode_step,
@@ -30,6 +30,7 @@ from .ssm import (
 __all__ = [
     "FusedRecurrentScan",
     "TriuneHipError",
+    "add_rms_norm",
     "decay_attn",
     "decay_attn_decode_step",
     "decay_attn_varlen",
@@ -42,9 +43,11 @@ __all__ = [
     "fused_qkvg_decode_step",
     "fused_qkvg_decode_step_pool",
     "gated_deltanet",
+    "gated_rms_norm",
     "gla",
     "gla_decode_step",
     "layer_norm",
+    "rms_norm",
     "short_conv",
     "short_conv_decode_step",
     "short_conv_varlen",

@@ -208,6 +208,21 @@ def _bind(lib):
             [_vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp],
             _i,
         ),
+        "triune_hip_rms_norm": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64p, _f, _f, _vp, _vp, _vp, _i64, _i64, _i64, _vp],
+            _i,
+        ),
+        "triune_hip_rms_norm_bwd_workspace_size": ([_i64, _i64], _sz),
+        "triune_hip_rms_norm_bwd": (
+            [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i64p, _f, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
+             _vp],
+            _i,
+        ),
+        "triune_hip_gated_rms_norm": ([_vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _i64, _i64, _i64, _vp], _i),
+        "triune_hip_gated_rms_norm_bwd": (
+            [_vp, _vp, _vp, _vp, _i, _i, _i64p, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp],
+            _i,
+        ),
         "triune_hip_layer_norm": (
             [_vp, _i64, _vp, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _vp],
             _i,
@@ -283,6 +298,11 @@ EXPORTS = (
     "triune_hip_decay_attn_bwd_workspace_size",
     "triune_hip_decay_attn_bwd",
     "triune_hip_decay_attn_decode_step",
+    "triune_hip_rms_norm",
+    "triune_hip_rms_norm_bwd_workspace_size",
+    "triune_hip_rms_norm_bwd",
+    "triune_hip_gated_rms_norm",
+    "triune_hip_gated_rms_norm_bwd",
     "triune_hip_layer_norm",
     "triune_hip_layer_norm_bwd_workspace_size",
     "triune_hip_layer_norm_bwd",

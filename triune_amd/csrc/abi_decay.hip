@@ -2,6 +2,7 @@
 // include/triune_hip.h): argument checks, workspace layout and launches.
 #include "abi_common.h"
 #include "decay.h"
+#include "rms_norm.h"
 
 using namespace triune;
 
@@ -299,6 +300,103 @@ int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* 
     a.slots = slots, a.n_rows = n_state_rows, a.Bn = B;
     a.H = (int)H, a.per = (int)(H / Hk), a.Dk = (int)Dk, a.Dv = (int)Dv;
     return status(launch_decay_step(a, io_dtype, (hipStream_t)stream));
+}
+
+// ---- norms ---------------------------------------------------------------------------------------
+static int rms_check(std::initializer_list<const void*> io, const void* w, const void* s, int io_dtype, int w_dtype,
+                     int s_dtype, int64_t R, int64_t G, int64_t D) {
+    auto par_ok = [&](const void* p, int dt) { return !p || dt == io_dtype || dt == TRIUNE_DT_F32; };
+    if (!dtype_ok(io_dtype) || !par_ok(w, w_dtype) || !par_ok(s, s_dtype)) return TRIUNE_ERR_DTYPE;
+    if (R < 0 || R > kMaxGrid || G <= 0 || G > kMaxGrid || D <= 0 || D > NORM_MAX_D) return TRIUNE_ERR_SHAPE;
+    if (!all_aligned(io_dtype, io) || !aligned(w, w_dtype) || !aligned(s, s_dtype)) return TRIUNE_ERR_LAYOUT;
+    return TRIUNE_OK;
+}
+
+int triune_hip_rms_norm(const void* x, const void* r, const void* w, const void* s, int io_dtype, int r_dtype,
+                        int w_dtype, int s_dtype, const int64_t* strides, float alpha, float eps, void* y, void* h,
+                        float* rstd, int64_t R, int64_t G, int64_t D, void* stream) {
+    if (!x || !y || !strides || (r == nullptr) != (h == nullptr)) return TRIUNE_ERR_NULL;
+    if (const int e = rms_check({x, y}, w, s, io_dtype, w_dtype, s_dtype, R, G, D)) return e;
+    if (r && r_dtype != io_dtype && r_dtype != TRIUNE_DT_F32) return TRIUNE_ERR_DTYPE;
+    if ((r && !all_aligned(r_dtype, {r, h})) || !aligned(rstd, TRIUNE_DT_F32)) return TRIUNE_ERR_LAYOUT;
+    if (R == 0) return TRIUNE_OK;
+    RmsParams a{};
+    a.x = {x, strides[0], strides[1]};
+    a.r = {r, strides[2], strides[3]};
+    a.w = w, a.s = s, a.w_dt = w_dtype, a.s_dt = s_dtype, a.alpha = alpha, a.eps = eps;
+    a.y = y, a.h = h, a.rstd = rstd, a.R = R, a.G = (int)G, a.D = (int)D, a.cus = compute_units();
+    return status(launch_rms_norm(a, io_dtype, r && r_dtype != io_dtype, (hipStream_t)stream));
+}
+
+size_t triune_hip_rms_norm_bwd_workspace_size(int64_t R, int64_t D) {
+    if (R <= 0 || R > kMaxGrid || D <= 0 || D > NORM_MAX_D) return 0;
+    return align_up((size_t)rms_bwd_parts(R, (int)D, compute_units()) * 2 * D * 4);
+}
+
+static int rms_parts(RmsBwdParams& p, void* ws, size_t have) {
+    p.parts = rms_bwd_parts(p.f.R, p.f.D, p.f.cus);
+    if (!p.dw && !p.ds) return TRIUNE_OK;
+    p.part = (float*)ws;
+    return check_ws(ws, have, (size_t)p.parts * 2 * p.f.D * 4);
+}
+
+int triune_hip_rms_norm_bwd(const void* h, const void* dy, const void* dh, const void* x, const void* w,
+                            const void* s, int io_dtype, int h_dtype, int w_dtype, int s_dtype, const int64_t* strides,
+                            float alpha, const float* rstd, void* dx, void* dr, void* dw, void* ds, int64_t R,
+                            int64_t G, int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!h || !dy || !rstd || !strides || (ds && (!x || !s))) return TRIUNE_ERR_NULL;
+    if (const int e = rms_check({dy, x, dx}, w, s, io_dtype, w_dtype, s_dtype, R, G, D)) return e;
+    if (h_dtype != io_dtype && h_dtype != TRIUNE_DT_F32) return TRIUNE_ERR_DTYPE;
+    if (!all_aligned(h_dtype, {h, dh, dr}) || !aligned(rstd, TRIUNE_DT_F32) || !aligned(dw, w_dtype) ||
+        !aligned(ds, s_dtype))
+        return TRIUNE_ERR_LAYOUT;
+    if (R == 0) return TRIUNE_ERR_SHAPE;
+    RmsBwdParams p{};
+    RmsParams& a = p.f;
+    a.r = {h, strides[0], strides[1]};
+    p.dy = {dy, strides[2], strides[3]};
+    p.dh = {dh, strides[4], strides[5]};
+    a.x = {x, strides[6], strides[7]};
+    a.w = w, a.s = s, a.w_dt = w_dtype, a.s_dt = s_dtype, a.alpha = alpha, a.rstd = const_cast<float*>(rstd);
+    a.R = R, a.G = (int)G, a.D = (int)D, a.cus = compute_units();
+    p.dx = dx, p.dr = dr, p.dw = dw, p.ds = ds;
+    if (const int e = rms_parts(p, workspace, workspace_bytes)) return e;
+    return status(launch_rms_norm_bwd(p, io_dtype, h_dtype != io_dtype, (hipStream_t)stream));
+}
+
+int triune_hip_gated_rms_norm(const void* x, const void* z, const void* w, int io_dtype, int w_dtype,
+                              const int64_t* strides, float eps, void* y, float* rstd, int64_t R, int64_t G, int64_t D,
+                              void* stream) {
+    if (!x || !z || !y || !strides) return TRIUNE_ERR_NULL;
+    if (const int e = rms_check({x, z, y}, w, nullptr, io_dtype, w_dtype, 0, R, G, D)) return e;
+    if (!aligned(rstd, TRIUNE_DT_F32)) return TRIUNE_ERR_LAYOUT;
+    if (R == 0) return TRIUNE_OK;
+    RmsParams a{};
+    a.x = {x, strides[0], strides[1]};
+    a.z = {z, strides[2], strides[3]};
+    a.w = w, a.w_dt = w_dtype, a.eps = eps, a.y = y, a.rstd = rstd;
+    a.R = R, a.G = (int)G, a.D = (int)D, a.cus = compute_units();
+    return status(launch_gated_norm(a, io_dtype, (hipStream_t)stream));
+}
+
+int triune_hip_gated_rms_norm_bwd(const void* x, const void* z, const void* dy, const void* w, int io_dtype,
+                                  int w_dtype, const int64_t* strides, const float* rstd, void* dx, void* dz, void* dw,
+                                  int64_t R, int64_t G, int64_t D, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    if (!x || !z || !dy || !rstd || !strides) return TRIUNE_ERR_NULL;
+    if (const int e = rms_check({x, z, dy, dx, dz}, w, nullptr, io_dtype, w_dtype, 0, R, G, D)) return e;
+    if (!aligned(rstd, TRIUNE_DT_F32) || !aligned(dw, w_dtype)) return TRIUNE_ERR_LAYOUT;
+    if (R == 0) return TRIUNE_ERR_SHAPE;
+    RmsBwdParams p{};
+    RmsParams& a = p.f;
+    a.x = {x, strides[0], strides[1]};
+    a.z = {z, strides[2], strides[3]};
+    p.dy = {dy, strides[4], strides[5]};
+    a.w = w, a.w_dt = w_dtype, a.rstd = const_cast<float*>(rstd);
+    a.R = R, a.G = (int)G, a.D = (int)D, a.cus = compute_units();
+    p.dx = dx, p.dz = dz, p.dw = dw;
+    if (const int e = rms_parts(p, workspace, workspace_bytes)) return e;
+    return status(launch_gated_norm_bwd(p, io_dtype, (hipStream_t)stream));
 }
 
 }  // extern "C"
