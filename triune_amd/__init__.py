@@ -4,7 +4,7 @@ Host code in Python over a C-ABI library of hand-written HIP kernels (libtriune_
 include/triune_hip.h).  Operator surface mirrors triune.ops.gla / triune.kernels.fast_gla.
 """
 
-from .decay_attn import decay_attn, decay_attn_decode_step, decay_attn_varlen
+from .decay import decay_attn, decay_attn_decode_step, decay_attn_varlen
 from .fast_gla import (
     FusedRecurrentScan,
     TriuneHipError,

@@ -131,6 +131,14 @@ struct Par {
     __device__ __forceinline__ float at(int k, int t, int j) const { return v[k][j >> 2][t][j & 3]; }
 };
 
+// x, not to be merged into a mixed-precision product that rounds to fp16 by itself: whether the compiler does so depends on
+// the kernel, and the norm of a kept sum would differ from that of the same row read again.
+template <typename T>
+__device__ __forceinline__ float apart(float x) {
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
+    return x;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* row_ptr(const NormRows& a, int64_t r, int G) {
     if (G == 1) return (const T*)a.p + r * a.st0;

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void rms_norm_kernel(RmsParams 
             for (int j = 0; j < 8; ++j) {
                 h[k][j] = (float)nx[k].v[j];
                 if constexpr (RES) {
-                    kept[k].v[j] = (TH)__builtin_fmaf(s_s.at(k, t, j), h[k][j], (float)nr[k].v[j]);
+                    kept[k].v[j] = (TH)apart<TH>(__builtin_fmaf(s_s.at(k, t, j), h[k][j], (float)nr[k].v[j]));
                     h[k][j] = (float)kept[k].v[j];  // the norm is of the sum as it is kept
                 }
                 sq = __builtin_fmaf(h[k][j], h[k][j], sq);
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void rms_norm_kernel(RmsParams 
             if (left <= 0) continue;
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = h[k][j] * rstd * s_w.at(k, t, j);
+            for (int j = 0; j < 8; ++j) y[j] = apart<T>(h[k][j] * rstd * s_w.at(k, t, j));
             store_raw<8>((T*)a.y + r * a.D + c, left, y);
             if constexpr (RES) store_raw<8>((TH*)a.h + r * a.D + c, left, kept[k]);
         }
