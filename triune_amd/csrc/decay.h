@@ -37,6 +37,19 @@ struct DecayParams {
 int decay_slice(int Dv);
 int decay_padded_dk(int Dk);
 int64_t decay_state_values(int Dk, int Dv);
+// Whether the rows of these tensors are whole 16-byte units (for fp16, eight bytes), aligned, and 32 of them within the
+// offsets of a buffer resource.
+inline bool decay_full(int Dk, int Dv, int io_dt, std::initializer_list<DecayTok> ts) {
+    const int e = io_dt == DT_BF16 ? 8 : 4, size = io_dt == DT_F32 ? 4 : 2;
+    if (Dk % e || Dv % e) return false;
+    for (const DecayTok& t : ts) {
+        if (!t.p) continue;
+        if (reinterpret_cast<uintptr_t>(t.p) % (e * size) || (t.sb | t.st | t.sh) & (e - 1)) return false;
+        if (t.st < 0 || t.st >= (TILE_SKIP >> 8)) return false;  // 63 rows of 4 bytes and a row's width stay below it
+    }
+    return true;
+}
+
 // The walks that form states.  rev: gradients of states, from the end.
 struct DecayWalkParams {
     DecayParams f;            // rows in k, columns in v

@@ -16,20 +16,16 @@
 
 namespace triune {
 
-namespace {
-
 constexpr int C = DECAY_CHUNK;
 
-}  // namespace
-
 // Outputs, from the state in front of the segment.
-template <typename TIO, typename TC, int DK, int NW, int NT>
-__global__ __launch_bounds__(NW * 64) void decay_attn_kernel(DecayParams a) {
+template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(WIDTH), TJ = C / KS;  // TJ: K steps over the tokens
     constexpr int DT = DK / 16;
     using Frag = typename Mat<TC>::Frag;
-    __shared__ __attribute__((aligned(16))) TC s_q[C * RK], s_k[C * RK], s_v[C * RV];
+    __shared__ __attribute__((aligned(16))) TC s_qs[2][C * RK], s_ks[2][C * RK], s_vs[2][C * RV];
     __shared__ __attribute__((aligned(16))) float s_g[NW][2][C];
     DecayWhere x;
     if (!decay_where(a, x)) return;
@@ -52,15 +48,28 @@ __global__ __launch_bounds__(NW * 64) void decay_attn_kernel(DecayParams a) {
         get_state(S, a.ws_state + (from * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4);
     }
 
-    for (int t0 = 0; t0 < x.seg.len; t0 += C) {
+    // a chunk's tiles go from registers to one of two places, and the next one's loads are issued
+    Tile<TIO, TC, C, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
+    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
+    GateBits tg;
+    auto fetch = [&](int t0) {
         const int rows = min(C, x.seg.len - t0);
-        __syncthreads();
-        load_tile<TIO, TC, C, DK, NTH>(s_q, pq + t0 * a.q.st, a.q.st, rows, a.Dk);
-        load_tile<TIO, TC, C, DK, NTH>(s_k, pk + t0 * a.k.st, a.k.st, rows, a.Dk);
-        load_tile<TIO, TC, C, WIDTH, NTH>(s_v, pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
-        const Sum2 gs = chunk_sums<C>(a.g, a.g_dt, pg + t0 * a.g.st, rows, lane);
+        tq.fetch(pq + t0 * a.q.st, a.q.st, rows, a.Dk);
+        tk.fetch(pk + t0 * a.k.st, a.k.st, rows, a.Dk);
+        tv.fetch(pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
+        tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
+    };
+    if (x.seg.len) fetch(0);
+    for (int t0 = 0; t0 < x.seg.len; t0 += C) {
+        const int rows = min(C, x.seg.len - t0), place = t0 / C & 1;
+        TC *s_q = s_qs[place], *s_k = s_ks[place], *s_v = s_vs[place];
+        tq.put(s_q);
+        tk.put(s_k);
+        tv.put(s_v);
+        const Sum2 gs = running_sums<C>(tg.value(a.g_dt), rows, lane);
         if (lane < C) s_g[w][0][lane] = gs.hi, s_g[w][1][lane] = gs.lo;
-        __syncthreads();
+        if (t0 + C < x.seg.len) fetch(t0 + C);
+        lds_barrier();
         const Sum2 end{s_g[w][0][C - 1], s_g[w][1][C - 1]};
         Sum2 Gj[2][4];  // of tokens 16 J + 4 g + r
 #pragma unroll
@@ -180,13 +189,13 @@ __global__ __launch_bounds__(NW * 64) void decay_attn_kernel(DecayParams a) {
 // follows, in the workspace; or from the carried-in states the state in front of every `every` tokens, in `states`,
 // and the final one.  REV: the same from the end of the sequence (gradients of states, rows q and columns do):
 //     R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
-template <typename TIO, typename TC, int DK, int NW, int NT, bool REV>
-__global__ __launch_bounds__(NW * 64) void decay_walk_kernel(DecayWalkParams p) {
+template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV>
+__global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams p) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(WIDTH), TJ = C / KS, DT = DK / 16;
     using Frag = typename Mat<TC>::Frag;
-    __shared__ __attribute__((aligned(16))) TC s_k[C * RK], s_v[C * RV];
+    __shared__ __attribute__((aligned(16))) TC s_ks[2][C * RK], s_vs[2][C * RV];
     __shared__ __attribute__((aligned(16))) float s_g[NW][2][C];
     DecayWhere x;
     if (!decay_where(a, x)) return;
@@ -216,20 +225,31 @@ __global__ __launch_bounds__(NW * 64) void decay_walk_kernel(DecayWalkParams p) 
 
     Sum2 all{0.f, 0.f};
     const int chunks = (x.seg.len + C - 1) / C;
+    Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st, a.Dk);
+    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
+    GateBits tg;
+    auto fetch = [&](int i) {
+        const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
+        tk.fetch(pk + t0 * a.k.st, a.k.st, rows, a.Dk);
+        tv.fetch(pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
+        tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
+    };
+    if (chunks) fetch(0);
     for (int i = 0; i < chunks; ++i) {
         const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
+        TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
         const int64_t at = x.seg.t0 + t0;
         if (each && (REV ? (at + C) % p.every == 0 || at + rows == a.T : at % p.every == 0)) {
             const int64_t nc = (a.T + p.every - 1) / p.every, wide = (int64_t)WIDTH * a.slices;
             float* to = p.states + ((x.seg.seq * a.H + x.h) * nc + at / p.every) * values;
             each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
         }
-        __syncthreads();
-        load_tile<TIO, TC, C, DK, NTH>(s_k, pk + t0 * a.k.st, a.k.st, rows, a.Dk);
-        load_tile<TIO, TC, C, WIDTH, NTH>(s_v, pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
-        const Sum2 gs = chunk_sums<C>(a.g, a.g_dt, pg + t0 * a.g.st, rows, lane);
+        tk.put(s_k);
+        tv.put(s_v);
+        const Sum2 gs = running_sums<C>(tg.value(a.g_dt), rows, lane);
         if (lane < C) s_g[w][0][lane] = gs.hi, s_g[w][1][lane] = gs.lo;
-        __syncthreads();
+        if (i + 1 < chunks) fetch(i + 1);
+        lds_barrier();
         const Sum2 end{s_g[w][0][C - 1], s_g[w][1][C - 1]};
         const float keep = __builtin_amdgcn_exp2f(end.hi + end.lo);
         all.hi = fmaxf(all.hi + end.hi, -1024.f);
@@ -383,8 +403,16 @@ enum class Job { OUT, WALK, WALK_REV };
 template <typename TIO, typename TC, Job J, int DK, int NW, int NT>
 hipError_t run_one(const DecayWalkParams& p, hipStream_t s) {
     const dim3 grid((unsigned)(p.f.n_work * p.f.H * p.f.slices));
-    if constexpr (J == Job::OUT) decay_attn_kernel<TIO, TC, DK, NW, NT><<<grid, NW * 64, 0, s>>>(p.f);
-    else decay_walk_kernel<TIO, TC, DK, NW, NT, J == Job::WALK_REV><<<grid, NW * 64, 0, s>>>(p);
+    constexpr int dt = std::is_same<TIO, float>::value ? DT_F32 : std::is_same<TIO, __bf16>::value ? DT_BF16 : DT_F16;
+    const bool full = decay_full(p.f.Dk, p.f.Dv, dt, {J == Job::OUT ? p.f.q : DecayTok{}, p.f.k, p.f.v});
+    if constexpr (J == Job::OUT) {
+        if (full) decay_attn_kernel<TIO, TC, DK, NW, NT, true><<<grid, NW * 64, 0, s>>>(p.f);
+        else decay_attn_kernel<TIO, TC, DK, NW, NT, false><<<grid, NW * 64, 0, s>>>(p.f);
+    } else {
+        constexpr bool REV = J == Job::WALK_REV;
+        if (full) decay_walk_kernel<TIO, TC, DK, NW, NT, true, REV><<<grid, NW * 64, 0, s>>>(p);
+        else decay_walk_kernel<TIO, TC, DK, NW, NT, false, REV><<<grid, NW * 64, 0, s>>>(p);
+    }
     return hipGetLastError();
 }
 template <typename TIO, typename TC, Job J, int DK>

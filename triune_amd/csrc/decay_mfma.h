@@ -9,6 +9,8 @@
 
 #include "decay.h"
 
+#include <type_traits>
+
 namespace triune {
 
 template <typename TC>
@@ -134,11 +136,82 @@ __device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a con
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
+// The same through registers, so that a chunk's loads are in flight while the one before it is worked on.  FULL: whole
+// units of 16-byte aligned rows (decay_full), through a buffer resource that moves with the chunks, so that a load
+// takes no address arithmetic; what lies outside reads 0 by an offset past the resource's end.
+template <typename TIO, typename TC, int ROWS, int D, int NTH, bool FULL>
+struct Tile {
+    static constexpr int E = Mat<TC>::E, UNITS = D / E, N = ROWS * UNITS, PER = (N + NTH - 1) / NTH;
+    Raw<TIO, E> x[PER];
+    int off[PER];  // bytes from the chunk's first row
+    __device__ __forceinline__ static int row_of(int i) { return (threadIdx.x + i * NTH) / UNITS; }
+    __device__ __forceinline__ static int col_of(int i) { return (threadIdx.x + i * NTH) % UNITS * E; }
+    __device__ __forceinline__ Tile(int64_t st, int cols) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)(row_of(i) * st + col_of(i)) * (int)sizeof(TIO) : TILE_SKIP;
+    }
+    __device__ __forceinline__ void fetch(const TIO* p, int64_t st, int rows, int cols) {
+        if constexpr (FULL) {
+            const __amdgpu_buffer_rsrc_t r =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<TIO*>(p), (short)0, TILE_SKIP, 0x00020000);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int o = rows == ROWS || row_of(i) < rows ? off[i] : TILE_SKIP;
+                x[i] = __builtin_bit_cast(Raw<TIO, E>, tile_load<TIO, E>(r, o));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const bool in = row_of(i) < rows && col_of(i) < cols;
+                x[i] = load_raw<E>(p + (in ? row_of(i) * st + col_of(i) : 0), in ? cols - col_of(i) : 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(TC* tile) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (N % NTH && row_of(i) >= ROWS) continue;
+            TC* to = tile + row_of(i) * tile_stride<TC>(D) + col_of(i);
+            if constexpr (std::is_same<TIO, TC>::value) {
+                *reinterpret_cast<typename Mat<TC>::Frag*>(to) = __builtin_bit_cast(typename Mat<TC>::Frag, x[i]);
+            } else {
+                typename Mat<TC>::Frag f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] = (TC)x[i].v[e];
+                *reinterpret_cast<typename Mat<TC>::Frag*>(to) = f;
+            }
+        }
+    }
+};
+
+// Orders LDS accesses around a barrier and leaves loads from memory in flight, which __syncthreads would wait for.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// A gate's bits; what the other of two loads reads is not used.  Both are issued, since a load behind a condition would
+// be waited for there.
+static __device__ const uint32_t kNoGate[1] = {0};
+struct GateBits {
+    uint32_t wide;
+    uint16_t half;
+    __device__ __forceinline__ void fetch(const DecayTok& g, int dt, int64_t at) {
+        const bool f32 = dt == DT_F32;
+        wide = *(f32 ? (const uint32_t*)g.p + at : kNoGate);
+        half = *(f32 ? (const uint16_t*)kNoGate : (const uint16_t*)g.p + at);
+    }
+    __device__ __forceinline__ float value(int dt) const {
+        return dt == DT_F32    ? __uint_as_float(wide)
+               : dt == DT_BF16 ? __uint_as_float((uint32_t)half << 16)
+                               : (float)__builtin_bit_cast(_Float16, half);
+    }
+};
+
 // The running sums of a chunk's gates: lane l holds token l's (of 32: l & 31's).  Tokens past the end count as 0.
 template <int CH>
-__device__ __forceinline__ Sum2 chunk_sums(const DecayTok& g, int dt, int64_t at, int rows, int lane) {
-    const int t = lane & (CH - 1);
-    Sum2 s = split_gate(t < rows ? log2_gate(load_dt(g.p, dt, at + t * g.st)) : 0.f);
+__device__ __forceinline__ Sum2 running_sums(float gate, int rows, int lane) {
+    Sum2 s = split_gate((lane & (CH - 1)) < rows ? log2_gate(gate) : 0.f);
     s.hi = row_inclusive_scan(s.hi);
     s.lo = row_inclusive_scan(s.lo);
     const float h0 = lane_value(s.hi, 15), l0 = lane_value(s.lo, 15);
@@ -149,6 +222,12 @@ __device__ __forceinline__ Sum2 chunk_sums(const DecayTok& g, int dt, int64_t at
         if (lane & 32) s.hi += h1, s.lo += l1;
     }
     return s;
+}
+
+template <int CH>
+__device__ __forceinline__ Sum2 chunk_sums(const DecayTok& g, int dt, int64_t at, int rows, int lane) {
+    const int t = lane & (CH - 1);
+    return running_sums<CH>(t < rows ? load_dt(g.p, dt, at + t * g.st) : 0.f, rows, lane);
 }
 
 // Work items of a walk: (segment, head, slice), slices fastest.
