@@ -26,7 +26,7 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
     constexpr int DT = DK / 16;
     using Frag = typename Mat<TC>::Frag;
     __shared__ __attribute__((aligned(16))) TC s_qs[2][C * RK], s_ks[2][C * RK], s_vs[2][C * RV];
-    __shared__ __attribute__((aligned(16))) float s_g[NW][2][C];
+    __shared__ __attribute__((aligned(16))) ChunkGates s_gs[2];
     DecayWhere x;
     if (!decay_where(a, x)) return;
     const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15;
@@ -66,19 +66,10 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
         tq.put(s_q);
         tk.put(s_k);
         tv.put(s_v);
-        const Sum2 gs = running_sums<C>(tg.value(a.g_dt), rows, lane);
-        if (lane < C) s_g[w][0][lane] = gs.hi, s_g[w][1][lane] = gs.lo;
+        ChunkGates& s_g = s_gs[place];
+        if (w == 0) s_g.put(tg.value(a.g_dt), rows, lane);
         if (t0 + C < x.seg.len) fetch(t0 + C);
         lds_barrier();
-        const Sum2 end{s_g[w][0][C - 1], s_g[w][1][C - 1]};
-        Sum2 Gj[2][4];  // of tokens 16 J + 4 g + r
-#pragma unroll
-        for (int J = 0; J < 2; ++J) {
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(&s_g[w][0][16 * J + 4 * g]);
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(&s_g[w][1][16 * J + 4 * g]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) Gj[J][r] = {hi[r], lo[r]};
-        }
         Frag vf[NT][TJ];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
@@ -120,17 +111,22 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
         }
 #pragma unroll
         for (int I = 0; I < 2; ++I) {
-            const Sum2 Gi{s_g[w][0][16 * I + n], s_g[w][1][16 * I + n]};
-            const float from = __builtin_amdgcn_exp2f(Gi.hi + Gi.lo);
+            const float from = s_g.from[16 * I + n];
 #pragma unroll
             for (int c = 0; c < NT; ++c)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) O[c][I][r] *= from;
+            if (I == 1) {
+                const f32x4 written = four(&s_g.half[4 * g]);
+                const float read = s_g.half[16 + n];
 #pragma unroll
-            for (int J = 0; J <= I; ++J)
+                for (int r = 0; r < 4; ++r) P[1][0][r] *= written[r] * read;
+            }
+            const Sum2 Gi{s_g.hi[16 * I + n], s_g.lo[16 * I + n]};
+            const f32x4 hi = four(&s_g.hi[16 * I + 4 * g]), lo = four(&s_g.lo[16 * I + 4 * g]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    P[I][J][r] = J < I || 4 * g + r <= n ? P[I][J][r] * decay_between(Gi, Gj[J][r]) : 0.f;
+            for (int r = 0; r < 4; ++r)
+                P[I][I][r] = 4 * g + r <= n ? P[I][I][r] * decay_between(Gi, Sum2{hi[r], lo[r]}) : 0.f;
 #pragma unroll
             for (int j = 0; j < (TJ == 1 ? 1 : I + 1); ++j) {
                 float pt[E];
@@ -147,21 +143,18 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
                     float o[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[r] = a.scale * O[c][I][r];
-                    store_raw<4>(po + (int64_t)(t0 + t) * a.o.st + dv, a.Dv - col0 - dv, o);
+                    if (!FULL || dv < a.Dv - col0)
+                        store_raw<4>(po + (int64_t)(t0 + t) * a.o.st + dv, FULL ? 4 : a.Dv - col0 - dv, o);
                 }
             }
         }
         // the state: rows of k by weighted rows of v
-        const float keep = __builtin_amdgcn_exp2f(end.hi + end.lo);
+        const float keep = s_g.from[C - 1];
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
             for (int t = 0; t < DT; ++t) S[c][t] *= keep;
-        float wj[2][4];
-#pragma unroll
-        for (int J = 0; J < 2; ++J)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) wj[J][r] = decay_between(end, Gj[J][r]);
+        const f32x4 wj[2] = {four(&s_g.to[4 * g]), four(&s_g.to[16 + 4 * g])};
 #pragma unroll
         for (int j = 0; j < TJ; ++j) {
             Frag kf[DT];
@@ -183,160 +176,6 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
     each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
         if (in) a.fin[soff + off] = v;
     });
-}
-
-// States alone, from rows (k of a.k) by columns (v): the segments' own end states (states null) of those that another one
-// follows, in the workspace; or from the carried-in states the state in front of every `every` tokens, in `states`,
-// and the final one.  REV: the same from the end of the sequence (gradients of states, rows q and columns do):
-//     R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
-template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV>
-__global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams p) {
-    const DecayParams& a = p.f;
-    constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
-    constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(WIDTH), TJ = C / KS, DT = DK / 16;
-    using Frag = typename Mat<TC>::Frag;
-    __shared__ __attribute__((aligned(16))) TC s_ks[2][C * RK], s_vs[2][C * RV];
-    __shared__ __attribute__((aligned(16))) float s_g[NW][2][C];
-    DecayWhere x;
-    if (!decay_where(a, x)) return;
-    const bool each = p.states, begins = REV ? x.seg.last : x.seg.index == 0, ends = REV ? x.seg.index == 0 : x.seg.last;
-    if (!each && ends) return;
-    const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15, col0 = x.slice * WIDTH;
-    const TIO* pk = (const TIO*)a.k.p + decay_base(a, x, a.k, x.h / a.per);
-    const TIO* pv = (const TIO*)a.v.p + decay_base(a, x, a.v, x.h) + col0;
-    const int64_t pg = decay_base(a, x, a.g, x.h);
-    const int64_t srow = ssm_row(a.slots, a.n_slots, x.seg.seq), soff = (srow * a.H + x.h) * a.Dk * a.Dv;
-    const int64_t values = (int64_t)DK * WIDTH * a.slices, in_ws = ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
-    auto ws = [&](int64_t item) { return a.ws_state + (item * a.H + x.h) * values + in_ws; };
-
-    f32x4 S[NT][DT];
-    if (begins) {
-        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
-            v = in && a.s0 && srow >= 0 ? a.s0[soff + off] : 0.f;
-        });
-        // The last segment of a cut sequence has no use for its place in the workspace: it takes the initial state,
-        // since s0 may be the pool that the last segment's outputs leave their state in while the first one starts.
-        if (!REV && !each) put_state(S, ws(x.last));
-    } else if (each) {
-        get_state(S, ws(REV ? x.w + 1 : x.w - 1));
-    } else {
-        each_state<TC>(S, 0, 0, 0, 0, [](float& v, int64_t, bool) { v = 0.f; });
-    }
-
-    Sum2 all{0.f, 0.f};
-    const int chunks = (x.seg.len + C - 1) / C;
-    Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st, a.Dk);
-    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
-    GateBits tg;
-    auto fetch = [&](int i) {
-        const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
-        tk.fetch(pk + t0 * a.k.st, a.k.st, rows, a.Dk);
-        tv.fetch(pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
-        tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
-    };
-    if (chunks) fetch(0);
-    for (int i = 0; i < chunks; ++i) {
-        const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
-        TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
-        const int64_t at = x.seg.t0 + t0;
-        if (each && (REV ? (at + C) % p.every == 0 || at + rows == a.T : at % p.every == 0)) {
-            const int64_t nc = (a.T + p.every - 1) / p.every, wide = (int64_t)WIDTH * a.slices;
-            float* to = p.states + ((x.seg.seq * a.H + x.h) * nc + at / p.every) * values;
-            each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
-        }
-        tk.put(s_k);
-        tv.put(s_v);
-        const Sum2 gs = running_sums<C>(tg.value(a.g_dt), rows, lane);
-        if (lane < C) s_g[w][0][lane] = gs.hi, s_g[w][1][lane] = gs.lo;
-        if (i + 1 < chunks) fetch(i + 1);
-        lds_barrier();
-        const Sum2 end{s_g[w][0][C - 1], s_g[w][1][C - 1]};
-        const float keep = __builtin_amdgcn_exp2f(end.hi + end.lo);
-        all.hi = fmaxf(all.hi + end.hi, -1024.f);
-        all.lo += end.lo;
-        float wj[2][4];
-#pragma unroll
-        for (int J = 0; J < 2; ++J)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const Sum2 Gj{s_g[w][0][16 * J + 4 * g + r], s_g[w][1][16 * J + 4 * g + r]};
-                wj[J][r] = REV ? a.scale * __builtin_amdgcn_exp2f(Gj.hi + Gj.lo) : decay_between(end, Gj);
-            }
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int t = 0; t < DT; ++t) S[c][t] *= keep;
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) {
-            Frag kf[DT];
-#pragma unroll
-            for (int t = 0; t < DT; ++t) kf[t] = col_frag<TC, true>(s_k, RK, t, j, g, n);
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                const Frag vf = col_frag<TC, false>(s_v, RV, w * NT + c, j, g, n);
-                float v[E];
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = (float)vf[e] * wj[TJ == 1 ? e >> 2 : j][e & 3];
-                const auto vp = parts<TC, 3>(v);
-#pragma unroll
-                for (int t = 0; t < DT; ++t) S[c][t] = mma<TC>(kf[t], vp, S[c][t]);
-            }
-        }
-    }
-
-    if (each) {
-        if (!ends || !a.fin || srow < 0) return;
-        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
-            if (in) a.fin[soff + off] = v;
-        });
-    } else {
-        put_state(S, ws(x.w));
-        if (x.slice == 0 && threadIdx.x == 0) {
-            float* sum = a.ws_sum + (x.w * a.H + x.h) * 2;
-            sum[0] = all.hi, sum[1] = all.lo;
-        }
-    }
-}
-
-// Joins the segments' end states in order: S_p = 2^{sum_p} S_{p-1} + own_p, in place, for the segments that another
-// one follows (rev: from the last one to the second).  A thread per value of a (sequence, head).
-__global__ __launch_bounds__(256) void decay_carry_kernel(DecayParams a, int64_t values, bool rev) {
-    const int64_t blocks = (values + 255) / 256;
-    const int64_t sh = blockIdx.x / blocks, i = (blockIdx.x % blocks) * 256 + threadIdx.x;
-    const int64_t seq = sh / a.H, h = sh % a.H;
-    if (i >= values) return;
-    int64_t first, n;
-    if (a.cu) {
-        first = a.seg_off[seq];
-        n = a.seg_off[seq + 1] - first;
-    } else {
-        first = seq * a.nseg;
-        n = a.nseg;
-    }
-    if (n < 3) return;  // one state to carry: the first segment's own
-    const int64_t step = rev ? -a.H * values : a.H * values, step_sum = rev ? -2 * a.H : 2 * a.H;
-    if (rev) first += n - 1;
-    float* p = a.ws_state + (first * a.H + h) * values + i;
-    const float* sum = a.ws_sum + (first * a.H + h) * 2;
-    float s = p[0];
-    constexpr int AHEAD = 8;
-    for (int64_t k0 = 1; k0 < n - 1; k0 += AHEAD) {
-        float x[AHEAD], d[AHEAD];
-        const int m = (int)min((int64_t)AHEAD, n - 1 - k0);
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (k < m) {
-                x[k] = p[(k0 + k) * step];
-                const float* e = sum + (k0 + k) * step_sum;
-                d[k] = __builtin_amdgcn_exp2f(e[0] + e[1]);
-            }
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (k < m) {
-                s = __builtin_fmaf(d[k], s, x[k]);
-                p[(k0 + k) * step] = s;
-            }
-    }
 }
 
 // One token for every row: a block takes a (row, head), a thread V columns of every RG-th state row.
@@ -398,45 +237,13 @@ int64_t decay_state_values(int Dk, int Dv) {
 
 namespace {
 
-enum class Job { OUT, WALK, WALK_REV };
-
-template <typename TIO, typename TC, Job J, int DK, int NW, int NT>
-hipError_t run_one(const DecayWalkParams& p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.f.n_work * p.f.H * p.f.slices));
-    constexpr int dt = std::is_same<TIO, float>::value ? DT_F32 : std::is_same<TIO, __bf16>::value ? DT_BF16 : DT_F16;
-    const bool full = decay_full(p.f.Dk, p.f.Dv, dt, {J == Job::OUT ? p.f.q : DecayTok{}, p.f.k, p.f.v});
-    if constexpr (J == Job::OUT) {
-        if (full) decay_attn_kernel<TIO, TC, DK, NW, NT, true><<<grid, NW * 64, 0, s>>>(p.f);
-        else decay_attn_kernel<TIO, TC, DK, NW, NT, false><<<grid, NW * 64, 0, s>>>(p.f);
-    } else {
-        constexpr bool REV = J == Job::WALK_REV;
-        if (full) decay_walk_kernel<TIO, TC, DK, NW, NT, true, REV><<<grid, NW * 64, 0, s>>>(p);
-        else decay_walk_kernel<TIO, TC, DK, NW, NT, false, REV><<<grid, NW * 64, 0, s>>>(p);
+template <typename TIO, typename TC>
+struct Attn {
+    template <int DK, int NW, int NT, bool FULL>
+    static void run(const DecayParams& a, dim3 grid, hipStream_t s) {
+        decay_attn_kernel<TIO, TC, DK, NW, NT, FULL><<<grid, NW * 64, 0, s>>>(a);
     }
-    return hipGetLastError();
-}
-template <typename TIO, typename TC, Job J, int DK>
-hipError_t run_width(const DecayWalkParams& p, hipStream_t s) {
-    switch (decay_slice(p.f.Dv)) {
-        case 32: return run_one<TIO, TC, J, DK, 2, 1>(p, s);
-        case 64: return run_one<TIO, TC, J, DK, 4, 1>(p, s);
-        default: return run_one<TIO, TC, J, DK, 4, 2>(p, s);
-    }
-}
-template <typename TIO, typename TC, Job J>
-hipError_t run_dk(const DecayWalkParams& p, hipStream_t s) {
-    switch (decay_padded_dk(p.f.Dk)) {
-        case 32: return run_width<TIO, TC, J, 32>(p, s);
-        case 64: return run_width<TIO, TC, J, 64>(p, s);
-        default: return run_width<TIO, TC, J, 128>(p, s);
-    }
-}
-template <Job J>
-hipError_t run(const DecayWalkParams& p, int dt, hipStream_t s) {
-    if (dt == DT_F32) return run_dk<float, float, J>(p, s);
-    if (dt == DT_BF16) return run_dk<__bf16, __bf16, J>(p, s);
-    return run_dk<_Float16, float, J>(p, s);
-}
+};
 
 template <typename TIO>
 hipError_t run_step(const DecayStepParams& a, hipStream_t s) {
@@ -450,16 +257,9 @@ hipError_t run_step(const DecayStepParams& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_decay_walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
-    return rev ? run<Job::WALK_REV>(p, io_dt, s) : run<Job::WALK>(p, io_dt, s);
-}
 hipError_t launch_decay_attn(const DecayParams& a, int io_dt, hipStream_t s) {
-    return run<Job::OUT>(DecayWalkParams{a, nullptr, 0}, io_dt, s);
-}
-hipError_t launch_decay_carry(const DecayParams& a, bool rev, hipStream_t s) {
-    const int64_t values = decay_state_values(a.Dk, a.Dv);
-    decay_carry_kernel<<<dim3((unsigned)(a.n_seqs * a.H * ((values + 255) / 256))), 256, 0, s>>>(a, values, rev);
-    return hipGetLastError();
+    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.q, a.k, a.v});
+    return decay_by_type<Attn>(a, a, io_dt, full, s);
 }
 hipError_t launch_decay_step(const DecayStepParams& a, int io_dt, hipStream_t s) {
     if (io_dt == DT_F32) return run_step<float>(a, s);

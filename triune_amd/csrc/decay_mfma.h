@@ -224,6 +224,23 @@ __device__ __forceinline__ Sum2 running_sums(float gate, int rows, int lane) {
     return s;
 }
 
+// What a chunk of 32 tokens takes of its gates, formed once for all waves: the sums G (hi, lo), 2^G, 2^{G_end - G}, and for
+// the scores of the second 16 tokens with the first 16 the factors 2^{G - G_15} (read) and 2^{G_15 - G} (written).
+struct ChunkGates {
+    float hi[32], lo[32], from[32], to[32], half[32];
+    __device__ __forceinline__ void put(float gate, int rows, int lane) {
+        const Sum2 s = running_sums<32>(gate, rows, lane);
+        const Sum2 end{lane_value(s.hi, 31), lane_value(s.lo, 31)}, mid{lane_value(s.hi, 15), lane_value(s.lo, 15)};
+        if (lane >= 32) return;
+        hi[lane] = s.hi;
+        lo[lane] = s.lo;
+        from[lane] = __builtin_amdgcn_exp2f(s.hi + s.lo);
+        to[lane] = decay_between(end, s);
+        half[lane] = lane < 16 ? decay_between(mid, s) : decay_between(s, mid);
+    }
+};
+__device__ __forceinline__ f32x4 four(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
+
 template <int CH>
 __device__ __forceinline__ Sum2 chunk_sums(const DecayTok& g, int dt, int64_t at, int rows, int lane) {
     const int t = lane & (CH - 1);
@@ -237,13 +254,20 @@ struct DecayWhere {
     int h, slice;
 };
 __device__ __forceinline__ bool decay_where(const DecayParams& a, DecayWhere& x) {
-    int64_t b = blockIdx.x;
-    x.slice = (int)(b % a.slices);
-    b /= a.slices;
-    x.h = (int)(b % a.H);
-    x.w = b / a.H;
-    if (!ssm_segment(a, x.w, x.seg)) return false;
-    x.last = !a.cu ? x.w - x.seg.index + a.nseg - 1 : a.seg_off ? a.seg_off[x.seg.seq + 1] - 1 : x.w;
+    uint32_t b = blockIdx.x;
+    x.slice = (int)(b % (uint32_t)a.slices);
+    b /= (uint32_t)a.slices;
+    x.h = (int)(b % (uint32_t)a.H);
+    x.w = b / (uint32_t)a.H;
+    if (a.cu) {
+        if (!ssm_segment(a, x.w, x.seg)) return false;
+        x.last = a.seg_off ? a.seg_off[x.seg.seq + 1] - 1 : x.w;
+        return true;
+    }
+    const uint32_t seq = (uint32_t)x.w / (uint32_t)a.nseg, p = (uint32_t)x.w - seq * (uint32_t)a.nseg;
+    const int64_t t0 = (int64_t)p * a.seg;
+    x.seg = SsmSeg{seq, 0, t0, (int)min((int64_t)a.seg, a.T - t0), (int)p, p == (uint32_t)a.nseg - 1};
+    x.last = x.w - p + a.nseg - 1;
     return true;
 }
 // The first element of a work item's tokens.
@@ -285,6 +309,36 @@ __device__ __forceinline__ void get_state(f32x4 (&S)[NT][DT], const float* from)
     for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int t = 0; t < DT; ++t) S[c][t] = *reinterpret_cast<const f32x4*>(from + (c * DT + t) * 256);
+}
+
+// F<TIO, TC>::run<DK, NW, NT, FULL>(p, grid, stream) for the types and sizes of a: NW waves that own NT tiles of 16 columns
+// each, a workgroup for each (segment, head, slice).
+template <template <typename, typename> class F, typename TIO, typename TC, int DK, bool FULL, typename P>
+void decay_by_width(const P& p, const DecayParams& a, dim3 grid, hipStream_t s) {
+    switch (decay_slice(a.Dv)) {
+        case 32: return F<TIO, TC>::template run<DK, 2, 1, FULL>(p, grid, s);
+        case 64: return F<TIO, TC>::template run<DK, 4, 1, FULL>(p, grid, s);
+        default: return F<TIO, TC>::template run<DK, 4, 2, FULL>(p, grid, s);
+    }
+}
+template <template <typename, typename> class F, typename TIO, typename TC, bool FULL, typename P>
+void decay_by_dk(const P& p, const DecayParams& a, dim3 grid, hipStream_t s) {
+    switch (decay_padded_dk(a.Dk)) {
+        case 32: return decay_by_width<F, TIO, TC, 32, FULL>(p, a, grid, s);
+        case 64: return decay_by_width<F, TIO, TC, 64, FULL>(p, a, grid, s);
+        default: return decay_by_width<F, TIO, TC, 128, FULL>(p, a, grid, s);
+    }
+}
+template <template <typename, typename> class F, typename P>
+hipError_t decay_by_type(const P& p, const DecayParams& a, int dt, bool full, hipStream_t s) {
+    const dim3 grid((unsigned)(a.n_work * a.H * a.slices));
+    if (dt == DT_F32)
+        full ? decay_by_dk<F, float, float, true>(p, a, grid, s) : decay_by_dk<F, float, float, false>(p, a, grid, s);
+    else if (dt == DT_BF16)
+        full ? decay_by_dk<F, __bf16, __bf16, true>(p, a, grid, s) : decay_by_dk<F, __bf16, __bf16, false>(p, a, grid, s);
+    else
+        full ? decay_by_dk<F, _Float16, float, true>(p, a, grid, s) : decay_by_dk<F, _Float16, float, false>(p, a, grid, s);
+    return hipGetLastError();
 }
 
 }  // namespace triune
