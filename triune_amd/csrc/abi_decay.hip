@@ -72,7 +72,7 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
 struct GradPlan {
     DecayPlan p;
     int64_t chunk, nc;
-    size_t off_S, off_R, off_q, off_k, off_g, total;
+    size_t off_S, off_R, off_own, off_sum, off_seg, off_q, off_k, off_g, total;
 };
 
 GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int io_dtype, int g_head,
@@ -81,20 +81,19 @@ GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int6
     r.chunk = decay_grad_chunk(io_dtype == TRIUNE_DT_BF16);
     r.nc = (T + r.chunk - 1) / r.chunk;
     r.p = plan_dense(B, T, H, Dk, Dv, flags);
-    if (r.p.nseg > 1) {
-        r.p.seg = round_up(r.p.seg, r.chunk);
-        r.p.nseg = (T + r.p.seg - 1) / r.p.seg;
-        r.p.n_work = B * r.p.nseg;
-        plan_bytes(r.p, H, Dk, Dv, 0);
-    }
-    const size_t states = align_up((size_t)(B * H * r.nc) * decay_state_values((int)Dk, (int)Dv) * 4);
+    r.p.seg = round_up(r.p.seg, r.chunk);
+    r.p.nseg = (T + r.p.seg - 1) / r.p.seg;
+    r.p.n_work = B * r.p.nseg;
+    const size_t state = (size_t)decay_state_values((int)Dk, (int)Dv) * 4, heads = (size_t)(B * H);
     const size_t shared = H > Hk ? align_up((size_t)(B * T * H) * Dk * 4) : 0;
-    r.off_S = r.p.total;
-    r.off_R = r.off_S + states;
-    r.off_q = r.off_R + states;
+    r.off_R = r.off_S + align_up(heads * r.nc * state);
+    r.off_own = r.off_R + align_up(heads * r.nc * state);
+    r.off_sum = r.off_own + align_up(heads * state);
+    r.off_seg = r.off_sum + align_up(heads * r.nc * 16);
+    r.off_q = r.off_seg + align_up(heads * r.p.nseg * 8);
     r.off_k = r.off_q + shared;
     r.off_g = r.off_k + shared;
-    r.total = r.off_g + (g_head ? align_up((size_t)(B * r.nc * H) * 4) : 0);
+    r.total = r.off_g + (g_head ? align_up(heads * r.nc * 4) : 0);
     return r;
 }
 
@@ -105,7 +104,7 @@ bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t
 }
 
 bool grad_grids_ok(const GradPlan& r, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv) {
-    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 512) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
+    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 256) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
 }
 
 void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -128,8 +127,7 @@ void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk,
 
 int run_attn(const DecayParams& a, int nseg, int io_dtype, hipStream_t s) {
     if (nseg > 1) {
-        if (const int e = status(launch_decay_walk(DecayWalkParams{a, nullptr, 0}, false, io_dtype, s))) return e;
-        if (const int e = status(launch_decay_carry(a, false, s))) return e;
+        if (const int e = status(launch_decay_ends(a, io_dtype, s))) return e;
     }
     return status(launch_decay_attn(a, io_dtype, s));
 }
@@ -262,17 +260,17 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
     p.dq = dq, p.dk = dk, p.dv = dv, p.dg = dg;
     if (H > Hk) p.part_q = (float*)(ws + r.off_q), p.part_k = (float*)(ws + r.off_k);
     if (g_head) p.part_g = (float*)(ws + r.off_g);
+    p.sum_S = (float*)(ws + r.off_sum), p.sum_R = p.sum_S + 2 * B * H * r.nc, p.per = r.p.seg / r.chunk;
+    p.wide = a.slices * decay_slice((int)Dv);
+    // the segments' sums are formed by each walk
+    a.ws_sum = (float*)(ws + r.off_seg);
     for (const bool rev : {false, true}) {
-        DecayWalkParams x{a, nullptr, (int)r.chunk};
+        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), (float*)(rev ? p.sum_R : p.sum_S), (float*)(ws + r.off_own),
+                          (int)r.chunk};
         x.f.s0 = rev ? ds_final : s0;
         x.f.fin = rev ? ds0 : nullptr;
         if (rev) x.f.k = a.q, x.f.v = a.o;
-        if (r.p.nseg > 1) {
-            if (const int e = status(launch_decay_walk(x, rev, io_dtype, s))) return e;
-            if (const int e = status(launch_decay_carry(x.f, rev, s))) return e;
-        }
-        x.states = const_cast<float*>(rev ? p.R : p.S);
-        if (const int e = status(launch_decay_walk(x, rev, io_dtype, s))) return e;
+        if (const int e = status(launch_decay_states(x, rev, io_dtype, s))) return e;
     }
     return status(launch_decay_grad(p, io_dtype, s));
 }

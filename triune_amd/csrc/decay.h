@@ -50,14 +50,26 @@ inline bool decay_full(int Dk, int Dv, int io_dt, std::initializer_list<DecayTok
     return true;
 }
 
-// The walks that form states.  rev: gradients of states, from the end.
+// Segments' end states and what the join makes of them, in the workspace.
+hipError_t launch_decay_ends(const DecayParams& a, int io_dt, hipStream_t s);
+
+// The states in front of every chunk; rev: the gradients of those behind them.
 struct DecayWalkParams {
     DecayParams f;            // rows in k, columns in v
-    float* states;            // [n_seqs, H, ceil(T / every), values] or null: the segments' end states instead
-    int every;                // of 32 tokens' multiples; segments are multiples of it
+    float* states;            // [n_seqs, H, nc, values], nc = ceil(T / every)
+    float* sums;              // [n_seqs, H, nc, 2]: log2 decay from the segment's first place
+    float* own;               // [n_seqs, H, values]: f.fin of the walk's last segment, before the join
+    int every;                // a multiple of 32 tokens; segments are multiples of it
 };
-hipError_t launch_decay_walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
-hipError_t launch_decay_carry(const DecayParams& a, bool rev, hipStream_t s);
+struct DecayCarryParams {
+    DecayParams f;
+    float *states, *own;      // as above, or null: the end states in f.ws_state
+    int every;
+    int64_t nc, values;
+    int dk;                   // rows of a state
+    bool rev;
+};
+hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
 hipError_t launch_decay_attn(const DecayParams& a, int io_dt, hipStream_t s);
 
 // Tokens of a chunk of the gradients: 64, or 32 for operands in fp32, whose tiles take twice the LDS.
@@ -65,7 +77,9 @@ constexpr int decay_grad_chunk(bool bf16) { return bf16 ? 64 : 32; }
 
 struct DecayGradParams {
     DecayParams f;            // o: the gradient of the outputs
-    const float *S, *R;       // [n_seqs, H, nc, values]: states in front of the chunks, gradients of those behind them
+    // states in front of the chunks and gradients of those behind them, and their sums (DecayWalkParams)
+    const float *S, *R, *sum_S, *sum_R;
+    int64_t per, wide;        // chunks of a segment; columns of a state as kept
     int64_t nc;               // chunks of a sequence
     void *dq, *dk, *dv;       // contiguous, I/O dtype
     float *part_q, *part_k;   // [n_seqs T, H, Dk] where heads share q and k, else null

@@ -20,7 +20,7 @@ constexpr int C = DECAY_CHUNK;
 
 // Outputs, from the state in front of the segment.
 template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL>
-__global__ __launch_bounds__(NW * 64, 2) void decay_attn_kernel(DecayParams a) {
+__global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) void decay_attn_kernel(DecayParams a) {
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(WIDTH), TJ = C / KS;  // TJ: K steps over the tokens
     constexpr int DT = DK / 16;

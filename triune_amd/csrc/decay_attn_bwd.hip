@@ -10,9 +10,10 @@
 // with dq', dk' the terms with S_0 and R.  Only pairs that span t are added, so steep gates, whose own pairs are large
 // and spanning ones small, lose nothing to cancellation.
 //
-// The states in front of the chunks and the gradients behind them come from two walks (decay_walk_kernel), so a
+// The states in front of the chunks and the gradients behind them come from two walks (decay_walk.hip), so a
 // workgroup takes one (chunk, head) by itself.  A and B are formed once, in tiles over the waves, and shared through
-// LDS; a wave owns 16-wide tiles of key dims (dq, dk) and of value dims (dv), so a state is read once for each use.
+// LDS, B in the place of A; a wave owns 16-wide tiles of key dims (dq, dk) and of value dims (dv), which are taken in
+// slices of 64, so a state is read once for each use and two workgroups fit a compute unit.
 #include "decay_mfma.h"
 
 namespace triune {
@@ -49,20 +50,38 @@ __device__ __forceinline__ float row_suffix_scan(float x) {
     return x;
 }
 
-template <int E>
-__device__ __forceinline__ void load_floats(const float* p, float (&x)[E]) {
-#pragma unroll
-    for (int i = 0; i < E; i += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i + e] = v[e];
-    }
-}
-
 }  // namespace
 
-template <typename TIO, typename TC, int DK, int DVW, int NW>
-__global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) {
+// The state of a place: what is kept there plus, decayed, what its segment's first place holds.  Through buffer resources,
+// whose scalar offsets step through the values (64-bit addresses for each would take two registers apiece and spill).
+struct StateAt {
+    __amdgpu_buffer_rsrc_t own, first;
+    float f;
+    __device__ __forceinline__ StateAt(const float* p, int64_t to_first, float f, int64_t values) : f(f) {
+        const int bytes = (int)(values * 4);
+        own = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), (short)0, bytes, 0x00020000);
+        first = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p + to_first), (short)0, bytes, 0x00020000);
+    }
+    // E consecutive values, at byte offsets of the lane and of all lanes
+    template <int E>
+    __device__ __forceinline__ void row(int lane, int all, float (&x)[E]) const {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(own, lane + 4 * i, all, 0));
+            const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(first, lane + 4 * i, all, 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] = __builtin_fmaf(f, b[e], a[e]);
+        }
+    }
+    __device__ __forceinline__ float one(int lane, int all) const {
+        const float a = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(own, lane, all, 0));
+        const float b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(first, lane, all, 0));
+        return __builtin_fmaf(f, b, a);
+    }
+};
+
+template <typename TIO, typename TC, int DK, int DVW, int NW, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams p) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, CH = decay_grad_chunk(E == 8), CT = CH / 16, TJ = CH / KS;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(DVW), RC = tile_stride<TC>(CH), NTH = NW * 64;
@@ -70,29 +89,47 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
     constexpr int NDK = DK / 16 < NW ? 1 : DK / 16 / NW, NDV = DVW / 16 < NW ? 1 : DVW / 16 / NW;
     using Frag = typename Mat<TC>::Frag;
     __shared__ __attribute__((aligned(16))) TC s_q[CH * RK], s_k[CH * RK], s_v[CH * RV], s_d[CH * RV];
-    __shared__ __attribute__((aligned(16))) TC s_A[NP * PL], s_B[NP * PL];
+    __shared__ __attribute__((aligned(16))) TC s_A[NP * PL];  // A, then B
     __shared__ float s_g[2][CH], s_x[NW][CH], s_y[NW][CH], s_z[NW];
     __shared__ float s_r[TILES][16], s_c[TILES][16], s_tot[TILES], s_diag[CT][16];
     const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15;
     const int h = (int)(blockIdx.x % a.H);
     const int64_t sc = blockIdx.x / a.H, seq = sc / p.nc, c = sc - seq * p.nc, t0 = c * CH;
     const int rows = (int)min((int64_t)CH, a.T - t0), hk = h / a.per;
-    const int64_t wide = (int64_t)DVW * a.slices, values = DK * wide;
-    const float* pS = p.S + ((seq * a.H + h) * p.nc + c) * values;
-    const float* pR = p.R + ((seq * a.H + h) * p.nc + c) * values;
+    const int wide = (int)p.wide;
+    const int64_t values = (int64_t)DK * wide, place = (seq * a.H + h) * p.nc + c;
+    // places that hold what their own segment made, and the segment's first place (its last one for R)
+    const int64_t c0 = c / p.per * p.per, c1 = min(c0 + p.per, p.nc) - 1;
+    const bool joinS = c0 > 0 && c > c0, joinR = c1 + 1 < p.nc && c < c1;
+    auto factor = [&](const float* sums) { return __builtin_amdgcn_exp2f(sums[2 * place] + sums[2 * place + 1]); };
+    const StateAt S(p.S + place * values, joinS ? (c0 - c) * values : 0, joinS ? factor(p.sum_S) : 0.f, values);
+    const StateAt R(p.R + place * values, joinR ? (c1 - c) * values : 0, joinR ? factor(p.sum_R) : 0.f, values);
     auto at = [&](const DecayTok& t, int head) { return seq * t.sb + t0 * t.st + head * t.sh; };
 
-    load_tile<TIO, TC, CH, DK, NTH>(s_q, (const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
-    load_tile<TIO, TC, CH, DK, NTH>(s_k, (const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
+    const TIO *pv = (const TIO*)a.v.p + at(a.v, h), *pd = (const TIO*)a.o.p + at(a.o, h);
+    auto fetch_values = [&](int col0, auto&& between) {
+        Tile<TIO, TC, CH, DVW, NTH, FULL> tv(a.v.st, a.Dv - col0), td(a.o.st, a.Dv - col0);
+        tv.fetch(pv + col0, a.v.st, rows, a.Dv - col0);
+        td.fetch(pd + col0, a.o.st, rows, a.Dv - col0);
+        between();
+        tv.put(s_v);
+        td.put(s_d);
+    };
+    Tile<TIO, TC, CH, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
+    tq.fetch((const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
+    tk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
+    fetch_values(0, [&] {
+        tq.put(s_q);
+        tk.put(s_k);
+    });
     if (w == 0) {
         const Sum2 gs = chunk_sums<CH>(a.g, a.g_dt, at(a.g, h), rows, lane);
         if (lane < CH) s_g[0][lane] = gs.hi, s_g[1][lane] = gs.lo;
     }
     if constexpr (E == 8) {  // a K step of 32 tokens takes the tile above the diagonal along: zeros
-        for (int u = threadIdx.x; u < CT / 2 * NP * 2 * 16 * 4; u += NTH) {
-            const int q = u & 3, row = (u >> 2) & 15, pl = (u >> 6) & 1, b = u >> 7 & (NP - 1), I = 2 * (u >> 8);
-            TC* to = (pl ? s_B : s_A) + b * PL + (16 * I + row) * RC + 16 * (I + 1) + 4 * q;
-            *reinterpret_cast<uint2*>(to) = uint2{0, 0};
+        for (int u = threadIdx.x; u < CT / 2 * NP * 16 * 4; u += NTH) {
+            const int q = u & 3, row = (u >> 2) & 15, b = (u >> 6) & (NP - 1), I = 2 * (u >> 7);
+            *reinterpret_cast<uint2*>(s_A + b * PL + (16 * I + row) * RC + 16 * (I + 1) + 4 * q) = uint2{0, 0};
         }
     }
     __syncthreads();
@@ -126,11 +163,8 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
 #pragma unroll
         for (int I = 0; I < CT; ++I) dq[d][I] = dk[d][I] = zero4();
     float z = 0.f;
-    for (int sl = 0; sl < a.slices; ++sl) {
-        const int col0 = sl * DVW;
-        if (sl) __syncthreads();
-        load_tile<TIO, TC, CH, DVW, NTH>(s_v, (const TIO*)a.v.p + at(a.v, h) + col0, a.v.st, rows, a.Dv - col0);
-        load_tile<TIO, TC, CH, DVW, NTH>(s_d, (const TIO*)a.o.p + at(a.o, h) + col0, a.o.st, rows, a.Dv - col0);
+    for (int col0 = 0; col0 < a.Dv; col0 += DVW) {
+        if (col0) fetch_values(col0, [] { __syncthreads(); });
         __syncthreads();
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -146,12 +180,12 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
         for (int d = 0; d < NDK; ++d) {
             const int t = w * NDK + d;
             if (t >= DK / 16) continue;
-            const int64_t off = (16 * t + n) * wide + col0 + E * g;
+            const int off = 4 * (n * wide + E * g);
 #pragma unroll
             for (int s = 0; s < DVW / KS; ++s) {
                 float xs[E], xr[E];
-                load_floats<E>(pS + off + s * KS, xs);
-                load_floats<E>(pR + off + s * KS, xr);
+                S.row<E>(off, 4 * (16 * t * wide + col0 + s * KS), xs);
+                R.row<E>(off, 4 * (16 * t * wide + col0 + s * KS), xr);
 #pragma unroll
                 for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[e], xr[e], z);
                 const auto ps = parts<TC, 3>(xs);
@@ -174,7 +208,8 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
             for (int s = 0; s < DK / KS; ++s) {
                 float xr[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) xr[e] = pR[(s * KS + E * g + e) * wide + col0 + 16 * t + n];
+                for (int e = 0; e < E; ++e)
+                    xr[e] = R.one(4 * (E * g * wide + n), 4 * ((s * KS + e) * wide + col0 + 16 * t));
                 const auto pr = parts<TC, 3>(xr);
 #pragma unroll
                 for (int J = 0; J < CT; ++J) dv[J] = mma<TC>(pr, row_frag(s_k, RK, 16 * J + n, s, g), dv[J]);
@@ -198,6 +233,7 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
     }
 
     // B, and the sums of (q . k) B over its tiles that the gates' gradients take
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int idx = w + NW * m;
@@ -210,7 +246,7 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
             x[r] = J < I || 4 * g + r <= n ? bm[m][r] * dec[m][r] : 0.f;
             M[r] = J < I || 4 * g + r < n ? am[m][r] * x[r] : 0.f;
         }
-        put4<TC, NP>(s_B, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
+        put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
         if (J < I) {
             float col = (M[0] + M[1]) + (M[2] + M[3]);
             col = xor_sum<32>(xor_sum<16>(col));
@@ -263,14 +299,14 @@ __global__ __launch_bounds__(NW * 64) void decay_grad_kernel(DecayGradParams p) 
                 const Frag x = col_frag<TC, false>(s_k, RK, t, s, g, n);
 #pragma unroll
                 for (int b = NP - 1; b >= 0; --b)
-                    dq[d][I] = Mat<TC>::mma(x, row_frag_tok(s_B + b * PL, RC, i, s, g), dq[d][I]);
+                    dq[d][I] = Mat<TC>::mma(x, row_frag_tok(s_A + b * PL, RC, i, s, g), dq[d][I]);
             }
 #pragma unroll
             for (int s = 16 * I / KS; s < TJ; ++s) {
                 const Frag x = col_frag<TC, false>(s_q, RK, t, s, g, n);
 #pragma unroll
                 for (int b = NP - 1; b >= 0; --b)
-                    dk[d][I] = Mat<TC>::mma(x, col_frag<TC, false>(s_B + b * PL, RC, I, s, g, n), dk[d][I]);
+                    dk[d][I] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, I, s, g, n), dk[d][I]);
             }
             if (i >= rows) continue;
             const float oq[4] = {dq[d][I][0], dq[d][I][1], dq[d][I][2], dq[d][I][3]};
@@ -363,27 +399,24 @@ __global__ __launch_bounds__(1024) void decay_gate_kernel(DecayGradParams p, int
 namespace {
 
 template <typename TIO, typename TC, int DK, int DVW>
-hipError_t grad_one(const DecayGradParams& p, hipStream_t s) {
-    constexpr int NW = DK == 128 || DVW == 128 ? 8 : 4;
-    decay_grad_kernel<TIO, TC, DK, DVW, NW>
-        <<<dim3((unsigned)(p.f.n_seqs * p.nc * p.f.H)), NW * 64, 0, s>>>(p);
-    return hipGetLastError();
+void grad_one(const DecayGradParams& p, bool full, hipStream_t s) {
+    const dim3 grid((unsigned)(p.f.n_seqs * p.nc * p.f.H));
+    if (full) decay_grad_kernel<TIO, TC, DK, DVW, 4, true><<<grid, 256, 0, s>>>(p);
+    else decay_grad_kernel<TIO, TC, DK, DVW, 4, false><<<grid, 256, 0, s>>>(p);
 }
 template <typename TIO, typename TC, int DK>
-hipError_t grad_width(const DecayGradParams& p, hipStream_t s) {
-    switch (decay_slice(p.f.Dv)) {
-        case 32: return grad_one<TIO, TC, DK, 32>(p, s);
-        case 64: return grad_one<TIO, TC, DK, 64>(p, s);
-        default: return grad_one<TIO, TC, DK, 128>(p, s);
-    }
+void grad_width(const DecayGradParams& p, bool full, hipStream_t s) {
+    if (p.f.Dv <= 32) grad_one<TIO, TC, DK, 32>(p, full, s);
+    else grad_one<TIO, TC, DK, 64>(p, full, s);
 }
 template <typename TIO, typename TC>
-hipError_t grad_dk(const DecayGradParams& p, hipStream_t s) {
+hipError_t grad_dk(const DecayGradParams& p, bool full, hipStream_t s) {
     switch (decay_padded_dk(p.f.Dk)) {
-        case 32: return grad_width<TIO, TC, 32>(p, s);
-        case 64: return grad_width<TIO, TC, 64>(p, s);
-        default: return grad_width<TIO, TC, 128>(p, s);
+        case 32: grad_width<TIO, TC, 32>(p, full, s); break;
+        case 64: grad_width<TIO, TC, 64>(p, full, s); break;
+        default: grad_width<TIO, TC, 128>(p, full, s);
     }
+    return hipGetLastError();
 }
 template <typename TIO>
 hipError_t share(const DecayGradParams& p, hipStream_t s) {
@@ -395,9 +428,11 @@ hipError_t share(const DecayGradParams& p, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_decay_grad(const DecayGradParams& p, int io_dt, hipStream_t s) {
-    hipError_t e = io_dt == DT_F32    ? grad_dk<float, float>(p, s)
-                   : io_dt == DT_BF16 ? grad_dk<__bf16, __bf16>(p, s)
-                                      : grad_dk<_Float16, float>(p, s);
+    const DecayParams& a = p.f;
+    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.q, a.k, a.v, a.o});
+    hipError_t e = io_dt == DT_F32    ? grad_dk<float, float>(p, full, s)
+                   : io_dt == DT_BF16 ? grad_dk<__bf16, __bf16>(p, full, s)
+                                      : grad_dk<_Float16, float>(p, full, s);
     if (e != hipSuccess) return e;
     if (p.part_q) {
         e = io_dt == DT_F32 ? share<float>(p, s) : io_dt == DT_BF16 ? share<__bf16>(p, s) : share<_Float16>(p, s);

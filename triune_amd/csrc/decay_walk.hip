@@ -5,11 +5,15 @@ namespace triune {
 
 constexpr int C = DECAY_CHUNK;
 
-// States alone, from rows (k of a.k) by columns (v): the segments' own end states (states null) of those that another one
-// follows, in the workspace; or from the carried-in states the state in front of every `every` tokens, in `states`,
-// and the final one.  REV: the same from the end of the sequence (gradients of states, rows q and columns do):
-//     R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
-template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV>
+// States alone, from rows (a.k) by columns (a.v), REV: from the end of the sequence (gradients of states, whose rows are q
+// and whose columns are do):
+//     S <- e^{G_C} S + sum_j e^{G_C - G_j} k_j v_j^T,   R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
+// The first segment of a walk starts from a.s0, the others from zero, and decay_carry_kernel adds what comes in.
+// EACH false: the segments' own end states, in the order of the lanes, of those that another one follows.
+// EACH true: the state in front of (REV: behind) every chunk of p.every tokens, in `states`, [DK][columns] each.  A
+// segment leaves its own end state in the next one's first place, and that one's later places hold what its own tokens
+// made: whoever reads them adds the first place's state, decayed by `sums`.
+template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV, bool EACH>
 __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams p) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
@@ -19,31 +23,15 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
     __shared__ __attribute__((aligned(16))) ChunkGates s_gs[2];
     DecayWhere x;
     if (!decay_where(a, x)) return;
-    const bool each = p.states, begins = REV ? x.seg.last : x.seg.index == 0, ends = REV ? x.seg.index == 0 : x.seg.last;
-    if (!each && ends) return;
+    const bool begins = REV ? x.seg.last : x.seg.index == 0, ends = REV ? x.seg.index == 0 : x.seg.last;
+    if (!EACH && ends) return;
     const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15, col0 = x.slice * WIDTH;
     const TIO* pk = (const TIO*)a.k.p + decay_base(a, x, a.k, x.h / a.per);
     const TIO* pv = (const TIO*)a.v.p + decay_base(a, x, a.v, x.h) + col0;
     const int64_t pg = decay_base(a, x, a.g, x.h);
     const int64_t srow = ssm_row(a.slots, a.n_slots, x.seg.seq), soff = (srow * a.H + x.h) * a.Dk * a.Dv;
-    const int64_t values = (int64_t)DK * WIDTH * a.slices, in_ws = ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
-    auto ws = [&](int64_t item) { return a.ws_state + (item * a.H + x.h) * values + in_ws; };
+    const int64_t wide = (int64_t)WIDTH * a.slices, values = DK * wide;
 
-    f32x4 S[NT][DT];
-    if (begins) {
-        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
-            v = in && a.s0 && srow >= 0 ? a.s0[soff + off] : 0.f;
-        });
-        // The last segment of a cut sequence has no use for its place in the workspace: it takes the initial state,
-        // since s0 may be the pool that the last segment's outputs leave their state in while the first one starts.
-        if (!REV && !each) put_state(S, ws(x.last));
-    } else if (each) {
-        get_state(S, ws(REV ? x.w + 1 : x.w - 1));
-    } else {
-        each_state<TC>(S, 0, 0, 0, 0, [](float& v, int64_t, bool) { v = 0.f; });
-    }
-
-    Sum2 all{0.f, 0.f};
     const int chunks = (x.seg.len + C - 1) / C;
     Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st, a.Dk);
     Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
@@ -55,15 +43,35 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
         tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
     };
     if (chunks) fetch(0);
+
+    f32x4 S[NT][DT];
+    if (begins && a.s0) {
+        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
+            v = in && srow >= 0 ? a.s0[soff + off] : 0.f;
+        });
+    } else {
+        each_state<TC>(S, 0, 0, 0, 0, [](float& v, int64_t, bool) { v = 0.f; });
+    }
+    // The last segment of a cut sequence has no use for its place in the workspace: it takes the initial state, since
+    // s0 may be the pool that the last segment's outputs leave their state in while the first one starts.
+    auto ws = [&](int64_t item) {
+        return a.ws_state + (item * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
+    };
+    if (!EACH && begins) put_state(S, ws(x.last));
+    const int64_t nc = EACH ? (a.T + p.every - 1) / p.every : 0;
+    auto keep_at = [&](int64_t c, const Sum2& sum) {
+        const int64_t at = (x.seg.seq * a.H + x.h) * nc + c;
+        float* to = p.states + at * values;
+        each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
+        if (x.slice == 0 && threadIdx.x == 0) p.sums[2 * at] = sum.hi, p.sums[2 * at + 1] = sum.lo;
+    };
+
+    Sum2 all{0.f, 0.f};
     for (int i = 0; i < chunks; ++i) {
         const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
-        TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
         const int64_t at = x.seg.t0 + t0;
-        if (each && (REV ? (at + C) % p.every == 0 || at + rows == a.T : at % p.every == 0)) {
-            const int64_t nc = (a.T + p.every - 1) / p.every, wide = (int64_t)WIDTH * a.slices;
-            float* to = p.states + ((x.seg.seq * a.H + x.h) * nc + at / p.every) * values;
-            each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
-        }
+        if (EACH && (i ? (REV ? at + C : at) % p.every == 0 : begins)) keep_at(at / p.every, all);
+        TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
         tk.put(s_k);
         tv.put(s_v);
         ChunkGates& s_g = s_gs[i & 1];
@@ -98,88 +106,121 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
         }
     }
 
-    if (each) {
-        if (!ends || !a.fin || srow < 0) return;
-        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
-            if (in) a.fin[soff + off] = v;
-        });
-    } else {
+    float* sum = a.ws_sum + (x.w * a.H + x.h) * 2;
+    if (a.ws_sum && x.slice == 0 && threadIdx.x == 0) sum[0] = all.hi, sum[1] = all.lo;
+    if constexpr (!EACH) {
         put_state(S, ws(x.w));
-        if (x.slice == 0 && threadIdx.x == 0) {
-            float* sum = a.ws_sum + (x.w * a.H + x.h) * 2;
-            sum[0] = all.hi, sum[1] = all.lo;
+    } else if (!ends) {
+        keep_at(REV ? x.seg.t0 / p.every - 1 : (x.seg.t0 + a.seg) / p.every, Sum2{0.f, 0.f});
+    } else if (a.fin) {
+        if (begins) {
+            each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
+                if (in) a.fin[soff + off] = v;
+            });
+        } else {  // the carry completes it
+            float* to = p.own + (x.seg.seq * a.H + x.h) * values;
+            each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
         }
     }
 }
 
-// Joins the segments' end states in order: S_p = 2^{sum_p} S_{p-1} + own_p, in place, for the segments that another
-// one follows (rev: from the last one to the second).  A thread per value of a (sequence, head).
-__global__ __launch_bounds__(256) void decay_carry_kernel(DecayParams a, int64_t values, bool rev) {
-    const int64_t blocks = (values + 255) / 256;
-    const int64_t sh = blockIdx.x / blocks, i = (blockIdx.x % blocks) * 256 + threadIdx.x;
-    const int64_t seq = sh / a.H, h = sh % a.H;
-    if (i >= values) return;
-    int64_t first, n;
+// Joins the segments' end states in place: S_p = 2^{sum_p} S_{p-1} + own_p, p = 1 .. n - 2 in the walk's direction, with S_0
+// the first segment's own; the state in front of segment p + 1 is then S_p.  A thread per value of a (sequence, head),
+// with the next states in flight.
+__global__ __launch_bounds__(256) void decay_carry_kernel(DecayCarryParams p) {
+    const DecayParams& a = p.f;
+    const uint32_t blocks = (uint32_t)((p.values + 255) / 256);
+    const uint32_t sh = blockIdx.x / blocks, seq = sh / (uint32_t)a.H, h = sh - seq * (uint32_t)a.H;
+    const int64_t i = (int64_t)(blockIdx.x - sh * blocks) * 256 + threadIdx.x;
+    if (i >= p.values) return;
+    int64_t first = 0, n = a.nseg;
     if (a.cu) {
         first = a.seg_off[seq];
         n = a.seg_off[seq + 1] - first;
     } else {
-        first = seq * a.nseg;
-        n = a.nseg;
+        first = (int64_t)seq * a.nseg;
     }
-    if (n < 3) return;  // one state to carry: the first segment's own
-    const int64_t step = rev ? -a.H * values : a.H * values, step_sum = rev ? -2 * a.H : 2 * a.H;
-    if (rev) first += n - 1;
-    float* p = a.ws_state + (first * a.H + h) * values + i;
-    const float* sum = a.ws_sum + (first * a.H + h) * 2;
-    float s = p[0];
-    constexpr int AHEAD = 8;
-    for (int64_t k0 = 1; k0 < n - 1; k0 += AHEAD) {
-        float x[AHEAD], d[AHEAD];
-        const int m = (int)min((int64_t)AHEAD, n - 1 - k0);
+    const int64_t own = p.own ? 1 : 0;  // one more join, into the final state
+    if (n + own < 3) return;
+    // segment k of the walk
+    auto segment = [&](int64_t k) { return first + (p.rev ? n - 1 - k : k); };
+    auto factor = [&](int64_t k) {
+        const float* e = a.ws_sum + (segment(k) * a.H + h) * 2;
+        return __builtin_amdgcn_exp2f(e[0] + e[1]);
+    };
+    float* s0;
+    int64_t step;
+    if (p.states) {  // the place in front of the walk's second segment, and those of the following ones
+        const int64_t per = a.seg / p.every, at = p.rev ? (n - 1) * per - 1 : per;
+        s0 = p.states + ((int64_t)sh * p.nc + at) * p.values + i;
+        step = (p.rev ? -per : per) * p.values;
+    } else {
+        s0 = a.ws_state + (first * a.H + h) * p.values + i;
+        step = a.H * p.values;
+    }
+    const int64_t joins = n - 2;
+    float s = s0[0];
+    constexpr int AHEAD = 16;
+    float x[AHEAD];
+    auto fetch = [&](int64_t k0) {  // past the end the last one again, so that no load stands behind a condition
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) x[k] = s0[min(k0 + k, joins) * step];
+    };
+    if (joins > 0) fetch(1);
+    for (int64_t k0 = 1; k0 <= joins; k0 += AHEAD) {
+        float y[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) y[k] = x[k];
+        fetch(min(k0 + AHEAD, joins));
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-            if (k < m) {
-                x[k] = p[(k0 + k) * step];
-                const float* e = sum + (k0 + k) * step_sum;
-                d[k] = __builtin_amdgcn_exp2f(e[0] + e[1]);
+            if (k0 + k <= joins) {
+                s = __builtin_fmaf(factor(k0 + k), s, y[k]);
+                s0[(k0 + k) * step] = s;
             }
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (k < m) {
-                s = __builtin_fmaf(d[k], s, x[k]);
-                p[(k0 + k) * step] = s;
-            }
+    }
+    if (own) {
+        const int64_t wide = p.values / p.dk, d = i / wide, c = i - d * wide;
+        if (d < a.Dk && c < a.Dv)
+            a.fin[((int64_t)sh * a.Dk + d) * a.Dv + c] = __builtin_fmaf(factor(n - 1), s, p.own[sh * p.values + i]);
     }
 }
 
 namespace {
 
-template <typename TIO, typename TC>
-struct Walk {
-    template <int DK, int NW, int NT, bool FULL>
-    static void run(const DecayWalkParams& p, dim3 grid, hipStream_t s) {
-        decay_walk_kernel<TIO, TC, DK, NW, NT, FULL, false><<<grid, NW * 64, 0, s>>>(p);
-    }
+template <bool REV, bool EACH>
+struct Walks {
+    template <typename TIO, typename TC>
+    struct Of {
+        template <int DK, int NW, int NT, bool FULL>
+        static void run(const DecayWalkParams& p, dim3 grid, hipStream_t s) {
+            decay_walk_kernel<TIO, TC, DK, NW, NT, FULL, REV, EACH><<<grid, NW * 64, 0, s>>>(p);
+        }
+    };
 };
-template <typename TIO, typename TC>
-struct WalkBack {
-    template <int DK, int NW, int NT, bool FULL>
-    static void run(const DecayWalkParams& p, dim3 grid, hipStream_t s) {
-        decay_walk_kernel<TIO, TC, DK, NW, NT, FULL, true><<<grid, NW * 64, 0, s>>>(p);
-    }
-};
+
+hipError_t carry(const DecayCarryParams& p, hipStream_t s) {
+    decay_carry_kernel<<<dim3((unsigned)(p.f.n_seqs * p.f.H * ((p.values + 255) / 256))), 256, 0, s>>>(p);
+    return hipGetLastError();
+}
 
 }  // namespace
 
-hipError_t launch_decay_walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
-    const bool full = decay_full(p.f.Dk, p.f.Dv, io_dt, {p.f.k, p.f.v});
-    return rev ? decay_by_type<WalkBack>(p, p.f, io_dt, full, s) : decay_by_type<Walk>(p, p.f, io_dt, full, s);
+hipError_t launch_decay_ends(const DecayParams& a, int io_dt, hipStream_t s) {
+    const DecayWalkParams p{a, nullptr, nullptr, nullptr, 0};
+    const hipError_t e = decay_by_type<Walks<false, false>::Of>(p, a, io_dt, decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v}), s);
+    if (e != hipSuccess) return e;
+    return carry(DecayCarryParams{a, nullptr, nullptr, 0, 0, decay_state_values(a.Dk, a.Dv), 0, false}, s);
 }
-hipError_t launch_decay_carry(const DecayParams& a, bool rev, hipStream_t s) {
-    const int64_t values = decay_state_values(a.Dk, a.Dv);
-    decay_carry_kernel<<<dim3((unsigned)(a.n_seqs * a.H * ((values + 255) / 256))), 256, 0, s>>>(a, values, rev);
-    return hipGetLastError();
+
+hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
+    const DecayParams& a = p.f;
+    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v});
+    const hipError_t e = rev ? decay_by_type<Walks<true, true>::Of>(p, a, io_dt, full, s)
+                             : decay_by_type<Walks<false, true>::Of>(p, a, io_dt, full, s);
+    if (e != hipSuccess || a.nseg < 2) return e;
+    return carry(DecayCarryParams{a, p.states, rev && a.fin ? p.own : nullptr, p.every, (a.T + p.every - 1) / p.every,
+                                  decay_state_values(a.Dk, a.Dv), decay_padded_dk(a.Dk), rev}, s);
 }
 
 }  // namespace triune
