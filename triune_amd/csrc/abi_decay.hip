@@ -20,8 +20,15 @@ bool seqs_ok(int64_t n_seqs, int64_t H, int64_t Dv) { return grid_ok(n_seqs, H *
 int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * DECAY_CHUNK; }
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Workgroups that fill the chip.
-constexpr int kSlots = 4;
+// Workgroups that split calls are cut into, and the tokens that a segment has at least: a cut costs a state written,
+// joined and read, 16 bytes a value.
+int64_t chip_slots(int64_t Dk, int64_t Dv) {
+    return (int64_t)compute_units() * (decay_padded_dk((int)Dk) * decay_slice((int)Dv) > 8192 ? 3 : 6) / 2;
+}
+int64_t least_segment(int64_t Dk, int64_t Dv) {
+    const int values = decay_padded_dk((int)Dk) * decay_slice((int)Dv);
+    return values > 8192 ? 192 : values > 4096 ? 128 : 64;
+}
 
 struct DecayPlan {
     int64_t seg, nseg, n_work, cut;
@@ -41,8 +48,8 @@ DecayPlan plan_dense(int64_t n_seqs, int64_t T, int64_t H, int64_t Dk, int64_t D
     const int64_t whole = round_up(T, DECAY_CHUNK), blocks = n_seqs * H * slices_of(Dv);
     p.seg = forced_segment(flags);
     if (!p.seg) {
-        int64_t n = (int64_t)compute_units() * kSlots / blocks;
-        if (n > T / 64) n = T / 64;
+        int64_t n = chip_slots(Dk, Dv) / blocks;
+        if (n > T / least_segment(Dk, Dv)) n = T / least_segment(Dk, Dv);
         p.seg = n < 2 ? whole : round_up((T + n - 1) / n, DECAY_CHUNK);
     }
     if (p.seg > whole) p.seg = whole;
@@ -58,10 +65,11 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
     DecayPlan p{};
     p.seg = forced_segment(flags);
     if (!p.seg) {
-        p.seg = round_up(total * H * slices_of(Dv) / ((int64_t)compute_units() * kSlots), DECAY_CHUNK);
-        if (p.seg < 64) p.seg = 64;
+        p.seg = round_up(total * H * slices_of(Dv) / chip_slots(Dk, Dv), DECAY_CHUNK);
+        if (p.seg < least_segment(Dk, Dv)) p.seg = least_segment(Dk, Dv);
+        p.cut = p.seg * 3 / 2;
     }
-    p.cut = p.seg;
+    if (p.cut < p.seg) p.cut = p.seg;
     p.nseg = p.cut < total ? 2 : 1;
     p.n_work = p.nseg > 1 ? total / p.seg + n_seqs : n_seqs;
     plan_bytes(p, H, Dk, Dv, n_seqs + 1);

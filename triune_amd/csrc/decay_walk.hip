@@ -125,29 +125,21 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
 }
 
 // Joins the segments' end states in place: S_p = 2^{sum_p} S_{p-1} + own_p, p = 1 .. n - 2 in the walk's direction, with S_0
-// the first segment's own; the state in front of segment p + 1 is then S_p.  A thread per value of a (sequence, head),
-// with the next states in flight.
+// the first segment's own; the state in front of segment p + 1 is then S_p.  A thread per four values of a (sequence,
+// head), with the next states and sums in flight.
 __global__ __launch_bounds__(256) void decay_carry_kernel(DecayCarryParams p) {
     const DecayParams& a = p.f;
-    const uint32_t blocks = (uint32_t)((p.values + 255) / 256);
+    const uint32_t blocks = (uint32_t)((p.values + 1023) / 1024);
     const uint32_t sh = blockIdx.x / blocks, seq = sh / (uint32_t)a.H, h = sh - seq * (uint32_t)a.H;
-    const int64_t i = (int64_t)(blockIdx.x - sh * blocks) * 256 + threadIdx.x;
+    const int64_t i = (int64_t)(blockIdx.x - sh * blocks) * 1024 + threadIdx.x * 4;
     if (i >= p.values) return;
-    int64_t first = 0, n = a.nseg;
+    int64_t first = (int64_t)seq * a.nseg, n = a.nseg;
     if (a.cu) {
         first = a.seg_off[seq];
         n = a.seg_off[seq + 1] - first;
-    } else {
-        first = (int64_t)seq * a.nseg;
     }
     const int64_t own = p.own ? 1 : 0;  // one more join, into the final state
     if (n + own < 3) return;
-    // segment k of the walk
-    auto segment = [&](int64_t k) { return first + (p.rev ? n - 1 - k : k); };
-    auto factor = [&](int64_t k) {
-        const float* e = a.ws_sum + (segment(k) * a.H + h) * 2;
-        return __builtin_amdgcn_exp2f(e[0] + e[1]);
-    };
     float* s0;
     int64_t step;
     if (p.states) {  // the place in front of the walk's second segment, and those of the following ones
@@ -158,31 +150,46 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(DecayCarryParams p) {
         s0 = a.ws_state + (first * a.H + h) * p.values + i;
         step = a.H * p.values;
     }
-    const int64_t joins = n - 2;
-    float s = s0[0];
-    constexpr int AHEAD = 16;
-    float x[AHEAD];
-    auto fetch = [&](int64_t k0) {  // past the end the last one again, so that no load stands behind a condition
+    // sums of segment k of the walk
+    const float* sum0 = a.ws_sum + ((first + (p.rev ? n - 1 : 0)) * a.H + h) * 2;
+    const int64_t sum_step = (p.rev ? -2 : 2) * a.H;
+    const int joins = (int)(n - 2);
+    f32x4 s = *reinterpret_cast<const f32x4*>(s0);
+    constexpr int AHEAD = 8;
+    f32x4 x[AHEAD];
+    float d[AHEAD];
+    auto fetch = [&](int k0) {  // past the end the last one again, so that no load stands behind a condition
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) x[k] = s0[min(k0 + k, joins) * step];
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t at = min(k0 + k, joins);
+            x[k] = *reinterpret_cast<const f32x4*>(s0 + at * step);
+            d[k] = sum0[at * sum_step] + sum0[at * sum_step + 1];
+        }
     };
     if (joins > 0) fetch(1);
-    for (int64_t k0 = 1; k0 <= joins; k0 += AHEAD) {
-        float y[AHEAD];
+    for (int k0 = 1; k0 <= joins; k0 += AHEAD) {
+        f32x4 y[AHEAD];
+        float f[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) y[k] = x[k];
-        fetch(min(k0 + AHEAD, joins));
+        for (int k = 0; k < AHEAD; ++k) y[k] = x[k], f[k] = __builtin_amdgcn_exp2f(d[k]);
+        if (k0 + AHEAD <= joins) fetch(k0 + AHEAD);
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
             if (k0 + k <= joins) {
-                s = __builtin_fmaf(factor(k0 + k), s, y[k]);
-                s0[(k0 + k) * step] = s;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(f[k], s[e], y[k][e]);
+                *reinterpret_cast<f32x4*>(s0 + (k0 + k) * step) = s;
             }
     }
     if (own) {
-        const int64_t wide = p.values / p.dk, d = i / wide, c = i - d * wide;
-        if (d < a.Dk && c < a.Dv)
-            a.fin[((int64_t)sh * a.Dk + d) * a.Dv + c] = __builtin_fmaf(factor(n - 1), s, p.own[sh * p.values + i]);
+        const float f = __builtin_amdgcn_exp2f(sum0[(n - 1) * sum_step] + sum0[(n - 1) * sum_step + 1]);
+        const f32x4 end = *reinterpret_cast<const f32x4*>(p.own + sh * p.values + i);
+        const int64_t wide = p.values / p.dk, r = i / wide, c = i - r * wide;
+        if (r >= a.Dk) return;
+        float* to = a.fin + ((int64_t)sh * a.Dk + r) * a.Dv + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < a.Dv) to[e] = __builtin_fmaf(f, s[e], end[e]);
     }
 }
 
@@ -200,7 +207,7 @@ struct Walks {
 };
 
 hipError_t carry(const DecayCarryParams& p, hipStream_t s) {
-    decay_carry_kernel<<<dim3((unsigned)(p.f.n_seqs * p.f.H * ((p.values + 255) / 256))), 256, 0, s>>>(p);
+    decay_carry_kernel<<<dim3((unsigned)(p.f.n_seqs * p.f.H * ((p.values + 1023) / 1024))), 256, 0, s>>>(p);
     return hipGetLastError();
 }
 
