@@ -564,15 +564,18 @@ int triune_hip_decay_attn_varlen(const void* q, const void* k, const void* v, co
                                  int flags, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients: dout [B, T, H, Dv] in io_dtype; strides[15] = (batch, token, head) of q, k, v, g, dout; ds_final (NULL: zeros)
  * and ds0 (NULL: not wanted) fp32 contiguous [B, H, Dk, Dv], not one tensor; dq, dk, dv contiguous in io_dtype; dg
- * contiguous in g_dtype, [B, T, H], or with g_head != 0 [H], the sum over batch and tokens.  B, T > 0.  Sums are taken in a
- * fixed order.  The workspace holds the states of every 64th token (32nd for fp32 and fp16), twice. */
+ * contiguous in g_dtype, [B, T, H], or with g_head != 0 [H], the sum over batch and tokens.  B, T > 0.
+ * fwd_workspace: what triune_hip_decay_attn on these inputs and flags left in its workspace, not written since, or NULL.
+ * Sums are taken in a fixed order.  The workspace holds three times the states of every 64th token (32nd for fp32 and
+ * fp16). */
 size_t triune_hip_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
                                                 int io_dtype, int g_head, int flags);
 int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const void* dout,
                               int io_dtype, int g_dtype, const int64_t* strides, float scale, const float* s0,
                               const float* ds_final, void* dq, void* dk, void* dv, void* dg, int g_head, float* ds0,
                               int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int flags,
-                              void* workspace, size_t workspace_bytes, void* stream);
+                              const void* fwd_workspace, size_t fwd_workspace_bytes, void* workspace,
+                              size_t workspace_bytes, void* stream);
 /* One token for each of B rows; strides[10] = (batch, head) of q, k, v, g, o.  Row b uses state row slots[b] (b when
  * slots is NULL) of state_in and state_out, which may be one tensor; a row outside [0, n_state_rows) has no state and
  * zero outputs; other slots must be distinct. */

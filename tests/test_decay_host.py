@@ -13,7 +13,7 @@ from triune_amd import norm as N
 
 DENSE = "q k v g io gdt st scale s0 o fin B T H Hk Dk Dv flags ws wsb stream".split()
 VARLEN = "q k v g io gdt st scale cu n total s0 fin slots rows o H Hk Dk Dv flags ws wsb stream".split()
-BWD = "q k v g do io gdt st scale s0 dfin dq dk dv dg head ds0 B T H Hk Dk Dv flags ws wsb stream".split()
+BWD = "q k v g do io gdt st scale s0 dfin dq dk dv dg head ds0 B T H Hk Dk Dv flags fws fwsb ws wsb stream".split()
 STEP = "q k v g io gdt st scale s_in s_out slots rows o B H Hk Dk Dv stream".split()
 ENTRIES = [("triune_hip_decay_attn", DENSE), ("triune_hip_decay_attn_varlen", VARLEN),
            ("triune_hip_decay_attn_bwd", BWD), ("triune_hip_decay_attn_decode_step", STEP)]
@@ -22,7 +22,7 @@ ENTRIES = [("triune_hip_decay_attn", DENSE), ("triune_hip_decay_attn_varlen", VA
 def base(names, **kw):
     b = {k: FAKE for k in names}
     b.update(io=1, gdt=0, st=st(15), scale=1.0, slots=None, ws=None, wsb=0, stream=None, flags=0, B=2, T=64, H=4, Hk=2,
-             Dk=64, Dv=64, n=2, total=64, rows=2, head=0)
+             Dk=64, Dv=64, n=2, total=64, rows=2, head=0, fws=None, fwsb=0)
     return {**b, **kw}
 
 
@@ -57,11 +57,12 @@ def test_attention_entries_need_their_workspace():
     for k in ("do", "dq", "dk", "dv", "dg"):
         assert call(**{k: None}) == NULL, k
     assert call(B=0) == SHAPE and call(T=0) == SHAPE
-    flags = 1 << 8  # segments of 32 tokens
-    need = lib.triune_hip_decay_attn_workspace_size(2, 64, 4, 2, 64, 64, flags)
+    flags = 1 << 8  # segments of 64 tokens (packed: 32)
+    need = lib.triune_hip_decay_attn_workspace_size(2, 128, 4, 2, 64, 64, flags)
     assert need >= 2 * 2 * 4 * 64 * 64 * 4
     dense = caller("triune_hip_decay_attn", DENSE, **base(DENSE))
-    assert dense(flags=flags, ws=FAKE, wsb=need - 1) == WORKSPACE
+    assert dense(T=128, flags=flags, ws=FAKE, wsb=need - 1) == WORKSPACE
+    assert call(T=128, flags=flags, fws=FAKE, fwsb=need - 1, ws=FAKE, wsb=1 << 40) == WORKSPACE
     need = lib.triune_hip_decay_attn_varlen_workspace_size(2, 640, 4, 2, 64, 64, flags)
     varlen = caller("triune_hip_decay_attn_varlen", VARLEN, **base(VARLEN))
     assert need > 0 and varlen(flags=flags, total=640, ws=FAKE, wsb=need - 1) == WORKSPACE

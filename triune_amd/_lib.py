@@ -201,7 +201,7 @@ def _bind(lib):
         "triune_hip_decay_attn_bwd_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _i], _sz),
         "triune_hip_decay_attn_bwd": (
             [_vp, _vp, _vp, _vp, _vp, _i, _i, _i64p, _f, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i64, _i64, _i64,
-             _i64, _i64, _i, _vp, _sz, _vp],
+             _i64, _i64, _i, _vp, _sz, _vp, _sz, _vp],
             _i,
         ),
         "triune_hip_decay_attn_decode_step": (

@@ -50,8 +50,9 @@ DecayPlan plan_dense(int64_t n_seqs, int64_t T, int64_t H, int64_t Dk, int64_t D
     if (!p.seg) {
         int64_t n = chip_slots(Dk, Dv) / blocks;
         if (n > T / least_segment(Dk, Dv)) n = T / least_segment(Dk, Dv);
-        p.seg = n < 2 ? whole : round_up((T + n - 1) / n, DECAY_CHUNK);
+        p.seg = n < 2 ? whole : (T + n - 1) / n;
     }
+    p.seg = round_up(p.seg, 64);  // whole chunks of the gradients
     if (p.seg > whole) p.seg = whole;
     p.nseg = (T + p.seg - 1) / p.seg;
     p.n_work = n_seqs * p.nseg;
@@ -76,29 +77,27 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
     return p;
 }
 
-// Gradients: segments of whole chunks, the states of every chunk, and sums of shared heads and of constant gates.
+// Gradients: the forward's segments (its joined end states, formed again where they are not kept, and those of the
+// states' gradients), the states of every chunk, and sums of shared heads and of constant gates.
 struct GradPlan {
     DecayPlan p;
     int64_t chunk, nc;
-    size_t off_S, off_R, off_own, off_sum, off_seg, off_q, off_k, off_g, total;
+    size_t off_R_ends, off_S, off_R, off_cols, off_q, off_k, off_g, total;
 };
 
 GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int io_dtype, int g_head,
                    int flags) {
     GradPlan r{};
+    r.p = plan_dense(B, T, H, Dk, Dv, flags);
     r.chunk = decay_grad_chunk(io_dtype == TRIUNE_DT_BF16);
     r.nc = (T + r.chunk - 1) / r.chunk;
-    r.p = plan_dense(B, T, H, Dk, Dv, flags);
-    r.p.seg = round_up(r.p.seg, r.chunk);
-    r.p.nseg = (T + r.p.seg - 1) / r.p.seg;
-    r.p.n_work = B * r.p.nseg;
-    const size_t state = (size_t)decay_state_values((int)Dk, (int)Dv) * 4, heads = (size_t)(B * H);
+    const size_t heads = (size_t)(B * H), states = align_up(heads * r.nc * decay_state_values((int)Dk, (int)Dv) * 4);
     const size_t shared = H > Hk ? align_up((size_t)(B * T * H) * Dk * 4) : 0;
-    r.off_R = r.off_S + align_up(heads * r.nc * state);
-    r.off_own = r.off_R + align_up(heads * r.nc * state);
-    r.off_sum = r.off_own + align_up(heads * state);
-    r.off_seg = r.off_sum + align_up(heads * r.nc * 16);
-    r.off_q = r.off_seg + align_up(heads * r.p.nseg * 8);
+    r.off_R_ends = r.p.total;
+    r.off_S = r.off_R_ends + r.p.total;
+    r.off_R = r.off_S + states;
+    r.off_cols = r.off_R + states;
+    r.off_q = r.off_cols + states;
     r.off_k = r.off_q + shared;
     r.off_g = r.off_k + shared;
     r.total = r.off_g + (g_head ? align_up(heads * r.nc * 4) : 0);
@@ -112,7 +111,7 @@ bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t
 }
 
 bool grad_grids_ok(const GradPlan& r, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv) {
-    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 256) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
+    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 512) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
 }
 
 void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -135,7 +134,7 @@ void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk,
 
 int run_attn(const DecayParams& a, int nseg, int io_dtype, hipStream_t s) {
     if (nseg > 1) {
-        if (const int e = status(launch_decay_ends(a, io_dtype, s))) return e;
+        if (const int e = status(launch_decay_ends(a, false, io_dtype, s))) return e;
     }
     return status(launch_decay_attn(a, io_dtype, s));
 }
@@ -242,7 +241,8 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
                               int io_dtype, int g_dtype, const int64_t* strides, float scale, const float* s0,
                               const float* ds_final, void* dq, void* dk, void* dv, void* dg, int g_head, float* ds0,
                               int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int flags,
-                              void* workspace, size_t workspace_bytes, void* stream) {
+                              const void* fwd_workspace, size_t fwd_workspace_bytes, void* workspace,
+                              size_t workspace_bytes, void* stream) {
     if (!q || !k || !v || !g || !dout || !strides || !dq || !dk || !dv || !dg) return TRIUNE_ERR_NULL;
     if (!dtype_ok(io_dtype) || (g_dtype != io_dtype && g_dtype != TRIUNE_DT_F32)) return TRIUNE_ERR_DTYPE;
     if (B <= 0 || T <= 0 || !tokens_ok(B, T) || !decay_shape_ok(H, Hk, Dk, Dv) || !seqs_ok(B, H, Dv))
@@ -252,6 +252,8 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
         return TRIUNE_ERR_LAYOUT;
     const GradPlan r = plan_grad(B, T, H, Hk, Dk, Dv, io_dtype, g_head, flags);
     if (!grad_grids_ok(r, B, T, H, Hk, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (fwd_workspace)
+        if (const int e = check_ws(fwd_workspace, fwd_workspace_bytes, r.p.total)) return e;
     if (const int e = check_ws(workspace, workspace_bytes, r.total)) return e;
     char* ws = (char*)workspace;
     const hipStream_t s = (hipStream_t)stream;
@@ -264,20 +266,22 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
     a.o = {dout, strides[12], strides[13], strides[14]};
     a.g_dt = g_dtype, a.scale = scale;
     set_sizes(a, B, T, H, Hk, Dk, Dv, r.p, ws);
-    p.S = (float*)(ws + r.off_S), p.R = (float*)(ws + r.off_R), p.nc = r.nc;
+    p.S = (float*)(ws + r.off_S), p.R = (float*)(ws + r.off_R), p.R_cols = (uint32_t*)(ws + r.off_cols);
+    p.nc = r.nc, p.wide = a.slices * decay_slice((int)Dv);
     p.dq = dq, p.dk = dk, p.dv = dv, p.dg = dg;
     if (H > Hk) p.part_q = (float*)(ws + r.off_q), p.part_k = (float*)(ws + r.off_k);
     if (g_head) p.part_g = (float*)(ws + r.off_g);
-    p.sum_S = (float*)(ws + r.off_sum), p.sum_R = p.sum_S + 2 * B * H * r.nc, p.per = r.p.seg / r.chunk;
-    p.wide = a.slices * decay_slice((int)Dv);
-    // the segments' sums are formed by each walk
-    a.ws_sum = (float*)(ws + r.off_seg);
     for (const bool rev : {false, true}) {
-        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), (float*)(rev ? p.sum_R : p.sum_S), (float*)(ws + r.off_own),
-                          (int)r.chunk};
+        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), rev ? (uint32_t*)p.R_cols : nullptr, (int)r.chunk};
         x.f.s0 = rev ? ds_final : s0;
         x.f.fin = rev ? ds0 : nullptr;
         if (rev) x.f.k = a.q, x.f.v = a.o;
+        if (r.p.nseg > 1) {
+            x.f.ws_state = (float*)(!rev && fwd_workspace ? (char*)fwd_workspace : ws + (rev ? r.off_R_ends : 0));
+            x.f.ws_sum = (float*)((char*)x.f.ws_state + r.p.off_sum);
+            if (rev || !fwd_workspace)
+                if (const int e = status(launch_decay_ends(x.f, rev, io_dtype, s))) return e;
+        }
         if (const int e = status(launch_decay_states(x, rev, io_dtype, s))) return e;
     }
     return status(launch_decay_grad(p, io_dtype, s));

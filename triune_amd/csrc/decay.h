@@ -50,24 +50,15 @@ inline bool decay_full(int Dk, int Dv, int io_dt, std::initializer_list<DecayTok
     return true;
 }
 
-// Segments' end states and what the join makes of them, in the workspace.
-hipError_t launch_decay_ends(const DecayParams& a, int io_dt, hipStream_t s);
+// Segments' end states and what the join makes of them, in the workspace; rev: gradients of states, from the end.
+hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStream_t s);
 
 // The states in front of every chunk; rev: the gradients of those behind them.
 struct DecayWalkParams {
     DecayParams f;            // rows in k, columns in v
-    float* states;            // [n_seqs, H, nc, values], nc = ceil(T / every)
-    float* sums;              // [n_seqs, H, nc, 2]: log2 decay from the segment's first place
-    float* own;               // [n_seqs, H, values]: f.fin of the walk's last segment, before the join
+    float* states;            // [n_seqs, H, nc, DK, columns], nc = ceil(T / every)
+    uint32_t* columns;        // rev: the same values by columns, [columns / 16][K step][parts][lane][16 bytes]
     int every;                // a multiple of 32 tokens; segments are multiples of it
-};
-struct DecayCarryParams {
-    DecayParams f;
-    float *states, *own;      // as above, or null: the end states in f.ws_state
-    int every;
-    int64_t nc, values;
-    int dk;                   // rows of a state
-    bool rev;
 };
 hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
 hipError_t launch_decay_attn(const DecayParams& a, int io_dt, hipStream_t s);
@@ -77,9 +68,9 @@ constexpr int decay_grad_chunk(bool bf16) { return bf16 ? 64 : 32; }
 
 struct DecayGradParams {
     DecayParams f;            // o: the gradient of the outputs
-    // states in front of the chunks and gradients of those behind them, and their sums (DecayWalkParams)
-    const float *S, *R, *sum_S, *sum_R;
-    int64_t per, wide;        // chunks of a segment; columns of a state as kept
+    const float *S, *R;       // states in front of the chunks, gradients of those behind them (DecayWalkParams)
+    const uint32_t* R_cols;
+    int64_t wide;             // columns of a state as kept
     int64_t nc;               // chunks of a sequence
     void *dq, *dk, *dv;       // contiguous, I/O dtype
     float *part_q, *part_k;   // [n_seqs T, H, Dk] where heads share q and k, else null

@@ -52,41 +52,37 @@ __device__ __forceinline__ float row_suffix_scan(float x) {
 
 }  // namespace
 
-// The state of a place: what is kept there plus, decayed, what its segment's first place holds.  Through buffer resources,
-// whose scalar offsets step through the values (64-bit addresses for each would take two registers apiece and spill).
+// A state through a buffer resource, whose scalar offset steps through the values (64-bit addresses for each would take
+// two registers apiece and spill).
 struct StateAt {
-    __amdgpu_buffer_rsrc_t own, first;
-    float f;
-    __device__ __forceinline__ StateAt(const float* p, int64_t to_first, float f, int64_t values) : f(f) {
-        const int bytes = (int)(values * 4);
-        own = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), (short)0, bytes, 0x00020000);
-        first = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p + to_first), (short)0, bytes, 0x00020000);
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ StateAt(const void* p, int64_t values)
+        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)(values * 4), 0x00020000)) {}
+    // 16 bytes at byte offsets of the lane and of all lanes
+    __device__ __forceinline__ f32x4 at(int lane, int all) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane, all, 0));
     }
-    // E consecutive values, at byte offsets of the lane and of all lanes
     template <int E>
     __device__ __forceinline__ void row(int lane, int all, float (&x)[E]) const {
 #pragma unroll
         for (int i = 0; i < E; i += 4) {
-            const f32x4 a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(own, lane + 4 * i, all, 0));
-            const f32x4 b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(first, lane + 4 * i, all, 0));
+            const f32x4 v = at(lane + 4 * i, all);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[i + e] = __builtin_fmaf(f, b[e], a[e]);
+            for (int e = 0; e < 4; ++e) x[i + e] = v[e];
         }
-    }
-    __device__ __forceinline__ float one(int lane, int all) const {
-        const float a = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(own, lane, all, 0));
-        const float b = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(first, lane, all, 0));
-        return __builtin_fmaf(f, b, a);
     }
 };
 
 template <typename TIO, typename TC, int DK, int DVW, int NW, bool FULL>
-__global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams p) {
+__global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams p) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, CH = decay_grad_chunk(E == 8), CT = CH / 16, TJ = CH / KS;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(DVW), RC = tile_stride<TC>(CH), NTH = NW * 64;
     constexpr int TILES = CT * (CT + 1) / 2, MT = (TILES + NW - 1) / NW, NP = E == 8 ? 2 : 1, PL = CH * RC;
-    constexpr int NDK = DK / 16 < NW ? 1 : DK / 16 / NW, NDV = DVW / 16 < NW ? 1 : DVW / 16 / NW;
+    // a wave owns one tile of dims, for all 16-token tiles of the chunk or where there are waves enough a share of them
+    constexpr int TK = DK / 16, HK = NW / TK < CT ? NW / TK : CT, CTK = CT / HK;
+    constexpr int TV = DVW / 16, HV = NW / TV < CT ? NW / TV : CT, CTV = CT / HV;
+    static_assert(TK <= NW && TV <= NW, "a tile of dims for a wave");
     using Frag = typename Mat<TC>::Frag;
     __shared__ __attribute__((aligned(16))) TC s_q[CH * RK], s_k[CH * RK], s_v[CH * RV], s_d[CH * RV];
     __shared__ __attribute__((aligned(16))) TC s_A[NP * PL];  // A, then B
@@ -98,12 +94,7 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
     const int rows = (int)min((int64_t)CH, a.T - t0), hk = h / a.per;
     const int wide = (int)p.wide;
     const int64_t values = (int64_t)DK * wide, place = (seq * a.H + h) * p.nc + c;
-    // places that hold what their own segment made, and the segment's first place (its last one for R)
-    const int64_t c0 = c / p.per * p.per, c1 = min(c0 + p.per, p.nc) - 1;
-    const bool joinS = c0 > 0 && c > c0, joinR = c1 + 1 < p.nc && c < c1;
-    auto factor = [&](const float* sums) { return __builtin_amdgcn_exp2f(sums[2 * place] + sums[2 * place + 1]); };
-    const StateAt S(p.S + place * values, joinS ? (c0 - c) * values : 0, joinS ? factor(p.sum_S) : 0.f, values);
-    const StateAt R(p.R + place * values, joinR ? (c1 - c) * values : 0, joinR ? factor(p.sum_R) : 0.f, values);
+    const StateAt S(p.S + place * values, values), R(p.R + place * values, values), Rc(p.R_cols + place * values, values);
     auto at = [&](const DecayTok& t, int head) { return seq * t.sb + t0 * t.st + head * t.sh; };
 
     const TIO *pv = (const TIO*)a.v.p + at(a.v, h), *pd = (const TIO*)a.o.p + at(a.o, h);
@@ -115,12 +106,12 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
         tv.put(s_v);
         td.put(s_d);
     };
-    Tile<TIO, TC, CH, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
-    tq.fetch((const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
-    tk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
+    Tile<TIO, TC, CH, DK, NTH, FULL> fq(a.q.st, a.Dk), fk(a.k.st, a.Dk);
+    fq.fetch((const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
+    fk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
     fetch_values(0, [&] {
-        tq.put(s_q);
-        tk.put(s_k);
+        fq.put(s_q);
+        fk.put(s_k);
     });
     if (w == 0) {
         const Sum2 gs = chunk_sums<CH>(a.g, a.g_dt, at(a.g, h), rows, lane);
@@ -157,15 +148,35 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
         put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
     }
 
-    f32x4 dq[NDK][CT], dk[NDK][CT];
+    const int tk = w % TK, Ik = w / TK * CTK, tv = w % TV, Jv = w / TV * CTV;
+    const bool ownsK = w < TK * HK, ownsV = w < TV * HV;
+    f32x4 dq[CTK], dk[CTK];
 #pragma unroll
-    for (int d = 0; d < NDK; ++d)
-#pragma unroll
-        for (int I = 0; I < CT; ++I) dq[d][I] = dk[d][I] = zero4();
+    for (int I = 0; I < CTK; ++I) dq[I] = dk[I] = zero4();
     float z = 0.f;
     for (int col0 = 0; col0 < a.Dv; col0 += DVW) {
         if (col0) fetch_values(col0, [] { __syncthreads(); });
         __syncthreads();
+        if (ownsK) {
+            const int off = 4 * (n * wide + E * g);
+#pragma unroll
+            for (int s = 0; s < DVW / KS; ++s) {
+                float xs[E], xr[E];
+                S.row<E>(off, 4 * (16 * tk * wide + col0 + s * KS), xs);
+                R.row<E>(off, 4 * (16 * tk * wide + col0 + s * KS), xr);
+                if (Ik == 0) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[e], xr[e], z);
+                }
+                const auto ps = parts<TC, 3>(xs);
+                const auto pr = parts<TC, 3>(xr);
+#pragma unroll
+                for (int I = 0; I < CTK; ++I) {
+                    dq[I] = mma<TC>(ps, row_frag(s_d, RV, 16 * (Ik + I) + n, s, g), dq[I]);
+                    dk[I] = mma<TC>(pr, row_frag(s_v, RV, 16 * (Ik + I) + n, s, g), dk[I]);
+                }
+            }
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int idx = w + NW * m;
@@ -176,58 +187,33 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
             for (int s = 0; s < DVW / KS; ++s)
                 bm[m] = Mat<TC>::mma(row_frag(s_v, RV, 16 * J + n, s, g), row_frag(s_d, RV, 16 * I + n, s, g), bm[m]);
         }
+        if (ownsV) {
+            f32x4 dv[CTV];
 #pragma unroll
-        for (int d = 0; d < NDK; ++d) {
-            const int t = w * NDK + d;
-            if (t >= DK / 16) continue;
-            const int off = 4 * (n * wide + E * g);
-#pragma unroll
-            for (int s = 0; s < DVW / KS; ++s) {
-                float xs[E], xr[E];
-                S.row<E>(off, 4 * (16 * t * wide + col0 + s * KS), xs);
-                R.row<E>(off, 4 * (16 * t * wide + col0 + s * KS), xr);
-#pragma unroll
-                for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[e], xr[e], z);
-                const auto ps = parts<TC, 3>(xs);
-                const auto pr = parts<TC, 3>(xr);
-#pragma unroll
-                for (int I = 0; I < CT; ++I) {
-                    dq[d][I] = mma<TC>(ps, row_frag(s_d, RV, 16 * I + n, s, g), dq[d][I]);
-                    dk[d][I] = mma<TC>(pr, row_frag(s_v, RV, 16 * I + n, s, g), dk[d][I]);
-                }
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < NDV; ++d) {
-            const int t = w * NDV + d;
-            if (t >= DVW / 16) continue;
-            f32x4 dv[CT];
-#pragma unroll
-            for (int J = 0; J < CT; ++J) dv[J] = zero4();
+            for (int J = 0; J < CTV; ++J) dv[J] = zero4();
 #pragma unroll
             for (int s = 0; s < DK / KS; ++s) {
-                float xr[E];
+                Parts<TC, NP> pr;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    xr[e] = R.one(4 * (E * g * wide + n), 4 * ((s * KS + e) * wide + col0 + 16 * t));
-                const auto pr = parts<TC, 3>(xr);
+                for (int b = 0; b < NP; ++b)
+                    pr.p[b] = __builtin_bit_cast(Frag, Rc.at(16 * lane, 64 * DK * (col0 / 16 + tv) + 64 * KS * s + 1024 * b));
 #pragma unroll
-                for (int J = 0; J < CT; ++J) dv[J] = mma<TC>(pr, row_frag(s_k, RK, 16 * J + n, s, g), dv[J]);
+                for (int J = 0; J < CTV; ++J) dv[J] = mma<TC>(pr, row_frag(s_k, RK, 16 * (Jv + J) + n, s, g), dv[J]);
             }
 #pragma unroll
-            for (int J = 0; J < CT; ++J) {
-                const int j = 16 * J + n;
+            for (int J = 0; J < CTV; ++J) {
+                const int j = 16 * (Jv + J) + n;
                 dv[J] *= decay_between(end, sum_at(j));
-#pragma unroll
-                for (int s = 16 * J / KS; s < TJ; ++s) {
-                    const Frag x = col_frag<TC, false>(s_d, RV, t, s, g, n);
+                for (int s = 16 * (Jv + J) / KS; s < TJ; ++s) {
+                    const Frag x = col_frag<TC, false>(s_d, RV, tv, s, g, n);
 #pragma unroll
                     for (int b = NP - 1; b >= 0; --b)
-                        dv[J] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, J, s, g, n), dv[J]);
+                        dv[J] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, Jv + J, s, g, n), dv[J]);
                 }
-                const int dim = col0 + 16 * t + 4 * g;
+                const int dim = col0 + 16 * tv + 4 * g;
                 const float o[4] = {dv[J][0], dv[J][1], dv[J][2], dv[J][3]};
-                if (j < rows) store_raw<4>((TIO*)p.dv + ((seq * a.T + t0 + j) * a.H + h) * a.Dv + dim, a.Dv - dim, o);
+                if (j < rows && dim < a.Dv)
+                    store_raw<4>((TIO*)p.dv + ((seq * a.T + t0 + j) * a.H + h) * a.Dv + dim, FULL ? 4 : a.Dv - dim, o);
             }
         }
     }
@@ -274,59 +260,52 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
     }
     __syncthreads();
 
-    float xs[CT], ys[CT];
+    for (int t = lane; t < CH; t += 64) s_x[w][t] = s_y[w][t] = 0.f;
+    if (ownsK) {
+        const int dim = 16 * tk + 4 * g;
 #pragma unroll
-    for (int I = 0; I < CT; ++I) xs[I] = ys[I] = 0.f;
-#pragma unroll
-    for (int d = 0; d < NDK; ++d) {
-        const int t = w * NDK + d;
-        if (t >= DK / 16) continue;
-        const int dim = 16 * t + 4 * g;
-#pragma unroll
-        for (int I = 0; I < CT; ++I) {
-            const int i = 16 * I + n;
+        for (int u = 0; u < CTK; ++u) {
+            const int I = Ik + u, i = 16 * I + n;
             const Sum2 Gi = sum_at(i);
-            const float fq = a.scale * __builtin_amdgcn_exp2f(Gi.hi + Gi.lo), fk = decay_between(end, Gi);
+            const float eq = a.scale * __builtin_amdgcn_exp2f(Gi.hi + Gi.lo), ek = decay_between(end, Gi);
+            float x = 0.f, y = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                dq[d][I][r] *= fq;
-                dk[d][I][r] *= fk;
-                xs[I] = __builtin_fmaf((float)s_q[i * RK + dim + r], dq[d][I][r], xs[I]);
-                ys[I] = __builtin_fmaf((float)s_k[i * RK + dim + r], dk[d][I][r], ys[I]);
+                dq[u][r] *= eq;
+                dk[u][r] *= ek;
+                x = __builtin_fmaf((float)s_q[i * RK + dim + r], dq[u][r], x);
+                y = __builtin_fmaf((float)s_k[i * RK + dim + r], dk[u][r], y);
             }
-#pragma unroll
+            x = xor_sum<32>(xor_sum<16>(x));
+            y = xor_sum<32>(xor_sum<16>(y));
+            if (g == 0) s_x[w][i] = x, s_y[w][i] = y;
             for (int s = 0; s <= (16 * I + 15) / KS; ++s) {
-                const Frag x = col_frag<TC, false>(s_k, RK, t, s, g, n);
+                const Frag f = col_frag<TC, false>(s_k, RK, tk, s, g, n);
 #pragma unroll
                 for (int b = NP - 1; b >= 0; --b)
-                    dq[d][I] = Mat<TC>::mma(x, row_frag_tok(s_A + b * PL, RC, i, s, g), dq[d][I]);
+                    dq[u] = Mat<TC>::mma(f, row_frag_tok(s_A + b * PL, RC, i, s, g), dq[u]);
             }
-#pragma unroll
             for (int s = 16 * I / KS; s < TJ; ++s) {
-                const Frag x = col_frag<TC, false>(s_q, RK, t, s, g, n);
+                const Frag f = col_frag<TC, false>(s_q, RK, tk, s, g, n);
 #pragma unroll
                 for (int b = NP - 1; b >= 0; --b)
-                    dk[d][I] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, I, s, g, n), dk[d][I]);
+                    dk[u] = Mat<TC>::mma(f, col_frag<TC, false>(s_A + b * PL, RC, I, s, g, n), dk[u]);
             }
-            if (i >= rows) continue;
-            const float oq[4] = {dq[d][I][0], dq[d][I][1], dq[d][I][2], dq[d][I][3]};
-            const float ok[4] = {dk[d][I][0], dk[d][I][1], dk[d][I][2], dk[d][I][3]};
+            if (i >= rows || dim >= a.Dk) continue;
+            const float oq[4] = {dq[u][0], dq[u][1], dq[u][2], dq[u][3]};
+            const float ok[4] = {dk[u][0], dk[u][1], dk[u][2], dk[u][3]};
             const int64_t tok = seq * a.T + t0 + i;
+            const int left = FULL ? 4 : a.Dk - dim;
             if (p.part_q) {  // of one head of several that share q and k
                 const int64_t off = (tok * a.H + h) * a.Dk + dim;
-                store_raw<4>(p.part_q + off, a.Dk - dim, oq);
-                store_raw<4>(p.part_k + off, a.Dk - dim, ok);
+                store_raw<4>(p.part_q + off, left, oq);
+                store_raw<4>(p.part_k + off, left, ok);
             } else {
                 const int64_t off = (tok * (a.H / a.per) + hk) * a.Dk + dim;
-                store_raw<4>((TIO*)p.dq + off, a.Dk - dim, oq);
-                store_raw<4>((TIO*)p.dk + off, a.Dk - dim, ok);
+                store_raw<4>((TIO*)p.dq + off, left, oq);
+                store_raw<4>((TIO*)p.dk + off, left, ok);
             }
         }
-    }
-#pragma unroll
-    for (int I = 0; I < CT; ++I) {
-        const float x = xor_sum<32>(xor_sum<16>(xs[I])), y = xor_sum<32>(xor_sum<16>(ys[I]));
-        if (g == 0) s_x[w][16 * I + n] = x, s_y[w][16 * I + n] = y;
     }
     z = xor_sum<16>(xor_sum<32>(dpp_sum16(z)));
     if (lane == 0) s_z[w] = z;
@@ -401,8 +380,8 @@ namespace {
 template <typename TIO, typename TC, int DK, int DVW>
 void grad_one(const DecayGradParams& p, bool full, hipStream_t s) {
     const dim3 grid((unsigned)(p.f.n_seqs * p.nc * p.f.H));
-    if (full) decay_grad_kernel<TIO, TC, DK, DVW, 4, true><<<grid, 256, 0, s>>>(p);
-    else decay_grad_kernel<TIO, TC, DK, DVW, 4, false><<<grid, 256, 0, s>>>(p);
+    if (full) decay_grad_kernel<TIO, TC, DK, DVW, 8, true><<<grid, 512, 0, s>>>(p);
+    else decay_grad_kernel<TIO, TC, DK, DVW, 8, false><<<grid, 512, 0, s>>>(p);
 }
 template <typename TIO, typename TC, int DK>
 void grad_width(const DecayGradParams& p, bool full, hipStream_t s) {

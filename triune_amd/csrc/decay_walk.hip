@@ -8,11 +8,9 @@ constexpr int C = DECAY_CHUNK;
 // States alone, from rows (a.k) by columns (a.v), REV: from the end of the sequence (gradients of states, whose rows are q
 // and whose columns are do):
 //     S <- e^{G_C} S + sum_j e^{G_C - G_j} k_j v_j^T,   R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
-// The first segment of a walk starts from a.s0, the others from zero, and decay_carry_kernel adds what comes in.
-// EACH false: the segments' own end states, in the order of the lanes, of those that another one follows.
-// EACH true: the state in front of (REV: behind) every chunk of p.every tokens, in `states`, [DK][columns] each.  A
-// segment leaves its own end state in the next one's first place, and that one's later places hold what its own tokens
-// made: whoever reads them adds the first place's state, decayed by `sums`.
+// EACH false: the segments' own end states of those that another one follows, the first one's from a.s0, in the
+// workspace in the order of the lanes; decay_carry_kernel joins them.
+// EACH true: from the joined states the state in front of (REV: behind) every chunk of p.every tokens, and the final one.
 template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV, bool EACH>
 __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams p) {
     const DecayParams& a = p.f;
@@ -44,8 +42,13 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
     };
     if (chunks) fetch(0);
 
+    auto ws = [&](int64_t item) {
+        return a.ws_state + (item * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
+    };
     f32x4 S[NT][DT];
-    if (begins && a.s0) {
+    if (EACH && !begins) {
+        get_state(S, ws(REV ? x.w + 1 : x.w - 1));
+    } else if (begins && a.s0) {
         each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
             v = in && srow >= 0 ? a.s0[soff + off] : 0.f;
         });
@@ -54,23 +57,33 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
     }
     // The last segment of a cut sequence has no use for its place in the workspace: it takes the initial state, since
     // s0 may be the pool that the last segment's outputs leave their state in while the first one starts.
-    auto ws = [&](int64_t item) {
-        return a.ws_state + (item * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
-    };
-    if (!EACH && begins) put_state(S, ws(x.last));
+    if (!EACH && !REV && begins) put_state(S, ws(x.last));
     const int64_t nc = EACH ? (a.T + p.every - 1) / p.every : 0;
-    auto keep_at = [&](int64_t c, const Sum2& sum) {
+    auto keep_at = [&](int64_t c) {
         const int64_t at = (x.seg.seq * a.H + x.h) * nc + c;
         float* to = p.states + at * values;
         each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
-        if (x.slice == 0 && threadIdx.x == 0) p.sums[2 * at] = sum.hi, p.sums[2 * at + 1] = sum.lo;
+        if constexpr (REV) {  // and as operands of the products with k, whose K index is the key dim
+            uint32_t* cols = p.columns + at * values + (x.slice * (WIDTH / 16) + w * NT) * (DK * 16) + lane * 4;
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int k = 0; k < DK / KS; ++k) {
+                    float e[E];
+                    acc_slots<TC>(S[c], k, e);
+                    const auto q = parts<TC, 2>(e);
+#pragma unroll
+                    for (int i = 0; i < (E == 8 ? 2 : 1); ++i)
+                        *reinterpret_cast<Frag*>(cols + c * (DK * 16) + k * (KS * 16) + i * 256) = q.p[i];
+                }
+        }
     };
 
     Sum2 all{0.f, 0.f};
     for (int i = 0; i < chunks; ++i) {
         const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
         const int64_t at = x.seg.t0 + t0;
-        if (EACH && (i ? (REV ? at + C : at) % p.every == 0 : begins)) keep_at(at / p.every, all);
+        if (EACH && (REV ? (at + C) % p.every == 0 || at + rows == a.T : at % p.every == 0)) keep_at(at / p.every);
         TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
         tk.put(s_k);
         tv.put(s_v);
@@ -106,53 +119,35 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
         }
     }
 
-    float* sum = a.ws_sum + (x.w * a.H + x.h) * 2;
-    if (a.ws_sum && x.slice == 0 && threadIdx.x == 0) sum[0] = all.hi, sum[1] = all.lo;
     if constexpr (!EACH) {
         put_state(S, ws(x.w));
-    } else if (!ends) {
-        keep_at(REV ? x.seg.t0 / p.every - 1 : (x.seg.t0 + a.seg) / p.every, Sum2{0.f, 0.f});
-    } else if (a.fin) {
-        if (begins) {
-            each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
-                if (in) a.fin[soff + off] = v;
-            });
-        } else {  // the carry completes it
-            float* to = p.own + (x.seg.seq * a.H + x.h) * values;
-            each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
-        }
+        float* sum = a.ws_sum + (x.w * a.H + x.h) * 2;
+        if (x.slice == 0 && threadIdx.x == 0) sum[0] = all.hi, sum[1] = all.lo;
+    } else if (ends && a.fin) {
+        each_state<TC>(S, col0, a.Dk, a.Dv, a.Dv, [&](float& v, int64_t off, bool in) {
+            if (in) a.fin[soff + off] = v;
+        });
     }
 }
 
 // Joins the segments' end states in place: S_p = 2^{sum_p} S_{p-1} + own_p, p = 1 .. n - 2 in the walk's direction, with S_0
 // the first segment's own; the state in front of segment p + 1 is then S_p.  A thread per four values of a (sequence,
 // head), with the next states and sums in flight.
-__global__ __launch_bounds__(256) void decay_carry_kernel(DecayCarryParams p) {
-    const DecayParams& a = p.f;
-    const uint32_t blocks = (uint32_t)((p.values + 1023) / 1024);
+__global__ __launch_bounds__(256) void decay_carry_kernel(DecayParams a, int64_t values, bool rev) {
+    const uint32_t blocks = (uint32_t)((values + 1023) / 1024);
     const uint32_t sh = blockIdx.x / blocks, seq = sh / (uint32_t)a.H, h = sh - seq * (uint32_t)a.H;
     const int64_t i = (int64_t)(blockIdx.x - sh * blocks) * 1024 + threadIdx.x * 4;
-    if (i >= p.values) return;
+    if (i >= values) return;
     int64_t first = (int64_t)seq * a.nseg, n = a.nseg;
     if (a.cu) {
         first = a.seg_off[seq];
         n = a.seg_off[seq + 1] - first;
     }
-    const int64_t own = p.own ? 1 : 0;  // one more join, into the final state
-    if (n + own < 3) return;
-    float* s0;
-    int64_t step;
-    if (p.states) {  // the place in front of the walk's second segment, and those of the following ones
-        const int64_t per = a.seg / p.every, at = p.rev ? (n - 1) * per - 1 : per;
-        s0 = p.states + ((int64_t)sh * p.nc + at) * p.values + i;
-        step = (p.rev ? -per : per) * p.values;
-    } else {
-        s0 = a.ws_state + (first * a.H + h) * p.values + i;
-        step = a.H * p.values;
-    }
-    // sums of segment k of the walk
-    const float* sum0 = a.ws_sum + ((first + (p.rev ? n - 1 : 0)) * a.H + h) * 2;
-    const int64_t sum_step = (p.rev ? -2 : 2) * a.H;
+    if (n < 3) return;  // one state to carry: the first segment's own
+    if (rev) first += n - 1;
+    float* s0 = a.ws_state + (first * a.H + h) * values + i;
+    const float* sum0 = a.ws_sum + (first * a.H + h) * 2;  // sums of the walk's first segment
+    const int64_t step = rev ? -a.H * values : a.H * values, sum_step = rev ? -2 * a.H : 2 * a.H;
     const int joins = (int)(n - 2);
     f32x4 s = *reinterpret_cast<const f32x4*>(s0);
     constexpr int AHEAD = 8;
@@ -181,16 +176,6 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(DecayCarryParams p) {
                 *reinterpret_cast<f32x4*>(s0 + (k0 + k) * step) = s;
             }
     }
-    if (own) {
-        const float f = __builtin_amdgcn_exp2f(sum0[(n - 1) * sum_step] + sum0[(n - 1) * sum_step + 1]);
-        const f32x4 end = *reinterpret_cast<const f32x4*>(p.own + sh * p.values + i);
-        const int64_t wide = p.values / p.dk, r = i / wide, c = i - r * wide;
-        if (r >= a.Dk) return;
-        float* to = a.fin + ((int64_t)sh * a.Dk + r) * a.Dv + c;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < a.Dv) to[e] = __builtin_fmaf(f, s[e], end[e]);
-    }
 }
 
 namespace {
@@ -206,28 +191,25 @@ struct Walks {
     };
 };
 
-hipError_t carry(const DecayCarryParams& p, hipStream_t s) {
-    decay_carry_kernel<<<dim3((unsigned)(p.f.n_seqs * p.f.H * ((p.values + 1023) / 1024))), 256, 0, s>>>(p);
-    return hipGetLastError();
+template <bool EACH>
+hipError_t walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
+    const DecayParams& a = p.f;
+    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v});
+    return rev ? decay_by_type<Walks<true, EACH>::template Of>(p, a, io_dt, full, s)
+               : decay_by_type<Walks<false, EACH>::template Of>(p, a, io_dt, full, s);
 }
 
 }  // namespace
 
-hipError_t launch_decay_ends(const DecayParams& a, int io_dt, hipStream_t s) {
-    const DecayWalkParams p{a, nullptr, nullptr, nullptr, 0};
-    const hipError_t e = decay_by_type<Walks<false, false>::Of>(p, a, io_dt, decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v}), s);
+hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStream_t s) {
+    const hipError_t e = walk<false>(DecayWalkParams{a, nullptr, nullptr, 0}, rev, io_dt, s);
     if (e != hipSuccess) return e;
-    return carry(DecayCarryParams{a, nullptr, nullptr, 0, 0, decay_state_values(a.Dk, a.Dv), 0, false}, s);
+    const int64_t values = decay_state_values(a.Dk, a.Dv);
+    decay_carry_kernel<<<dim3((unsigned)(a.n_seqs * a.H * ((values + 1023) / 1024))), 256, 0, s>>>(a, values, rev);
+    return hipGetLastError();
 }
-
 hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
-    const DecayParams& a = p.f;
-    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v});
-    const hipError_t e = rev ? decay_by_type<Walks<true, true>::Of>(p, a, io_dt, full, s)
-                             : decay_by_type<Walks<false, true>::Of>(p, a, io_dt, full, s);
-    if (e != hipSuccess || a.nseg < 2) return e;
-    return carry(DecayCarryParams{a, p.states, rev && a.fin ? p.own : nullptr, p.every, (a.T + p.every - 1) / p.every,
-                                  decay_state_values(a.Dk, a.Dv), decay_padded_dk(a.Dk), rev}, s);
+    return walk<true>(p, rev, io_dt, s);
 }
 
 }  // namespace triune

@@ -87,7 +87,7 @@ def _initial(s0, like, shape):
 
 
 def _attn(q, k, v, g, scale, s0, out, flags=0):
-    """(o, final state) of a dense call with B, T > 0."""
+    """(o, final state, workspace or None) of a dense call with B, T > 0."""
     B, T, H, Dv = v.shape
     Hk, Dk = q.shape[2:]
     q, k, v = _rows(q), _rows(k), _rows(v)
@@ -98,7 +98,7 @@ def _attn(q, k, v, g, scale, s0, out, flags=0):
     st = strides(*(_head_strides(x) for x in (q, k, v)), _head_strides(g, 3), _head_strides(o))
     call_on(q, "triune_hip_decay_attn", ptr(q), ptr(k), ptr(v), ptr(g), dtype_code(q), dtype_code(g), st, scale, ptr(s0),
             ptr(o), ptr(fin), B, T, H, Hk, Dk, Dv, flags, ptr(ws), wsb)
-    return o, fin
+    return o, fin, ws
 
 
 def _no_tokens(q, H, Dv, s0):
@@ -108,7 +108,7 @@ def _no_tokens(q, H, Dv, s0):
     return s0.to(torch.float32).clone()
 
 
-def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0):
+def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0, kept=None):
     B, T, H, Dv = v.shape
     Hk, Dk = q.shape[2:]
     dev, f32 = q.device, torch.float32
@@ -124,22 +124,23 @@ def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0):
     ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
     st = strides(*(_head_strides(x) for x in (q, k, v)), _head_strides(g, 3), _head_strides(do))
     call_on(q, "triune_hip_decay_attn_bwd", ptr(q), ptr(k), ptr(v), ptr(g), ptr(do), dtype_code(q), dtype_code(g), st, scale,
-            ptr(s0), ptr(dfin), ptr(dq), ptr(dk), ptr(dv), ptr(dg), head, ptr(ds0), B, T, H, Hk, Dk, Dv, flags, ptr(ws), wsb)
+            ptr(s0), ptr(dfin), ptr(dq), ptr(dk), ptr(dv), ptr(dg), head, ptr(ds0), B, T, H, Hk, Dk, Dv, flags, ptr(kept),
+            0 if kept is None else kept.numel(), ptr(ws), wsb)
     return dq, dk, dv, dg, ds0
 
 
 class _DecayAttn(torch.autograd.Function):
-    """decay_attn with gradients.  The backward forms the states of every 64th token again, so nothing is kept
-    but the inputs."""
+    """decay_attn with gradients.  The forward keeps the states of its segments (none of short calls); the backward forms
+    those of every 64th token from them."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, s0, scale):
         s0f = None if s0 is None else s0.to(torch.float32).contiguous()
         if q.shape[0] == 0 or q.shape[1] == 0:
-            o, fin = torch.empty(v.shape, device=v.device, dtype=v.dtype), _no_tokens(q, *v.shape[2:], s0f)
+            o, fin, kept = torch.empty(v.shape, device=v.device, dtype=v.dtype), _no_tokens(q, *v.shape[2:], s0f), None
         else:
-            o, fin = _attn(q, k, v, g, scale, s0f, None)
-        ctx.save_for_backward(q, k, v, g, s0)
+            o, fin, kept = _attn(q, k, v, g, scale, s0f, None)
+        ctx.save_for_backward(q, k, v, g, s0, kept)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, fin
@@ -147,7 +148,7 @@ class _DecayAttn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, dfin):
-        q, k, v, g, s0 = ctx.saved_tensors
+        q, k, v, g, s0, kept = ctx.saved_tensors
         if do is None and dfin is None:
             return (None,) * 6
         want = s0 is not None and ctx.needs_input_grad[4]
@@ -155,7 +156,7 @@ class _DecayAttn(torch.autograd.Function):
             zero = [torch.zeros_like(t) for t in (q, k, v, g)]
             return (*zero, dfin.to(s0.dtype) if want and dfin is not None else None, None)
         s0f = None if s0 is None else s0.to(torch.float32).contiguous()
-        dq, dk, dv, dg, ds0 = _attn_bwd(q, k, v, g, ctx.scale, s0f, do, dfin, want)
+        dq, dk, dv, dg, ds0 = _attn_bwd(q, k, v, g, ctx.scale, s0f, do, dfin, want, kept=kept)
         return dq, dk, dv, dg, ds0.to(s0.dtype) if want else None, None
 
 
@@ -180,7 +181,7 @@ def decay_attn(q, k, v, g, initial_state=None, scale=1.0, out=None):
     s0 = _initial(initial_state, q, (B, H, Dk, Dv))
     if B == 0 or T == 0:  # nothing to read: the final state is the initial state
         return _out(out, v), _no_tokens(q, H, Dv, s0)
-    return _attn(q, k, v, g, float(scale), s0, out)
+    return _attn(q, k, v, g, float(scale), s0, out)[:2]
 
 
 def decay_attn_varlen(q, k, v, g, cu_seqlens, initial_state=None, scale=1.0, out=None, *, state_pool=None, slots=None):
