@@ -82,7 +82,7 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
 struct GradPlan {
     DecayPlan p;
     int64_t chunk, nc;
-    size_t off_R_ends, off_S, off_R, off_cols, off_q, off_k, off_g, total;
+    size_t off_R_ends, off_S, off_R, off_q, off_k, off_g, total;
 };
 
 GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int io_dtype, int g_head,
@@ -96,8 +96,7 @@ GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int6
     r.off_R_ends = r.p.total;
     r.off_S = r.off_R_ends + r.p.total;
     r.off_R = r.off_S + states;
-    r.off_cols = r.off_R + states;
-    r.off_q = r.off_cols + states;
+    r.off_q = r.off_R + states;
     r.off_k = r.off_q + shared;
     r.off_g = r.off_k + shared;
     r.total = r.off_g + (g_head ? align_up(heads * r.nc * 4) : 0);
@@ -266,13 +265,13 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
     a.o = {dout, strides[12], strides[13], strides[14]};
     a.g_dt = g_dtype, a.scale = scale;
     set_sizes(a, B, T, H, Hk, Dk, Dv, r.p, ws);
-    p.S = (float*)(ws + r.off_S), p.R = (float*)(ws + r.off_R), p.R_cols = (uint32_t*)(ws + r.off_cols);
+    p.S = (float*)(ws + r.off_S), p.R = (float*)(ws + r.off_R);
     p.nc = r.nc, p.wide = a.slices * decay_slice((int)Dv);
     p.dq = dq, p.dk = dk, p.dv = dv, p.dg = dg;
     if (H > Hk) p.part_q = (float*)(ws + r.off_q), p.part_k = (float*)(ws + r.off_k);
     if (g_head) p.part_g = (float*)(ws + r.off_g);
     for (const bool rev : {false, true}) {
-        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), rev ? (uint32_t*)p.R_cols : nullptr, (int)r.chunk};
+        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), (int)r.chunk};
         x.f.s0 = rev ? ds_final : s0;
         x.f.fin = rev ? ds0 : nullptr;
         if (rev) x.f.k = a.q, x.f.v = a.o;

@@ -57,7 +57,6 @@ hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStrea
 struct DecayWalkParams {
     DecayParams f;            // rows in k, columns in v
     float* states;            // [n_seqs, H, nc, DK, columns], nc = ceil(T / every)
-    uint32_t* columns;        // rev: the same values by columns, [columns / 16][K step][parts][lane][16 bytes]
     int every;                // a multiple of 32 tokens; segments are multiples of it
 };
 hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
@@ -69,7 +68,6 @@ constexpr int decay_grad_chunk(bool bf16) { return bf16 ? 64 : 32; }
 struct DecayGradParams {
     DecayParams f;            // o: the gradient of the outputs
     const float *S, *R;       // states in front of the chunks, gradients of those behind them (DecayWalkParams)
-    const uint32_t* R_cols;
     int64_t wide;             // columns of a state as kept
     int64_t nc;               // chunks of a sequence
     void *dq, *dk, *dv;       // contiguous, I/O dtype

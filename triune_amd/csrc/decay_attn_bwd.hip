@@ -12,8 +12,9 @@
 //
 // The states in front of the chunks and the gradients behind them come from two walks (decay_walk.hip), so a
 // workgroup takes one (chunk, head) by itself.  A and B are formed once, in tiles over the waves, and shared through
-// LDS, B in the place of A; a wave owns 16-wide tiles of key dims (dq, dk) and of value dims (dv), which are taken in
-// slices of 64, so a state is read once for each use and two workgroups fit a compute unit.
+// LDS, B in the place of A; a wave owns a 16-wide tile of key dims (dq, dk) and one of value dims (dv), which are taken in
+// slices of 32.  Its rows of S and R come from memory once, the products with k take R by columns from LDS (in q's place,
+// which is read again behind them), and two workgroups fit a compute unit.
 #include "decay_mfma.h"
 
 namespace triune {
@@ -73,46 +74,62 @@ struct StateAt {
     }
 };
 
-template <typename TIO, typename TC, int DK, int DVW, int NW, bool FULL>
-__global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams p) {
+template <typename TIO, typename TC, int DK, int NW, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams p) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, CH = decay_grad_chunk(E == 8), CT = CH / 16, TJ = CH / KS;
-    constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(DVW), RC = tile_stride<TC>(CH), NTH = NW * 64;
-    constexpr int TILES = CT * (CT + 1) / 2, MT = (TILES + NW - 1) / NW, NP = E == 8 ? 2 : 1, PL = CH * RC;
-    // a wave owns one tile of dims, for all 16-token tiles of the chunk or where there are waves enough a share of them
-    constexpr int TK = DK / 16, HK = NW / TK < CT ? NW / TK : CT, CTK = CT / HK;
+    constexpr int DVW = 32, RK = tile_stride<TC>(DK), RV = tile_stride<TC>(DVW), RC = tile_stride<TC>(CH), NTH = NW * 64;
+    constexpr int TILES = CT * (CT + 1) / 2, MT = (TILES + NW - 1) / NW, NP = E == 8 ? 2 : 1, PL = CH * RC, PR = DK * DVW;
+    // a wave owns NDK tiles of key dims and one of value dims, for all 16-token tiles of the chunk or where there are waves
+    // enough a share of them
+    constexpr int TK = DK / 16, NDK = TK > NW ? TK / NW : 1, HK = TK > NW ? 1 : NW / TK < CT ? NW / TK : CT, CTK = CT / HK;
     constexpr int TV = DVW / 16, HV = NW / TV < CT ? NW / TV : CT, CTV = CT / HV;
-    static_assert(TK <= NW && TV <= NW, "a tile of dims for a wave");
+    static_assert(TV <= NW && TK % NDK == 0, "tiles of dims for a wave");
+    static_assert(NP * PR <= CH * RK, "R's planes take q's place");
     using Frag = typename Mat<TC>::Frag;
     __shared__ __attribute__((aligned(16))) TC s_q[CH * RK], s_k[CH * RK], s_v[CH * RV], s_d[CH * RV];
     __shared__ __attribute__((aligned(16))) TC s_A[NP * PL];  // A, then B
     __shared__ float s_g[2][CH], s_x[NW][CH], s_y[NW][CH], s_z[NW];
     __shared__ float s_r[TILES][16], s_c[TILES][16], s_tot[TILES], s_diag[CT][16];
+    TC* const s_R = s_q;  // between A and the last steps: a slice of R, [DK][DVW] in parts
     const int lane = threadIdx.x & 63, w = wave_index(), g = lane >> 4, n = lane & 15;
-    const int h = (int)(blockIdx.x % a.H);
-    const int64_t sc = blockIdx.x / a.H, seq = sc / p.nc, c = sc - seq * p.nc, t0 = c * CH;
+    const int h = (int)(blockIdx.x % (uint32_t)a.H);
+    const uint32_t sc = blockIdx.x / (uint32_t)a.H, seq32 = sc / (uint32_t)p.nc;
+    const int64_t seq = seq32, c = sc - seq32 * (uint32_t)p.nc, t0 = c * CH;
     const int rows = (int)min((int64_t)CH, a.T - t0), hk = h / a.per;
     const int wide = (int)p.wide;
     const int64_t values = (int64_t)DK * wide, place = (seq * a.H + h) * p.nc + c;
-    const StateAt S(p.S + place * values, values), R(p.R + place * values, values), Rc(p.R_cols + place * values, values);
+    const StateAt S(p.S + place * values, values), R(p.R + place * values, values);
     auto at = [&](const DecayTok& t, int head) { return seq * t.sb + t0 * t.st + head * t.sh; };
 
+    constexpr int UK = TK / NDK;  // waves that share the key dims
+    const int tk = w % UK * NDK, Ik = w / UK * CTK, tv = w % TV, Jv = w / TV * CTV;
+    const bool ownsK = w < UK * HK, ownsV = w < TV * HV;
+    // a slice of 32 value dims: v, do, and the wave's rows of the states, in flight while the one before is worked on
     const TIO *pv = (const TIO*)a.v.p + at(a.v, h), *pd = (const TIO*)a.o.p + at(a.o, h);
-    auto fetch_values = [&](int col0, auto&& between) {
-        Tile<TIO, TC, CH, DVW, NTH, FULL> tv(a.v.st, a.Dv - col0), td(a.o.st, a.Dv - col0);
-        tv.fetch(pv + col0, a.v.st, rows, a.Dv - col0);
-        td.fetch(pd + col0, a.o.st, rows, a.Dv - col0);
-        between();
-        tv.put(s_v);
-        td.put(s_d);
+    Tile<TIO, TC, CH, DVW, NTH, FULL> fv(a.v.st, DVW), fd(a.o.st, DVW);
+    constexpr int NS = DVW / KS;
+    float xs[NDK * NS][E], xr[NDK * NS][E];
+    auto fetch = [&](int col0) {
+        fv.fetch(pv + col0, a.v.st, rows, a.Dv - col0);
+        fd.fetch(pd + col0, a.o.st, rows, a.Dv - col0);
+#pragma unroll
+        for (int i = 0; i < NDK * NS; ++i) {
+            const int all = 4 * (16 * (tk + i / NS) * wide + col0 + i % NS * KS);
+            S.row<E>(4 * (n * wide + E * g), all, xs[i]);
+            R.row<E>(4 * (n * wide + E * g), all, xr[i]);
+        }
     };
-    Tile<TIO, TC, CH, DK, NTH, FULL> fq(a.q.st, a.Dk), fk(a.k.st, a.Dk);
-    fq.fetch((const TIO*)a.q.p + at(a.q, hk), a.q.st, rows, a.Dk);
-    fk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
-    fetch_values(0, [&] {
+    Tile<TIO, TC, CH, DK, NTH, FULL> fq(a.q.st, a.Dk);
+    const TIO* pq = (const TIO*)a.q.p + at(a.q, hk);
+    {
+        Tile<TIO, TC, CH, DK, NTH, FULL> fk(a.k.st, a.Dk);
+        fq.fetch(pq, a.q.st, rows, a.Dk);
+        fk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
+        fetch(0);
         fq.put(s_q);
         fk.put(s_k);
-    });
+    }
     if (w == 0) {
         const Sum2 gs = chunk_sums<CH>(a.g, a.g_dt, at(a.g, h), rows, lane);
         if (lane < CH) s_g[0][lane] = gs.hi, s_g[1][lane] = gs.lo;
@@ -123,14 +140,23 @@ __global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams 
             *reinterpret_cast<uint2*>(s_A + b * PL + (16 * I + row) * RC + 16 * (I + 1) + 4 * q) = uint2{0, 0};
         }
     }
-    __syncthreads();
+    lds_barrier();
     auto sum_at = [&](int t) { return Sum2{s_g[0][t], s_g[1][t]}; };
     const Sum2 end = sum_at(CH - 1);
 
-    f32x4 am[MT], bm[MT], dec[MT];
+    // scale e^{G_i - G_j} of a tile's value, 0 above the diagonal (whose products may be anything)
+    auto weighed = [&](const f32x4& x, int I, int J) {
+        const Sum2 Gi = sum_at(16 * I + n);
+        f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            y[r] = J < I || 4 * g + r <= n ? x[r] * (a.scale * decay_between(Gi, sum_at(16 * J + 4 * g + r))) : 0.f;
+        return y;
+    };
+    f32x4 am[MT], bm[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-        am[m] = bm[m] = dec[m] = zero4();
+        am[m] = bm[m] = zero4();
         const int idx = w + NW * m;
         if (idx >= TILES) continue;
         int I, J;
@@ -138,45 +164,46 @@ __global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams 
 #pragma unroll
         for (int s = 0; s < DK / KS; ++s)
             am[m] = Mat<TC>::mma(row_frag(s_k, RK, 16 * J + n, s, g), row_frag(s_q, RK, 16 * I + n, s, g), am[m]);
-        const Sum2 Gi = sum_at(16 * I + n);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            dec[m][r] = J < I || 4 * g + r <= n ? a.scale * decay_between(Gi, sum_at(16 * J + 4 * g + r)) : 0.f;
-        f32x4 x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = J < I || 4 * g + r <= n ? am[m][r] * dec[m][r] : 0.f;
-        put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
+        put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, weighed(am[m], I, J));
     }
 
-    const int tk = w % TK, Ik = w / TK * CTK, tv = w % TV, Jv = w / TV * CTV;
-    const bool ownsK = w < TK * HK, ownsV = w < TV * HV;
-    f32x4 dq[CTK], dk[CTK];
+    f32x4 dq[NDK][CTK], dk[NDK][CTK];
 #pragma unroll
-    for (int I = 0; I < CTK; ++I) dq[I] = dk[I] = zero4();
+    for (int d = 0; d < NDK; ++d)
+#pragma unroll
+        for (int I = 0; I < CTK; ++I) dq[d][I] = dk[d][I] = zero4();
     float z = 0.f;
     for (int col0 = 0; col0 < a.Dv; col0 += DVW) {
-        if (col0) fetch_values(col0, [] { __syncthreads(); });
-        __syncthreads();
+        lds_barrier();
+        fv.put(s_v, a.Dv - col0);
+        fd.put(s_d, a.Dv - col0);
+        if (ownsK && Ik == 0) {
+#pragma unroll
+            for (int i = 0; i < NDK * NS; ++i) {
+                const auto r = parts<TC, 2>(xr[i]);
+#pragma unroll
+                for (int b = 0; b < NP; ++b)
+                    *reinterpret_cast<Frag*>(s_R + b * PR + (16 * (tk + i / NS) + n) * DVW + i % NS * KS + E * g) = r.p[b];
+#pragma unroll
+                for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[i][e], xr[i][e], z);
+            }
+        }
+        lds_barrier();
         if (ownsK) {
-            const int off = 4 * (n * wide + E * g);
 #pragma unroll
-            for (int s = 0; s < DVW / KS; ++s) {
-                float xs[E], xr[E];
-                S.row<E>(off, 4 * (16 * tk * wide + col0 + s * KS), xs);
-                R.row<E>(off, 4 * (16 * tk * wide + col0 + s * KS), xr);
-                if (Ik == 0) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[e], xr[e], z);
-                }
-                const auto ps = parts<TC, 3>(xs);
-                const auto pr = parts<TC, 3>(xr);
+            for (int i = 0; i < NDK * NS; ++i) {
+                const int d = i / NS, s = i % NS;
+                const auto ps = parts<TC, 3>(xs[i]);
+                const auto pr = parts<TC, 3>(xr[i]);
 #pragma unroll
                 for (int I = 0; I < CTK; ++I) {
-                    dq[I] = mma<TC>(ps, row_frag(s_d, RV, 16 * (Ik + I) + n, s, g), dq[I]);
-                    dk[I] = mma<TC>(pr, row_frag(s_v, RV, 16 * (Ik + I) + n, s, g), dk[I]);
+                    dq[d][I] = mma<TC>(ps, row_frag(s_d, RV, 16 * (Ik + I) + n, s, g), dq[d][I]);
+                    dk[d][I] = mma<TC>(pr, row_frag(s_v, RV, 16 * (Ik + I) + n, s, g), dk[d][I]);
                 }
             }
         }
+        if (col0 + DVW < a.Dv) fetch(col0 + DVW);
+        else fq.fetch(pq, a.q.st, rows, a.Dk);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int idx = w + NW * m;
@@ -188,30 +215,26 @@ __global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams 
                 bm[m] = Mat<TC>::mma(row_frag(s_v, RV, 16 * J + n, s, g), row_frag(s_d, RV, 16 * I + n, s, g), bm[m]);
         }
         if (ownsV) {
-            f32x4 dv[CTV];
 #pragma unroll
-            for (int J = 0; J < CTV; ++J) dv[J] = zero4();
+            for (int u = 0; u < CTV; ++u) {
+                const int J = Jv + u, j = 16 * J + n;
+                f32x4 dv = zero4();
 #pragma unroll
-            for (int s = 0; s < DK / KS; ++s) {
-                Parts<TC, NP> pr;
+                for (int s = 0; s < DK / KS; ++s) {
+                    const Frag x = row_frag_tok(s_k, RK, j, s, g);
 #pragma unroll
-                for (int b = 0; b < NP; ++b)
-                    pr.p[b] = __builtin_bit_cast(Frag, Rc.at(16 * lane, 64 * DK * (col0 / 16 + tv) + 64 * KS * s + 1024 * b));
-#pragma unroll
-                for (int J = 0; J < CTV; ++J) dv[J] = mma<TC>(pr, row_frag(s_k, RK, 16 * (Jv + J) + n, s, g), dv[J]);
-            }
-#pragma unroll
-            for (int J = 0; J < CTV; ++J) {
-                const int j = 16 * (Jv + J) + n;
-                dv[J] *= decay_between(end, sum_at(j));
-                for (int s = 16 * (Jv + J) / KS; s < TJ; ++s) {
+                    for (int b = NP - 1; b >= 0; --b)
+                        dv = Mat<TC>::mma(col_frag<TC, false>(s_R + b * PR, DVW, tv, s, g, n), x, dv);
+                }
+                dv *= decay_between(end, sum_at(j));
+                for (int s = 16 * J / KS; s < TJ; ++s) {
                     const Frag x = col_frag<TC, false>(s_d, RV, tv, s, g, n);
 #pragma unroll
                     for (int b = NP - 1; b >= 0; --b)
-                        dv[J] = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, Jv + J, s, g, n), dv[J]);
+                        dv = Mat<TC>::mma(x, col_frag<TC, false>(s_A + b * PL, RC, J, s, g, n), dv);
                 }
                 const int dim = col0 + 16 * tv + 4 * g;
-                const float o[4] = {dv[J][0], dv[J][1], dv[J][2], dv[J][3]};
+                const float o[4] = {dv[0], dv[1], dv[2], dv[3]};
                 if (j < rows && dim < a.Dv)
                     store_raw<4>((TIO*)p.dv + ((seq * a.T + t0 + j) * a.H + h) * a.Dv + dim, FULL ? 4 : a.Dv - dim, o);
             }
@@ -219,19 +242,18 @@ __global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams 
     }
 
     // B, and the sums of (q . k) B over its tiles that the gates' gradients take
-    __syncthreads();
+    lds_barrier();
+    fq.put(s_q);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
         const int idx = w + NW * m;
         if (idx >= TILES) continue;
         int I, J;
         tile_of(idx, I, J);
-        f32x4 x, M;
+        const f32x4 x = weighed(bm[m], I, J);
+        f32x4 M;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            x[r] = J < I || 4 * g + r <= n ? bm[m][r] * dec[m][r] : 0.f;
-            M[r] = J < I || 4 * g + r < n ? am[m][r] * x[r] : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) M[r] = J < I || 4 * g + r < n ? am[m][r] * x[r] : 0.f;
         put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, x);
         if (J < I) {
             float col = (M[0] + M[1]) + (M[2] + M[3]);
@@ -258,53 +280,56 @@ __global__ __launch_bounds__(NW * 64, 4) void decay_grad_kernel(DecayGradParams 
             }
         }
     }
-    __syncthreads();
+    lds_barrier();
 
     for (int t = lane; t < CH; t += 64) s_x[w][t] = s_y[w][t] = 0.f;
     if (ownsK) {
-        const int dim = 16 * tk + 4 * g;
 #pragma unroll
         for (int u = 0; u < CTK; ++u) {
             const int I = Ik + u, i = 16 * I + n;
             const Sum2 Gi = sum_at(i);
             const float eq = a.scale * __builtin_amdgcn_exp2f(Gi.hi + Gi.lo), ek = decay_between(end, Gi);
+            const int64_t tok = seq * a.T + t0 + i;
             float x = 0.f, y = 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                dq[u][r] *= eq;
-                dk[u][r] *= ek;
-                x = __builtin_fmaf((float)s_q[i * RK + dim + r], dq[u][r], x);
-                y = __builtin_fmaf((float)s_k[i * RK + dim + r], dk[u][r], y);
+            for (int d = 0; d < NDK; ++d) {
+                const int dim = 16 * (tk + d) + 4 * g;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    dq[d][u][r] *= eq;
+                    dk[d][u][r] *= ek;
+                    x = __builtin_fmaf((float)s_q[i * RK + dim + r], dq[d][u][r], x);
+                    y = __builtin_fmaf((float)s_k[i * RK + dim + r], dk[d][u][r], y);
+                }
+                for (int s = 0; s <= (16 * I + 15) / KS; ++s) {
+                    const Frag f = col_frag<TC, false>(s_k, RK, tk + d, s, g, n);
+#pragma unroll
+                    for (int b = NP - 1; b >= 0; --b)
+                        dq[d][u] = Mat<TC>::mma(f, row_frag_tok(s_A + b * PL, RC, i, s, g), dq[d][u]);
+                }
+                for (int s = 16 * I / KS; s < TJ; ++s) {
+                    const Frag f = col_frag<TC, false>(s_q, RK, tk + d, s, g, n);
+#pragma unroll
+                    for (int b = NP - 1; b >= 0; --b)
+                        dk[d][u] = Mat<TC>::mma(f, col_frag<TC, false>(s_A + b * PL, RC, I, s, g, n), dk[d][u]);
+                }
+                if (i >= rows || dim >= a.Dk) continue;
+                const float oq[4] = {dq[d][u][0], dq[d][u][1], dq[d][u][2], dq[d][u][3]};
+                const float ok[4] = {dk[d][u][0], dk[d][u][1], dk[d][u][2], dk[d][u][3]};
+                const int left = FULL ? 4 : a.Dk - dim;
+                if (p.part_q) {  // of one head of several that share q and k
+                    const int64_t off = (tok * a.H + h) * a.Dk + dim;
+                    store_raw<4>(p.part_q + off, left, oq);
+                    store_raw<4>(p.part_k + off, left, ok);
+                } else {
+                    const int64_t off = (tok * (a.H / a.per) + hk) * a.Dk + dim;
+                    store_raw<4>((TIO*)p.dq + off, left, oq);
+                    store_raw<4>((TIO*)p.dk + off, left, ok);
+                }
             }
             x = xor_sum<32>(xor_sum<16>(x));
             y = xor_sum<32>(xor_sum<16>(y));
             if (g == 0) s_x[w][i] = x, s_y[w][i] = y;
-            for (int s = 0; s <= (16 * I + 15) / KS; ++s) {
-                const Frag f = col_frag<TC, false>(s_k, RK, tk, s, g, n);
-#pragma unroll
-                for (int b = NP - 1; b >= 0; --b)
-                    dq[u] = Mat<TC>::mma(f, row_frag_tok(s_A + b * PL, RC, i, s, g), dq[u]);
-            }
-            for (int s = 16 * I / KS; s < TJ; ++s) {
-                const Frag f = col_frag<TC, false>(s_q, RK, tk, s, g, n);
-#pragma unroll
-                for (int b = NP - 1; b >= 0; --b)
-                    dk[u] = Mat<TC>::mma(f, col_frag<TC, false>(s_A + b * PL, RC, I, s, g, n), dk[u]);
-            }
-            if (i >= rows || dim >= a.Dk) continue;
-            const float oq[4] = {dq[u][0], dq[u][1], dq[u][2], dq[u][3]};
-            const float ok[4] = {dk[u][0], dk[u][1], dk[u][2], dk[u][3]};
-            const int64_t tok = seq * a.T + t0 + i;
-            const int left = FULL ? 4 : a.Dk - dim;
-            if (p.part_q) {  // of one head of several that share q and k
-                const int64_t off = (tok * a.H + h) * a.Dk + dim;
-                store_raw<4>(p.part_q + off, left, oq);
-                store_raw<4>(p.part_k + off, left, ok);
-            } else {
-                const int64_t off = (tok * (a.H / a.per) + hk) * a.Dk + dim;
-                store_raw<4>((TIO*)p.dq + off, left, oq);
-                store_raw<4>((TIO*)p.dk + off, left, ok);
-            }
         }
     }
     z = xor_sum<16>(xor_sum<32>(dpp_sum16(z)));
@@ -377,23 +402,18 @@ __global__ __launch_bounds__(1024) void decay_gate_kernel(DecayGradParams p, int
 
 namespace {
 
-template <typename TIO, typename TC, int DK, int DVW>
+template <typename TIO, typename TC, int DK>
 void grad_one(const DecayGradParams& p, bool full, hipStream_t s) {
     const dim3 grid((unsigned)(p.f.n_seqs * p.nc * p.f.H));
-    if (full) decay_grad_kernel<TIO, TC, DK, DVW, 8, true><<<grid, 512, 0, s>>>(p);
-    else decay_grad_kernel<TIO, TC, DK, DVW, 8, false><<<grid, 512, 0, s>>>(p);
-}
-template <typename TIO, typename TC, int DK>
-void grad_width(const DecayGradParams& p, bool full, hipStream_t s) {
-    if (p.f.Dv <= 32) grad_one<TIO, TC, DK, 32>(p, full, s);
-    else grad_one<TIO, TC, DK, 64>(p, full, s);
+    if (full) decay_grad_kernel<TIO, TC, DK, 4, true><<<grid, 256, 0, s>>>(p);
+    else decay_grad_kernel<TIO, TC, DK, 4, false><<<grid, 256, 0, s>>>(p);
 }
 template <typename TIO, typename TC>
 hipError_t grad_dk(const DecayGradParams& p, bool full, hipStream_t s) {
     switch (decay_padded_dk(p.f.Dk)) {
-        case 32: grad_width<TIO, TC, 32>(p, full, s); break;
-        case 64: grad_width<TIO, TC, 64>(p, full, s); break;
-        default: grad_width<TIO, TC, 128>(p, full, s);
+        case 32: grad_one<TIO, TC, 32>(p, full, s); break;
+        case 64: grad_one<TIO, TC, 64>(p, full, s); break;
+        default: grad_one<TIO, TC, 128>(p, full, s);
     }
     return hipGetLastError();
 }

@@ -168,10 +168,12 @@ struct Tile {
             }
         }
     }
-    __device__ __forceinline__ void put(TC* tile) const {
+    // left: columns of the tile inside the tensor, for a Tile that moves over its columns
+    __device__ __forceinline__ void put(TC* tile, int left = D) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (N % NTH && row_of(i) >= ROWS) continue;
+            if (FULL && left < D && col_of(i) >= left) x[i] = Raw<TIO, E>{};
             TC* to = tile + row_of(i) * tile_stride<TC>(D) + col_of(i);
             if constexpr (std::is_same<TIO, TC>::value) {
                 *reinterpret_cast<typename Mat<TC>::Frag*>(to) = __builtin_bit_cast(typename Mat<TC>::Frag, x[i]);

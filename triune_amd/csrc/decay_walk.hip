@@ -63,20 +63,6 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
         const int64_t at = (x.seg.seq * a.H + x.h) * nc + c;
         float* to = p.states + at * values;
         each_state<TC>(S, col0, DK, (int)wide, wide, [&](float& v, int64_t off, bool) { to[off] = v; });
-        if constexpr (REV) {  // and as operands of the products with k, whose K index is the key dim
-            uint32_t* cols = p.columns + at * values + (x.slice * (WIDTH / 16) + w * NT) * (DK * 16) + lane * 4;
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-                for (int k = 0; k < DK / KS; ++k) {
-                    float e[E];
-                    acc_slots<TC>(S[c], k, e);
-                    const auto q = parts<TC, 2>(e);
-#pragma unroll
-                    for (int i = 0; i < (E == 8 ? 2 : 1); ++i)
-                        *reinterpret_cast<Frag*>(cols + c * (DK * 16) + k * (KS * 16) + i * 256) = q.p[i];
-                }
-        }
     };
 
     Sum2 all{0.f, 0.f};
@@ -202,7 +188,7 @@ hipError_t walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStream_t s) {
-    const hipError_t e = walk<false>(DecayWalkParams{a, nullptr, nullptr, 0}, rev, io_dt, s);
+    const hipError_t e = walk<false>(DecayWalkParams{a, nullptr, 0}, rev, io_dt, s);
     if (e != hipSuccess) return e;
     const int64_t values = decay_state_values(a.Dk, a.Dv);
     decay_carry_kernel<<<dim3((unsigned)(a.n_seqs * a.H * ((values + 1023) / 1024))), 256, 0, s>>>(a, values, rev);
