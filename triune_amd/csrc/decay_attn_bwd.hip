@@ -167,6 +167,20 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
         put4<TC, NP>(s_A, PL, (16 * I + n) * RC + 16 * J + 4 * g, weighed(am[m], I, J));
     }
 
+    // The wave's columns of R's slice; rows 4 to 7 of eight have their halves swapped, since rows without padding would meet
+    // on the banks there.
+    auto R_cols = [&](int b, int s) {
+        if constexpr (E == 8) {
+            const int row = 32 * s + 4 * g + (n >> 2), col = 16 * tv + 4 * (n & 3);
+            const TC* x = s_R + b * PR + row * DVW + (col ^ ((g & 1) << 4));
+            const bf16x4 lo = lds_read_tr(x), hi = lds_read_tr(x + 16 * DVW);
+            return Frag{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        } else {
+            const TC* x = s_R + (16 * s + 4 * g) * DVW + ((16 * tv + n) ^ ((g & 1) << 4));
+            return Frag{x[0], x[DVW], x[2 * DVW], x[3 * DVW]};
+        }
+    };
+
     f32x4 dq[NDK][CTK], dk[NDK][CTK];
 #pragma unroll
     for (int d = 0; d < NDK; ++d)
@@ -183,7 +197,8 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
                 const auto r = parts<TC, 2>(xr[i]);
 #pragma unroll
                 for (int b = 0; b < NP; ++b)
-                    *reinterpret_cast<Frag*>(s_R + b * PR + (16 * (tk + i / NS) + n) * DVW + i % NS * KS + E * g) = r.p[b];
+                    *reinterpret_cast<Frag*>(s_R + b * PR + (16 * (tk + i / NS) + n) * DVW +
+                                             ((i % NS * KS + E * g) ^ ((n & 4) << 2))) = r.p[b];
 #pragma unroll
                 for (int e = 0; e < E; ++e) z = __builtin_fmaf(xs[i][e], xr[i][e], z);
             }
@@ -224,7 +239,7 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
                     const Frag x = row_frag_tok(s_k, RK, j, s, g);
 #pragma unroll
                     for (int b = NP - 1; b >= 0; --b)
-                        dv = Mat<TC>::mma(col_frag<TC, false>(s_R + b * PR, DVW, tv, s, g, n), x, dv);
+                        dv = Mat<TC>::mma(R_cols(b, s), x, dv);
                 }
                 dv *= decay_between(end, sum_at(j));
                 for (int s = 16 * J / KS; s < TJ; ++s) {

@@ -78,10 +78,12 @@ __device__ __forceinline__ int tile_dim(int t, int m) {
     else return 16 * t + m;
 }
 
-// A row of an LDS tile with D values: one 16-byte unit of padding spreads rows over the banks.
+// A row of an LDS tile with D values, padded so that rows fall on other banks.  bf16: by 32 bytes, so that the eight rows by
+// two units of a cycle of ds_read_b128 and the eight rows by four of a transposed read both fill the banks; fp32, whose
+// columns are read value by value: by 16 bytes, so that the four rows of a read do.
 template <typename TC>
 constexpr int tile_stride(int D) {
-    return D + 16 / (int)sizeof(TC);
+    return D + (sizeof(TC) == 2 ? 16 : 4);
 }
 
 // K step s of row `row`.
