@@ -48,7 +48,8 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
         get_state(S, a.ws_state + (from * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4);
     }
 
-    // a chunk's tiles go from registers to one of two places, and the next one's loads are issued
+    // A chunk's tiles go from registers to one of two places, and the next one's loads are issued; gates are loaded two chunks
+    // ahead and formed one ahead.
     Tile<TIO, TC, C, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
     Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
     GateBits tg;
@@ -57,9 +58,14 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
         tq.fetch(pq + t0 * a.q.st, a.q.st, rows, a.Dk);
         tk.fetch(pk + t0 * a.k.st, a.k.st, rows, a.Dk);
         tv.fetch(pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
-        tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
     };
-    if (x.seg.len) fetch(0);
+    auto fetch_gates = [&](int t0) { tg.fetch(a.g, a.g_dt, pg + min(t0 + (lane & (C - 1)), x.seg.len - 1) * a.g.st); };
+    if (x.seg.len) {
+        fetch_gates(0);
+        fetch(0);
+        if (w == NW - 1) s_gs[0].put(tg.value(a.g_dt), x.seg.len, lane);
+        fetch_gates(C);
+    }
     for (int t0 = 0; t0 < x.seg.len; t0 += C) {
         const int rows = min(C, x.seg.len - t0), place = t0 / C & 1;
         TC *s_q = s_qs[place], *s_k = s_ks[place], *s_v = s_vs[place];
@@ -67,9 +73,14 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
         tk.put(s_k);
         tv.put(s_v);
         ChunkGates& s_g = s_gs[place];
-        if (w == 0) s_g.put(tg.value(a.g_dt), rows, lane);
-        if (t0 + C < x.seg.len) fetch(t0 + C);
+        const GateBits gates = tg;
+        if (t0 + C < x.seg.len) {
+            fetch(t0 + C);
+            fetch_gates(t0 + 2 * C);
+        }
         lds_barrier();
+        // the next chunk's gates, by the waves in turn, beside the others' products
+        if (w == (t0 / C & (NW - 1))) s_gs[place ^ 1].put(gates.value(a.g_dt), x.seg.len - t0 - C, lane);
         Frag vf[NT][TJ];
 #pragma unroll
         for (int c = 0; c < NT; ++c)

@@ -31,16 +31,25 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
     const int64_t wide = (int64_t)WIDTH * a.slices, values = DK * wide;
 
     const int chunks = (x.seg.len + C - 1) / C;
+    // loads and gates ahead as in decay_attn_kernel
     Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st, a.Dk);
     Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
     GateBits tg;
+    auto first = [&](int i) { return (REV ? chunks - 1 - i : i) * C; };
     auto fetch = [&](int i) {
-        const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
+        const int t0 = first(i), rows = min(C, x.seg.len - t0);
         tk.fetch(pk + t0 * a.k.st, a.k.st, rows, a.Dk);
         tv.fetch(pv + t0 * a.v.st, a.v.st, rows, a.Dv - col0);
-        tg.fetch(a.g, a.g_dt, pg + (t0 + min(lane & (C - 1), rows - 1)) * a.g.st);
     };
-    if (chunks) fetch(0);
+    auto fetch_gates = [&](int i) {
+        tg.fetch(a.g, a.g_dt, pg + min(first(min(i, chunks - 1)) + (lane & (C - 1)), x.seg.len - 1) * a.g.st);
+    };
+    if (chunks) {
+        fetch_gates(0);
+        fetch(0);
+        if (w == NW - 1) s_gs[0].put(tg.value(a.g_dt), x.seg.len - first(0), lane);
+        fetch_gates(1);
+    }
 
     auto ws = [&](int64_t item) {
         return a.ws_state + (item * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4;
@@ -67,16 +76,21 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
 
     Sum2 all{0.f, 0.f};
     for (int i = 0; i < chunks; ++i) {
-        const int t0 = (REV ? chunks - 1 - i : i) * C, rows = min(C, x.seg.len - t0);
+        const int t0 = first(i), place = i & 1;
         const int64_t at = x.seg.t0 + t0;
-        if (EACH && (REV ? (at + C) % p.every == 0 || at + rows == a.T : at % p.every == 0)) keep_at(at / p.every);
-        TC *s_k = s_ks[i & 1], *s_v = s_vs[i & 1];
+        if (EACH && (REV ? (at + C) % p.every == 0 || at + min(C, x.seg.len - t0) == a.T : at % p.every == 0))
+            keep_at(at / p.every);
+        TC *s_k = s_ks[place], *s_v = s_vs[place];
         tk.put(s_k);
         tv.put(s_v);
-        ChunkGates& s_g = s_gs[i & 1];
-        if (w == 0) s_g.put(tg.value(a.g_dt), rows, lane);
-        if (i + 1 < chunks) fetch(i + 1);
+        ChunkGates& s_g = s_gs[place];
+        const GateBits gates = tg;
+        if (i + 1 < chunks) {
+            fetch(i + 1);
+            fetch_gates(i + 2);
+        }
         lds_barrier();
+        if (i + 1 < chunks && w == (i & (NW - 1))) s_gs[place ^ 1].put(gates.value(a.g_dt), x.seg.len - first(i + 1), lane);
         const float keep = s_g.from[C - 1];
         all.hi = fmaxf(all.hi + s_g.hi[C - 1], -1024.f);
         all.lo += s_g.lo[C - 1];
