@@ -189,15 +189,20 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
     });
 }
 
-// One token for every row: a block takes a (row, head), a thread V columns of every RG-th state row.
-template <typename TIO, int V>
+// One token for every row: a block takes a (row, head), a thread four columns of every RG-th state row.  Bound by the
+// state, read and written once, past the caches.  ALIGNED: rows of whole 16 bytes, eight of which a thread has in flight.
+template <typename TIO, bool ALIGNED>
 __global__ __launch_bounds__(256) void decay_step_kernel(DecayStepParams a, int lanes) {
+    constexpr int V = 4, ROWS = 8;
     __shared__ float s_q[DECAY_MAX_DK], s_k[DECAY_MAX_DK];
     __shared__ float s_o[256 * V];
-    const int64_t b = blockIdx.x / a.H;
-    const int h = (int)(blockIdx.x % a.H), hk = h / a.per;
+    const uint32_t b = blockIdx.x / (uint32_t)a.H;
+    const int h = (int)(blockIdx.x - b * (uint32_t)a.H), hk = h / a.per;
     const int cl = threadIdx.x & (lanes - 1), rg = threadIdx.x / lanes, RG = 256 / lanes;
     const int64_t row = ssm_row(a.slots, a.n_rows, b);
+    const int64_t off = (row * a.H + h) * a.Dk * a.Dv;
+    const float *from = a.s_in + off;
+    float* to = a.s_out + off;
     for (int d = threadIdx.x; d < a.Dk; d += 256) {
         s_q[d] = (float)((const TIO*)a.q.p)[b * a.q.sb + hk * a.q.sh + d];
         s_k[d] = (float)((const TIO*)a.k.p)[b * a.k.sb + hk * a.k.sh + d];
@@ -205,29 +210,50 @@ __global__ __launch_bounds__(256) void decay_step_kernel(DecayStepParams a, int 
     const float decay = __builtin_amdgcn_exp2f(log2_gate(load_dt(a.g.p, a.g_dt, b * a.g.sb + h * a.g.sh)));
     const TIO* pv = (const TIO*)a.v.p + b * a.v.sb + h * a.v.sh;
     TIO* po = (TIO*)a.o.p + b * a.o.sb + h * a.o.sh;
-    const int64_t off = (row * a.H + h) * a.Dk * a.Dv;
-    __syncthreads();
     for (int c0 = 0; c0 < a.Dv; c0 += lanes * V) {
         const int col = c0 + cl * V, left = a.Dv - col;
-        float o[V];
+        const bool in = row >= 0 && left > 0;
+        f32x4 x[ROWS], o = zero4();
+        // past the last row the last one again: no load stands behind a condition
+        auto fetch = [&](int d0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = 0.f;
-        if (row >= 0 && left > 0) {
-            float v[V];
-            const Raw<TIO, V> rv = load_raw<V>(pv + col, left);
+            for (int i = 0; i < ROWS; ++i) {
+                const float* p = from + (int64_t)min(d0 + i * RG, a.Dk - 1) * a.Dv + col;
+                if constexpr (ALIGNED) {
+                    x[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+                } else {
+                    const Raw<float, V> r = load_raw<V>(p, left);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = (float)rv.v[j];
-            for (int d = rg; d < a.Dk; d += RG) {
-                Raw<float, V> s = load_raw<V>(a.s_in + off + (int64_t)d * a.Dv + col, left);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    s.v[j] = __builtin_fmaf(decay, s.v[j], s_k[d] * v[j]);
-                    o[j] = __builtin_fmaf(s_q[d], s.v[j], o[j]);
+                    for (int j = 0; j < V; ++j) x[i][j] = r.v[j];
                 }
-                store_raw<V>(a.s_out + off + (int64_t)d * a.Dv + col, left, s);
+            }
+        };
+        if (in) fetch(rg);
+        Raw<TIO, V> rv = load_raw<V>(pv + (in ? col : 0), in ? left : 0);
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (float)rv.v[j];
+        __syncthreads();
+        if (in) {
+            for (int d0 = rg; d0 < a.Dk; d0 += ROWS * RG) {
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    const int d = d0 + i * RG;
+                    if (d >= a.Dk) continue;
+                    float y[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        y[j] = __builtin_fmaf(decay, x[i][j], s_k[d] * v[j]);
+                        o[j] = __builtin_fmaf(s_q[d], y[j], o[j]);
+                    }
+                    if constexpr (ALIGNED)
+                        __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]},
+                                                    reinterpret_cast<f32x4*>(to + (int64_t)d * a.Dv + col));
+                    else store_raw<V>(to + (int64_t)d * a.Dv + col, left, y);
+                }
+                if (d0 + ROWS * RG < a.Dk) fetch(d0 + ROWS * RG);
             }
         }
-        __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) s_o[(rg * lanes + cl) * V + j] = o[j];
         __syncthreads();
@@ -262,7 +288,9 @@ hipError_t run_step(const DecayStepParams& a, hipStream_t s) {
     const int need = (a.Dv + 3) / 4;
     int lanes = 4;
     while (lanes < need && lanes < 64) lanes *= 2;
-    decay_step_kernel<TIO, 4><<<grid, 256, 0, s>>>(a, lanes);
+    const auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if (a.Dv % 4 == 0 && whole(a.s_in) && whole(a.s_out)) decay_step_kernel<TIO, true><<<grid, 256, 0, s>>>(a, lanes);
+    else decay_step_kernel<TIO, false><<<grid, 256, 0, s>>>(a, lanes);
     return hipGetLastError();
 }
 
