@@ -67,17 +67,29 @@ __global__ __launch_bounds__(block_threads(TPR)) void gated_norm_bwd_kernel(RmsB
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[k][j] = 0.f;
     __syncthreads();
-    const int64_t step = (int64_t)gridDim.x * RPB;
-    for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; r < a.R; r += step) {
+    constexpr bool AHEAD = TPR <= 256 && K <= 3;  // the next row's loads in flight where its registers are free
+    Raw<T, 8> fx[K], fz[K], fy[K];
+    float frstd;
+    auto fetch = [&](int64_t r) {
         const T *px = row_ptr<T>(a.x, r, a.G), *pz = row_ptr<T>(a.z, r, a.G), *py = row_ptr<T>(g.dy, r, a.G);
-        Raw<T, 8> nx[K], nz[K], ny[K];
+        frstd = a.rstd[r];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            nx[k] = load_group<EIGHTS>(px, column<TPR>(t, k), a.D);
-            nz[k] = load_group<EIGHTS>(pz, column<TPR>(t, k), a.D);
-            ny[k] = load_group<EIGHTS>(py, column<TPR>(t, k), a.D);
+            fx[k] = load_group<EIGHTS>(px, column<TPR>(t, k), a.D);
+            fz[k] = load_group<EIGHTS>(pz, column<TPR>(t, k), a.D);
+            fy[k] = load_group<EIGHTS>(py, column<TPR>(t, k), a.D);
         }
-        const float rstd = a.rstd[r];
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (AHEAD && r < a.R) fetch(r);
+    for (; r < a.R; r += step) {
+        if constexpr (!AHEAD) fetch(r);
+        Raw<T, 8> nx[K], nz[K], ny[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) nx[k] = fx[k], nz[k] = fz[k], ny[k] = fy[k];
+        const float rstd = frstd;
+        if (AHEAD && r + step < a.R) fetch(r + step);
         float xh[K][8], d[K][8], dz[K][8], sum = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)

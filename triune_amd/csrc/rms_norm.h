@@ -50,7 +50,10 @@ int64_t rms_bwd_parts(int64_t R, int D, int cus);
 
 namespace rms {
 
-constexpr int FWD_BLOCKS = 8, BWD_BLOCKS = 2;  // blocks of 256 threads a compute unit
+// Blocks of 256 threads a compute unit.  The backward's parts of dw and ds grow with them, and rows of few threads leave
+// its waves short of loads (16384 rows of 1536, gradients and their sums, bf16: 71 us with two, 79 with three, 88 with
+// four; 98304 rows of 128, gated: 44, 38 and 37, 44 with six).
+constexpr int FWD_BLOCKS = 8, BWD_BLOCKS = 2, BWD_BLOCKS_NARROW = 4;
 constexpr int block_threads(int tpr) { return tpr <= 256 ? 256 : tpr; }
 // Rows that a block takes at once, by the width (see `by_width`).
 inline int rows_per_block(int D) {

@@ -78,33 +78,38 @@ __global__ __launch_bounds__(block_threads(TPR)) void rms_norm_bwd_kernel(RmsBwd
 #pragma unroll
         for (int j = 0; j < 8; ++j) dw[k][j] = ds[k][j] = 0.f;
     __syncthreads();
-    const int64_t step = (int64_t)gridDim.x * RPB;
-    for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; r < a.R; r += step) {
-        Raw<TH, 8> nh[K], nd[K];
-        Raw<T, 8> ny[K], nx[K];
-        const TH* ph = row_ptr<TH>(a.r, r, a.G);
-        const T* py = row_ptr<T>(g.dy, r, a.G);
+    // the next row's loads in flight where its registers are free; without dh or ds a row that is read anyway stands for
+    // theirs, so that no load stands behind a condition
+    constexpr bool AHEAD = TPR <= 256 && K <= 3;
+    const bool adds = g.dh.p;
+    const NormRows rows_d = adds ? g.dh : a.r, rows_x = g.ds ? a.x : g.dy;
+    Raw<TH, 8> fh[K], fd[K];
+    Raw<T, 8> fy[K], fx[K];
+    float frstd;
+    auto fetch = [&](int64_t r) {
+        const TH *ph = row_ptr<TH>(a.r, r, a.G), *pd = row_ptr<TH>(rows_d, r, a.G);
+        const T *py = row_ptr<T>(g.dy, r, a.G), *px = row_ptr<T>(rows_x, r, a.G);
+        frstd = a.rstd[r];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            nh[k] = load_group<EIGHTS>(ph, column<TPR>(t, k), a.D);
-            ny[k] = load_group<EIGHTS>(py, column<TPR>(t, k), a.D);
+            const int c = column<TPR>(t, k);
+            fh[k] = load_group<EIGHTS>(ph, c, a.D);
+            fy[k] = load_group<EIGHTS>(py, c, a.D);
+            if (AHEAD || adds) fd[k] = load_group<EIGHTS>(pd, c, a.D);
+            if (AHEAD || g.ds) fx[k] = load_group<EIGHTS>(px, c, a.D);
         }
-        if (g.dh.p) {
-            const TH* pd = row_ptr<TH>(g.dh, r, a.G);
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (AHEAD && r < a.R) fetch(r);
+    for (; r < a.R; r += step) {
+        if constexpr (!AHEAD) fetch(r);
+        Raw<TH, 8> nh[K], nd[K];
+        Raw<T, 8> ny[K], nx[K];
 #pragma unroll
-            for (int k = 0; k < K; ++k) nd[k] = load_group<EIGHTS>(pd, column<TPR>(t, k), a.D);
-        } else {
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) nd[k].v[j] = (TH)0.f;
-        }
-        if (g.ds) {
-            const T* px = row_ptr<T>(a.x, r, a.G);
-#pragma unroll
-            for (int k = 0; k < K; ++k) nx[k] = load_group<EIGHTS>(px, column<TPR>(t, k), a.D);
-        }
-        const float rstd = a.rstd[r];
+        for (int k = 0; k < K; ++k) nh[k] = fh[k], nd[k] = fd[k], ny[k] = fy[k], nx[k] = fx[k];
+        const float rstd = frstd;
+        if (AHEAD && r + step < a.R) fetch(r + step);
         float xh[K][8], d[K][8], sum = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -124,9 +129,9 @@ __global__ __launch_bounds__(block_threads(TPR)) void rms_norm_bwd_kernel(RmsBwd
             float o[8], sc[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                o[j] = __builtin_fmaf(rstd, d[k][j] - xh[k][j] * m, (float)nd[k].v[j]);
+                o[j] = __builtin_fmaf(rstd, d[k][j] - xh[k][j] * m, adds ? (float)nd[k].v[j] : 0.f);
                 sc[j] = o[j] * s_s.at(k, t, j);
-                if (g.ds) ds[k][j] = __builtin_fmaf(o[j], (float)nx[k].v[j], ds[k][j]);
+                ds[k][j] = __builtin_fmaf(o[j], (float)nx[k].v[j], ds[k][j]);  // not used without g.ds
             }
             if (g.dr) store_raw<8>((TH*)g.dr + r * a.D + c, left, o);
             if (g.dx) store_raw<8>((T*)g.dx + r * a.D + c, left, sc);
@@ -155,7 +160,8 @@ __global__ __launch_bounds__(1024) void rms_bwd_sum_kernel(RmsBwdParams g) {
 }
 
 int64_t rms_bwd_parts(int64_t R, int D, int cus) {
-    const int64_t rpb = rows_per_block(D), blocks = (R + rpb - 1) / rpb, most = (int64_t)cus * BWD_BLOCKS;
+    const int64_t rpb = rows_per_block(D), blocks = (R + rpb - 1) / rpb;
+    const int64_t most = (int64_t)cus * (rpb > 4 ? BWD_BLOCKS_NARROW : BWD_BLOCKS);
     return blocks < most ? blocks : most;
 }
 
