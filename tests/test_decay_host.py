@@ -127,7 +127,7 @@ def test_rows_of_two_strides():
     """Rows of one outer and one inner stride go as they are, others are copied."""
     x = torch.zeros(4, 6, 5, 16)
     for v, want in ((x, (80, 16)), (x[:, :, 1:4], (80, 16)), (x[..., :8], (80, 16)), (x[0], (80, 16)), (x[0, 0], (16, 16)),
-                    (x[0, 0, 0], (0, 0)), (x[:1, ::2], (160, 16)), (x[:, 0], (480, 16))):
+                    (x[0, 0, 0], (16, 16)), (x[:1, ::2], (160, 16)), (x[:, 0], (480, 16))):
         got, outer, inner = N._pair(v, N._inner(v))
         assert got is v and (outer, inner) == want, v.shape
     for v in (x[:, 1:3], x.transpose(-1, -2), x[..., ::2], x[:1].expand(3, 6, 5, 16)):

@@ -20,11 +20,20 @@ bool seqs_ok(int64_t n_seqs, int64_t H, int64_t Dv) { return grid_ok(n_seqs, H *
 int forced_segment(int flags) { return ((flags >> TRIUNE_FLAG_SEG_SHIFT) & 0xff) * DECAY_CHUNK; }
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Workgroups that split calls are cut into, and the tokens that a segment has at least: a cut costs a state written,
-// joined and read, 16 bytes a value.
+// Workgroups that split calls are cut into: three to every two compute units where a workgroup holds a whole state of more
+// than 8192 values, three to each otherwise.  A cut costs a state written, joined and read, 16 bytes a value, a long
+// segment leaves compute units idle.  Forward in us, bf16, by tokens a segment ([x]: what this takes):
+//   4 x 16384, 6 heads of 64:     256 97.2, 384 95.7, [512] 85.4, 768 103.1
+//   1 x 8192, 24 heads, 128 x 64: 128 84.9, [256] 68.8, 384 66.9, 512 75.9
+//   4 x 2048, 12 heads of 128:    128 82.5, 192 78.8, [256] 72.1, 384 84.0
+//   1 x 2048, 16 heads of 128:    64 48.1, [128] 39.8, 192 40.8, 256 47.6
+//   2 x 512, 8 heads of 128:      [64] 26.4, 128 30.8, 256 42.1
+// It loses most at 1 x 4096, 12 heads of 128 ([128] 54.7, 192 48.0) and 1 x 16384 of them ([512] 123.5, 768 118.2).
 int64_t chip_slots(int64_t Dk, int64_t Dv) {
     return (int64_t)compute_units() * (decay_padded_dk((int)Dk) * decay_slice((int)Dv) > 8192 ? 3 : 6) / 2;
 }
+// The least tokens of a packed call's segment; its sequences end in shorter ones as they are.  Dense: 64, whole chunks of
+// the gradients.
 int64_t least_segment(int64_t Dk, int64_t Dv) {
     const int values = decay_padded_dk((int)Dk) * decay_slice((int)Dv);
     return values > 8192 ? 192 : values > 4096 ? 128 : 64;
@@ -49,7 +58,7 @@ DecayPlan plan_dense(int64_t n_seqs, int64_t T, int64_t H, int64_t Dk, int64_t D
     p.seg = forced_segment(flags);
     if (!p.seg) {
         int64_t n = chip_slots(Dk, Dv) / blocks;
-        if (n > T / least_segment(Dk, Dv)) n = T / least_segment(Dk, Dv);
+        if (n > T / 64) n = T / 64;
         p.seg = n < 2 ? whole : (T + n - 1) / n;
     }
     p.seg = round_up(p.seg, 64);  // whole chunks of the gradients

@@ -108,6 +108,8 @@ def _inner(x):
 
 def _pair(x, G):
     """(x, stride of every G-th row, stride of the rows between): a copy where the rows have none."""
+    if x.is_contiguous():
+        return x, G * x.shape[-1], x.shape[-1]
     if x.stride(-1) != 1 and x.shape[-1] != 1:
         x = x.contiguous()
     lead = [(n, s) for n, s in zip(x.shape[:-1], x.stride()[:-1])]
@@ -120,16 +122,15 @@ def _pair(x, G):
     return x, step, step if inner is None else inner
 
 
-def _rms_check(x, eps, **others):
-    _one_device(x, *(t for t in others.values() if torch.is_tensor(t)))
+def _rms_check(x, other, eps, weight, scale=None):
+    _one_device(x, other, weight, scale)
     dtype_code(x)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"rows of 1 to {MAX_WIDTH} elements are supported")
-    for name in ("weight", "scale"):
-        p = others.get(name)
-        if not torch.is_tensor(p):
+    for name, p in (("weight", weight), ("scale", scale)):
+        if p is None:
             continue
-        if tuple(p.shape) != (x.shape[-1],):
+        if p.dim() != 1 or p.shape[0] != x.shape[-1]:
             raise ValueError(f"{name} must be [{x.shape[-1]}]")
         if p.dtype not in (x.dtype, torch.float32):
             raise TypeError(f"{name} must have x's dtype or float32")
@@ -208,7 +209,7 @@ class _RmsNorm(torch.autograd.Function):
 def rms_norm(x, weight=None, eps=1e-6):
     """RMS norm over the last dim of x (at most 16384 wide, any leading dims and strides); weight: [D] in x's dtype or
     float32, or None.  Returns y like x, contiguous.  Differentiable (once); the gradients do not depend on timing."""
-    _rms_check(x, eps, weight=weight)
+    _rms_check(x, None, eps, weight)
     weight = None if weight is None else weight.contiguous()
     if _needs_grad(x, weight):
         return _RmsNorm.apply(x, None, weight, None, 1.0, float(eps))
@@ -223,15 +224,15 @@ def add_rms_norm(x, residual, weight=None, scale=None, eps=1e-6):
     rms_norm.  Returns (y in x's dtype, h in residual's dtype), contiguous; y is the norm of h as rounded, so that
     rms_norm(h) gives it again.  Differentiable in every tensor argument (once); the gradients do not depend on
     timing."""
-    _rms_check(x, eps, residual=residual, weight=weight, scale=scale)
+    alpha = 1.0
+    if scale is not None and not torch.is_tensor(scale):
+        scale, alpha = None, float(scale)
+    _rms_check(x, residual, eps, weight, scale)
     if residual.shape != x.shape:
         raise ValueError(f"residual must be {list(x.shape)}")
     if residual.dtype not in (x.dtype, torch.float32):
         raise TypeError("residual must have x's dtype or float32")
     weight = None if weight is None else weight.contiguous()
-    alpha = 1.0
-    if scale is not None and not torch.is_tensor(scale):
-        scale, alpha = None, float(scale)
     scale = None if scale is None else scale.contiguous()
     if _needs_grad(x, residual, weight, scale):
         return _RmsNorm.apply(x, residual, weight, scale, alpha, float(eps))
@@ -282,7 +283,7 @@ def gated_rms_norm(x, z, weight=None, eps=1e-6):
     """rms_norm(x, weight) silu(z): the norm behind a recurrent layer with its gate, over the last dim ([..., heads, dim]
     norms each head).  x and z: one shape and dtype, any leading dims and strides, at most 16384 wide; weight: as in
     rms_norm.  Returns y like x, contiguous.  Differentiable (once); the gradients do not depend on timing."""
-    _rms_check(x, eps, z=z, weight=weight)
+    _rms_check(x, z, eps, weight)
     if z.shape != x.shape or z.dtype != x.dtype:
         raise ValueError(f"z must be {list(x.shape)} of {x.dtype}")
     weight = None if weight is None else weight.contiguous()
