@@ -279,19 +279,20 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
     p.dq = dq, p.dk = dk, p.dv = dv, p.dg = dg;
     if (H > Hk) p.part_q = (float*)(ws + r.off_q), p.part_k = (float*)(ws + r.off_k);
     if (g_head) p.part_g = (float*)(ws + r.off_g);
+    DecayWalkParams x[2];  // forward, backward
     for (const bool rev : {false, true}) {
-        DecayWalkParams x{a, (float*)(rev ? p.R : p.S), (int)r.chunk};
-        x.f.s0 = rev ? ds_final : s0;
-        x.f.fin = rev ? ds0 : nullptr;
-        if (rev) x.f.k = a.q, x.f.v = a.o;
-        if (r.p.nseg > 1) {
-            x.f.ws_state = (float*)(!rev && fwd_workspace ? (char*)fwd_workspace : ws + (rev ? r.off_R_ends : 0));
-            x.f.ws_sum = (float*)((char*)x.f.ws_state + r.p.off_sum);
-            if (rev || !fwd_workspace)
-                if (const int e = status(launch_decay_ends(x.f, rev, io_dtype, s))) return e;
-        }
-        if (const int e = status(launch_decay_states(x, rev, io_dtype, s))) return e;
+        x[rev] = {a, (float*)(rev ? p.R : p.S), (int)r.chunk};
+        DecayParams& f = x[rev].f;
+        f.s0 = rev ? ds_final : s0;
+        f.fin = rev ? ds0 : nullptr;
+        if (rev) f.k = a.q, f.v = a.o;
+        if (r.p.nseg <= 1) continue;
+        f.ws_state = (float*)(!rev && fwd_workspace ? (char*)fwd_workspace : ws + (rev ? r.off_R_ends : 0));
+        f.ws_sum = (float*)((char*)f.ws_state + r.p.off_sum);
+        if (rev || !fwd_workspace)
+            if (const int e = status(launch_decay_ends(f, rev, io_dtype, s))) return e;
     }
+    if (const int e = status(launch_decay_states(x[0], x[1], io_dtype, s))) return e;
     return status(launch_decay_grad(p, io_dtype, s));
 }
 

@@ -53,13 +53,13 @@ inline bool decay_full(int Dk, int Dv, int io_dt, std::initializer_list<DecayTok
 // Segments' end states and what the join makes of them, in the workspace; rev: gradients of states, from the end.
 hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStream_t s);
 
-// The states in front of every chunk; rev: the gradients of those behind them.
+// The states in front of every chunk, and the gradients of those behind them.
 struct DecayWalkParams {
     DecayParams f;            // rows in k, columns in v
     float* states;            // [n_seqs, H, nc, DK, columns], nc = ceil(T / every)
     int every;                // a multiple of 32 tokens; segments are multiples of it
 };
-hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s);
+hipError_t launch_decay_states(const DecayWalkParams& states, const DecayWalkParams& grads, int io_dt, hipStream_t s);
 hipError_t launch_decay_attn(const DecayParams& a, int io_dt, hipStream_t s);
 
 // Tokens of a chunk of the gradients: 64, or 32 for operands in fp32, whose tiles take twice the LDS.

@@ -119,26 +119,12 @@ __device__ __forceinline__ typename Mat<TC>::Frag row_frag_tok(const TC* tile, i
     }
 }
 
-// ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`.
-template <typename TIO, typename TC, int ROWS, int D, int NTH>
-__device__ __forceinline__ void load_tile(TC* tile, const TIO* p, int64_t st, int rows, int cols) {
-    constexpr int E = Mat<TC>::E, UNITS = D / E, RS = tile_stride<TC>(D);
-#pragma unroll
-    for (int u = threadIdx.x; u < ROWS * UNITS; u += NTH) {
-        const int row = u / UNITS, c = u % UNITS * E;
-        Raw<TIO, E> r = load_raw<E>(p + (row < rows ? row * st + c : 0), row < rows ? cols - c : 0);
-        typename Mat<TC>::Frag f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = (TC)r.v[e];
-        *reinterpret_cast<typename Mat<TC>::Frag*>(tile + row * RS + c) = f;
-    }
-}
-
 __device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a constant
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
-// The same through registers, so that a chunk's loads are in flight while the one before it is worked on.  FULL: whole
+// ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`, through registers, so that a chunk's loads
+// are in flight while the one before it is worked on.  FULL: whole
 // units of 16-byte aligned rows (decay_full), through a buffer resource that moves with the chunks, so that a load
 // takes no address arithmetic; what lies outside reads 0 by an offset past the resource's end.
 template <typename TIO, typename TC, int ROWS, int D, int NTH, bool FULL>
@@ -151,7 +137,7 @@ struct Tile {
     __device__ __forceinline__ Tile(int64_t st, int cols) {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)(row_of(i) * st + col_of(i)) * (int)sizeof(TIO) : TILE_SKIP;
+            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)((row_of(i) * st + col_of(i)) * (int64_t)sizeof(TIO)) : TILE_SKIP;
     }
     __device__ __forceinline__ void fetch(const TIO* p, int64_t st, int rows, int cols) {
         if constexpr (FULL) {

@@ -5,6 +5,13 @@ namespace triune {
 
 constexpr int C = DECAY_CHUNK;
 
+// LDS of a walk.
+template <typename TC, int DK, int WIDTH>
+struct WalkTiles {
+    __attribute__((aligned(16))) TC k[2][C * tile_stride<TC>(DK)], v[2][C * tile_stride<TC>(WIDTH)];
+    __attribute__((aligned(16))) ChunkGates g[2];
+};
+
 // States alone, from rows (a.k) by columns (a.v), REV: from the end of the sequence (gradients of states, whose rows are q
 // and whose columns are do):
 //     S <- e^{G_C} S + sum_j e^{G_C - G_j} k_j v_j^T,   R <- e^{G_C} R + scale sum_i e^{G_i} q_i do_i^T
@@ -12,13 +19,11 @@ constexpr int C = DECAY_CHUNK;
 // workspace in the order of the lanes; decay_carry_kernel joins them.
 // EACH true: from the joined states the state in front of (REV: behind) every chunk of p.every tokens, and the final one.
 template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV, bool EACH>
-__global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams p) {
+__device__ __forceinline__ void walk(const DecayWalkParams& p, WalkTiles<TC, DK, NW * NT * 16>& lds) {
     const DecayParams& a = p.f;
     constexpr int E = Mat<TC>::E, KS = Mat<TC>::KS, WIDTH = NW * NT * 16, NTH = NW * 64;
     constexpr int RK = tile_stride<TC>(DK), RV = tile_stride<TC>(WIDTH), TJ = C / KS, DT = DK / 16;
     using Frag = typename Mat<TC>::Frag;
-    __shared__ __attribute__((aligned(16))) TC s_ks[2][C * RK], s_vs[2][C * RV];
-    __shared__ __attribute__((aligned(16))) ChunkGates s_gs[2];
     DecayWhere x;
     if (!decay_where(a, x)) return;
     const bool begins = REV ? x.seg.last : x.seg.index == 0, ends = REV ? x.seg.index == 0 : x.seg.last;
@@ -47,7 +52,7 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
     if (chunks) {
         fetch_gates(0);
         fetch(0);
-        if (w == NW - 1) s_gs[0].put(tg.value(a.g_dt), x.seg.len - first(0), lane);
+        if (w == NW - 1) lds.g[0].put(tg.value(a.g_dt), x.seg.len - first(0), lane);
         fetch_gates(1);
     }
 
@@ -80,17 +85,17 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
         const int64_t at = x.seg.t0 + t0;
         if (EACH && (REV ? (at + C) % p.every == 0 || at + min(C, x.seg.len - t0) == a.T : at % p.every == 0))
             keep_at(at / p.every);
-        TC *s_k = s_ks[place], *s_v = s_vs[place];
+        TC *s_k = lds.k[place], *s_v = lds.v[place];
         tk.put(s_k);
         tv.put(s_v);
-        ChunkGates& s_g = s_gs[place];
+        ChunkGates& s_g = lds.g[place];
         const GateBits gates = tg;
         if (i + 1 < chunks) {
             fetch(i + 1);
             fetch_gates(i + 2);
         }
         lds_barrier();
-        if (i + 1 < chunks && w == (i & (NW - 1))) s_gs[place ^ 1].put(gates.value(a.g_dt), x.seg.len - first(i + 1), lane);
+        if (i + 1 < chunks && w == (i & (NW - 1))) lds.g[place ^ 1].put(gates.value(a.g_dt), x.seg.len - first(i + 1), lane);
         const float keep = s_g.from[C - 1];
         all.hi = fmaxf(all.hi + s_g.hi[C - 1], -1024.f);
         all.lo += s_g.lo[C - 1];
@@ -128,6 +133,19 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_walk_kernel(DecayWalkParams 
             if (in) a.fin[soff + off] = v;
         });
     }
+}
+
+template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL, bool REV>
+__global__ __launch_bounds__(NW * 64, 2) void decay_ends_kernel(DecayWalkParams p) {
+    __shared__ WalkTiles<TC, DK, NW * NT * 16> lds;
+    walk<TIO, TC, DK, NW, NT, FULL, REV, false>(p, lds);
+}
+// Both directions in one launch, which a compute unit takes side by side.
+template <typename TIO, typename TC, int DK, int NW, int NT, bool FULL>
+__global__ __launch_bounds__(NW * 64, 2) void decay_states_kernel(DecayWalkParams p, DecayWalkParams r) {
+    __shared__ WalkTiles<TC, DK, NW * NT * 16> lds;
+    if (blockIdx.y) walk<TIO, TC, DK, NW, NT, FULL, true, true>(r, lds);
+    else walk<TIO, TC, DK, NW, NT, FULL, false, true>(p, lds);
 }
 
 // Joins the segments' end states in place: S_p = 2^{sum_p} S_{p-1} + own_p, p = 1 .. n - 2 in the walk's direction, with S_0
@@ -180,36 +198,42 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(DecayParams a, int64_t
 
 namespace {
 
-template <bool REV, bool EACH>
-struct Walks {
+template <bool REV>
+struct Ends {
     template <typename TIO, typename TC>
     struct Of {
         template <int DK, int NW, int NT, bool FULL>
         static void run(const DecayWalkParams& p, dim3 grid, hipStream_t s) {
-            decay_walk_kernel<TIO, TC, DK, NW, NT, FULL, REV, EACH><<<grid, NW * 64, 0, s>>>(p);
+            decay_ends_kernel<TIO, TC, DK, NW, NT, FULL, REV><<<grid, NW * 64, 0, s>>>(p);
         }
     };
 };
-
-template <bool EACH>
-hipError_t walk(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
-    const DecayParams& a = p.f;
-    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v});
-    return rev ? decay_by_type<Walks<true, EACH>::template Of>(p, a, io_dt, full, s)
-               : decay_by_type<Walks<false, EACH>::template Of>(p, a, io_dt, full, s);
-}
+struct TwoWalks {
+    DecayWalkParams p, r;
+};
+template <typename TIO, typename TC>
+struct States {
+    template <int DK, int NW, int NT, bool FULL>
+    static void run(const TwoWalks& x, dim3 grid, hipStream_t s) {
+        decay_states_kernel<TIO, TC, DK, NW, NT, FULL><<<dim3(grid.x, 2), NW * 64, 0, s>>>(x.p, x.r);
+    }
+};
 
 }  // namespace
 
 hipError_t launch_decay_ends(const DecayParams& a, bool rev, int io_dt, hipStream_t s) {
-    const hipError_t e = walk<false>(DecayWalkParams{a, nullptr, 0}, rev, io_dt, s);
+    const DecayWalkParams p{a, nullptr, 0};
+    const bool full = decay_full(a.Dk, a.Dv, io_dt, {a.k, a.v});
+    const hipError_t e = rev ? decay_by_type<Ends<true>::template Of>(p, a, io_dt, full, s)
+                             : decay_by_type<Ends<false>::template Of>(p, a, io_dt, full, s);
     if (e != hipSuccess) return e;
     const int64_t values = decay_state_values(a.Dk, a.Dv);
     decay_carry_kernel<<<dim3((unsigned)(a.n_seqs * a.H * ((values + 1023) / 1024))), 256, 0, s>>>(a, values, rev);
     return hipGetLastError();
 }
-hipError_t launch_decay_states(const DecayWalkParams& p, bool rev, int io_dt, hipStream_t s) {
-    return walk<true>(p, rev, io_dt, s);
+hipError_t launch_decay_states(const DecayWalkParams& p, const DecayWalkParams& r, int io_dt, hipStream_t s) {
+    const bool full = decay_full(p.f.Dk, p.f.Dv, io_dt, {p.f.k, p.f.v, r.f.k, r.f.v});
+    return decay_by_type<States>(TwoWalks{p, r}, p.f, io_dt, full, s);
 }
 
 }  // namespace triune
