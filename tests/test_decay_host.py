@@ -133,3 +133,25 @@ def test_rows_of_two_strides():
     for v in (x[:, 1:3], x.transpose(-1, -2), x[..., ::2], x[:1].expand(3, 6, 5, 16)):
         got, outer, inner = N._pair(v, N._inner(v))
         assert got.is_contiguous() and got.shape == v.shape and inner == v.shape[-1] and outer == v.shape[-2] * inner
+
+
+def test_segments_by_length_and_heads():
+    """Dense calls are cut where their (sequence, head) pairs leave the card idle, and nowhere else."""
+    size = L.lib().triune_hip_decay_attn_workspace_size
+
+    def segments(B, T, H, Dk, Dv, values, flags=0):
+        """Segments of a sequence, from the states and sums that a workspace holds."""
+        have = size(B, T, H, H, Dk, Dv, flags)
+        pad = lambda n: -(-n // 256) * 256  # noqa: E731
+        return next((n for n in range(2, T // 64 + 2)
+                     if have == pad(4 * B * n * H * values) + pad(8 * B * n * H)), 1 if have == 0 else None)
+
+    for T in (1, 63, 64):
+        assert segments(1, T, 1, 64, 64, 64 * 64) == 1, T
+    for T in (65, 127, 128):
+        assert segments(1, T, 1, 64, 64, 64 * 64) in (1, 2), T
+    assert segments(1, 640, 1, 64, 64, 64 * 64) == 10  # never shorter than 64 tokens
+    assert segments(1, 640, 1, 128, 300, 128 * 384) == 10  # value dims in whole slices
+    assert segments(1, 640, 1, 64, 64, 64 * 64, 4 << 8) == 5  # forced: of 4 x 32 tokens
+    assert segments(1 << 12, 640, 16, 64, 64, 64 * 64) == 1  # workgroups enough
+    assert size(1, 640, 1, 1, 0, 64, 0) == 0 and size(0, 640, 1, 1, 64, 64, 0) == 0
