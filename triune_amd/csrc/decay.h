@@ -1,5 +1,5 @@
-// decay.h -- parameter blocks and launchers of the decay attention kernels (decay_attn.hip, decay_attn_bwd.hip)
-// and of the norms beside it (rms_norm.hip).  Internal to libtriune_hip.
+// decay.h -- parameter blocks and launchers of the decay attention kernels (decay_attn.hip, decay_walk.hip,
+// decay_attn_bwd.hip).  Internal to libtriune_hip.
 #pragma once
 
 #include "ssm.h"
@@ -23,7 +23,8 @@ struct DecayParams {
     float* fin;               // [rows, H, Dk, Dv] or null
     const int32_t* slots;     // packed over a pool: the row of each sequence, else null
     int64_t n_slots;
-    float* ws_state;          // [n_work, H, values]: a segment's own end state, then the state behind it
+    float* ws_state;          // [n_work, H, values]: a segment's own end state, then the state behind it; the last
+                              // segment's place: the sequence's initial state
     float* ws_sum;            // [n_work, H, 2]: summed log2 decays
     int64_t n_seqs, T;        // T: length of a dense sequence, or all tokens of a packed call
     int H, per, Dk, Dv;       // per: heads of v for one of q and k

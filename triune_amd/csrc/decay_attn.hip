@@ -11,7 +11,14 @@
 // each, the state slice lies in their accumulators.  The scores of a chunk are six products of 16 x 16 x Dk, so every
 // wave forms them for itself instead of sharing them through LDS.  Accumulators (scores, state) become operands of the
 // next product in place (decay_mfma.h).  Where segments follow each other, a first pass forms their end states and a
-// scan joins them.
+// scan joins them (decay_walk.hip).
+//
+// What bounds it: a workgroup's chain of chunks where few are at work, vector issue where many are (4 x 16384 tokens, 6
+// heads of 64, bf16: 69 % of the SIMDs' cycles issue vector work and 24 % matrix work, 51.9 us for 202 MB; 16 prompts,
+// 12 heads of 128: 44 and 22 %, 38.7 us).  Hence a chunk's loads are in flight while the one before it is worked on
+// (143 -> 126 us of all passes of a call of the first kind), its gates are formed once for all waves (103), and slices
+// are as wide as 128 columns, four waves of two tiles, so that q and k are read once for all of them.  Two chunks of
+// loads in flight, or two waves of two tiles for 64 columns, gave nothing.
 #include "decay_mfma.h"
 
 namespace triune {
@@ -48,8 +55,8 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
         get_state(S, a.ws_state + (from * a.H + x.h) * values + ((int64_t)x.slice * NW + w) * (NT * DT * 256) + lane * 4);
     }
 
-    // A chunk's tiles go from registers to one of two places, and the next one's loads are issued; gates are loaded two chunks
-    // ahead and formed one ahead.
+    // A chunk's tiles go from registers to one of two places, and the next one's loads are issued; gates are loaded two
+    // chunks ahead and formed one ahead.
     Tile<TIO, TC, C, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
     Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
     GateBits tg;
@@ -191,6 +198,8 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
 
 // One token for every row: a block takes a (row, head), a thread four columns of every RG-th state row.  Bound by the
 // state, read and written once, past the caches.  ALIGNED: rows of whole 16 bytes, eight of which a thread has in flight.
+// 256 sessions, 12 heads of 128: 78.6 us, 5.1 TB/s, the rate of a large copy (104 us with fewer in flight and through the
+// caches).
 template <typename TIO, bool ALIGNED>
 __global__ __launch_bounds__(256) void decay_step_kernel(DecayStepParams a, int lanes) {
     constexpr int V = 4, ROWS = 8;

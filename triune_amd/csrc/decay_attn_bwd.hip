@@ -15,6 +15,11 @@
 // LDS, B in the place of A; a wave owns a 16-wide tile of key dims (dq, dk) and one of value dims (dv), which are taken in
 // slices of 32.  Its rows of S and R come from memory once, the products with k take R by columns from LDS (in q's place,
 // which is read again behind them), and two workgroups fit a compute unit.
+//
+// 4 x 2048 tokens, 12 heads of 128, bf16: 117 us for 206 MB of states, 101 of tensors in and 75 out (3.3 TB/s); 30 % of
+// the SIMDs' cycles issue vector work and 14 % matrix work, 45 % of the waves' wait: a chain of products with little
+// beside it at two workgroups a compute unit, which registers (128) and LDS (74 KB) allow.  Chunks of 64 tokens instead
+// of 32 halve the states' bytes; fp32 tensors, whose tiles take twice the LDS, stay at 32.
 #include "decay_mfma.h"
 
 namespace triune {

@@ -5,6 +5,12 @@
 // The accumulator's rows 4 g + r of two neighbouring tiles (bf16) or one (fp32) are the K slots of the same lane,
 // so an accumulator becomes an operand without moving between lanes: slot e of lane group g is then row
 // 16 (e >> 2) + 4 g + (e & 3).
+//
+// Roundings.  bf16 tensors are operands as they are.  What is derived from them (scores, states, weighted rows) is a
+// sum of bf16 parts, each half a step (2^-8) off the rest: two parts, 2^-16, where it ends in a 16-bit output, three,
+// 2^-24, where it goes into a state that is carried on, and for the states' terms of dq and dk, which the gates'
+// gradients add up.  fp16 tensors take the fp32 form, since their range is not bf16's and their products with states
+// are not fp16's.
 #pragma once
 
 #include "decay.h"
@@ -123,8 +129,8 @@ __device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a con
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
-// ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`, through registers, so that a chunk's loads
-// are in flight while the one before it is worked on.  FULL: whole
+// ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`, through registers, so that a chunk's
+// loads are in flight while the one before it is worked on.  FULL: whole
 // units of 16-byte aligned rows (decay_full), through a buffer resource that moves with the chunks, so that a load
 // takes no address arithmetic; what lies outside reads 0 by an offset past the resource's end.
 template <typename TIO, typename TC, int ROWS, int D, int NTH, bool FULL>
@@ -137,7 +143,8 @@ struct Tile {
     __device__ __forceinline__ Tile(int64_t st, int cols) {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)((row_of(i) * st + col_of(i)) * (int64_t)sizeof(TIO)) : TILE_SKIP;
+            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)((row_of(i) * st + col_of(i)) * (int64_t)sizeof(TIO))
+                                                          : TILE_SKIP;
     }
     __device__ __forceinline__ void fetch(const TIO* p, int64_t st, int rows, int cols) {
         if constexpr (FULL) {

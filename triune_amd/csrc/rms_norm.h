@@ -10,6 +10,11 @@
 // a row of K groups of eight columns each, from 8 threads (heads of 64) to sixteen waves; blocks walk rows with the
 // next one's loads in flight.  The backward's blocks hold their columns' dw and ds in registers; a last kernel adds
 // the blocks' parts in a fixed order.
+//
+// Sum and norm of 16384 rows of 1536, bf16: 52.4 us forward (201 MB, 3.8 TB/s), 66.0 backward (302 MB, 4.6 TB/s; 89.3
+// without the next row's loads in flight).  9003 rows of 1001, fp16 with a float32 residual: 39.0 and 57.0 us (2.8 and
+// 2.5 TB/s): rows that do not start on 16 bytes.  Gated, 393216 rows of 64, bf16: 29.6 us (151 MB, 5.1 TB/s, a large
+// copy's rate); 98304 rows of 128: 16.3 forward, 29.9 backward.
 #pragma once
 
 #include "ssm.h"
