@@ -130,9 +130,9 @@ __device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a con
 }
 
 // ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`, through registers, so that a chunk's
-// loads are in flight while the one before it is worked on.  FULL: whole
-// units of 16-byte aligned rows (decay_full), through a buffer resource that moves with the chunks, so that a load
-// takes no address arithmetic; what lies outside reads 0 by an offset past the resource's end.
+// loads are in flight while the one before it is worked on.  FULL: whole units of 16-byte aligned rows (decay_full), through
+// a buffer resource that moves with the chunks, so that a load takes no address arithmetic; what lies outside reads 0 by an
+// offset past the resource's end.
 template <typename TIO, typename TC, int ROWS, int D, int NTH, bool FULL>
 struct Tile {
     static constexpr int E = Mat<TC>::E, UNITS = D / E, N = ROWS * UNITS, PER = (N + NTH - 1) / NTH;

@@ -9,7 +9,7 @@ innermost is made 1 by a copy where it is not), one dtype of float32, bfloat16 a
 H / Hk consecutive heads of v share one of q and k.  g: log-decays [B, T, H] in that dtype or float32, or [H]: one
 constant per head.  A log-decay above 0 counts as 0 (its gradient is 0 then), -inf forgets.  Dk is at most 128, Dv at
 most 16384.  States are float32 [B, H, Dk, Dv].  Sums and states are float32, outputs are rounded once.  Values are
-expected to be finite: one that is not reaches the outputs of the other tokens of its block of 32 (training: 64) in the
+expected to be finite: one that is not reaches the outputs of the other tokens of its block of 32 (gradients of bfloat16: 64) in the
 same sequence and head, earlier ones among them, and all later ones; other sequences and heads it does not reach.
 Tensors are on one HIP device; there is no CPU path and no forward-mode derivative.
 """
@@ -131,7 +131,7 @@ def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0, kept=None):
 
 class _DecayAttn(torch.autograd.Function):
     """decay_attn with gradients.  The forward keeps the states of its segments (none of short calls); the backward forms
-    those of every 64th token from them."""
+    those of every 64th token (32nd of float32 and float16) from them, as scratch."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, s0, scale):
