@@ -7,11 +7,11 @@ dim, as the member with one decay a head, which needs no factor on every element
 Layouts: q, k [B, T, Hk, Dk], v [B, T, H, Dv] (packed: [N, heads, dim] or [1, N, heads, dim]) with any strides (the
 innermost is made 1 by a copy where it is not), one dtype of float32, bfloat16 and float16; H is a multiple of Hk, and
 H / Hk consecutive heads of v share one of q and k.  g: log-decays [B, T, H] in that dtype or float32, or [H]: one
-constant per head.  A log-decay above 0 counts as 0 (its gradient is 0 then), -inf forgets.  Dk is at most 128, Dv at
-most 16384.  States are float32 [B, H, Dk, Dv].  Sums and states are float32, outputs are rounded once.  Values are
-expected to be finite: one that is not reaches the outputs of the other tokens of its block of 32 (gradients of bfloat16: 64) in the
-same sequence and head, earlier ones among them, and all later ones; other sequences and heads it does not reach.
-Tensors are on one HIP device; there is no CPU path and no forward-mode derivative.
+constant per head.  A log-decay above 0 counts as 0 (its gradient is 0 then), -inf forgets.  Dk is at most 128, Dv
+at most 16384.  States are float32 [B, H, Dk, Dv].  Sums and states are float32, outputs are rounded once.  Values
+are expected to be finite: one that is not reaches the outputs of the other tokens of its block of 32 (gradients of
+bfloat16: 64) in the same sequence and head, earlier ones among them, and all later ones; other sequences and heads
+it does not reach. Tensors are on one HIP device; there is no CPU path and no forward-mode derivative.
 """
 
 from __future__ import annotations
