@@ -57,8 +57,8 @@ __global__ __launch_bounds__(NW * 64, (Mat<TC>::E == 4 && DK == 128 ? 1 : 2)) vo
 
     // A chunk's tiles go from registers to one of two places, and the next one's loads are issued; gates are loaded two
     // chunks ahead and formed one ahead.
-    Tile<TIO, TC, C, DK, NTH, FULL> tq(a.q.st, a.Dk), tk(a.k.st, a.Dk);
-    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
+    Tile<TIO, TC, C, DK, NTH, FULL> tq(a.q.st), tk(a.k.st);
+    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st);
     GateBits tg;
     auto fetch = [&](int t0) {
         const int rows = min(C, x.seg.len - t0);

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
     const bool ownsK = w < UK * HK, ownsV = w < TV * HV;
     // a slice of 32 value dims: v, do, and the wave's rows of the states, in flight while the one before is worked on
     const TIO *pv = (const TIO*)a.v.p + at(a.v, h), *pd = (const TIO*)a.o.p + at(a.o, h);
-    Tile<TIO, TC, CH, DVW, NTH, FULL> fv(a.v.st, DVW), fd(a.o.st, DVW);
+    Tile<TIO, TC, CH, DVW, NTH, FULL> fv(a.v.st), fd(a.o.st);
     constexpr int NS = DVW / KS;
     float xs[NDK * NS][E], xr[NDK * NS][E];
     auto fetch = [&](int col0) {
@@ -125,10 +125,10 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
             R.row<E>(4 * (n * wide + E * g), all, xr[i]);
         }
     };
-    Tile<TIO, TC, CH, DK, NTH, FULL> fq(a.q.st, a.Dk);
+    Tile<TIO, TC, CH, DK, NTH, FULL> fq(a.q.st);
     const TIO* pq = (const TIO*)a.q.p + at(a.q, hk);
     {
-        Tile<TIO, TC, CH, DK, NTH, FULL> fk(a.k.st, a.Dk);
+        Tile<TIO, TC, CH, DK, NTH, FULL> fk(a.k.st);
         fq.fetch(pq, a.q.st, rows, a.Dk);
         fk.fetch((const TIO*)a.k.p + at(a.k, hk), a.k.st, rows, a.Dk);
         fetch(0);
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
     float z = 0.f;
     for (int col0 = 0; col0 < a.Dv; col0 += DVW) {
         lds_barrier();
-        fv.put(s_v, a.Dv - col0);
-        fd.put(s_d, a.Dv - col0);
+        fv.put(s_v);
+        fd.put(s_d);
         if (ownsK && Ik == 0) {
 #pragma unroll
             for (int i = 0; i < NDK * NS; ++i) {

@@ -131,44 +131,42 @@ __device__ __forceinline__ float lane_value(float x, int lane) {  // lane: a con
 
 // ROWS rows of a [tokens][D] tensor into an LDS tile, zeros past `rows` and `cols`, through registers, so that a chunk's
 // loads are in flight while the one before it is worked on.  FULL: whole units of 16-byte aligned rows (decay_full), through
-// a buffer resource that moves with the chunks, so that a load takes no address arithmetic; what lies outside reads 0 by an
-// offset past the resource's end.
+// a buffer resource that moves with the chunks, so that a load takes no address arithmetic; the resource has no end of its
+// own (rows are far apart), so every unit outside of `rows` and `cols` goes past it (TileUnits).
 template <typename TIO, typename TC, int ROWS, int D, int NTH, bool FULL>
 struct Tile {
-    static constexpr int E = Mat<TC>::E, UNITS = D / E, N = ROWS * UNITS, PER = (N + NTH - 1) / NTH;
+    static constexpr int E = Mat<TC>::E;
+    using Units = TileUnits<ROWS, D, E, NTH>;
+    static constexpr int N = Units::N, PER = Units::PER;
     Raw<TIO, E> x[PER];
     int off[PER];  // bytes from the chunk's first row
-    __device__ __forceinline__ static int row_of(int i) { return (threadIdx.x + i * NTH) / UNITS; }
-    __device__ __forceinline__ static int col_of(int i) { return (threadIdx.x + i * NTH) % UNITS * E; }
-    __device__ __forceinline__ Tile(int64_t st, int cols) {
+    __device__ __forceinline__ static int row_of(int i) { return Units::row(threadIdx.x, i); }
+    __device__ __forceinline__ static int col_of(int i) { return Units::col(threadIdx.x, i); }
+    __device__ __forceinline__ explicit Tile(int64_t st) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            off[i] = row_of(i) < ROWS && col_of(i) < cols ? (int)((row_of(i) * st + col_of(i)) * (int64_t)sizeof(TIO))
-                                                          : TILE_SKIP;
+        for (int i = 0; i < PER; ++i) off[i] = Units::offset(threadIdx.x, i, st, sizeof(TIO));
     }
+    // rows, cols: what the tensor has from p on
     __device__ __forceinline__ void fetch(const TIO* p, int64_t st, int rows, int cols) {
         if constexpr (FULL) {
             const __amdgpu_buffer_rsrc_t r =
                 __builtin_amdgcn_make_buffer_rsrc(const_cast<TIO*>(p), (short)0, TILE_SKIP, 0x00020000);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int o = rows == ROWS || row_of(i) < rows ? off[i] : TILE_SKIP;
-                x[i] = __builtin_bit_cast(Raw<TIO, E>, tile_load<TIO, E>(r, o));
-            }
+            for (int i = 0; i < PER; ++i)
+                x[i] = __builtin_bit_cast(Raw<TIO, E>,
+                                          tile_load<TIO, E>(r, Units::load_from(off[i], threadIdx.x, i, rows, cols)));
         } else {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const bool in = row_of(i) < rows && col_of(i) < cols;
+                const bool in = Units::in(threadIdx.x, i, rows, cols);
                 x[i] = load_raw<E>(p + (in ? row_of(i) * st + col_of(i) : 0), in ? cols - col_of(i) : 0);
             }
         }
     }
-    // left: columns of the tile inside the tensor, for a Tile that moves over its columns
-    __device__ __forceinline__ void put(TC* tile, int left = D) {
+    __device__ __forceinline__ void put(TC* tile) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             if (N % NTH && row_of(i) >= ROWS) continue;
-            if (FULL && left < D && col_of(i) >= left) x[i] = Raw<TIO, E>{};
             TC* to = tile + row_of(i) * tile_stride<TC>(D) + col_of(i);
             if constexpr (std::is_same<TIO, TC>::value) {
                 *reinterpret_cast<typename Mat<TC>::Frag*>(to) = __builtin_bit_cast(typename Mat<TC>::Frag, x[i]);

@@ -42,8 +42,8 @@ __device__ __forceinline__ void walk(const DecayWalkParams& p, WalkTiles<TC, DK,
 
     const int chunks = (x.seg.len + C - 1) / C;
     // loads and gates ahead as in decay_attn_kernel
-    Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st, a.Dk);
-    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st, a.Dv - col0);
+    Tile<TIO, TC, C, DK, NTH, FULL> tk(a.k.st);
+    Tile<TIO, TC, C, WIDTH, NTH, FULL> tv(a.v.st);
     GateBits tg;
     auto first = [&](int i) { return (REV ? chunks - 1 - i : i) * C; };
     auto fetch = [&](int i) {

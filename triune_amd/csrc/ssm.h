@@ -4,6 +4,7 @@
 #pragma once
 
 #include "common.h"
+#include "tile_units.h"
 
 #include <initializer_list>
 
@@ -294,7 +295,6 @@ __device__ __forceinline__ void store_states(float* p, int left, const float (&x
 // not written.  Accesses step through the vector offset, which the range check covers; a
 // branch around them, or one for whole tiles, would make the compiler join registers behind it, which
 // waits for the loads it should leave in flight.
-constexpr int TILE_SKIP = 0x40000000;  // an offset past every resource: reads 0, writes nothing
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const T* p, int64_t st, int64_t rows, uint32_t width) {
     const int64_t n = p && rows > 0 ? ((rows - 1) * st + width) * (int64_t)sizeof(T) : 0;
