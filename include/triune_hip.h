@@ -543,7 +543,10 @@ int triune_hip_layer_norm_bwd(const void* x, int64_t x_stride, const void* w, co
  *     S_t = e^{g_t} S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t         (g above 0 counts as 0)
  * q, k [B, T, Hk, Dk], v, o [B, T, H, Dv] in io_dtype, innermost stride 1, any other strides (in elements) and any
  * alignment of an element; H / Hk consecutive heads of v share one of q and k; g [B, T, H] in io_dtype or fp32 (strides of
- * 0 for constants).  Dk <= 128, Dv <= 16384, H < 65536.  strides[15] = (batch, token, head) of q, k, v, g, o.
+ * 0 for constants).  Dk <= 128, Dv <= 16384, H < 65536; a call of 2^24 workgroups or more is a shape error (one for each
+ * segment of a sequence, head and 128 value dims; gradients: one for each head and 64 tokens, of fp32 and fp16 32; forced
+ * segments: one for each 1024 values of the sequences' states).
+ * strides[15] = (batch, token, head) of q, k, v, g, o.
  * States: fp32 contiguous [B, H, Dk, Dv], s0 NULL: zeros, s_final NULL: not wanted; without tokens (T = 0) s0 goes to
  * s_final.  o overlaps no input.  A workspace is 16-byte aligned and belongs to one call at a time.  flags bits 8..15
  * force the length of a segment in units of 32 tokens (0: automatic). */

@@ -69,8 +69,16 @@ DecayPlan plan_dense(int64_t n_seqs, int64_t T, int64_t H, int64_t Dk, int64_t D
     return p;
 }
 
+// The grids of a call: its work items, and where there are segments the join's, four values of a state a thread.  States
+// themselves are addressed in 64 bits.
+bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t Dv) {
+    const int64_t values = decay_state_values((int)Dk, (int)Dv);
+    return grid_ok(p.n_work, H * slices_of(Dv), 256) &&
+           (p.nseg <= 1 || grid_ok(n_seqs, H * ((values + 1023) / 1024), 256));
+}
+
 // Packed: lengths are on the device, so a segment is an equal share of all tokens.  nseg > 1 says that there may be
-// segments.
+// segments; sequences whose join would outgrow a grid are enough without them.
 DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int64_t Dv, int flags) {
     DecayPlan p{};
     p.seg = forced_segment(flags);
@@ -82,6 +90,10 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
     if (p.cut < p.seg) p.cut = p.seg;
     p.nseg = p.cut < total ? 2 : 1;
     p.n_work = p.nseg > 1 ? total / p.seg + n_seqs : n_seqs;
+    if (!forced_segment(flags) && !grids_ok(p, n_seqs, H, Dk, Dv)) {
+        p.nseg = 1;
+        p.n_work = n_seqs;
+    }
     plan_bytes(p, H, Dk, Dv, n_seqs + 1);
     return p;
 }
@@ -112,14 +124,8 @@ GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int6
     return r;
 }
 
-bool grids_ok(const DecayPlan& p, int64_t n_seqs, int64_t H, int64_t Dk, int64_t Dv) {
-    const int64_t values = decay_state_values((int)Dk, (int)Dv);
-    return grid_ok(p.n_work, H * slices_of(Dv), 256) && grid_ok(n_seqs, H * ((values + 255) / 256), 256) &&
-           n_seqs <= kMaxGrid / (H * Dk * Dv);
-}
-
-bool grad_grids_ok(const GradPlan& r, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv) {
-    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 512) && grid_ok(B * T, (Hk * Dk + 255) / 256 + 1, 256);
+bool grad_grids_ok(const GradPlan& r, int64_t B, int64_t H, int64_t Dk, int64_t Dv) {
+    return grids_ok(r.p, B, H, Dk, Dv) && grid_ok(B * r.nc, H, 256);
 }
 
 void set_sizes(DecayParams& a, int64_t n_seqs, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -242,7 +248,7 @@ size_t triune_hip_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H,
         !seqs_ok(B, H, Dv))
         return 0;
     const GradPlan r = plan_grad(B, T, H, Hk, Dk, Dv, io_dtype, g_head, flags);
-    return grad_grids_ok(r, B, T, H, Hk, Dk, Dv) ? r.total : 0;
+    return grad_grids_ok(r, B, H, Dk, Dv) ? r.total : 0;
 }
 
 int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const void* g, const void* dout,
@@ -259,7 +265,7 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
         !all_aligned(TRIUNE_DT_F32, {s0, ds_final, ds0}))
         return TRIUNE_ERR_LAYOUT;
     const GradPlan r = plan_grad(B, T, H, Hk, Dk, Dv, io_dtype, g_head, flags);
-    if (!grad_grids_ok(r, B, T, H, Hk, Dk, Dv)) return TRIUNE_ERR_SHAPE;
+    if (!grad_grids_ok(r, B, H, Dk, Dv)) return TRIUNE_ERR_SHAPE;
     if (fwd_workspace)
         if (const int e = check_ws(fwd_workspace, fwd_workspace_bytes, r.p.total)) return e;
     if (const int e = check_ws(workspace, workspace_bytes, r.total)) return e;

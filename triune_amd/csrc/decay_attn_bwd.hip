@@ -391,21 +391,23 @@ __global__ __launch_bounds__(NW * 64, 2) void decay_grad_kernel(DecayGradParams 
     }
 }
 
-// dq and dk of shared heads: the sum over the heads that share them, in their order.
+// dq and dk of shared heads: the sum over the heads that share them, in their order.  A thread takes every
+// SHARE_BLOCKS * 256-th value, so that no size outgrows a grid.
+constexpr int64_t SHARE_BLOCKS = 1 << 16;
 template <typename TIO>
 __global__ __launch_bounds__(256) void decay_share_kernel(DecayGradParams p, int64_t n) {
     const DecayParams& a = p.f;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t head = i / a.Dk, d = i - head * a.Dk;
-    float q = 0.f, k = 0.f;
-    for (int s = 0; s < a.per; ++s) {
-        const int64_t off = (head * a.per + s) * a.Dk + d;
-        q += p.part_q[off];
-        k += p.part_k[off];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += SHARE_BLOCKS * 256) {
+        const int64_t head = i / a.Dk, d = i - head * a.Dk;
+        float q = 0.f, k = 0.f;
+        for (int s = 0; s < a.per; ++s) {
+            const int64_t off = (head * a.per + s) * a.Dk + d;
+            q += p.part_q[off];
+            k += p.part_k[off];
+        }
+        ((TIO*)p.dq)[i] = (TIO)q;
+        ((TIO*)p.dk)[i] = (TIO)k;
     }
-    ((TIO*)p.dq)[i] = (TIO)q;
-    ((TIO*)p.dk)[i] = (TIO)k;
 }
 
 // dg of constants per head: the chunks' sums, sixteen threads a head, then these, in a fixed order.
@@ -440,7 +442,8 @@ hipError_t grad_dk(const DecayGradParams& p, bool full, hipStream_t s) {
 template <typename TIO>
 hipError_t share(const DecayGradParams& p, hipStream_t s) {
     const int64_t n = p.f.n_seqs * p.f.T * (p.f.H / p.f.per) * p.f.Dk;
-    decay_share_kernel<TIO><<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(p, n);
+    const int64_t blocks = (n + 255) / 256;
+    decay_share_kernel<TIO><<<dim3((unsigned)(blocks < SHARE_BLOCKS ? blocks : SHARE_BLOCKS)), 256, 0, s>>>(p, n);
     return hipGetLastError();
 }
 
