@@ -568,7 +568,8 @@ int triune_hip_decay_attn_varlen(const void* q, const void* k, const void* v, co
 /* Gradients: dout [B, T, H, Dv] in io_dtype; strides[15] = (batch, token, head) of q, k, v, g, dout; ds_final (NULL: zeros)
  * and ds0 (NULL: not wanted) fp32 contiguous [B, H, Dk, Dv], not one tensor; dq, dk, dv contiguous in io_dtype; dg
  * contiguous in g_dtype, [B, T, H], or with g_head != 0 [H], the sum over batch and tokens.  B, T > 0.
- * fwd_workspace: what triune_hip_decay_attn on these inputs and flags left in its workspace, not written since, or NULL.
+ * fwd_workspace: what triune_hip_decay_attn on these inputs and flags left in its workspace, not written since, or NULL;
+ * with it the workspace may be smaller by triune_hip_decay_attn_workspace_size than its size function says.
  * Sums are taken in a fixed order.  The workspace holds the states of every 64th token (32nd for fp32 and fp16), twice. */
 size_t triune_hip_decay_attn_bwd_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
                                                 int io_dtype, int g_head, int flags);

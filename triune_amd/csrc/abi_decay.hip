@@ -98,12 +98,12 @@ DecayPlan plan_packed(int64_t n_seqs, int64_t total, int64_t H, int64_t Dk, int6
     return p;
 }
 
-// Gradients: the forward's segments (its joined end states, formed again where they are not kept, and those of the
-// states' gradients), the states of every chunk, and sums of shared heads and of constant gates.
+// Gradients: the segments' end states of the states' gradients, the states of every chunk, sums of shared heads and of
+// constant gates, and last the forward's end states, which take no place where the forward's workspace holds them.
 struct GradPlan {
     DecayPlan p;
     int64_t chunk, nc;
-    size_t off_R_ends, off_S, off_R, off_q, off_k, off_g, total;
+    size_t off_S, off_R, off_q, off_k, off_g, off_ends, total;
 };
 
 GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int io_dtype, int g_head,
@@ -114,13 +114,13 @@ GradPlan plan_grad(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int6
     r.nc = (T + r.chunk - 1) / r.chunk;
     const size_t heads = (size_t)(B * H), states = align_up(heads * r.nc * decay_state_values((int)Dk, (int)Dv) * 4);
     const size_t shared = H > Hk ? align_up((size_t)(B * T * H) * Dk * 4) : 0;
-    r.off_R_ends = r.p.total;
-    r.off_S = r.off_R_ends + r.p.total;
+    r.off_S = r.p.total;
     r.off_R = r.off_S + states;
     r.off_q = r.off_R + states;
     r.off_k = r.off_q + shared;
     r.off_g = r.off_k + shared;
-    r.total = r.off_g + (g_head ? align_up(heads * r.nc * 4) : 0);
+    r.off_ends = r.off_g + (g_head ? align_up(heads * r.nc * 4) : 0);
+    r.total = r.off_ends + r.p.total;
     return r;
 }
 
@@ -268,7 +268,7 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
     if (!grad_grids_ok(r, B, H, Dk, Dv)) return TRIUNE_ERR_SHAPE;
     if (fwd_workspace)
         if (const int e = check_ws(fwd_workspace, fwd_workspace_bytes, r.p.total)) return e;
-    if (const int e = check_ws(workspace, workspace_bytes, r.total)) return e;
+    if (const int e = check_ws(workspace, workspace_bytes, fwd_workspace ? r.off_ends : r.total)) return e;
     char* ws = (char*)workspace;
     const hipStream_t s = (hipStream_t)stream;
     DecayGradParams p{};
@@ -293,7 +293,7 @@ int triune_hip_decay_attn_bwd(const void* q, const void* k, const void* v, const
         f.fin = rev ? ds0 : nullptr;
         if (rev) f.k = a.q, f.v = a.o;
         if (r.p.nseg <= 1) continue;
-        f.ws_state = (float*)(!rev && fwd_workspace ? (char*)fwd_workspace : ws + (rev ? r.off_R_ends : 0));
+        f.ws_state = (float*)(!rev && fwd_workspace ? (char*)fwd_workspace : ws + (rev ? 0 : r.off_ends));
         f.ws_sum = (float*)((char*)f.ws_state + r.p.off_sum);
         if (rev || !fwd_workspace)
             if (const int e = status(launch_decay_ends(f, rev, io_dtype, s))) return e;

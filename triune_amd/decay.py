@@ -121,6 +121,7 @@ def _attn_bwd(q, k, v, g, scale, s0, do, dfin, want_s0, flags=0, kept=None):
     ds0 = torch.empty(B, H, Dk, Dv, device=dev, dtype=f32) if want_s0 else None
     head = int(g.dim() == 1)
     wsb = plan_on(q, "triune_hip_decay_attn_bwd_workspace_size", B, T, H, Hk, Dk, Dv, dtype_code(q), head, flags)
+    wsb -= 0 if kept is None else kept.numel()  # the forward's end states
     ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
     st = strides(*(_head_strides(x) for x in (q, k, v)), _head_strides(g, 3), _head_strides(do))
     call_on(q, "triune_hip_decay_attn_bwd", ptr(q), ptr(k), ptr(v), ptr(g), ptr(do), dtype_code(q), dtype_code(g), st, scale,
