@@ -549,7 +549,7 @@ int triune_hip_layer_norm_bwd(const void* x, int64_t x_stride, const void* w, co
  * strides[15] = (batch, token, head) of q, k, v, g, o.
  * States: fp32 contiguous [B, H, Dk, Dv], s0 NULL: zeros, s_final NULL: not wanted; without tokens (T = 0) s0 goes to
  * s_final.  o overlaps no input.  A workspace is 16-byte aligned and belongs to one call at a time.  flags bits 8..15
- * force the length of a segment in units of 32 tokens (0: automatic). */
+ * force the length of a segment in units of 32 tokens (0: automatic), which dense calls and gradients round up to 64. */
 size_t triune_hip_decay_attn_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
                                             int flags);
 int triune_hip_decay_attn(const void* q, const void* k, const void* v, const void* g, int io_dtype, int g_dtype,
