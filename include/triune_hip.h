@@ -587,7 +587,7 @@ int triune_hip_decay_attn_decode_step(const void* q, const void* k, const void* 
                                       float* state_out, const int32_t* slots, int64_t n_state_rows, void* o, int64_t B,
                                       int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, void* stream);
 
-/* RMS norm of R rows of D elements (D <= 16384), with the residual sum in front of it:
+/* RMS norm of R rows of D elements (R < 2^31, D <= 16384), with the residual sum in front of it:
  *     h = r + scale x (rounded to r_dtype),   y = h rstd w,   rstd = 1 / sqrt(mean h^2 + eps)
  * scale: s [D], or alpha where s is NULL.  r and h NULL: y is the norm of x.  x, y in io_dtype; r, h in r_dtype (io_dtype
  * or fp32); w, s [D] (each may be NULL) in io_dtype or fp32.  Row i of x starts (i / G) strides[0] + (i % G) strides[1]

@@ -8,7 +8,7 @@
 // Every exponent is a difference of sums and at most 0, so no factor leaves the range, whatever the gates.
 //
 // A workgroup walks a segment of a (sequence, head) for a slice of the state's columns; its waves own 16 or 32 of them
-// each, the state slice lies in their accumulators.  The scores of a chunk are six products of 16 x 16 x Dk, so every
+// each, the state slice lies in their accumulators.  The scores of a chunk are three products of 16 x 16 x Dk, so every
 // wave forms them for itself instead of sharing them through LDS.  Accumulators (scores, state) become operands of the
 // next product in place (decay_mfma.h).  Where segments follow each other, a first pass forms their end states and a
 // scan joins them (decay_walk.hip).

@@ -18,8 +18,8 @@
 //
 // 4 x 2048 tokens, 12 heads of 128, bf16: 117 us for 206 MB of states, 101 of tensors in and 75 out (3.3 TB/s); 30 % of
 // the SIMDs' cycles issue vector work and 14 % matrix work, 45 % of the waves' wait: a chain of products with little
-// beside it at two workgroups a compute unit, which registers (128) and LDS (74 KB) allow.  Chunks of 64 tokens instead
-// of 32 halve the states' bytes; fp32 tensors, whose tiles take twice the LDS, stay at 32.
+// beside it at two workgroups a compute unit, which registers (256, four spilled) and LDS (74 KB) allow.  Chunks of 64
+// tokens instead of 32 halve the states' bytes; fp32 tensors, whose tiles take twice the LDS, stay at 32.
 #include "decay_mfma.h"
 
 namespace triune {
